@@ -340,6 +340,72 @@ int ima_class_count_replay(const void* x_operand, const void* w_operand, const v
                            float* out_f32, int64_t ld_f32, int32_t* mismatch_rows, int32_t* tiles_out,
                            const int32_t* tiles_in, void* stream);
 
+/* ---- 8-bit integer linears (W8A8) ---------------------------------------------------
+ * No counterpart in the reference: a student linear whose activations carry one int8 scale per
+ * token and whose weights one per output channel, so that the whole linear is one exact int8
+ * product; a gated feed-forward block of two of them; and their gradients.
+ *
+ * Quantiser: x [M,K] (row stride ldx) -> q [M,K] int8 = rint(RN32(x / s)), scale [M] fp32 =
+ * s = max(RN32(amax / 127), 1e-12), IEEE divisions, ties to even.  Columns K..round_up(K, 16)
+ * of a row of q may be written (ldq a multiple of 16, q 16-byte aligned).  A row with a NaN or an
+ * infinity gets scale NaN or inf and codes 0.  Weights are quantised with the same call, one row
+ * per output channel. */
+int ima_int8_quantize_rows(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq,
+                           float* scale, void* stream);
+
+/* Every int8 operand below is [rows, K] with K contiguous, 16-byte aligned, its row stride a
+ * multiple of 16, and K <= 131071 (the int32 sums are then exact for every int8 value).
+ *
+ * c [M,N] int32 = a b^T (row stride ldc) and/or y [M,N] = (fp32(c) * x_scale[m]) * w_scale[n]
+ * (+ bias[n] when bias != NULL), rounded once to y_dtype; a [M,K], b [N,K].  At least one
+ * output. */
+int ima_int8_gemm(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
+                  int32_t* c, int64_t ldc, const float* x_scale, const float* w_scale, const void* bias, int bias_dtype,
+                  void* y, int y_dtype, int64_t ldy, void* stream);
+
+/* Gated feed-forward block in one kernel: y [M,N] = act(g) * u with g = (fp32(a gate^T) *
+ * x_scale[m]) * gate_scale[n] (+ gate_bias[n]) and u the same of up. */
+#define IMA_ACT_SILU 0
+#define IMA_ACT_GELU 1      /* with the error function */
+#define IMA_ACT_GELU_TANH 2 /* with its tanh approximation */
+int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
+                        int64_t M, int64_t N, int64_t K, const float* x_scale, const float* gate_scale,
+                        const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype,
+                        int activation, void* y, int y_dtype, int64_t ldy, void* stream);
+/* Gradients of g and u from dh [M,N] (row stride ldh): g and u are formed again from the codes,
+ * d[m, n] = dh u act'(g) and d[m, seg_pitch + n] = dh act(g), fp32 (row stride ldd). */
+int ima_int8_gated_backward_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up,
+                                 int64_t ldu, int64_t M, int64_t N, int64_t K, const float* x_scale,
+                                 const float* gate_scale, const float* up_scale, const void* gate_bias,
+                                 const void* up_bias, int bias_dtype, int activation, const void* dh, int dh_dtype,
+                                 int64_t ldh, float* d, int64_t ldd, int64_t seg_pitch, void* stream);
+
+/* Base-256 digit planes of a real matrix, the left operand of a gradient product: v = rint(D / s),
+ * s = rowmax |D| / (127 * 256 + 127) with planes == 2, / (127 * 65536 + 127 * 256 + 127) with
+ * planes == 3, v = sum_p 256^p d_p, d_p in [-128, 127].
+ * _rows: D[m, j] = src[m, j] * col_scale[j] (col_scale NULL: 1); out [planes][M][ldp], row_scale
+ *   [M].  src, col_scale and out consist of `segs` (1 or 2) segments of seg_len columns, seg_pitch
+ *   apart; other columns of out are zero.
+ * _cols: D = src[m, j] * row_scale[m] (NULL: 1) transposed: out [planes][L][ldp], col_scale [L],
+ *   columns M.. of out zero.  sum_out (optional, [L] of sum_dtype) = sum_m src[m, j], in a fixed
+ *   order.  planes == 0: the sums alone.  workspace: ima_int8_cols_workspace_bytes(M, L). */
+int ima_int8_digits_rows(const void* src, int src_dtype, int64_t M, int64_t seg_len, int64_t seg_pitch, int segs,
+                         int64_t ld, const float* col_scale, int planes, int8_t* out, int64_t ldp, float* row_scale,
+                         void* stream);
+int64_t ima_int8_cols_workspace_bytes(int64_t M, int64_t L);
+int ima_int8_digits_cols(const void* src, int src_dtype, int64_t M, int64_t L, int64_t ld, const float* row_scale,
+                         int planes, int8_t* out, int64_t ldp, float* col_scale, void* sum_out, int sum_dtype,
+                         void* workspace, void* stream);
+/* dst [cols, rows] (row stride ldd, columns rows..round_up(rows, 16) zero) = src [rows, cols] transposed. */
+int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst, int64_t ldd,
+                       void* stream);
+/* y [M,N] = row_scale[m] * sum_p 256^p (a_planes[p] b^T)[m, n], a_planes [planes][M][lda], b [N,K].
+ * With b2 [N,K] the product of a second segment of the planes is added: the planes then hold K
+ * columns at 0 and K at round_up(K, 128), zero between. */
+int ima_int8_digit_gemm(const int8_t* a_planes, int planes, int64_t lda, const float* row_scale, const int8_t* b,
+                        int64_t ldb, const int8_t* b2, int64_t ldb2, int64_t M, int64_t N, int64_t K, void* y,
+                        int y_dtype, int64_t ldy, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

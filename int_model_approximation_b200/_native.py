@@ -31,6 +31,10 @@ IMA_DTYPE_F16 = 2
 IMA_SCHEME_DIGITS3 = 3
 IMA_SCHEME_DIGITS5 = 5
 
+IMA_ACT_SILU = 0
+IMA_ACT_GELU = 1
+IMA_ACT_GELU_TANH = 2
+
 _VP = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int
@@ -133,6 +137,34 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ima_hawkeye_replay": (
         _I32,
         [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _I32, _I32, _I32, _VP, _I64, _VP, _I64, _VP],
+    ),
+    "ima_int8_quantize_rows": (_I32, [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),
+    "ima_int8_gemm": (
+        _I32,
+        [_VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _I32, _I64, _VP],
+    ),
+    "ima_int8_gated_gemm": (
+        _I32,
+        [_VP, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _I64, _VP],
+    ),
+    "ima_int8_gated_backward_gemm": (
+        _I32,
+        [_VP, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _I64, _VP,
+         _I64, _I64, _VP],
+    ),
+    "ima_int8_digits_rows": (
+        _I32,
+        [_VP, _I32, _I64, _I64, _I64, _I32, _I64, _VP, _I32, _VP, _I64, _VP, _VP],
+    ),
+    "ima_int8_cols_workspace_bytes": (_I64, [_I64, _I64]),
+    "ima_int8_digits_cols": (
+        _I32,
+        [_VP, _I32, _I64, _I64, _I64, _VP, _I32, _VP, _I64, _VP, _VP, _I32, _VP, _VP],
+    ),
+    "ima_int8_transpose": (_I32, [_VP, _I64, _I64, _I64, _VP, _I64, _VP]),
+    "ima_int8_digit_gemm": (
+        _I32,
+        [_VP, _I32, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _I32, _I64, _VP],
     ),
     "ima_freivalds_workspace_bytes": (_I64, [_I64]),
     "ima_freivalds_fp8": (

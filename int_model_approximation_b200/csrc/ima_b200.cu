@@ -7,3 +7,5 @@
 #include "int_gemm.cu"
 #include "class_counts.cu"
 #include "class_count_engine.cu"
+#include "int8_quant.cu"
+#include "int8_gemm.cu"

@@ -45,6 +45,8 @@ enum ImaWhere {
     IMA_WHERE_GEMM_MMA = 3,
     IMA_WHERE_GEMM_EPILOGUE = 4,
     IMA_WHERE_CLASS_COUNTS = 5,
+    IMA_WHERE_INT8_GEMM = 6,
+    IMA_WHERE_INT8_SKINNY = 7,
 };
 
 // Host-side helper: record the CUDA error of the last call for ima_last_cuda_error().

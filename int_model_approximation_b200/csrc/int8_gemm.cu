@@ -1,0 +1,618 @@
+// Products of 8-bit integer matrices on tcgen05 kind::i8, with the epilogues of the 8-bit linears.
+//
+//   I8_LINEAR     C = A B^T (int32, exact),  y = (fp32(C) s_m) t_n + b_n
+//   I8_GATED      two products of one A:  h = act(g) u,  g = (fp32(A G^T) s_m) t^g_n + b^g_n, u likewise
+//   I8_GATED_BWD  the same two products again, then with dh read in the epilogue
+//                 D^g = dh u act'(g),  D^u = dh act(g)
+//   I8_DIGIT      A in P base-256 digit planes (int8_quant.cu):  y = s_m sum_p 256^p (A_p B^T)
+//
+// Sums.  |C| <= 128 * 128 * K < 2^31 for K <= 131,071, the longest contraction accepted, so the
+// int32 accumulators are exact; the digits' accumulators are joined in int64 and rounded to fp32
+// once.
+//
+// Tile and roles (persistent, 10 warps per CTA): a tile is 128 rows of A by BN rows of B.  A stage
+// holds 128 bytes of K of the P planes of A and of the tile's rows of B, 128-byte swizzled.
+//   warp 0    TMA producer;
+//   warp 1    allocates tensor memory and issues the MMAs (one thread);
+//   warps 2-9 epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 (one output row per thread) and
+//             half of the tile's columns, and stores 64-byte row pieces through shared memory, so
+//             that a warp store covers 8 rows of 64 contiguous bytes.
+// With one plane there are two accumulators, so the epilogue of a tile runs under the MMAs of
+// the next.  The gated forms put 128 rows of G and 128 rows of U into one B tile: a single MMA of
+// N = 256 forms g and u of the same 128 output columns, and A is read once for both.
+//
+// Every wait is bounded: one that runs out records IMA_ERR_TIMEOUT, and every role drains and
+// returns.
+#include <cudaTypedefs.h>
+#include <algorithm>
+#include "sm100_primitives.cuh"
+
+namespace {
+
+constexpr int I8_BM = 128;      // rows of A per CTA
+constexpr int I8_KT = 128;      // bytes of K per stage: one 128-byte swizzle row
+constexpr int I8_EPI_WARPS = 8;
+constexpr int I8_THREADS = 64 + I8_EPI_WARPS * 32;
+constexpr int64_t I8_MAX_K = 131071;
+
+enum I8Epi { I8_LINEAR = 0, I8_GATED = 1, I8_GATED_BWD = 2, I8_DIGIT = 3 };
+
+template <int P, int BN>
+struct I8Cfg {
+    static constexpr int A_PLANE = I8_BM * I8_KT;
+    static constexpr int B_BYTES = BN * I8_KT;
+    static constexpr int STAGE_BYTES = P * A_PLANE + B_BYTES;
+    static constexpr int STAGES = 200 * 1024 / STAGE_BYTES < 6 ? 200 * 1024 / STAGE_BYTES : 6;
+    static constexpr int ACC = P * BN;                       // tensor-memory columns of one tile
+    static constexpr int BUFS = 2 * ACC <= 512 ? 2 : 1;
+    static_assert(ACC <= 512, "accumulators exceed tensor memory");
+    static constexpr int STG_OFFSET = STAGES * STAGE_BYTES;  // 2 KB of output staging per epilogue warp
+    static constexpr int COL_OFFSET = STG_OFFSET + I8_EPI_WARPS * 2048;   // 256 floats per epilogue warp
+    static constexpr int BAR_OFFSET = COL_OFFSET + I8_EPI_WARPS * 1024;
+    static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 2 * BUFS + 1) * 8 + 16;
+    static constexpr int ALLOC = TOTAL + 1024;               // slack to align the base to 1024 B
+    static_assert(ALLOC <= 227 * 1024, "shared memory per CTA");
+};
+
+struct __align__(64) I8Params {
+    CUtensorMap ma, mb, mb2;        // A planes, B (or G), U
+    int32_t* c;
+    void* y;
+    const float* xs;                // [M] row scales
+    const float* ws[2];             // [N] column scales of B (or G) and U
+    const void* bias[2];
+    const void* dh;
+    float* d;                       // I8_GATED_BWD: D^g, and D^u seg_pitch columns further
+    int64_t ldc, ldy, ldh, ldd, seg_pitch;
+    int32_t M, N, m_tiles, n_tiles, k_tiles, group_m;
+    int32_t y_dtype, bias_dtype, dh_dtype, act, vec_c, vec_y, vec_d;
+    int32_t seg_tiles;              // I8_DIGIT: k-tiles of the first B; later ones read the second (mb2)
+    uint64_t stall_ns;              // test knob (ima_set_gemm_wait_test); 0 in normal use
+};
+
+// Tile t -> (row tile, column tile): groups of group_m row tiles, rows fastest within a group, so
+// that the tiles in flight share their k-slices of both operands in L2.
+IMA_DEVINL void i8_tile(const I8Params& p, int64_t t, int32_t& mt, int32_t& nt) {
+    const int64_t per_group = (int64_t)p.group_m * p.n_tiles;
+    const int32_t g = (int32_t)(t / per_group);
+    const int32_t within = (int32_t)(t - (int64_t)g * per_group);
+    const int32_t gm = min(p.group_m, p.m_tiles - g * p.group_m);
+    mt = g * p.group_m + within % gm;
+    nt = within / gm;
+}
+
+// ---------------------------------------------------------------------------
+// activations and their derivatives, fp32
+// ---------------------------------------------------------------------------
+template <int ACT>
+IMA_DEVINL float act_value(float g) {
+    if (ACT == IMA_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));
+    if (ACT == IMA_ACT_GELU) return 0.5f * g * erfcf(-0.70710678f * g);
+    const float z = 0.79788456f * (g + 0.044715f * g * g * g);
+    return 0.5f * g * (1.0f + tanhf(z));
+}
+// value a = act(g) and slope act'(g)
+template <int ACT>
+IMA_DEVINL void act_both(float g, float& a, float& da) {
+    if (ACT == IMA_ACT_SILU) {
+        const float s = __fdividef(1.0f, 1.0f + __expf(-g));
+        a = g * s;
+        da = s * (1.0f + g * (1.0f - s));
+    } else if (ACT == IMA_ACT_GELU) {
+        const float cdf = 0.5f * erfcf(-0.70710678f * g);
+        a = g * cdf;
+        da = cdf + g * 0.39894228f * __expf(-0.5f * g * g);
+    } else {
+        const float z = 0.79788456f * (g + 0.044715f * g * g * g);
+        const float t = tanhf(z);
+        a = 0.5f * g * (1.0f + t);
+        da = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g * g);
+    }
+}
+
+IMA_DEVINL uint32_t pack_half2(float lo, float hi, int dtype) {
+    if (dtype == IMA_DTYPE_BF16) {
+        __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&b);
+    }
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// 64 bytes of each of a warp's 32 rows (w: this lane's row) through 2 KB of shared memory to
+// base + row * pitch: each store instruction writes 8 rows of 64 contiguous bytes.  Slot j of row r
+// lies at j ^ (r / 2 % 4), which keeps both sides free of bank conflicts.  `bytes` of each row
+// and `rows` rows are written; without 16-byte alignment (vec == 0) element by element.
+IMA_DEVINL void stage_store(unsigned char* st, int lane, const uint32_t (&w)[16], unsigned char* base, int64_t pitch,
+                            int rows, int bytes, int vec, int esize) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<uint4*>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+        const int r = it * 8 + (lane >> 2), j = lane & 3;
+        const uint4 v = *reinterpret_cast<const uint4*>(st + r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+        const int left = bytes - j * 16;
+        if (r < rows && left > 0) {
+            unsigned char* dst = base + r * pitch + j * 16;
+            if (vec && left >= 16) {
+                *reinterpret_cast<uint4*>(dst) = v;
+            } else {
+                const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+                if (esize == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e * 4 < left) reinterpret_cast<uint32_t*>(dst)[e] = q[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e * 2 < left) reinterpret_cast<uint16_t*>(dst)[e] = (uint16_t)(q[e >> 1] >> (16 * (e & 1)));
+                }
+            }
+        }
+    }
+}
+
+// 32 fp32 values of this lane's row at column `col` of y, in y's type.
+IMA_DEVINL void store_y32(const I8Params& p, unsigned char* st, int lane, const float (&v)[32], int64_t row0, int rows,
+                          int32_t col) {
+    unsigned char* y = reinterpret_cast<unsigned char*>(p.y);
+    uint32_t w[16];
+    if (p.y_dtype == IMA_DTYPE_F32) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[hf * 16 + j]);
+            const int32_t c = col + hf * 16;
+            stage_store(st, lane, w, y + (row0 * p.ldy + c) * 4, p.ldy * 4, rows, (p.N - c) * 4, p.vec_y, 4);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack_half2(v[2 * j], v[2 * j + 1], p.y_dtype);
+        stage_store(st, lane, w, y + (row0 * p.ldy + col) * 2, p.ldy * 2, rows, (p.N - col) * 2, p.vec_y, 2);
+    }
+}
+
+template <int P, int BN, int EPI>
+__global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_constant__ I8Params p) {
+    using L = I8Cfg<P, BN>;
+    constexpr bool PAIR = EPI == I8_GATED || EPI == I8_GATED_BWD;   // B tile = BN / 2 rows of G, then of U
+    constexpr int TN = PAIR ? BN / 2 : BN;                          // output columns of a tile
+    constexpr int HALF = TN / 2;                                    // output columns of an epilogue warp
+    extern __shared__ unsigned char i8_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
+    uint64_t* empty = full + L::STAGES;
+    uint64_t* acc_full = empty + L::STAGES;
+    uint64_t* acc_empty = acc_full + L::BUFS;
+    uint64_t* drained = acc_empty + L::BUFS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t num_tiles = (int64_t)p.m_tiles * p.n_tiles;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < L::BUFS; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], I8_EPI_WARPS);
+        }
+        mbar_init(drained, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        // ---------------- TMA producer ----------------
+        uint32_t stage = 0, phase = 0;
+        uint64_t issued = 0;
+        for (int64_t t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+            int32_t mt, nt;
+            i8_tile(p, t, mt, nt);
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                if (!mbar_wait_or_abort(&empty[stage], phase ^ 1u, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM,
+                                        (int)stage))
+                    break;
+                ++issued;
+                unsigned char* sb = smem + stage * L::STAGE_BYTES;
+                mbar_arrive_expect_tx(&full[stage], (uint32_t)L::STAGE_BYTES);
+#pragma unroll
+                for (int i = 0; i < P; ++i)
+                    tma_load_3d(sb + i * L::A_PLANE, &p.ma, &full[stage], kt * I8_KT, mt * I8_BM, i);
+                unsigned char* bb = sb + P * L::A_PLANE;
+                if (EPI == I8_DIGIT && kt >= p.seg_tiles)
+                    tma_load_2d(bb, &p.mb2, &full[stage], (kt - p.seg_tiles) * I8_KT, nt * TN);
+                else
+                    tma_load_2d(bb, &p.mb, &full[stage], kt * I8_KT, nt * TN);
+                if (PAIR) tma_load_2d(bb + TN * I8_KT, &p.mb2, &full[stage], kt * I8_KT, nt * TN);
+                if (++stage == (uint32_t)L::STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+        // Every load issued lands before the CTA exits, also after an abort.
+        for (int s = 0; s < L::STAGES; ++s) {
+            const uint64_t rounds = issued / L::STAGES + ((uint64_t)s < issued % L::STAGES ? 1u : 0u);
+            if (rounds > 0)
+                mbar_wait_bounded(&full[s], (uint32_t)((rounds - 1) & 1u), IMA_WHERE_INT8_GEMM, 100 + s);
+        }
+    } else if (warp == 1 && lane == 0) {
+        // ---------------- MMA issuer ----------------
+        constexpr uint32_t idesc = idesc_i8(I8_BM, BN);
+        uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
+        if (p.stall_ns)   // test knob: a wait that nothing ends runs out
+            mbar_wait_or_abort(drained, 0u, abort_flag, p.stall_ns, IMA_WHERE_INT8_GEMM, -2);
+        for (int64_t t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+            if (!mbar_wait_or_abort(&acc_empty[buf], bphase ^ 1u, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM, -1))
+                break;
+            tc_fence_after();
+            const uint32_t acc = tmem_base + buf * L::ACC;
+            bool fed = true;
+            for (int kt = 0; kt < p.k_tiles; ++kt) {
+                if (!mbar_wait_or_abort(&full[stage], phase, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM,
+                                        50 + (int)stage)) {
+                    fed = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t sa = smem_u32(smem + stage * L::STAGE_BYTES);
+                const uint32_t sb = sa + P * L::A_PLANE;
+#pragma unroll
+                for (int ks = 0; ks < I8_KT / 32; ++ks)
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        mma_i8(acc + i * BN, umma_desc_sw128_kmajor(sa + i * L::A_PLANE + ks * 32),
+                               umma_desc_sw128_kmajor(sb + ks * 32), idesc, (kt | ks) ? 1u : 0u);
+                mma_commit(&empty[stage]);
+                if (++stage == (uint32_t)L::STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (!fed) break;
+            mma_commit(&acc_full[buf]);
+            if (++buf == (uint32_t)L::BUFS) { buf = 0; bphase ^= 1u; }
+        }
+        // Every MMA issued completes before the CTA frees tensor memory.
+        mma_commit(drained);
+        mbar_wait_bounded(drained, 0u, IMA_WHERE_INT8_GEMM, -3);
+    } else if (warp >= 2) {
+        // ---------------- epilogue ----------------
+        const int ew = warp - 2, q = warp & 3, h = ew >> 2;
+        unsigned char* st = smem + L::STG_OFFSET + ew * 2048;
+        float* cols = reinterpret_cast<float*>(smem + L::COL_OFFSET) + ew * 256;
+        uint32_t buf = 0, bphase = 0;
+        for (int64_t t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+            int32_t mt, nt;
+            i8_tile(p, t, mt, nt);
+            const int64_t row0 = (int64_t)mt * I8_BM + q * 32;
+            const int rows = (int)max((int64_t)0, min((int64_t)32, (int64_t)p.M - row0));
+            const int32_t n0 = nt * TN + h * HALF;
+            // this warp's column scales and biases: [2 operands][scale, bias][HALF]
+            if (EPI != I8_DIGIT) {
+                __syncwarp();
+                for (int i = lane; i < HALF; i += 32) {
+                    const int32_t n = n0 + i;
+#pragma unroll
+                    for (int o = 0; o < (PAIR ? 2 : 1); ++o) {
+                        cols[(2 * o) * HALF + i] = n < p.N && p.ws[o] ? p.ws[o][n] : 0.0f;
+                        cols[(2 * o + 1) * HALF + i] = n < p.N && p.bias[o] ? load_as_f32(p.bias[o], p.bias_dtype, n) : 0.0f;
+                    }
+                }
+            }
+            const float xs = lane < rows && p.xs ? p.xs[row0 + lane] : 0.0f;
+            const bool ok = mbar_wait_or_abort(&acc_full[buf], bphase, abort_flag, IMA_WAIT_LIMIT_NS,
+                                               IMA_WHERE_INT8_GEMM, 200);
+            __syncwarp();
+            if (!__all_sync(0xFFFFFFFFu, ok)) { *abort_flag = 1; break; }
+            tc_fence_after();
+            const uint32_t tq = tmem_base + ((uint32_t)(q * 32) << 16) + buf * L::ACC + h * HALF;
+            const bool zero = p.k_tiles == 0;   // K == 0: no MMA wrote the accumulators
+            if constexpr (EPI == I8_LINEAR) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < HALF; c0 += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(tq + c0, r);
+                    tmem_wait_ld();
+                    if (zero) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) r[j] = 0;
+                    }
+                    if (n0 + c0 >= p.N || rows == 0) continue;
+                    if (p.c) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = r[hf * 16 + j];
+                            const int32_t c = n0 + c0 + hf * 16;
+                            stage_store(st, lane, w, reinterpret_cast<unsigned char*>(p.c + row0 * p.ldc + c),
+                                        p.ldc * 4, rows, (p.N - c) * 4, p.vec_c, 4);
+                        }
+                    }
+                    if (p.y) {
+                        float v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)r[j]), xs), cols[c0 + j]);
+                            if (p.bias[0]) v[j] = __fadd_rn(v[j], cols[HALF + c0 + j]);
+                        }
+                        store_y32(p, st, lane, v, row0, rows, n0 + c0);
+                    }
+                }
+            } else if constexpr (EPI == I8_GATED) {
+                auto chunks = [&](auto tag) {
+                    constexpr int ACT = decltype(tag)::value;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HALF; c0 += 32) {
+                        uint32_t rg[32], ru[32];
+                        tmem_ld32(tq + c0, rg);
+                        tmem_ld32(tq + TN + c0, ru);
+                        tmem_wait_ld();
+                        if (n0 + c0 >= p.N || rows == 0) continue;
+                        float v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float g0 = zero ? 0.0f : __int2float_rn((int32_t)rg[j]);
+                            const float u0 = zero ? 0.0f : __int2float_rn((int32_t)ru[j]);
+                            const float g = __fadd_rn(__fmul_rn(__fmul_rn(g0, xs), cols[c0 + j]), cols[HALF + c0 + j]);
+                            const float u = __fadd_rn(__fmul_rn(__fmul_rn(u0, xs), cols[2 * HALF + c0 + j]),
+                                                      cols[3 * HALF + c0 + j]);
+                            v[j] = act_value<ACT>(g) * u;
+                        }
+                        store_y32(p, st, lane, v, row0, rows, n0 + c0);
+                    }
+                };
+                if (p.act == IMA_ACT_SILU) chunks(std::integral_constant<int, IMA_ACT_SILU>{});
+                else if (p.act == IMA_ACT_GELU) chunks(std::integral_constant<int, IMA_ACT_GELU>{});
+                else chunks(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
+            } else if constexpr (EPI == I8_GATED_BWD) {
+                auto chunks = [&](auto tag) {
+                    constexpr int ACT = decltype(tag)::value;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < HALF; c0 += 16) {
+                        uint32_t rg[16], ru[16];
+                        tmem_ld16(tq + c0, rg);
+                        tmem_ld16(tq + TN + c0, ru);
+                        const int32_t n = n0 + c0;
+                        float dh[16];
+                        if (lane < rows && n < p.N) {
+                            const unsigned char* src = reinterpret_cast<const unsigned char*>(p.dh) +
+                                                       ((row0 + lane) * p.ldh + n) * dtype_bytes(p.dh_dtype);
+                            const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+                            float a[8], b[8];
+                            load8(src, p.dh_dtype, 0, p.N - n, vec, a);
+                            load8(src, p.dh_dtype, 8, p.N - n, vec, b);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) { dh[j] = a[j]; dh[8 + j] = b[j]; }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) dh[j] = 0.0f;
+                        }
+                        tmem_wait_ld();
+                        if (n >= p.N || rows == 0) continue;
+                        uint32_t wg[16], wu[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float g0 = zero ? 0.0f : __int2float_rn((int32_t)rg[j]);
+                            const float u0 = zero ? 0.0f : __int2float_rn((int32_t)ru[j]);
+                            const float g = __fadd_rn(__fmul_rn(__fmul_rn(g0, xs), cols[c0 + j]), cols[HALF + c0 + j]);
+                            const float u = __fadd_rn(__fmul_rn(__fmul_rn(u0, xs), cols[2 * HALF + c0 + j]),
+                                                      cols[3 * HALF + c0 + j]);
+                            float a, da;
+                            act_both<ACT>(g, a, da);
+                            wg[j] = __float_as_uint(dh[j] * u * da);
+                            wu[j] = __float_as_uint(dh[j] * a);
+                        }
+                        float* d = p.d + row0 * p.ldd + n;
+                        stage_store(st, lane, wg, reinterpret_cast<unsigned char*>(d), p.ldd * 4, rows, (p.N - n) * 4,
+                                    p.vec_d, 4);
+                        stage_store(st, lane, wu, reinterpret_cast<unsigned char*>(d + p.seg_pitch), p.ldd * 4, rows,
+                                    (p.N - n) * 4, p.vec_d, 4);
+                    }
+                };
+                if (p.act == IMA_ACT_SILU) chunks(std::integral_constant<int, IMA_ACT_SILU>{});
+                else if (p.act == IMA_ACT_GELU) chunks(std::integral_constant<int, IMA_ACT_GELU>{});
+                else chunks(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
+            } else {
+#pragma unroll 1
+                for (int c0 = 0; c0 < HALF; c0 += 32) {
+                    uint32_t r[P][32];
+#pragma unroll
+                    for (int i = 0; i < P; ++i) tmem_ld32(tq + i * BN + c0, r[i]);
+                    tmem_wait_ld();
+                    if (n0 + c0 >= p.N || rows == 0) continue;
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        int64_t s = 0;
+#pragma unroll
+                        for (int i = 0; i < P; ++i) s += (int64_t)(int32_t)r[i][j] << (8 * i);
+                        v[j] = zero ? __fmul_rn(0.0f, xs) : __fmul_rn(__ll2float_rn(s), xs);
+                    }
+                    store_y32(p, st, lane, v, row0, rows, n0 + c0);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (++buf == (uint32_t)L::BUFS) { buf = 0; bphase ^= 1u; }
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// Map over [planes][rows][K] bytes (row pitch ld) with a {128 B, box_rows(, 1)} box, 128-byte swizzle.
+int make_i8_map(CUtensorMap* map, const int8_t* base, int64_t K, int64_t ld, int64_t rows, int planes, int box_rows,
+                bool three_d) {
+    auto enc = get_encode_fn();
+    if (!enc) return IMA_ERR_CUDA;
+    cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(ld * rows)};
+    cuuint32_t box[3] = {(cuuint32_t)I8_KT, (cuuint32_t)box_rows, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, three_d ? 3 : 2, const_cast<int8_t*>(base), dims, strides, box,
+                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? IMA_OK : IMA_ERR_INVALID_ARGUMENT;
+}
+
+// An int8 operand as the loads need it: 16-byte aligned rows of at least K bytes.
+int check_i8_operand(const int8_t* p, int64_t rows, int64_t K, int64_t ld) {
+    if (rows < 0 || K < 0) return IMA_ERR_INVALID_ARGUMENT;
+    if (K > 0 && rows > 0 && !p) return IMA_ERR_INVALID_ARGUMENT;
+    if (ld < K || ld % 16 || (reinterpret_cast<uintptr_t>(p) & 15)) return IMA_ERR_INVALID_ARGUMENT;
+    if (rows > INT32_MAX / 2 || ld > INT32_MAX || K > I8_MAX_K) return IMA_ERR_UNSUPPORTED;
+    return IMA_OK;
+}
+
+bool aligned16(const void* p, int64_t pitch_bytes) { return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15); }
+
+template <int P, int BN, int EPI>
+int launch_i8(I8Params& p, cudaStream_t stream) {
+    using L = I8Cfg<P, BN>;
+    constexpr int TN = EPI == I8_GATED || EPI == I8_GATED_BWD ? BN / 2 : BN;
+    p.m_tiles = (p.M + I8_BM - 1) / I8_BM;
+    p.n_tiles = (p.N + TN - 1) / TN;
+    p.group_m = 16;
+    p.stall_ns = g_gemm_stall_ns;
+    auto kern = int8_gemm_kernel<P, BN, EPI>;
+    int rc = ima_note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+    if (rc != IMA_OK) return rc;
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    const int grid = (int)std::min<int64_t>(tiles, gemm_grid_limit());
+    kern<<<grid, I8_THREADS, L::ALLOC, stream>>>(p);
+    return IMA_LAUNCH_STATUS();
+}
+
+// The maps of a product: A planes (Ka columns) in 128-row boxes, B (or G and U; K columns) in boxes of
+// a tile's rows.
+int make_i8_maps(I8Params& p, const int8_t* a, int64_t lda, int planes, const int8_t* b, int64_t ldb, const int8_t* b2,
+                 int64_t ldb2, int64_t Ka, int64_t K, int b_rows) {
+    p.k_tiles = (int32_t)((Ka + I8_KT - 1) / I8_KT);
+    if (K == 0) return IMA_OK;   // nothing is loaded
+    int rc = make_i8_map(&p.ma, a, Ka, lda, p.M, planes, I8_BM, true);
+    if (rc == IMA_OK) rc = make_i8_map(&p.mb, b, K, ldb, p.N, 1, b_rows, false);
+    if (rc == IMA_OK && b2) rc = make_i8_map(&p.mb2, b2, K, ldb2, p.N, 1, b_rows, false);
+    return rc;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ima_int8_gemm(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
+                  int32_t* c, int64_t ldc, const float* x_scale, const float* w_scale, const void* bias, int bias_dtype,
+                  void* y, int y_dtype, int64_t ldy, void* stream) {
+    int rc = check_i8_operand(a, M, K, lda);
+    if (rc == IMA_OK) rc = check_i8_operand(b, N, K, ldb);
+    if (rc != IMA_OK) return rc;
+    if (M == 0 || N == 0) return IMA_OK;
+    if (!c && !y) return IMA_ERR_INVALID_ARGUMENT;
+    if (c && ldc < N && M > 1) return IMA_ERR_INVALID_ARGUMENT;
+    if (y && (!x_scale || !w_scale || (ldy < N && M > 1) || !known_dtype(y_dtype))) return IMA_ERR_INVALID_ARGUMENT;
+    if (y && bias && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    I8Params p;
+    memset(&p, 0, sizeof(p));
+    p.c = c; p.y = y; p.xs = x_scale; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
+    p.ldc = ldc; p.ldy = ldy; p.y_dtype = y_dtype;
+    p.M = (int32_t)M; p.N = (int32_t)N;
+    p.vec_c = c && aligned16(c, ldc * 4);
+    p.vec_y = y && aligned16(y, ldy * dtype_bytes(y_dtype));
+    rc = make_i8_maps(p, a, lda, 1, b, ldb, nullptr, 0, K, K, 256);
+    if (rc != IMA_OK) return rc;
+    return launch_i8<1, 256, I8_LINEAR>(p, (cudaStream_t)stream);
+}
+
+int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
+                        int64_t M, int64_t N, int64_t K, const float* x_scale, const float* gate_scale,
+                        const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype,
+                        int activation, void* y, int y_dtype, int64_t ldy, void* stream) {
+    int rc = check_i8_operand(a, M, K, lda);
+    if (rc == IMA_OK) rc = check_i8_operand(gate, N, K, ldg);
+    if (rc == IMA_OK) rc = check_i8_operand(up, N, K, ldu);
+    if (rc != IMA_OK) return rc;
+    if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
+    if (M == 0 || N == 0) return IMA_OK;
+    if (!y || !x_scale || !gate_scale || !up_scale || (ldy < N && M > 1) || !known_dtype(y_dtype))
+        return IMA_ERR_INVALID_ARGUMENT;
+    if ((gate_bias || up_bias) && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    I8Params p;
+    memset(&p, 0, sizeof(p));
+    p.y = y; p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
+    p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = activation;
+    p.M = (int32_t)M; p.N = (int32_t)N;
+    p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
+    rc = make_i8_maps(p, a, lda, 1, gate, ldg, up, ldu, K, K, 128);
+    if (rc != IMA_OK) return rc;
+    return launch_i8<1, 256, I8_GATED>(p, (cudaStream_t)stream);
+}
+
+int ima_int8_gated_backward_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up,
+                                 int64_t ldu, int64_t M, int64_t N, int64_t K, const float* x_scale,
+                                 const float* gate_scale, const float* up_scale, const void* gate_bias,
+                                 const void* up_bias, int bias_dtype, int activation, const void* dh, int dh_dtype,
+                                 int64_t ldh, float* d, int64_t ldd, int64_t seg_pitch, void* stream) {
+    int rc = check_i8_operand(a, M, K, lda);
+    if (rc == IMA_OK) rc = check_i8_operand(gate, N, K, ldg);
+    if (rc == IMA_OK) rc = check_i8_operand(up, N, K, ldu);
+    if (rc != IMA_OK) return rc;
+    if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
+    if (M == 0 || N == 0) return IMA_OK;
+    if (!dh || !d || !x_scale || !gate_scale || !up_scale || !known_dtype(dh_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    if ((ldh < N && M > 1) || seg_pitch < N || (ldd < seg_pitch + N && M > 1)) return IMA_ERR_INVALID_ARGUMENT;
+    if ((gate_bias || up_bias) && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    I8Params p;
+    memset(&p, 0, sizeof(p));
+    p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
+    p.bias_dtype = bias_dtype; p.act = activation; p.dh = dh; p.dh_dtype = dh_dtype; p.ldh = ldh;
+    p.d = d; p.ldd = ldd; p.seg_pitch = seg_pitch;
+    p.M = (int32_t)M; p.N = (int32_t)N;
+    p.vec_d = aligned16(d, ldd * 4) && seg_pitch % 4 == 0;
+    rc = make_i8_maps(p, a, lda, 1, gate, ldg, up, ldu, K, K, 128);
+    if (rc != IMA_OK) return rc;
+    return launch_i8<1, 256, I8_GATED_BWD>(p, (cudaStream_t)stream);
+}
+
+int ima_int8_digit_gemm(const int8_t* a_planes, int planes, int64_t lda, const float* row_scale, const int8_t* b,
+                        int64_t ldb, const int8_t* b2, int64_t ldb2, int64_t M, int64_t N, int64_t K, void* y,
+                        int y_dtype, int64_t ldy, void* stream) {
+    if (planes != 2 && planes != 3) return IMA_ERR_UNSUPPORTED;
+    // with a second B the planes hold two segments of K columns, the second on a k-tile boundary
+    const int64_t seg = b2 ? (K + I8_KT - 1) / I8_KT * I8_KT : 0;
+    int rc = check_i8_operand(a_planes, M, seg + K, lda);
+    if (rc == IMA_OK) rc = check_i8_operand(b, N, K, ldb);
+    if (rc == IMA_OK && b2) rc = check_i8_operand(b2, N, K, ldb2);
+    if (rc != IMA_OK) return rc;
+    if (M == 0 || N == 0) return IMA_OK;
+    if (!y || !row_scale || (ldy < N && M > 1) || !known_dtype(y_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    I8Params p;
+    memset(&p, 0, sizeof(p));
+    p.y = y; p.xs = row_scale; p.ldy = ldy; p.y_dtype = y_dtype;
+    p.M = (int32_t)M; p.N = (int32_t)N;
+    p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
+    rc = make_i8_maps(p, a_planes, lda, planes, b, ldb, b2, ldb2, seg + K, K, planes == 2 ? 256 : 128);
+    if (rc != IMA_OK) return rc;
+    p.seg_tiles = (int32_t)((K + I8_KT - 1) / I8_KT);
+    if (planes == 2) return launch_i8<2, 256, I8_DIGIT>(p, (cudaStream_t)stream);
+    return launch_i8<3, 128, I8_DIGIT>(p, (cudaStream_t)stream);
+}
+
+}  // extern "C"

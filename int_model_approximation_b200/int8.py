@@ -1,0 +1,565 @@
+"""8-bit integer linears (W8A8): one int8 scale per token and per output channel.
+
+The codebook student reproduces an FP8 linear bit for bit and pays nine int8 products per
+multiplication for it.  The operators here pay one: activations are quantised per token and
+weights per output channel to int8, the product is exact in int32 (and Freivalds-checkable
+like every integer product of this package), and the scales are applied in the epilogue.
+There is no counterpart in the reference.
+
+  per_token_int8    the quantiser of both sides
+  Int8Weight        a weight's codes and channel scales, laid out once
+  int8_gemm         codes in, exact int32 product and/or rescaled output (beside codebook.int_gemm)
+  int8_linear       y = x W^T + b
+  int8_gated        h = act(x Wg^T + bg) * (x Wu^T + bu), both projections, activation and product
+                    in one kernel
+  int8_linear_backward, int8_gated_backward   their gradients as plain calls
+
+int8_linear and int8_gated take part in autograd.  Gradients pass straight through the
+rounding: they are the derivatives at the dequantised activations and weights, with the
+scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
+gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
+products of a backward pass run on the int8 tensor cores too: the gradient is written in
+base-256 digits of its row maximum (two digits for bf16 tensors, three for fp16 and fp32; see
+csrc/int8_quant.cu).
+
+Shapes: every contraction (K; in the backward pass also N, the padded pair of N for the gated
+block, and the number of tokens for a weight gradient) is at most 131071, so that int32 sums are
+exact.  Rows whose activations hold a NaN or an infinity come out as NaN.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _native as nat
+
+MAX_K = 131071
+ACTIVATIONS = {"silu": nat.IMA_ACT_SILU, "gelu": nat.IMA_ACT_GELU, "gelu_tanh": nat.IMA_ACT_GELU_TANH}
+
+
+def _round_up(v: int, to: int) -> int:
+    return (v + to - 1) // to * to
+
+
+def _require_cuda(t: torch.Tensor, label: str) -> None:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{label} must be on CUDA; this repo has no CPU execution path")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t [..., K] as a matrix whose rows are contiguous and do not overlap (a copy if need be)."""
+    r = t if t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    if (r.stride(1) != 1 and r.shape[1] > 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
+        r = r.contiguous()
+    return r
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a matrix from _rows (a single row has none of its own)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _empty_codes(rows: int, k: int, device: torch.device) -> torch.Tensor:
+    """int8 [rows, k] whose rows start on 16 bytes."""
+    return torch.empty((rows, _round_up(max(k, 1), 16)), dtype=torch.int8, device=device)[:, :k]
+
+
+def _aligned_codes(t: torch.Tensor, label: str) -> torch.Tensor:
+    """An int8 matrix as the kernels load it: contiguous rows that start on 16 bytes (a copy
+    only if it is not)."""
+    if t.dtype != torch.int8 or t.ndim != 2:
+        raise RuntimeError(f"{label} must be a 2-D int8 tensor, got {t.dtype} {tuple(t.shape)}")
+    _require_cuda(t, label)
+    if t.shape[1] > MAX_K:
+        raise RuntimeError(f"{label}: contraction of {t.shape[1]} exceeds {MAX_K} (exact int32 sums)")
+    one_row = t.shape[0] <= 1
+    if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or t.data_ptr() % 16 or
+                      not one_row and (t.stride(0) % 16 or t.stride(0) < t.shape[1])):
+        out = _empty_codes(t.shape[0], t.shape[1], t.device)
+        out.copy_(t)
+        return out
+    return t
+
+
+def _code_ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else _round_up(max(t.shape[1], 1), 16)
+
+
+def _scales(t: torch.Tensor, n: int, label: str) -> torch.Tensor:
+    s = t.detach().reshape(-1).to(torch.float32).contiguous()
+    if s.numel() != n:
+        raise RuntimeError(f"{label} has {s.numel()} entries, expected {n}")
+    return s
+
+
+def per_token_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-token int8 quantisation of x [..., K] in one kernel: (codes int8 [M, K], scale fp32 [M, 1]).
+
+    scale = max(amax / 127, 1e-12) and codes = round(x / scale), both as IEEE fp32 divisions,
+    ties to even.  The codes are a view of rows padded to 16 bytes.  A row with a NaN or an
+    infinity has that scale and codes 0."""
+    _require_cuda(x, "int8 activation")
+    return _quantise(_rows(x.detach()))
+
+
+def _quantise(rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    m, k = rows.shape
+    dev = rows.device
+    q = _empty_codes(m, k, dev)
+    scale = torch.empty((m, 1), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("ima_int8_quantize_rows", rows.data_ptr(), nat.dtype_code(rows.dtype), m, k, _ld(rows), q.data_ptr(),
+                 _code_ld(q), scale.data_ptr(), nat.stream_of(dev))
+    return q, scale
+
+
+def _transpose(t: torch.Tensor) -> torch.Tensor:
+    """int8 [rows, cols] (aligned) -> [cols, rows]."""
+    rows, cols = t.shape
+    out = _empty_codes(cols, rows, t.device)
+    with torch.cuda.device(t.device):
+        nat.call("ima_int8_transpose", t.data_ptr(), rows, cols, _code_ld(t), out.data_ptr(), _code_ld(out),
+                 nat.stream_of(t.device))
+    return out
+
+
+class Int8Weight:
+    """A weight [N, K] as int8 codes and one fp32 scale per output channel, laid out once.
+
+    `codes` and `scale` stay the caller's tensors where their layout allows it (rows on 16-byte
+    boundaries); the transposed codes that a backward pass contracts over are made at the first
+    one and kept until the codes change."""
+
+    def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
+        self.codes = _aligned_codes(codes.detach(), "int8 weight")
+        nat.require_device(codes.device, ("weight scale", scale))
+        self.scale = _scales(scale, codes.shape[0], "weight scale")
+        self._transposed: tuple | None = None
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor) -> "Int8Weight":
+        """Quantise a floating weight [N, K], one scale per row."""
+        if weight.ndim != 2:
+            raise RuntimeError(f"int8 weight source must be 2-D, got {tuple(weight.shape)}")
+        _require_cuda(weight, "int8 weight source")
+        return cls(*per_token_int8(weight))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def transposed(self) -> torch.Tensor:
+        version = nat.tensor_version(self.codes)
+        if self._transposed is not None and version is not None and self._transposed[1] == version:
+            return self._transposed[0]
+        t = _transpose(self.codes)
+        self._transposed = (t, version)
+        return t
+
+
+# ---------------------------------------------------------------------------
+# products
+# ---------------------------------------------------------------------------
+def _check_out(t: torch.Tensor, shape: tuple[int, int], dtypes: tuple, label: str) -> None:
+    if tuple(t.shape) != shape or t.dtype not in dtypes:
+        raise RuntimeError(f"{label} is {t.dtype} {tuple(t.shape)}, expected {shape} of {dtypes}")
+    if t.numel() and (t.stride(1) != 1 and shape[1] > 1 or shape[0] > 1 and t.stride(0) < shape[1]):
+        raise RuntimeError(f"{label} must have contiguous rows that do not overlap")
+
+
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _bias_args(n: int, *biases: torch.Tensor | None) -> tuple[list[torch.Tensor | None], int]:
+    """Biases as contiguous vectors of one floating type, and that type's code."""
+    given = [b for b in biases if b is not None]
+    if not given:
+        return list(biases), 0
+    dtype = given[0].dtype if all(b.dtype == given[0].dtype for b in given) else torch.float32
+    if dtype not in _FLOATS:
+        dtype = torch.float32
+    out = []
+    for b in biases:
+        if b is not None:
+            b = b.detach().reshape(-1).to(dtype).contiguous()
+            if b.numel() != n:
+                raise RuntimeError(f"bias has {b.numel()} entries, expected {n}")
+        out.append(b)
+    return out, nat.dtype_code(dtype)
+
+
+def int8_gemm(
+    a: torch.Tensor,
+    b: torch.Tensor,
+    *,
+    want_c: bool = True,
+    x_scale: torch.Tensor | None = None,
+    w_scale: torch.Tensor | None = None,
+    bias: torch.Tensor | None = None,
+    y_dtype: torch.dtype | None = None,
+    c_out: torch.Tensor | None = None,
+    y_out: torch.Tensor | None = None,
+):
+    """C = A B^T exactly (int32) and/or y = (fp32(C) * x_scale[m]) * w_scale[n] (+ bias).
+
+    a: int8 [M, K]; b: int8 [N, K], any strides (rows that do not start on 16 bytes are copied).
+    Returns (c int32 [M, N] or None, y [M, N] or None)."""
+    a = _aligned_codes(a, "int8 activation matrix")
+    b = _aligned_codes(b, "int8 weight matrix")
+    m, k = a.shape
+    n = b.shape[0]
+    if b.shape[1] != k:
+        raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={b.shape[1]}")
+    dev = a.device
+    c = c_out if c_out is not None else (torch.empty((m, n), dtype=torch.int32, device=dev) if want_c else None)
+    if c is not None:
+        _check_out(c, (m, n), (torch.int32,), "int8 product")
+    y, bias_dtype = None, 0
+    if y_dtype is not None or y_out is not None:
+        if x_scale is None or w_scale is None:
+            raise RuntimeError("int8_gemm needs x_scale and w_scale for the rescaled output")
+        y = y_out if y_out is not None else torch.empty((m, n), dtype=y_dtype, device=dev)
+        _check_out(y, (m, n), _FLOATS, "output")
+        nat.require_device(dev, ("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias))
+        x_scale = _scales(x_scale, m, "x_scale")
+        w_scale = _scales(w_scale, n, "w_scale")
+        (bias,), bias_dtype = _bias_args(n, bias)
+    else:
+        x_scale = w_scale = bias = None
+    if c is None and y is None:
+        raise RuntimeError("int8_gemm has no output to compute: want_c, y_dtype or y_out")
+    nat.require_device(dev, ("B matrix", b), ("int32 output", c), ("output", y))
+    with torch.cuda.device(dev):
+        nat.call(
+            "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, nat.ptr(c),
+            _ld(c) if c is not None else n, nat.ptr(x_scale), nat.ptr(w_scale), nat.ptr(bias), bias_dtype, nat.ptr(y),
+            nat.dtype_code(y.dtype) if y is not None else 0, _ld(y) if y is not None else n, nat.stream_of(dev),
+        )
+    return c, y
+
+
+def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None):
+    """(y [M, N], codes, scale) of x rows."""
+    q, scale = _quantise(rows)
+    _c, y = int8_gemm(q, weight.codes, want_c=False, x_scale=scale, w_scale=weight.scale, bias=bias, y_dtype=rows.dtype)
+    return y, q, scale
+
+
+def _gated_args(q: torch.Tensor, scale: torch.Tensor, gate: Int8Weight, up: Int8Weight, biases, bias_dtype: int,
+                activation: str) -> tuple:
+    m, k = q.shape
+    return (q.data_ptr(), _code_ld(q), gate.codes.data_ptr(), _code_ld(gate.codes), up.codes.data_ptr(),
+            _code_ld(up.codes), m, gate.shape[0], k, scale.data_ptr(), gate.scale.data_ptr(), up.scale.data_ptr(),
+            nat.ptr(biases[0]), nat.ptr(biases[1]), bias_dtype, ACTIVATIONS[activation])
+
+
+def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bias, up_bias, activation: str):
+    q, scale = _quantise(rows)
+    dev = rows.device
+    m, n = rows.shape[0], gate.shape[0]
+    h = torch.empty((m, n), dtype=rows.dtype, device=dev)
+    biases, bias_dtype = _bias_args(n, gate_bias, up_bias)
+    with torch.cuda.device(dev):
+        nat.call("ima_int8_gated_gemm", *_gated_args(q, scale, gate, up, biases, bias_dtype, activation), h.data_ptr(),
+                 nat.dtype_code(h.dtype), max(n, 1), nat.stream_of(dev))
+    return h, q, scale
+
+
+# ---------------------------------------------------------------------------
+# gradients
+# ---------------------------------------------------------------------------
+def _digit_count(*dtypes: torch.dtype) -> int:
+    """Digits of a gradient: two reach 2^-16 of its row maximum, three 2^-24.  Over rows whose elements
+    differ a lot (a column of token gradients) two are off by up to 6e-4 of the result's norm: below
+    bf16's own rounding (2e-3), above fp16's (2e-4)."""
+    return 2 if all(t in (None, torch.bfloat16) for t in dtypes) else 3
+
+
+def _digits_rows(src: torch.Tensor, seg_len: int, seg_pitch: int, segs: int, col_scale: torch.Tensor, planes: int):
+    m = src.shape[0]
+    dev = src.device
+    width = _round_up(max((segs - 1) * seg_pitch + seg_len, 1), 16)
+    out = torch.empty((planes, m, width), dtype=torch.int8, device=dev)
+    scale = torch.empty((m,), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("ima_int8_digits_rows", src.data_ptr(), nat.dtype_code(src.dtype), m, seg_len, seg_pitch, segs, _ld(src),
+                 col_scale.data_ptr(), planes, out.data_ptr(), width, scale.data_ptr(), nat.stream_of(dev))
+    return out, scale
+
+
+def _digits_cols(src: torch.Tensor, row_scale: torch.Tensor, planes: int, sum_dtype: torch.dtype | None):
+    """Transposed digits of src [M, L] (planes == 0: none) and its column sums (sum_dtype None: none)."""
+    m, length = src.shape
+    dev = src.device
+    width = _round_up(max(m, 1), 16)
+    out = torch.empty((planes, length, width), dtype=torch.int8, device=dev) if planes else None
+    scale = torch.empty((length,), dtype=torch.float32, device=dev) if planes else None
+    sums = torch.empty((length,), dtype=sum_dtype, device=dev) if sum_dtype is not None else None
+    ws = torch.empty((int(nat.lib().ima_int8_cols_workspace_bytes(m, length)),), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("ima_int8_digits_cols", src.data_ptr(), nat.dtype_code(src.dtype), m, length, _ld(src),
+                 row_scale.data_ptr(), planes, nat.ptr(out), width, nat.ptr(scale), nat.ptr(sums),
+                 nat.dtype_code(sum_dtype) if sums is not None else 0, ws.data_ptr(), nat.stream_of(dev))
+    return out, scale, sums
+
+
+def _digit_gemm(planes: torch.Tensor, row_scale: torch.Tensor, b: torch.Tensor, b2: torch.Tensor | None, m: int,
+                k: int, dtype: torch.dtype) -> torch.Tensor:
+    n = b.shape[0]
+    dev = planes.device
+    y = torch.empty((m, n), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        nat.call("ima_int8_digit_gemm", planes.data_ptr(), planes.shape[0], planes.shape[2], row_scale.data_ptr(),
+                 b.data_ptr(), _code_ld(b), nat.ptr(b2), _code_ld(b2) if b2 is not None else 0, m, n, k, y.data_ptr(),
+                 nat.dtype_code(dtype), max(n, 1), nat.stream_of(dev))
+    return y
+
+
+def _check_backward(m: int, contraction: int, want_dw: bool) -> None:
+    if contraction > MAX_K:
+        raise RuntimeError(f"int8 backward: contraction of {contraction} exceeds {MAX_K} (exact int32 sums)")
+    if want_dw and m > MAX_K:
+        raise RuntimeError(f"int8 weight gradient over {m} tokens exceeds {MAX_K} (exact int32 sums); split the batch")
+
+
+def _grad_rows(grad: torch.Tensor, m: int, n: int, dev: torch.device) -> torch.Tensor:
+    if grad.shape[-1] != n or grad.numel() != m * n:
+        raise RuntimeError(f"output gradient has shape {tuple(grad.shape)}, expected {m} rows of {n}")
+    nat.require_device(dev, ("output gradient", grad))
+    nat.dtype_code(grad.dtype)
+    return _rows(grad.detach().reshape(m, n))
+
+
+def _weight_gradient(d: torch.Tensor, codes_t: torch.Tensor | None, scale: torch.Tensor, g_dtype: torch.dtype,
+                     w_dtype: torch.dtype | None, b_dtype: torch.dtype | None):
+    """(dW, db) of one projection from its output gradient d [M, N]; g_dtype: the type d came from."""
+    want_dw = w_dtype is not None
+    if not want_dw and b_dtype is None:
+        return None, None
+    m, n = d.shape
+    planes = _digit_count(g_dtype, w_dtype) if want_dw else 0
+    digits, digit_scale, db = _digits_cols(d, scale, planes, b_dtype)
+    dw = None
+    if want_dw:
+        if m == 0:
+            dw = torch.zeros((n, codes_t.shape[0]), dtype=w_dtype, device=d.device)
+        else:
+            dw = _digit_gemm(digits, digit_scale, codes_t, None, n, m, w_dtype)
+    return dw, db
+
+
+def int8_linear_backward(
+    grad: torch.Tensor,
+    codes: torch.Tensor,
+    scale: torch.Tensor,
+    weight: Int8Weight,
+    *,
+    dx_dtype: torch.dtype | None = None,
+    dw_dtype: torch.dtype | None = None,
+    db_dtype: torch.dtype | None = None,
+):
+    """Gradients of int8_linear as (dx [M, K], dw [N, K], db [N]); None where no type is given.
+
+    grad: output gradient [..., N]; codes, scale: per_token_int8 of the activations.  Launches only,
+    on the current stream."""
+    codes = _aligned_codes(codes, "int8 activation matrix")
+    m, n = codes.shape[0], weight.shape[0]
+    dev = codes.device
+    if weight.shape[1] != codes.shape[1]:
+        raise RuntimeError(f"int8 matmul shape mismatch: K={codes.shape[1]} vs K={weight.shape[1]}")
+    nat.require_device(dev, ("weight", weight.codes), ("scale", scale))
+    scale = _scales(scale, m, "scale")
+    d = _grad_rows(grad, m, n, dev)
+    _check_backward(m, n if dx_dtype is not None else 0, dw_dtype is not None)
+    dx = None
+    if dx_dtype is not None:
+        digits, digit_scale = _digits_rows(d, n, n, 1, weight.scale, _digit_count(d.dtype, dx_dtype))
+        dx = _digit_gemm(digits, digit_scale, weight.transposed(), None, m, n, dx_dtype)
+    codes_t = _transpose(codes) if dw_dtype is not None else None
+    dw, db = _weight_gradient(d, codes_t, scale, d.dtype, dw_dtype, db_dtype)
+    return dx, dw, db
+
+
+def int8_gated_backward(
+    grad: torch.Tensor,
+    codes: torch.Tensor,
+    scale: torch.Tensor,
+    gate: Int8Weight,
+    up: Int8Weight,
+    gate_bias: torch.Tensor | None = None,
+    up_bias: torch.Tensor | None = None,
+    *,
+    activation: str = "silu",
+    dx_dtype: torch.dtype | None = None,
+    dgate_dtype: torch.dtype | None = None,
+    dup_dtype: torch.dtype | None = None,
+    gate_db_dtype: torch.dtype | None = None,
+    up_db_dtype: torch.dtype | None = None,
+):
+    """Gradients of int8_gated as (dx, dgate, dup, dgate_bias, dup_bias); None where no type is given.
+
+    grad: gradient of h [..., N]; codes, scale: per_token_int8 of the activations.  Both projections
+    are formed again from the codes, so a forward pass keeps one byte per activation and nothing
+    of width N.  Launches only, on the current stream."""
+    codes = _aligned_codes(codes, "int8 activation matrix")
+    m, k = codes.shape
+    n = gate.shape[0]
+    dev = codes.device
+    _check_gated(k, gate, up, activation)
+    nat.require_device(dev, ("gate weight", gate.codes), ("up weight", up.codes), ("scale", scale),
+                       ("gate bias", gate_bias), ("up bias", up_bias))
+    scale = _scales(scale, m, "scale")
+    dh = _grad_rows(grad, m, n, dev)
+    pitch = _round_up(max(n, 1), 128)
+    want_dw = dgate_dtype is not None or dup_dtype is not None
+    _check_backward(m, pitch + n if dx_dtype is not None else 0, want_dw)
+    # one tensor for the gradients of both projections, fp32: their digits are taken against row
+    # and column maxima that are known only once it is complete
+    d = torch.empty((m, 2 * pitch), dtype=torch.float32, device=dev)
+    biases, bias_dtype = _bias_args(n, gate_bias, up_bias)
+    with torch.cuda.device(dev):
+        nat.call("ima_int8_gated_backward_gemm", *_gated_args(codes, scale, gate, up, biases, bias_dtype, activation),
+                 dh.data_ptr(), nat.dtype_code(dh.dtype), _ld(dh), d.data_ptr(), 2 * pitch, pitch, nat.stream_of(dev))
+    dx = None
+    if dx_dtype is not None:
+        channel = torch.zeros((2, pitch), dtype=torch.float32, device=dev)
+        channel[0, :n] = gate.scale
+        channel[1, :n] = up.scale
+        digits, digit_scale = _digits_rows(d, n, pitch, 2, channel, _digit_count(dh.dtype, dx_dtype))
+        dx = _digit_gemm(digits, digit_scale, gate.transposed(), up.transposed(), m, n, dx_dtype)
+    codes_t = _transpose(codes) if want_dw else None
+    dg, dgb = _weight_gradient(d[:, :n], codes_t, scale, dh.dtype, dgate_dtype, gate_db_dtype)
+    du, dub = _weight_gradient(d[:, pitch:pitch + n], codes_t, scale, dh.dtype, dup_dtype, up_db_dtype)
+    return dx, dg, du, dgb, dub
+
+
+# ---------------------------------------------------------------------------
+# the operators
+# ---------------------------------------------------------------------------
+def _weight_of(weight) -> Int8Weight:
+    return weight if isinstance(weight, Int8Weight) else Int8Weight.from_float(weight)
+
+
+def _check_gated(k: int, gate, up, activation: str) -> None:
+    if activation not in ACTIVATIONS:
+        raise RuntimeError(f"unknown activation {activation!r}; choose one of: {', '.join(sorted(ACTIVATIONS))}")
+    if tuple(gate.shape) != tuple(up.shape):
+        raise RuntimeError(f"gate and up weights differ in shape: {tuple(gate.shape)} vs {tuple(up.shape)}")
+    if gate.shape[1] != k:
+        raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={gate.shape[1]}")
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, handle):
+        w = handle if handle is not None else Int8Weight.from_float(weight)
+        y, q, scale = _linear_forward(_rows(x.detach()), w, bias)
+        ctx.save_for_backward(q, scale)
+        ctx.weight = w
+        ctx.types = tuple(t.dtype if t is not None and need else None
+                          for t, need in zip((x, weight, bias), ctx.needs_input_grad))
+        ctx.shapes = (x.shape, None if bias is None else bias.shape)
+        return y.reshape(*x.shape[:-1], w.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, scale = ctx.saved_tensors
+        dx, dw, db = int8_linear_backward(grad, q, scale, ctx.weight, dx_dtype=ctx.types[0], dw_dtype=ctx.types[1],
+                                          db_dtype=ctx.types[2])
+        return (None if dx is None else dx.reshape(ctx.shapes[0]), dw, None if db is None else db.reshape(ctx.shapes[1]),
+                None)
+
+
+class _GatedFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, gate, up, activation):
+        g = gate if gate is not None else Int8Weight.from_float(gate_weight)
+        u = up if up is not None else Int8Weight.from_float(up_weight)
+        h, q, scale = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation)
+        ctx.save_for_backward(q, scale, gate_bias, up_bias)
+        ctx.gate, ctx.up, ctx.activation = g, u, activation
+        inputs = (x, gate_weight, up_weight, gate_bias, up_bias)
+        ctx.types = tuple(t.dtype if t is not None and need else None for t, need in zip(inputs, ctx.needs_input_grad))
+        ctx.shapes = tuple(None if t is None else t.shape for t in inputs)
+        return h.reshape(*x.shape[:-1], g.shape[0])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, scale, gate_bias, up_bias = ctx.saved_tensors
+        tx, tg, tu, tgb, tub = ctx.types
+        grads = int8_gated_backward(grad, q, scale, ctx.gate, ctx.up, gate_bias, up_bias, activation=ctx.activation,
+                                    dx_dtype=tx, dgate_dtype=tg, dup_dtype=tu, gate_db_dtype=tgb, up_db_dtype=tub)
+        return (*(None if g is None else g.reshape(shape) for g, shape in zip(grads, ctx.shapes)), None, None, None)
+
+
+def _check_linear_inputs(x: torch.Tensor, *named) -> None:
+    _require_cuda(x, "int8 input")
+    if x.ndim < 1:
+        raise RuntimeError("int8 input must have at least one dimension")
+    nat.dtype_code(x.dtype)
+    for label, t in named:
+        if isinstance(t, torch.Tensor):
+            nat.require_device(x.device, (label, t))
+            nat.dtype_code(t.dtype)
+        elif isinstance(t, Int8Weight):
+            nat.require_device(x.device, (label, t.codes))
+        elif t is not None:
+            raise RuntimeError(f"{label} must be a tensor or an Int8Weight, got {type(t).__name__}")
+
+
+def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """y = x W^T + b with int8 codes on both sides, in x's type: x [..., K], weight [N, K].
+
+    weight: an Int8Weight (frozen) or a floating tensor, quantised in the call and differentiable.
+    """
+    _check_linear_inputs(x, ("weight", weight), ("bias", bias))
+    if weight.shape[-1] != x.shape[-1]:
+        raise RuntimeError(f"int8 matmul shape mismatch: K={x.shape[-1]} vs K={weight.shape[-1]}")
+    if _wants_grad(x, weight, bias):
+        frozen = isinstance(weight, Int8Weight)
+        _check_backward(x.numel() // max(x.shape[-1], 1), weight.shape[0] if x.requires_grad else 0,
+                        not frozen and weight.requires_grad)
+        return _LinearFunction.apply(x, None if frozen else weight, bias, weight if frozen else None)
+    w = _weight_of(weight)
+    y, _q, _s = _linear_forward(_rows(x.detach()), w, bias)
+    return y.reshape(*x.shape[:-1], w.shape[0])
+
+
+def int8_gated(
+    x: torch.Tensor,
+    gate: Int8Weight | torch.Tensor,
+    up: Int8Weight | torch.Tensor,
+    gate_bias: torch.Tensor | None = None,
+    up_bias: torch.Tensor | None = None,
+    *,
+    activation: str = "silu",
+) -> torch.Tensor:
+    """h = act(x Wg^T + bg) * (x Wu^T + bu) in x's type: x [..., K], gate and up [N, K].
+
+    Both projections, the activation ("silu", "gelu" with the error function, or "gelu_tanh") and the
+    product run in one kernel; g and u never reach memory.  Weights as in int8_linear."""
+    _check_linear_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
+    _check_gated(x.shape[-1], gate, up, activation)
+    if _wants_grad(x, gate, up, gate_bias, up_bias):
+        frozen = [isinstance(w, Int8Weight) for w in (gate, up)]
+        _check_backward(x.numel() // max(x.shape[-1], 1),
+                        _round_up(gate.shape[0], 128) + gate.shape[0] if x.requires_grad else 0,
+                        any(not f and w.requires_grad for f, w in zip(frozen, (gate, up))))
+        return _GatedFunction.apply(x, None if frozen[0] else gate, None if frozen[1] else up, gate_bias, up_bias,
+                                    gate if frozen[0] else None, up if frozen[1] else None, activation)
+    g, u = _weight_of(gate), _weight_of(up)
+    h, _q, _s = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation)
+    return h.reshape(*x.shape[:-1], g.shape[0])

@@ -24,9 +24,12 @@ from .codebook import DigitPlanes, codebook_planes_from_fp8, int_gemm, per_token
 from .hawkeye import _validate_params as _validate_hawkeye_params
 from .hawkeye import hawkeye_replay, quantize_and_stage, stage_weight
 from .hawkeye_freivalds import exact_hawkeye_fp8_sum, stage_class_count_weight
+from .int8 import ACTIVATIONS as INT8_ACTIVATIONS
+from .int8 import Int8Weight, int8_gated, int8_linear
 
 STUDENT_KERNEL = os.environ.get("IMA_STUDENT_KERNEL", "codebook")
-SUPPORTED_STUDENT_KERNELS = {"codebook", "hawkeye", "hawkeye-class-counts"}
+# "int8" (no counterpart in the reference): every linear as an Int8Linear, gated blocks fused
+SUPPORTED_STUDENT_KERNELS = {"codebook", "hawkeye", "hawkeye-class-counts", "int8"}
 HAWKEYE_PRODUCTS_PER_GROUP = int(os.environ.get("IMA_HAWKEYE_GROUP", "32"))
 HAWKEYE_INTERNAL_WIDTH = int(os.environ.get("IMA_HAWKEYE_WIDTH", "14"))
 HAWKEYE_CLASS_CHUNK = int(os.environ.get("IMA_HAWKEYE_CLASS_CHUNK", "32"))
@@ -330,6 +333,93 @@ class HawkeyeClassCountsLinear(nn.Module):
         return y.to(x.dtype).reshape(*in_shape[:-1], self.out_features)
 
 
+class Int8Linear(nn.Module):
+    """Linear with int8 activations (one scale per token) and int8 weights (one per output channel):
+    one exact int32 product per forward.  No counterpart in the reference; weight is the
+    dequantised one, like Int32Linear's."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None):
+        super().__init__()
+        _require_cuda_tensor(weight, "int8 weight source")
+        with torch.inference_mode(False):   # versioned even inside inference mode (see _owned_copy)
+            handle = Int8Weight.from_float(weight.detach())
+        self._handle = handle
+        self.register_buffer("weight", handle.codes, persistent=False)
+        self.register_buffer("weight_scale", handle.scale, persistent=False)
+        if bias is None:
+            self.bias = None
+        else:
+            self.register_buffer("bias", bias.detach(), persistent=False)
+        self.in_features = weight.shape[1]
+        self.out_features = weight.shape[0]
+
+    def int8_weight(self) -> Int8Weight:
+        """The codes and scales as int8_linear takes them (laid out anew if a buffer was replaced,
+        e.g. by moving the module)."""
+        if self._handle.codes is not self.weight or self._handle.scale is not self.weight_scale:
+            self._handle = Int8Weight(self.weight, self.weight_scale)
+            self.weight, self.weight_scale = self._handle.codes, self._handle.scale
+        return self._handle
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _require_cuda_tensor(x, "int8 input")
+        _bump_probe(1)
+        return int8_linear(x, self.int8_weight(), self.bias)
+
+
+class Int8GatedMLP(nn.Module):
+    """Gated feed-forward block down(act(gate(x)) * up(x)) on three Int8Linear: gate, up, activation and
+    product in one kernel, then the down projection."""
+
+    def __init__(self, gate_proj: Int8Linear, up_proj: Int8Linear, down_proj: Int8Linear, activation: str):
+        super().__init__()
+        if activation not in INT8_ACTIVATIONS:
+            raise RuntimeError(f"unknown activation {activation!r}; choose one of: {', '.join(sorted(INT8_ACTIVATIONS))}")
+        self.gate_proj, self.up_proj, self.down_proj = gate_proj, up_proj, down_proj
+        self.activation = activation
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _require_cuda_tensor(x, "int8 input")
+        _bump_probe(2)
+        h = int8_gated(x, self.gate_proj.int8_weight(), self.up_proj.int8_weight(), self.gate_proj.bias,
+                       self.up_proj.bias, activation=self.activation)
+        return self.down_proj(h)
+
+
+def _bump_probe(products: int) -> None:
+    if _ACTIVE_INT32_PROBE is not None:
+        _ACTIVE_INT32_PROBE.count += products
+
+
+def _gated_activation(module: nn.Module) -> str | None:
+    """The activation of a module whose children are exactly gate_proj, up_proj, down_proj and act_fn,
+    down(act(gate(x)) * up(x)) in the layout of every gated block this package's shapes come from; None
+    for anything else."""
+    children = dict(module.named_children())
+    if set(children) != {"gate_proj", "up_proj", "down_proj", "act_fn"}:
+        return None
+    if next(module.parameters(recurse=False), None) is not None:
+        return None
+    act = children["act_fn"]
+    if isinstance(act, nn.SiLU):
+        return "silu"
+    if isinstance(act, nn.GELU):
+        return "gelu_tanh" if act.approximate == "tanh" else "gelu"
+    return None
+
+
+def _fuse_gated_blocks(model: nn.Module) -> None:
+    """Replace every gated block whose three projections are Int8Linear by an Int8GatedMLP."""
+    blocks = [(name, module) for name, module in model.named_modules() if name]
+    for name, module in blocks:
+        activation = _gated_activation(module)
+        if activation is None:
+            continue
+        parts = [module.gate_proj, module.up_proj, module.down_proj]
+        if all(isinstance(p, Int8Linear) for p in parts) and parts[0].weight.shape == parts[1].weight.shape:
+            _set_submodule(model, name, Int8GatedMLP(*parts, activation))
+
+
 # ---------------------------------------------------------------------------
 # model integerisation (ref __main__.py:526-594)
 # ---------------------------------------------------------------------------
@@ -364,7 +454,9 @@ def _replace_int32_linears(model: nn.Module) -> list[str]:
         if isinstance(module, nn.Linear):
             replacements.append((name, module))
     for name, module in replacements:
-        if module.weight.dtype == torch.float8_e4m3fn and hasattr(module, "weight_scale"):
+        if STUDENT_KERNEL == "int8":
+            replacement = Int8Linear(_dequantized_weight(module), module.bias)
+        elif module.weight.dtype == torch.float8_e4m3fn and hasattr(module, "weight_scale"):
             if STUDENT_KERNEL == "hawkeye":
                 replacement = HawkeyeLinear(module.weight, module.weight_scale, module.bias)
             elif STUDENT_KERNEL == "hawkeye-class-counts":
@@ -376,6 +468,8 @@ def _replace_int32_linears(model: nn.Module) -> list[str]:
         _set_submodule(model, name, replacement)
     if not replacements:
         raise RuntimeError("No Linear modules were found to integerize.")
+    if STUDENT_KERNEL == "int8":
+        _fuse_gated_blocks(model)
     return [name for name, _ in replacements]
 
 
