@@ -372,6 +372,18 @@ int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_
                         int64_t M, int64_t N, int64_t K, const float* x_scale, const float* gate_scale,
                         const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype,
                         int activation, void* y, int y_dtype, int64_t ldy, void* stream);
+/* The two operators on floating activations x [M,K] (row stride ldx): y [M,N] in x's type.  q [M,ldq]
+ * int8 and scale [M] are workspace; with keep_codes != 0 they hold the codes and scales of x
+ * afterwards (what a backward pass needs), otherwise a product of few tokens quantises them in
+ * its own launch and leaves both alone. */
+int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                    int keep_codes, const int8_t* w, int64_t ldw, int64_t N, const float* w_scale, const void* bias,
+                    int bias_dtype, void* y, int64_t ldy, void* stream);
+int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                   int keep_codes, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu, int64_t N,
+                   const float* gate_scale, const float* up_scale, const void* gate_bias, const void* up_bias,
+                   int bias_dtype, int activation, void* y, int64_t ldy, void* stream);
+
 /* Gradients of g and u from dh [M,N] (row stride ldh): g and u are formed again from the codes,
  * d[m, n] = dh u act'(g) and d[m, seg_pitch + n] = dh act(g), fp32 (row stride ldd). */
 int ima_int8_gated_backward_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up,

@@ -8,4 +8,4 @@
 #include "class_counts.cu"
 #include "class_count_engine.cu"
 #include "int8_quant.cu"
-#include "int8_gemm.cu"
+#include "int8_api.cu"

@@ -23,6 +23,7 @@
 //
 // Every wait is bounded: one that runs out records IMA_ERR_TIMEOUT, and every role drains and
 // returns.
+#pragma once
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include "sm100_primitives.cuh"
@@ -37,10 +38,10 @@ constexpr int64_t I8_MAX_K = 131071;
 
 enum I8Epi { I8_LINEAR = 0, I8_GATED = 1, I8_GATED_BWD = 2, I8_DIGIT = 3 };
 
-template <int P, int BN>
+template <int P, int BN, int CG>
 struct I8Cfg {
     static constexpr int A_PLANE = I8_BM * I8_KT;
-    static constexpr int B_BYTES = BN * I8_KT;
+    static constexpr int B_BYTES = BN / CG * I8_KT;          // a CTA pair holds half of B each
     static constexpr int STAGE_BYTES = P * A_PLANE + B_BYTES;
     static constexpr int STAGES = 200 * 1024 / STAGE_BYTES < 6 ? 200 * 1024 / STAGE_BYTES : 6;
     static constexpr int ACC = P * BN;                       // tensor-memory columns of one tile
@@ -176,9 +177,9 @@ IMA_DEVINL void store_y32(const I8Params& p, unsigned char* st, int lane, const 
     }
 }
 
-template <int P, int BN, int EPI>
+template <int P, int BN, int EPI, int CG>
 __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_constant__ I8Params p) {
-    using L = I8Cfg<P, BN>;
+    using L = I8Cfg<P, BN, CG>;
     constexpr bool PAIR = EPI == I8_GATED || EPI == I8_GATED_BWD;   // B tile = BN / 2 rows of G, then of U
     constexpr int TN = PAIR ? BN / 2 : BN;                          // output columns of a tile
     constexpr int HALF = TN / 2;                                    // output columns of an epilogue warp
@@ -194,6 +195,8 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t num_tiles = (int64_t)p.m_tiles * p.n_tiles;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;   // CTA of the pair; 0 issues its MMAs
+    const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::STAGES; ++s) {
@@ -202,17 +205,23 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         }
         for (int b = 0; b < L::BUFS; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], I8_EPI_WARPS);
+            mbar_init(&acc_empty[b], I8_EPI_WARPS * CG);
         }
         mbar_init(drained, 1);
         *abort_flag = 0;
         mbar_fence_init();
     }
     if (warp == 1) {
-        tmem_alloc(tmem_slot, 512);
-        tmem_relinquish();
+        if (CG == 2) {
+            tmem_alloc_pair(tmem_slot, 512);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, 512);
+            tmem_relinquish();
+        }
     }
     __syncthreads();
+    if (CG == 2) cluster_sync_all();   // both CTAs' barriers exist before either signals the other's
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -220,7 +229,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         // ---------------- TMA producer ----------------
         uint32_t stage = 0, phase = 0;
         uint64_t issued = 0;
-        for (int64_t t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+        for (int64_t t = first; t < num_tiles && !*abort_flag; t += step) {
             int32_t mt, nt;
             i8_tile(p, t, mt, nt);
             for (int kt = 0; kt < p.k_tiles; ++kt) {
@@ -229,32 +238,49 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                     break;
                 ++issued;
                 unsigned char* sb = smem + stage * L::STAGE_BYTES;
-                mbar_arrive_expect_tx(&full[stage], (uint32_t)L::STAGE_BYTES);
-#pragma unroll
-                for (int i = 0; i < P; ++i)
-                    tma_load_3d(sb + i * L::A_PLANE, &p.ma, &full[stage], kt * I8_KT, mt * I8_BM, i);
                 unsigned char* bb = sb + P * L::A_PLANE;
-                if (EPI == I8_DIGIT && kt >= p.seg_tiles)
-                    tma_load_2d(bb, &p.mb2, &full[stage], (kt - p.seg_tiles) * I8_KT, nt * TN);
-                else
-                    tma_load_2d(bb, &p.mb, &full[stage], kt * I8_KT, nt * TN);
-                if (PAIR) tma_load_2d(bb + TN * I8_KT, &p.mb2, &full[stage], kt * I8_KT, nt * TN);
+                const bool second = EPI == I8_DIGIT && kt >= p.seg_tiles;
+                const int32_t bx = (second ? kt - p.seg_tiles : kt) * I8_KT;
+                if constexpr (CG == 1) {
+                    mbar_arrive_expect_tx(&full[stage], (uint32_t)L::STAGE_BYTES);
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        tma_load_3d(sb + i * L::A_PLANE, &p.ma, &full[stage], kt * I8_KT, mt * I8_BM, i);
+                    tma_load_2d(bb, second ? &p.mb2 : &p.mb, &full[stage], bx, nt * TN);
+                    if (PAIR) tma_load_2d(bb + TN * I8_KT, &p.mb2, &full[stage], bx, nt * TN);
+                } else {
+                    // both CTAs' loads count on the barrier of CTA 0, whose MMA thread waits for them; the
+                    // stage is free in both (a commit of that thread), so its barrier is in this round's phase
+                    const uint32_t bar = cluster_map(&full[stage], 0);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)L::STAGE_BYTES);
+#pragma unroll
+                    for (int i = 0; i < P; ++i)
+                        tma_load_3d_pair(sb + i * L::A_PLANE, &p.ma, bar, kt * I8_KT, (mt * 2 + (int)rank) * I8_BM, i);
+                    if (PAIR)
+                        tma_load_2d_pair(bb, rank ? &p.mb2 : &p.mb, bar, bx, nt * TN);
+                    else
+                        tma_load_2d_pair(bb, second ? &p.mb2 : &p.mb, bar, bx, nt * TN + (int)rank * (BN / 2));
+                }
                 if (++stage == (uint32_t)L::STAGES) { stage = 0; phase ^= 1u; }
             }
         }
-        // Every load issued lands before the CTA exits, also after an abort.
+        // Every load issued lands before the CTA exits, also after an abort; in a pair, the commits
+        // that free this CTA's stages have arrived as well.
         for (int s = 0; s < L::STAGES; ++s) {
             const uint64_t rounds = issued / L::STAGES + ((uint64_t)s < issued % L::STAGES ? 1u : 0u);
-            if (rounds > 0)
+            if (rounds > 0 && rank == 0)
                 mbar_wait_bounded(&full[s], (uint32_t)((rounds - 1) & 1u), IMA_WHERE_INT8_GEMM, 100 + s);
+            if (CG == 2 && rounds > 0 && !*abort_flag)
+                mbar_wait_or_abort(&empty[s], (uint32_t)((rounds - 1) & 1u), abort_flag, IMA_WAIT_LIMIT_NS,
+                                   IMA_WHERE_INT8_GEMM, 150 + s);
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
         // ---------------- MMA issuer ----------------
-        constexpr uint32_t idesc = idesc_i8(I8_BM, BN);
+        constexpr uint32_t idesc = idesc_i8(I8_BM * CG, BN);
         uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
         if (p.stall_ns)   // test knob: a wait that nothing ends runs out
             mbar_wait_or_abort(drained, 0u, abort_flag, p.stall_ns, IMA_WHERE_INT8_GEMM, -2);
-        for (int64_t t = blockIdx.x; t < num_tiles && !*abort_flag; t += gridDim.x) {
+        for (int64_t t = first; t < num_tiles && !*abort_flag; t += step) {
             if (!mbar_wait_or_abort(&acc_empty[buf], bphase ^ 1u, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM, -1))
                 break;
             tc_fence_after();
@@ -272,18 +298,24 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
 #pragma unroll
                 for (int ks = 0; ks < I8_KT / 32; ++ks)
 #pragma unroll
-                    for (int i = 0; i < P; ++i)
-                        mma_i8(acc + i * BN, umma_desc_sw128_kmajor(sa + i * L::A_PLANE + ks * 32),
-                               umma_desc_sw128_kmajor(sb + ks * 32), idesc, (kt | ks) ? 1u : 0u);
-                mma_commit(&empty[stage]);
+                    for (int i = 0; i < P; ++i) {
+                        const uint64_t da = umma_desc_sw128_kmajor(sa + i * L::A_PLANE + ks * 32);
+                        const uint64_t db = umma_desc_sw128_kmajor(sb + ks * 32);
+                        if (CG == 2) mma_i8_pair(acc + i * BN, da, db, idesc, (kt | ks) ? 1u : 0u);
+                        else mma_i8(acc + i * BN, da, db, idesc, (kt | ks) ? 1u : 0u);
+                    }
+                if (CG == 2) mma_commit_pair(&empty[stage]);
+                else mma_commit(&empty[stage]);
                 if (++stage == (uint32_t)L::STAGES) { stage = 0; phase ^= 1u; }
             }
             if (!fed) break;
-            mma_commit(&acc_full[buf]);
+            if (CG == 2) mma_commit_pair(&acc_full[buf]);
+            else mma_commit(&acc_full[buf]);
             if (++buf == (uint32_t)L::BUFS) { buf = 0; bphase ^= 1u; }
         }
         // Every MMA issued completes before the CTA frees tensor memory.
-        mma_commit(drained);
+        if (CG == 2) mma_commit_pair_local(drained);
+        else mma_commit(drained);
         mbar_wait_bounded(drained, 0u, IMA_WHERE_INT8_GEMM, -3);
     } else if (warp >= 2) {
         // ---------------- epilogue ----------------
@@ -291,10 +323,10 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         unsigned char* st = smem + L::STG_OFFSET + ew * 2048;
         float* cols = reinterpret_cast<float*>(smem + L::COL_OFFSET) + ew * 256;
         uint32_t buf = 0, bphase = 0;
-        for (int64_t t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+        for (int64_t t = first; t < num_tiles; t += step) {
             int32_t mt, nt;
             i8_tile(p, t, mt, nt);
-            const int64_t row0 = (int64_t)mt * I8_BM + q * 32;
+            const int64_t row0 = ((int64_t)mt * CG + rank) * I8_BM + q * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, (int64_t)p.M - row0));
             const int32_t n0 = nt * TN + h * HALF;
             // this warp's column scales and biases: [2 operands][scale, bias][HALF]
@@ -444,15 +476,20 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (lane == 0) {
+                if (CG == 2) mbar_arrive_cluster(cluster_map(&acc_empty[buf], 0));
+                else mbar_arrive(&acc_empty[buf]);
+            }
             if (++buf == (uint32_t)L::BUFS) { buf = 0; bphase ^= 1u; }
         }
     }
     __syncthreads();
+    if (CG == 2) cluster_sync_all();   // no CTA leaves while the other may still signal or use its memory
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem_base, 512);
+        if (CG == 2) tmem_dealloc_pair(tmem_base, 512);
+        else tmem_dealloc(tmem_base, 512);
     }
 }
 
@@ -485,134 +522,63 @@ int check_i8_operand(const int8_t* p, int64_t rows, int64_t K, int64_t ld) {
 
 bool aligned16(const void* p, int64_t pitch_bytes) { return !((reinterpret_cast<uintptr_t>(p) | (uintptr_t)pitch_bytes) & 15); }
 
-template <int P, int BN, int EPI>
-int launch_i8(I8Params& p, cudaStream_t stream) {
-    using L = I8Cfg<P, BN>;
+// Rows of B in a load box: a CTA's share of a tile, of each operand in the gated forms.
+template <int BN, int EPI, int CG>
+constexpr int i8_box_rows() { return EPI == I8_GATED || EPI == I8_GATED_BWD ? BN / 2 : BN / CG; }
+
+struct I8Operands {
+    const int8_t *a, *b, *b2;
+    int64_t lda, ldb, ldb2, Ka, K;   // A has Ka columns per plane, B and b2 K
+};
+
+template <int P, int BN, int EPI, int CG>
+int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
+    using L = I8Cfg<P, BN, CG>;
     constexpr int TN = EPI == I8_GATED || EPI == I8_GATED_BWD ? BN / 2 : BN;
-    p.m_tiles = (p.M + I8_BM - 1) / I8_BM;
+    constexpr int BOX = i8_box_rows<BN, EPI, CG>();
+    p.m_tiles = (p.M + CG * I8_BM - 1) / (CG * I8_BM);
     p.n_tiles = (p.N + TN - 1) / TN;
-    p.group_m = 16;
+    p.k_tiles = (int32_t)((o.Ka + I8_KT - 1) / I8_KT);
+    p.group_m = 16 / CG;
     p.stall_ns = g_gemm_stall_ns;
-    auto kern = int8_gemm_kernel<P, BN, EPI>;
-    int rc = ima_note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+    int rc = IMA_OK;
+    if (o.K > 0) {   // K == 0 loads nothing
+        rc = make_i8_map(&p.ma, o.a, o.Ka, o.lda, p.M, P, I8_BM, true);
+        if (rc == IMA_OK) rc = make_i8_map(&p.mb, o.b, o.K, o.ldb, p.N, 1, BOX, false);
+        if (rc == IMA_OK && o.b2) rc = make_i8_map(&p.mb2, o.b2, o.K, o.ldb2, p.N, 1, BOX, false);
+        if (rc != IMA_OK) return rc;
+    }
+    auto kern = int8_gemm_kernel<P, BN, EPI, CG>;
+    rc = ima_note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
     if (rc != IMA_OK) return rc;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-    const int grid = (int)std::min<int64_t>(tiles, gemm_grid_limit());
-    kern<<<grid, I8_THREADS, L::ALLOC, stream>>>(p);
-    return IMA_LAUNCH_STATUS();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, gemm_grid_limit() / CG) * CG));
+    cfg.blockDim = dim3(I8_THREADS);
+    cfg.dynamicSmemBytes = L::ALLOC;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CG;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = CG == 2 ? 1 : 0;
+    return ima_note_cuda(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-// The maps of a product: A planes (Ka columns) in 128-row boxes, B (or G and U; K columns) in boxes of
-// a tile's rows.
-int make_i8_maps(I8Params& p, const int8_t* a, int64_t lda, int planes, const int8_t* b, int64_t ldb, const int8_t* b2,
-                 int64_t ldb2, int64_t Ka, int64_t K, int b_rows) {
-    p.k_tiles = (int32_t)((Ka + I8_KT - 1) / I8_KT);
-    if (K == 0) return IMA_OK;   // nothing is loaded
-    int rc = make_i8_map(&p.ma, a, Ka, lda, p.M, planes, I8_BM, true);
-    if (rc == IMA_OK) rc = make_i8_map(&p.mb, b, K, ldb, p.N, 1, b_rows, false);
-    if (rc == IMA_OK && b2) rc = make_i8_map(&p.mb2, b2, K, ldb2, p.N, 1, b_rows, false);
-    return rc;
+// A CTA pair computes 256 rows by BN columns with half of B in each CTA, so a stage moves 2/3 of
+// the bytes of two single CTAs (P == 1), which is what the L2 -> SM path limits; one CTA halves the
+// tile.  The pair is taken when it needs no more than 4/3 of the single form's time in whole rounds of
+// tiles over the machine.
+template <int P, int BN, int EPI>
+int launch_i8(I8Params& p, const I8Operands& o, cudaStream_t stream) {
+    constexpr int TN = EPI == I8_GATED || EPI == I8_GATED_BWD ? BN / 2 : BN;
+    const int64_t sms = gemm_grid_limit(), nt = (p.N + TN - 1) / TN;
+    const int64_t one = ((p.M + I8_BM - 1) / I8_BM * nt + sms - 1) / sms;
+    const int64_t two = sms < 2 ? INT32_MAX : ((p.M + 2 * I8_BM - 1) / (2 * I8_BM) * nt + sms / 2 - 1) / (sms / 2);
+    if (two * 3 <= one * 4) return launch_i8_tile<P, BN, EPI, 2>(p, o, stream);
+    return launch_i8_tile<P, BN, EPI, 1>(p, o, stream);
 }
 
 }  // namespace
-
-extern "C" {
-
-int ima_int8_gemm(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
-                  int32_t* c, int64_t ldc, const float* x_scale, const float* w_scale, const void* bias, int bias_dtype,
-                  void* y, int y_dtype, int64_t ldy, void* stream) {
-    int rc = check_i8_operand(a, M, K, lda);
-    if (rc == IMA_OK) rc = check_i8_operand(b, N, K, ldb);
-    if (rc != IMA_OK) return rc;
-    if (M == 0 || N == 0) return IMA_OK;
-    if (!c && !y) return IMA_ERR_INVALID_ARGUMENT;
-    if (c && ldc < N && M > 1) return IMA_ERR_INVALID_ARGUMENT;
-    if (y && (!x_scale || !w_scale || (ldy < N && M > 1) || !known_dtype(y_dtype))) return IMA_ERR_INVALID_ARGUMENT;
-    if (y && bias && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    I8Params p;
-    memset(&p, 0, sizeof(p));
-    p.c = c; p.y = y; p.xs = x_scale; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
-    p.ldc = ldc; p.ldy = ldy; p.y_dtype = y_dtype;
-    p.M = (int32_t)M; p.N = (int32_t)N;
-    p.vec_c = c && aligned16(c, ldc * 4);
-    p.vec_y = y && aligned16(y, ldy * dtype_bytes(y_dtype));
-    rc = make_i8_maps(p, a, lda, 1, b, ldb, nullptr, 0, K, K, 256);
-    if (rc != IMA_OK) return rc;
-    return launch_i8<1, 256, I8_LINEAR>(p, (cudaStream_t)stream);
-}
-
-int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
-                        int64_t M, int64_t N, int64_t K, const float* x_scale, const float* gate_scale,
-                        const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype,
-                        int activation, void* y, int y_dtype, int64_t ldy, void* stream) {
-    int rc = check_i8_operand(a, M, K, lda);
-    if (rc == IMA_OK) rc = check_i8_operand(gate, N, K, ldg);
-    if (rc == IMA_OK) rc = check_i8_operand(up, N, K, ldu);
-    if (rc != IMA_OK) return rc;
-    if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
-    if (M == 0 || N == 0) return IMA_OK;
-    if (!y || !x_scale || !gate_scale || !up_scale || (ldy < N && M > 1) || !known_dtype(y_dtype))
-        return IMA_ERR_INVALID_ARGUMENT;
-    if ((gate_bias || up_bias) && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    I8Params p;
-    memset(&p, 0, sizeof(p));
-    p.y = y; p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
-    p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = activation;
-    p.M = (int32_t)M; p.N = (int32_t)N;
-    p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
-    rc = make_i8_maps(p, a, lda, 1, gate, ldg, up, ldu, K, K, 128);
-    if (rc != IMA_OK) return rc;
-    return launch_i8<1, 256, I8_GATED>(p, (cudaStream_t)stream);
-}
-
-int ima_int8_gated_backward_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up,
-                                 int64_t ldu, int64_t M, int64_t N, int64_t K, const float* x_scale,
-                                 const float* gate_scale, const float* up_scale, const void* gate_bias,
-                                 const void* up_bias, int bias_dtype, int activation, const void* dh, int dh_dtype,
-                                 int64_t ldh, float* d, int64_t ldd, int64_t seg_pitch, void* stream) {
-    int rc = check_i8_operand(a, M, K, lda);
-    if (rc == IMA_OK) rc = check_i8_operand(gate, N, K, ldg);
-    if (rc == IMA_OK) rc = check_i8_operand(up, N, K, ldu);
-    if (rc != IMA_OK) return rc;
-    if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
-    if (M == 0 || N == 0) return IMA_OK;
-    if (!dh || !d || !x_scale || !gate_scale || !up_scale || !known_dtype(dh_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    if ((ldh < N && M > 1) || seg_pitch < N || (ldd < seg_pitch + N && M > 1)) return IMA_ERR_INVALID_ARGUMENT;
-    if ((gate_bias || up_bias) && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    I8Params p;
-    memset(&p, 0, sizeof(p));
-    p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
-    p.bias_dtype = bias_dtype; p.act = activation; p.dh = dh; p.dh_dtype = dh_dtype; p.ldh = ldh;
-    p.d = d; p.ldd = ldd; p.seg_pitch = seg_pitch;
-    p.M = (int32_t)M; p.N = (int32_t)N;
-    p.vec_d = aligned16(d, ldd * 4) && seg_pitch % 4 == 0;
-    rc = make_i8_maps(p, a, lda, 1, gate, ldg, up, ldu, K, K, 128);
-    if (rc != IMA_OK) return rc;
-    return launch_i8<1, 256, I8_GATED_BWD>(p, (cudaStream_t)stream);
-}
-
-int ima_int8_digit_gemm(const int8_t* a_planes, int planes, int64_t lda, const float* row_scale, const int8_t* b,
-                        int64_t ldb, const int8_t* b2, int64_t ldb2, int64_t M, int64_t N, int64_t K, void* y,
-                        int y_dtype, int64_t ldy, void* stream) {
-    if (planes != 2 && planes != 3) return IMA_ERR_UNSUPPORTED;
-    // with a second B the planes hold two segments of K columns, the second on a k-tile boundary
-    const int64_t seg = b2 ? (K + I8_KT - 1) / I8_KT * I8_KT : 0;
-    int rc = check_i8_operand(a_planes, M, seg + K, lda);
-    if (rc == IMA_OK) rc = check_i8_operand(b, N, K, ldb);
-    if (rc == IMA_OK && b2) rc = check_i8_operand(b2, N, K, ldb2);
-    if (rc != IMA_OK) return rc;
-    if (M == 0 || N == 0) return IMA_OK;
-    if (!y || !row_scale || (ldy < N && M > 1) || !known_dtype(y_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    I8Params p;
-    memset(&p, 0, sizeof(p));
-    p.y = y; p.xs = row_scale; p.ldy = ldy; p.y_dtype = y_dtype;
-    p.M = (int32_t)M; p.N = (int32_t)N;
-    p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
-    rc = make_i8_maps(p, a_planes, lda, planes, b, ldb, b2, ldb2, seg + K, K, planes == 2 ? 256 : 128);
-    if (rc != IMA_OK) return rc;
-    p.seg_tiles = (int32_t)((K + I8_KT - 1) / I8_KT);
-    if (planes == 2) return launch_i8<2, 256, I8_DIGIT>(p, (cudaStream_t)stream);
-    return launch_i8<3, 128, I8_DIGIT>(p, (cudaStream_t)stream);
-}
-
-}  // extern "C"

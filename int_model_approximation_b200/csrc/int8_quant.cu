@@ -20,14 +20,27 @@
 
 namespace {
 
-// x -> rint(RN32(x / s)) without a division per element: t = x * RN(1/s) is off by at most
-// 2^-22 |t| < 4e-5 from the quotient (|t| < 128), so only a t that close to a half-integer
-// needs the division itself.  NaN gives 0.
-IMA_DEVINL int32_t i8_code(float x, float s, float inv) {
-    const float t = __fmul_rn(x, inv);
-    const float k = rintf(t);
-    if (fabsf(fabsf(t - k) - 0.5f) < 1e-4f) return __float2int_rn(__fdiv_rn(x, s));
-    return __float2int_rn(k);
+// Codes of eight elements, rint(RN32(x / s)) each, without a division per element.  With inv =
+// RN(1/s), fma(x, inv, 1.5 * 2^23) holds rint(x * inv) in its low mantissa bits; x * inv is off by at
+// most 2^-23 |x / s| < 2e-5 from the quotient, so only where it is that close to a half-integer
+// (0.02 % of all elements) the division itself decides.  A scale that is NaN or inf gives codes 0.
+IMA_DEVINL uint2 i8_codes8(const float (&v)[8], float s, float inv) {
+    constexpr float kRound = 12582912.0f;
+    uint32_t b[8];
+    float worst = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float t = __fmaf_rn(v[j], inv, kRound);
+        b[j] = __float_as_uint(t);
+        worst = fmaxf(worst, fabsf(__fmaf_rn(v[j], inv, kRound - t)));
+    }
+    if (worst > 0.4999f) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = (uint32_t)__float2int_rn(__fdiv_rn(v[j], s));
+    }
+    if (!(s <= 3.402823466e38f)) return make_uint2(0, 0);
+    return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
 }
 
 IMA_DEVINL float i8_row_scale(float amax, bool nan) {
@@ -41,25 +54,51 @@ IMA_DEVINL uint32_t pack4(const int32_t* v) {
                        __byte_perm((uint32_t)v[2], (uint32_t)v[3], 0x0040), 0x5410);
 }
 
-// Eight consecutive elements as loaded (16 bytes of a 16-bit type, 32 of fp32).
+// Eight consecutive elements as loaded (16 bytes of a 16-bit type, 32 of fp32).  max_bits() is the fp32
+// bit pattern of the largest magnitude: magnitudes order like their bit patterns, NaN above all.
 template <int DT>
 struct Raw8;
 template <>
 struct Raw8<IMA_DTYPE_F32> {
     float v[8];
+    IMA_DEVINL void clear() {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    }
+    IMA_DEVINL void load_whole(const void* row, int64_t k0) {
+        const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k0);
+        const float4 a = __ldg(p), b = __ldg(p + 1);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
     IMA_DEVINL void load(const void* row, int64_t k0, int64_t K, bool vec) { load8(row, IMA_DTYPE_F32, k0, K, vec, v); }
     IMA_DEVINL void unpack(float (&o)[8]) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = v[j];
     }
+    IMA_DEVINL uint32_t max_bits() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+        return m;
+    }
 };
 template <bool BF16>
 struct RawHalf8 {
     uint4 u;
+    IMA_DEVINL void clear() { u = make_uint4(0, 0, 0, 0); }
+    IMA_DEVINL void load_whole(const void* row, int64_t k0) {
+        u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k0));
+    }
     IMA_DEVINL void load(const void* row, int64_t k0, int64_t K, bool vec) {
         u = qz_load_half8(reinterpret_cast<const uint16_t*>(row), k0, K, vec);
     }
     IMA_DEVINL void unpack(float (&o)[8]) const { qz_unpack_half8(u, BF16, o); }
+    IMA_DEVINL uint32_t max_bits() const {
+        uint32_t m = __vmaxu2(__vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu),
+                              __vmaxu2(u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu));
+        m = max(m & 0xFFFFu, m >> 16);
+        return BF16 ? m << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    }
 };
 template <>
 struct Raw8<IMA_DTYPE_BF16> : RawHalf8<true> {};
@@ -68,28 +107,18 @@ struct Raw8<IMA_DTYPE_F16> : RawHalf8<false> {};
 
 __host__ __device__ __forceinline__ int dtype_bytes(int dtype) { return dtype == IMA_DTYPE_F32 ? 4 : 2; }
 
-// Maximum of |v| and "saw a NaN" over the TPR threads of a row (TPR == 32, or the block).
+// Maximum over the TPR threads of a row (TPR == 32, or the block).
 template <int TPR>
-IMA_DEVINL void row_max(float& amax, int& nan, float* s_max, int* s_nan) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-        nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, o);
-    }
+IMA_DEVINL uint32_t row_max(uint32_t m, uint32_t* s_max) {
+    m = __reduce_max_sync(0xFFFFFFFFu, m);
     if (TPR > 32) {
-        const int w = threadIdx.x >> 5;
-        if ((threadIdx.x & 31) == 0) {
-            s_max[w] = amax;
-            s_nan[w] = nan;
-        }
+        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < TPR / 32; ++i) {
-            amax = fmaxf(amax, s_max[i]);
-            nan |= s_nan[i];
-        }
+        for (int i = 0; i < TPR / 32; ++i) m = max(m, s_max[i]);
         __syncthreads();
     }
+    return m;
 }
 
 // ---------------------------------------------------------------------------
@@ -98,57 +127,46 @@ IMA_DEVINL void row_max(float& amax, int& nan, float* s_max, int* s_nan) {
 // L2).  Bound by memory: 2 or 4 bytes in and 1 out per element.
 // ---------------------------------------------------------------------------
 template <int DT, int TPR, int V>
-__global__ void __launch_bounds__(256) int8_quantize_rows_kernel(const void* x, int64_t M, int64_t K, int64_t ldx,
-                                                                 int8_t* q, int64_t ldq, float* scale) {
-    __shared__ float s_max[8];
-    __shared__ int s_nan[8];
+__global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* x, int64_t M, int64_t K, int64_t ldx,
+                                                                    int8_t* q, int64_t ldq, float* scale) {
+    __shared__ uint32_t s_max[8];
     constexpr int ROWS = 256 / TPR;
     const int tid = threadIdx.x % TPR;
     for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; m < M; m += (int64_t)gridDim.x * ROWS) {
         const unsigned char* row = reinterpret_cast<const unsigned char*>(x) + m * ldx * dtype_bytes(DT);
         const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+        // whole aligned groups of eight that this thread keeps; the rest is loaded twice
+        const int64_t whole = vec ? min(K / 8 * 8, (int64_t)V * TPR * 8) : 0;
         Raw8<DT> keep[V];
-        float amax = 0.0f, v[8];
-        int nan = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i) keep[i].load(row, ((int64_t)i * TPR + tid) * 8, K, vec);
+        uint32_t mx = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            keep[i].unpack(v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                nan |= v[j] != v[j];
-                amax = fmaxf(amax, fabsf(v[j]));
-            }
+            keep[i].clear();
+            if ((i * TPR + tid) * 8 < whole) keep[i].load_whole(row, (int64_t)(i * TPR + tid) * 8);
         }
-        for (int64_t k0 = ((int64_t)V * TPR + tid) * 8; k0 < K; k0 += TPR * 8) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) mx = max(mx, keep[i].max_bits());
+#pragma unroll 1
+        for (int64_t k0 = whole + tid * 8; k0 < K; k0 += TPR * 8) {
             Raw8<DT> r;
             r.load(row, k0, K, vec);
-            r.unpack(v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                nan |= v[j] != v[j];
-                amax = fmaxf(amax, fabsf(v[j]));
-            }
+            mx = max(mx, r.max_bits());
         }
-        row_max<TPR>(amax, nan, s_max, s_nan);
-        const float s = i8_row_scale(amax, nan != 0);
+        const float amax = __uint_as_float(row_max<TPR>(mx, s_max));
+        const float s = i8_row_scale(amax, amax != amax);
         const float inv = __frcp_rn(s);
         if (tid == 0) scale[m] = s;
         int8_t* qr = q + m * ldq;
         auto emit = [&](const Raw8<DT>& r, int64_t k0) {
+            float v[8];
             r.unpack(v);
-            int32_t c[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) c[j] = i8_code(v[j], s, inv);
-            *reinterpret_cast<uint2*>(qr + k0) = make_uint2(pack4(c), pack4(c + 4));
+            *reinterpret_cast<uint2*>(qr + k0) = i8_codes8(v, s, inv);
         };
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int64_t k0 = ((int64_t)i * TPR + tid) * 8;
-            if (k0 < K) emit(keep[i], k0);
-        }
-        for (int64_t k0 = ((int64_t)V * TPR + tid) * 8; k0 < K; k0 += TPR * 8) {
+        for (int i = 0; i < V; ++i)
+            if ((i * TPR + tid) * 8 < whole) emit(keep[i], (int64_t)(i * TPR + tid) * 8);
+#pragma unroll 1
+        for (int64_t k0 = whole + tid * 8; k0 < K; k0 += TPR * 8) {
             Raw8<DT> r;
             r.load(row, k0, K, vec);
             emit(r, k0);
@@ -197,13 +215,12 @@ struct DigitRows {
 
 template <int DT, int P>
 __global__ void __launch_bounds__(256) int8_digit_rows_kernel(const DigitRows a) {
-    __shared__ float s_max[8];
-    __shared__ int s_nan[8];
+    __shared__ uint32_t s_max[8];
     const int tid = threadIdx.x;
     for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
         const unsigned char* row = reinterpret_cast<const unsigned char*>(a.src) + m * a.ld * dtype_bytes(DT);
-        float amax = 0.0f, v[8];
-        int nan = 0;
+        float v[8];
+        uint32_t mx = 0;
         auto scaled = [&](int sg, int64_t j0, float (&o)[8]) {
             const unsigned char* base = row + sg * a.seg_pitch * dtype_bytes(DT);
             Raw8<DT> r;
@@ -220,13 +237,10 @@ __global__ void __launch_bounds__(256) int8_digit_rows_kernel(const DigitRows a)
             for (int64_t j0 = (int64_t)tid * 8; j0 < a.seg_len; j0 += 2048) {
                 scaled(sg, j0, v);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    nan |= v[j] != v[j];
-                    amax = fmaxf(amax, fabsf(v[j]));
-                }
+                for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7FFFFFFFu);
             }
-        row_max<256>(amax, nan, s_max, s_nan);
-        const float s = digit_scale<P>(amax, nan != 0);
+        const float amax = __uint_as_float(row_max<256>(mx, s_max));
+        const float s = digit_scale<P>(amax, amax != amax);
         const float inv = __frcp_rn(s);
         if (tid == 0) a.row_scale[m] = s;
         for (int sg = 0; sg < a.segs; ++sg) {
@@ -412,15 +426,16 @@ bool known_dtype(int d) { return d == IMA_DTYPE_F32 || d == IMA_DTYPE_BF16 || d 
 template <int DT>
 int launch_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                     cudaStream_t st) {
-    if (K <= 1024) {   // one warp per row
-        const int64_t grid = std::min<int64_t>((M + 7) / 8, 148 * 32);
-        int8_quantize_rows_kernel<DT, 32, 4><<<(unsigned)grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+    // A warp per row where the row fits its registers (16 KB of rows in flight per warp group without a
+    // block-wide barrier: 8 B per element of fp32 at 2048, 16-bit at 4096), else a block per row.
+    constexpr int W = DT == IMA_DTYPE_F32 ? 8 : 16;
+    if (K <= 32 * 8 * W) {
+        const unsigned grid = (unsigned)std::min<int64_t>((M + 7) / 8, 148 * 32);
+        if (K <= 1024) int8_quantize_rows_kernel<DT, 32, 4><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+        else int8_quantize_rows_kernel<DT, 32, W><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
     } else {
-        const int64_t grid = std::min<int64_t>(M, 148 * 32);
-        if (K <= 4096)
-            int8_quantize_rows_kernel<DT, 256, 2><<<(unsigned)grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
-        else
-            int8_quantize_rows_kernel<DT, 256, 10><<<(unsigned)grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+        const unsigned grid = (unsigned)std::min<int64_t>(M, 148 * 32);
+        int8_quantize_rows_kernel<DT, 256, 10><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
     }
     return IMA_LAUNCH_STATUS();
 }

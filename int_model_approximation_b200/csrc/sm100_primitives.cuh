@@ -234,6 +234,11 @@ IMA_DEVINL void mma_commit_pair(uint64_t* bar) {
         ::"r"(smem_u32(bar)), "h"((uint16_t)3)
         : "memory");
 }
+// Arrive on this CTA's mbarrier once the pair's MMAs issued by this thread complete.
+IMA_DEVINL void mma_commit_pair_local(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
 // 32 lanes x 32 bits, 32 consecutive columns per thread.
 IMA_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile(

@@ -40,6 +40,20 @@ MAX_K = 131071
 ACTIVATIONS = {"silu": nat.IMA_ACT_SILU, "gelu": nat.IMA_ACT_GELU, "gelu_tanh": nat.IMA_ACT_GELU_TANH}
 
 
+_DTYPE_CODES = {torch.float32: nat.IMA_DTYPE_F32, torch.bfloat16: nat.IMA_DTYPE_BF16, torch.float16: nat.IMA_DTYPE_F16}
+
+
+def _call(dev: torch.device, fn: str, *args) -> None:
+    """A C entry whose last argument is the stream, on `dev` and its current stream."""
+    if torch.cuda.current_device() == dev.index:
+        status = getattr(nat.lib(), fn)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            status = getattr(nat.lib(), fn)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if status:
+        raise nat.NativeError(fn, status)
+
+
 def _round_up(v: int, to: int) -> int:
     return (v + to - 1) // to * to
 
@@ -110,9 +124,8 @@ def _quantise(rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     dev = rows.device
     q = _empty_codes(m, k, dev)
     scale = torch.empty((m, 1), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("ima_int8_quantize_rows", rows.data_ptr(), nat.dtype_code(rows.dtype), m, k, _ld(rows), q.data_ptr(),
-                 _code_ld(q), scale.data_ptr(), nat.stream_of(dev))
+    _call(dev, "ima_int8_quantize_rows", rows.data_ptr(), nat.dtype_code(rows.dtype), m, k, _ld(rows), q.data_ptr(),
+          _code_ld(q), scale.data_ptr())
     return q, scale
 
 
@@ -120,9 +133,7 @@ def _transpose(t: torch.Tensor) -> torch.Tensor:
     """int8 [rows, cols] (aligned) -> [cols, rows]."""
     rows, cols = t.shape
     out = _empty_codes(cols, rows, t.device)
-    with torch.cuda.device(t.device):
-        nat.call("ima_int8_transpose", t.data_ptr(), rows, cols, _code_ld(t), out.data_ptr(), _code_ld(out),
-                 nat.stream_of(t.device))
+    _call(t.device, "ima_int8_transpose", t.data_ptr(), rows, cols, _code_ld(t), out.data_ptr(), _code_ld(out))
     return out
 
 
@@ -236,20 +247,27 @@ def int8_gemm(
     if c is None and y is None:
         raise RuntimeError("int8_gemm has no output to compute: want_c, y_dtype or y_out")
     nat.require_device(dev, ("B matrix", b), ("int32 output", c), ("output", y))
-    with torch.cuda.device(dev):
-        nat.call(
-            "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, nat.ptr(c),
-            _ld(c) if c is not None else n, nat.ptr(x_scale), nat.ptr(w_scale), nat.ptr(bias), bias_dtype, nat.ptr(y),
-            nat.dtype_code(y.dtype) if y is not None else 0, _ld(y) if y is not None else n, nat.stream_of(dev),
-        )
+    _call(dev, "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, nat.ptr(c),
+          _ld(c) if c is not None else n, nat.ptr(x_scale), nat.ptr(w_scale), nat.ptr(bias), bias_dtype, nat.ptr(y),
+          nat.dtype_code(y.dtype) if y is not None else 0, _ld(y) if y is not None else n)
     return c, y
 
 
-def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None):
-    """(y [M, N], codes, scale) of x rows."""
-    q, scale = _quantise(rows)
-    _c, y = int8_gemm(q, weight.codes, want_c=False, x_scale=scale, w_scale=weight.scale, bias=bias, y_dtype=rows.dtype)
-    return y, q, scale
+def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None, keep: bool = False):
+    """(y [M, N], codes, scale) of x rows; codes and scale hold something only with keep."""
+    m, k = rows.shape
+    n = weight.shape[0]
+    dev = rows.device
+    y = torch.empty((m, n), dtype=rows.dtype, device=dev)
+    ld = _round_up(max(k, 1), 16)
+    q = torch.empty((m, ld), dtype=torch.int8, device=dev)
+    scale = torch.empty((m,), dtype=torch.float32, device=dev)
+    (bias,), bias_dtype = _bias_args(n, bias)
+    codes = weight.codes
+    _call(dev, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q.data_ptr(), ld,
+          scale.data_ptr(), keep, codes.data_ptr(), _code_ld(codes), n, weight.scale.data_ptr(), nat.ptr(bias),
+          bias_dtype, y.data_ptr(), max(n, 1))
+    return y, q[:, :k] if keep else None, scale
 
 
 def _gated_args(q: torch.Tensor, scale: torch.Tensor, gate: Int8Weight, up: Int8Weight, biases, bias_dtype: int,
@@ -260,16 +278,21 @@ def _gated_args(q: torch.Tensor, scale: torch.Tensor, gate: Int8Weight, up: Int8
             nat.ptr(biases[0]), nat.ptr(biases[1]), bias_dtype, ACTIVATIONS[activation])
 
 
-def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bias, up_bias, activation: str):
-    q, scale = _quantise(rows)
+def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bias, up_bias, activation: str,
+                   keep: bool = False):
+    m, k = rows.shape
+    n = gate.shape[0]
     dev = rows.device
-    m, n = rows.shape[0], gate.shape[0]
     h = torch.empty((m, n), dtype=rows.dtype, device=dev)
-    biases, bias_dtype = _bias_args(n, gate_bias, up_bias)
-    with torch.cuda.device(dev):
-        nat.call("ima_int8_gated_gemm", *_gated_args(q, scale, gate, up, biases, bias_dtype, activation), h.data_ptr(),
-                 nat.dtype_code(h.dtype), max(n, 1), nat.stream_of(dev))
-    return h, q, scale
+    ld = _round_up(max(k, 1), 16)
+    q = torch.empty((m, ld), dtype=torch.int8, device=dev)
+    scale = torch.empty((m,), dtype=torch.float32, device=dev)
+    (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
+    _call(dev, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q.data_ptr(), ld,
+          scale.data_ptr(), keep, gate.codes.data_ptr(), _code_ld(gate.codes), up.codes.data_ptr(), _code_ld(up.codes),
+          n, gate.scale.data_ptr(), up.scale.data_ptr(), nat.ptr(gate_bias), nat.ptr(up_bias), bias_dtype,
+          ACTIVATIONS[activation], h.data_ptr(), max(n, 1))
+    return h, q[:, :k] if keep else None, scale
 
 
 # ---------------------------------------------------------------------------
@@ -288,9 +311,8 @@ def _digits_rows(src: torch.Tensor, seg_len: int, seg_pitch: int, segs: int, col
     width = _round_up(max((segs - 1) * seg_pitch + seg_len, 1), 16)
     out = torch.empty((planes, m, width), dtype=torch.int8, device=dev)
     scale = torch.empty((m,), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("ima_int8_digits_rows", src.data_ptr(), nat.dtype_code(src.dtype), m, seg_len, seg_pitch, segs, _ld(src),
-                 col_scale.data_ptr(), planes, out.data_ptr(), width, scale.data_ptr(), nat.stream_of(dev))
+    _call(dev, "ima_int8_digits_rows", src.data_ptr(), nat.dtype_code(src.dtype), m, seg_len, seg_pitch, segs, _ld(src),
+          col_scale.data_ptr(), planes, out.data_ptr(), width, scale.data_ptr())
     return out, scale
 
 
@@ -303,10 +325,9 @@ def _digits_cols(src: torch.Tensor, row_scale: torch.Tensor, planes: int, sum_dt
     scale = torch.empty((length,), dtype=torch.float32, device=dev) if planes else None
     sums = torch.empty((length,), dtype=sum_dtype, device=dev) if sum_dtype is not None else None
     ws = torch.empty((int(nat.lib().ima_int8_cols_workspace_bytes(m, length)),), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("ima_int8_digits_cols", src.data_ptr(), nat.dtype_code(src.dtype), m, length, _ld(src),
-                 row_scale.data_ptr(), planes, nat.ptr(out), width, nat.ptr(scale), nat.ptr(sums),
-                 nat.dtype_code(sum_dtype) if sums is not None else 0, ws.data_ptr(), nat.stream_of(dev))
+    _call(dev, "ima_int8_digits_cols", src.data_ptr(), nat.dtype_code(src.dtype), m, length, _ld(src),
+          row_scale.data_ptr(), planes, nat.ptr(out), width, nat.ptr(scale), nat.ptr(sums),
+          nat.dtype_code(sum_dtype) if sums is not None else 0, ws.data_ptr())
     return out, scale, sums
 
 
@@ -315,10 +336,9 @@ def _digit_gemm(planes: torch.Tensor, row_scale: torch.Tensor, b: torch.Tensor, 
     n = b.shape[0]
     dev = planes.device
     y = torch.empty((m, n), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
-        nat.call("ima_int8_digit_gemm", planes.data_ptr(), planes.shape[0], planes.shape[2], row_scale.data_ptr(),
-                 b.data_ptr(), _code_ld(b), nat.ptr(b2), _code_ld(b2) if b2 is not None else 0, m, n, k, y.data_ptr(),
-                 nat.dtype_code(dtype), max(n, 1), nat.stream_of(dev))
+    _call(dev, "ima_int8_digit_gemm", planes.data_ptr(), planes.shape[0], planes.shape[2], row_scale.data_ptr(),
+          b.data_ptr(), _code_ld(b), nat.ptr(b2), _code_ld(b2) if b2 is not None else 0, m, n, k, y.data_ptr(),
+          nat.dtype_code(dtype), max(n, 1))
     return y
 
 
@@ -424,9 +444,8 @@ def int8_gated_backward(
     # and column maxima that are known only once it is complete
     d = torch.empty((m, 2 * pitch), dtype=torch.float32, device=dev)
     biases, bias_dtype = _bias_args(n, gate_bias, up_bias)
-    with torch.cuda.device(dev):
-        nat.call("ima_int8_gated_backward_gemm", *_gated_args(codes, scale, gate, up, biases, bias_dtype, activation),
-                 dh.data_ptr(), nat.dtype_code(dh.dtype), _ld(dh), d.data_ptr(), 2 * pitch, pitch, nat.stream_of(dev))
+    _call(dev, "ima_int8_gated_backward_gemm", *_gated_args(codes, scale, gate, up, biases, bias_dtype, activation),
+          dh.data_ptr(), nat.dtype_code(dh.dtype), _ld(dh), d.data_ptr(), 2 * pitch, pitch)
     dx = None
     if dx_dtype is not None:
         channel = torch.zeros((2, pitch), dtype=torch.float32, device=dev)
@@ -464,7 +483,7 @@ class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, handle):
         w = handle if handle is not None else Int8Weight.from_float(weight)
-        y, q, scale = _linear_forward(_rows(x.detach()), w, bias)
+        y, q, scale = _linear_forward(_rows(x.detach()), w, bias, keep=True)
         ctx.save_for_backward(q, scale)
         ctx.weight = w
         ctx.types = tuple(t.dtype if t is not None and need else None
@@ -487,7 +506,7 @@ class _GatedFunction(torch.autograd.Function):
     def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, gate, up, activation):
         g = gate if gate is not None else Int8Weight.from_float(gate_weight)
         u = up if up is not None else Int8Weight.from_float(up_weight)
-        h, q, scale = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation)
+        h, q, scale = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation, keep=True)
         ctx.save_for_backward(q, scale, gate_bias, up_bias)
         ctx.gate, ctx.up, ctx.activation = g, u, activation
         inputs = (x, gate_weight, up_weight, gate_bias, up_bias)
