@@ -67,6 +67,7 @@ struct __align__(64) I8Params {
     int64_t ldc, ldy, ldh, ldd, seg_pitch;
     int32_t M, N, m_tiles, n_tiles, k_tiles, group_m;
     int32_t y_dtype, bias_dtype, dh_dtype, act, vec_c, vec_y, vec_d;
+    int32_t dependent;              // launched while the kernel before it (a quantiser) still runs
     int32_t seg_tiles;              // I8_DIGIT: k-tiles of the first B; later ones read the second (mb2)
     uint64_t stall_ns;              // test knob (ima_set_gemm_wait_test); 0 in normal use
 };
@@ -224,6 +225,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
     if (CG == 2) cluster_sync_all();   // both CTAs' barriers exist before either signals the other's
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");   // codes and scales are complete
 
     if (warp == 0 && lane == 0) {
         // ---------------- TMA producer ----------------
@@ -557,13 +559,22 @@ int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
     cfg.blockDim = dim3(I8_THREADS);
     cfg.dynamicSmemBytes = L::ALLOC;
     cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = CG;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (CG == 2) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = CG;
+        attr[n].val.clusterDim.y = 1;
+        attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (p.dependent) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = (unsigned)n;
     return ima_note_cuda(cudaLaunchKernelEx(&cfg, kern, p));
 }
 

@@ -20,23 +20,41 @@
 
 namespace {
 
-// Codes of eight elements, rint(RN32(x / s)) each, without a division per element.  With inv =
-// RN(1/s), fma(x, inv, 1.5 * 2^23) holds rint(x * inv) in its low mantissa bits; x * inv is off by at
-// most 2^-23 |x / s| < 2e-5 from the quotient, so only where it is that close to a half-integer
-// (0.02 % of all elements) the division itself decides.  A scale that is NaN or inf gives codes 0.
-IMA_DEVINL uint2 i8_codes8(const float (&v)[8], float s, float inv) {
+// Reciprocals of a scale that bracket it: x * lo and x * hi lie on either side of RN32(x / s), which is off
+// by at most 2^-24 of the quotient, as are the products.
+struct I8Inv {
+    float lo, hi;
+};
+IMA_DEVINL I8Inv i8_inv(float s) {
+    const float inv = __frcp_rn(s);
+    return {__fmul_rn(inv, 1.0f - 0x1p-21f), __fmul_rn(inv, 1.0f + 0x1p-21f)};
+}
+
+// Codes of eight elements, rint(RN32(x / s)) each, without a division per element: fma(x, inv, 1.5 *
+// 2^23) holds rint(x * inv) in its low mantissa bits, and rounding is monotonic, so where both
+// brackets round to the same integer the quotient does too.  Where they differ (a quotient within
+// 2^-20 of itself of a half-integer, some 3 in 10^5) the division decides.  A scale that is NaN or
+// inf gives codes 0.
+IMA_DEVINL uint2 i8_codes8(const float (&v)[8], float s, I8Inv inv) {
     constexpr float kRound = 12582912.0f;
-    uint32_t b[8];
-    float worst = 0.0f;
+    uint32_t b[8], differ = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float t = __fmaf_rn(v[j], inv, kRound);
-        b[j] = __float_as_uint(t);
-        worst = fmaxf(worst, fabsf(__fmaf_rn(v[j], inv, kRound - t)));
+        b[j] = __float_as_uint(__fmaf_rn(v[j], inv.lo, kRound));
+        differ |= b[j] ^ __float_as_uint(__fmaf_rn(v[j], inv.hi, kRound));
     }
-    if (worst > 0.4999f) {
+    if (differ) {
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            float x = v[0];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) b[j] = (uint32_t)__float2int_rn(__fdiv_rn(v[j], s));
+            for (int e = 1; e < 8; ++e) x = j == e ? v[e] : x;
+            if (__fmaf_rn(x, inv.lo, kRound) != __fmaf_rn(x, inv.hi, kRound)) {
+                const uint32_t k = (uint32_t)__float2int_rn(__fdiv_rn(x, s));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) b[e] = j == e ? k : b[e];
+            }
+        }
     }
     if (!(s <= 3.402823466e38f)) return make_uint2(0, 0);
     return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
@@ -129,6 +147,8 @@ IMA_DEVINL uint32_t row_max(uint32_t m, uint32_t* s_max) {
 template <int DT, int TPR, int V>
 __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* x, int64_t M, int64_t K, int64_t ldx,
                                                                     int8_t* q, int64_t ldq, float* scale) {
+    // a product launched to follow this kernel may start now; it waits for this kernel's end before it reads
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ uint32_t s_max[8];
     constexpr int ROWS = 256 / TPR;
     const int tid = threadIdx.x % TPR;
@@ -154,7 +174,7 @@ __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* 
         }
         const float amax = __uint_as_float(row_max<TPR>(mx, s_max));
         const float s = i8_row_scale(amax, amax != amax);
-        const float inv = __frcp_rn(s);
+        const I8Inv inv = i8_inv(s);
         if (tid == 0) scale[m] = s;
         int8_t* qr = q + m * ldq;
         auto emit = [&](const Raw8<DT>& r, int64_t k0) {
@@ -426,16 +446,17 @@ bool known_dtype(int d) { return d == IMA_DTYPE_F32 || d == IMA_DTYPE_BF16 || d 
 template <int DT>
 int launch_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                     cudaStream_t st) {
-    // A warp per row where the row fits its registers (16 KB of rows in flight per warp group without a
-    // block-wide barrier: 8 B per element of fp32 at 2048, 16-bit at 4096), else a block per row.
+    // A warp per row where the row fits its registers and the rows fill the machine (no barrier across the
+    // block), else a block per row: all of a long row's loads in flight at once.
     constexpr int W = DT == IMA_DTYPE_F32 ? 8 : 16;
-    if (K <= 32 * 8 * W) {
+    if (K <= 32 * 8 * 4 || (K <= 32 * 8 * W && M >= 148 * 8)) {
         const unsigned grid = (unsigned)std::min<int64_t>((M + 7) / 8, 148 * 32);
         if (K <= 1024) int8_quantize_rows_kernel<DT, 32, 4><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
         else int8_quantize_rows_kernel<DT, 32, W><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
     } else {
         const unsigned grid = (unsigned)std::min<int64_t>(M, 148 * 32);
-        int8_quantize_rows_kernel<DT, 256, 10><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+        if (K <= 4096) int8_quantize_rows_kernel<DT, 256, 2><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+        else int8_quantize_rows_kernel<DT, 256, 10><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
     }
     return IMA_LAUNCH_STATUS();
 }
