@@ -376,6 +376,7 @@ int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_
  * int8 and scale [M] are workspace; with keep_codes != 0 they hold the codes and scales of x
  * afterwards (what a backward pass needs), otherwise a product of few tokens quantises them in
  * its own launch and leaves both alone. */
+int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated); /* 1: q and scale may be NULL (keep_codes == 0) */
 int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                     int keep_codes, const int8_t* w, int64_t ldw, int64_t N, const float* w_scale, const void* bias,
                     int bias_dtype, void* y, int64_t ldy, void* stream);
@@ -384,39 +385,35 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
                    const float* gate_scale, const float* up_scale, const void* gate_bias, const void* up_bias,
                    int bias_dtype, int activation, void* y, int64_t ldy, void* stream);
 
-/* Gradients of g and u from dh [M,N] (row stride ldh): g and u are formed again from the codes,
- * d[m, n] = dh u act'(g) and d[m, seg_pitch + n] = dh act(g), fp32 (row stride ldd). */
-int ima_int8_gated_backward_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up,
-                                 int64_t ldu, int64_t M, int64_t N, int64_t K, const float* x_scale,
-                                 const float* gate_scale, const float* up_scale, const void* gate_bias,
-                                 const void* up_bias, int bias_dtype, int activation, const void* dh, int dh_dtype,
-                                 int64_t ldh, float* d, int64_t ldd, int64_t seg_pitch, void* stream);
-
-/* Base-256 digit planes of a real matrix, the left operand of a gradient product: v = rint(D / s),
- * s = rowmax |D| / (127 * 256 + 127) with planes == 2, / (127 * 65536 + 127 * 256 + 127) with
- * planes == 3, v = sum_p 256^p d_p, d_p in [-128, 127].
- * _rows: D[m, j] = src[m, j] * col_scale[j] (col_scale NULL: 1); out [planes][M][ldp], row_scale
- *   [M].  src, col_scale and out consist of `segs` (1 or 2) segments of seg_len columns, seg_pitch
- *   apart; other columns of out are zero.
- * _cols: D = src[m, j] * row_scale[m] (NULL: 1) transposed: out [planes][L][ldp], col_scale [L],
- *   columns M.. of out zero.  sum_out (optional, [L] of sum_dtype) = sum_m src[m, j], in a fixed
- *   order.  planes == 0: the sums alone.  workspace: ima_int8_cols_workspace_bytes(M, L). */
-int ima_int8_digits_rows(const void* src, int src_dtype, int64_t M, int64_t seg_len, int64_t seg_pitch, int segs,
-                         int64_t ld, const float* col_scale, int planes, int8_t* out, int64_t ldp, float* row_scale,
-                         void* stream);
-int64_t ima_int8_cols_workspace_bytes(int64_t M, int64_t L);
-int ima_int8_digits_cols(const void* src, int src_dtype, int64_t M, int64_t L, int64_t ld, const float* row_scale,
-                         int planes, int8_t* out, int64_t ldp, float* col_scale, void* sum_out, int sum_dtype,
-                         void* workspace, void* stream);
-/* dst [cols, rows] (row stride ldd, columns rows..round_up(rows, 16) zero) = src [rows, cols] transposed. */
+/* dst [cols, rows] (row stride ldd, a multiple of 16; columns rows..round_up(rows, 16) zero) = src
+ * [rows, cols] transposed. */
 int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst, int64_t ldd,
                        void* stream);
-/* y [M,N] = row_scale[m] * sum_p 256^p (a_planes[p] b^T)[m, n], a_planes [planes][M][lda], b [N,K].
- * With b2 [N,K] the product of a second segment of the planes is added: the planes then hold K
- * columns at 0 and K at round_up(K, 128), zero between. */
-int ima_int8_digit_gemm(const int8_t* a_planes, int planes, int64_t lda, const float* row_scale, const int8_t* b,
-                        int64_t ldb, const int8_t* b2, int64_t ldb2, int64_t M, int64_t N, int64_t K, void* y,
-                        int y_dtype, int64_t ldy, void* stream);
+
+/* Gradients of the two operators from grad [M,N] (row stride ldg), straight through the rounding; q [M,K]
+ * and scale [M] are the codes of the activations.
+ *   linear: dx = (grad * w_scale) w, dw = (grad * scale)^T q, db = sum_m grad
+ *   gated:  g and u are formed again from the codes; D_gate = grad u act'(g), D_up = grad act(g);
+ *           dx sums both projections, dgate and dup, the biases' gradients
+ * dx [M,K], dw [N,K], db [N] are contiguous, each optional (NULL).  w_t (gate_t, up_t): the transposed
+ * codes [K,N] if the caller keeps them, else NULL and they are made in the workspace.  planes: base-256
+ * digits of the real factor of each product against its row maximum, 2 (2^-16 of it) or 3 (2^-24).
+ * Contractions are at most 131072 - 1: N (gated: round_up(N, 128) + N) for dx, M for dw
+ * (IMA_ERR_UNSUPPORTED beyond).  workspace: ima_int8_backward_workspace_bytes(...), 256-byte aligned;
+ * own_transposed != 0 when a w_t is NULL. */
+int64_t ima_int8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int planes, int dx, int dw, int db,
+                                          int own_transposed);
+int ima_int8_linear_backward(const void* grad, int grad_dtype, int64_t ldg, int64_t M, int64_t N, int64_t K,
+                             const int8_t* q, int64_t ldq, const float* scale, const int8_t* w, int64_t ldw,
+                             const int8_t* w_t, int64_t ldwt, const float* w_scale, int planes, void* dx, int dx_dtype,
+                             void* dw, int dw_dtype, void* db, int db_dtype, void* workspace, void* stream);
+int ima_int8_gated_backward(const void* grad, int grad_dtype, int64_t ldg, int64_t M, int64_t N, int64_t K,
+                            const int8_t* q, int64_t ldq, const float* scale, const int8_t* gate, int64_t ldgate,
+                            const int8_t* up, int64_t ldup, const int8_t* gate_t, int64_t ldgate_t, const int8_t* up_t,
+                            int64_t ldup_t, const float* gate_scale, const float* up_scale, const void* gate_bias,
+                            const void* up_bias, int bias_dtype, int activation, int planes, void* dx, int dx_dtype,
+                            void* dgate, void* dup, int dw_dtype, void* dgate_bias, void* dup_bias, int db_dtype,
+                            void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -147,6 +147,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I32,
         [_VP, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _I64, _VP],
     ),
+    "ima_int8_fused": (_I32, [_I64, _I64, _I64, _I32]),
     "ima_int8_linear": (
         _I32,
         [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _I32, _VP, _I64, _I64, _VP, _VP, _I32, _VP, _I64, _VP],
@@ -156,24 +157,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _I32, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _VP, _VP, _I32, _I32,
          _VP, _I64, _VP],
     ),
-    "ima_int8_gated_backward_gemm": (
-        _I32,
-        [_VP, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _I64, _VP,
-         _I64, _I64, _VP],
-    ),
-    "ima_int8_digits_rows": (
-        _I32,
-        [_VP, _I32, _I64, _I64, _I64, _I32, _I64, _VP, _I32, _VP, _I64, _VP, _VP],
-    ),
-    "ima_int8_cols_workspace_bytes": (_I64, [_I64, _I64]),
-    "ima_int8_digits_cols": (
-        _I32,
-        [_VP, _I32, _I64, _I64, _I64, _VP, _I32, _VP, _I64, _VP, _VP, _I32, _VP, _VP],
-    ),
     "ima_int8_transpose": (_I32, [_VP, _I64, _I64, _I64, _VP, _I64, _VP]),
-    "ima_int8_digit_gemm": (
+    "ima_int8_backward_workspace_bytes": (_I64, [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "ima_int8_linear_backward": (
         _I32,
-        [_VP, _I32, _I64, _VP, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _I32, _I64, _VP],
+        [_VP, _I32, _I64, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _I64, _VP, _I64, _VP, _I32, _VP, _I32, _VP, _I32, _VP,
+         _I32, _VP, _VP],
+    ),
+    "ima_int8_gated_backward": (
+        _I32,
+        [_VP, _I32, _I64, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _VP,
+         _VP, _I32, _I32, _I32, _VP, _I32, _VP, _VP, _I32, _VP, _VP, _I32, _VP, _VP],
     ),
     "ima_freivalds_workspace_bytes": (_I64, [_I64]),
     "ima_freivalds_fp8": (

@@ -46,8 +46,10 @@ int run_fused(SkParams& p, int x_dtype, const SkPlan& q, cudaStream_t st) {
 
 // Whether the tokens are quantised inside the product: every cluster then does it for itself, which
 // pays while the workers hold a CTA's share in one batch of loads.
-bool fused_wanted(int64_t M, const SkPlan& q) {
-    return q.ok && M <= 16 && M * ((q.k_steps + q.splits - 1) / q.splits) * I8_KT <= SK_WORKERS * 32 * SK_BATCH * 8;
+bool fused_plan(int64_t M, int64_t N, int64_t K, int ops, SkPlan& q) {
+    if (M < 1 || M > 16 || N < 1) return false;
+    q = sk_plan(M, N, i8_steps(K), 1, ops, true);
+    return q.ok && M * ((q.k_steps + q.splits - 1) / q.splits) * I8_KT <= SK_WORKERS * 32 * SK_BATCH * 8;
 }
 
 }  // namespace
@@ -72,7 +74,7 @@ int int8_gemm_entry(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, 
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
     p.vec_c = c && aligned16(c, ldc * 4);
     p.vec_y = y && aligned16(y, ldy * dtype_bytes(y_dtype));
-    return run_linear(p, {a, b, nullptr, lda, ldb, 0, K, K}, (cudaStream_t)stream);
+    return run_linear(p, {a, b, nullptr, lda, ldb, 0, K, K, M * lda}, (cudaStream_t)stream);
 }
 
 int int8_gated_entry(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
@@ -94,7 +96,7 @@ int int8_gated_entry(const int8_t* a, int64_t lda, const int8_t* gate, int64_t l
     p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = activation;
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
     p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
-    return run_gated(p, {a, gate, up, lda, ldg, ldu, K, K}, (cudaStream_t)stream);
+    return run_gated(p, {a, gate, up, lda, ldg, ldu, K, K, M * lda}, (cudaStream_t)stream);
 }
 
 }  // namespace
@@ -115,55 +117,13 @@ int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_
                             bias_dtype, activation, y, y_dtype, ldy, 0, stream);
 }
 
-int ima_int8_gated_backward_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up,
-                                 int64_t ldu, int64_t M, int64_t N, int64_t K, const float* x_scale,
-                                 const float* gate_scale, const float* up_scale, const void* gate_bias,
-                                 const void* up_bias, int bias_dtype, int activation, const void* dh, int dh_dtype,
-                                 int64_t ldh, float* d, int64_t ldd, int64_t seg_pitch, void* stream) {
-    int rc = check_i8_operand(a, M, K, lda);
-    if (rc == IMA_OK) rc = check_i8_operand(gate, N, K, ldg);
-    if (rc == IMA_OK) rc = check_i8_operand(up, N, K, ldu);
-    if (rc != IMA_OK) return rc;
-    if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
-    if (M == 0 || N == 0) return IMA_OK;
-    if (!dh || !d || !x_scale || !gate_scale || !up_scale || !known_dtype(dh_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    if ((ldh < N && M > 1) || seg_pitch < N || (ldd < seg_pitch + N && M > 1)) return IMA_ERR_INVALID_ARGUMENT;
-    if ((gate_bias || up_bias) && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    I8Params p;
-    memset(&p, 0, sizeof(p));
-    p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
-    p.bias_dtype = bias_dtype; p.act = activation; p.dh = dh; p.dh_dtype = dh_dtype; p.ldh = ldh;
-    p.d = d; p.ldd = ldd; p.seg_pitch = seg_pitch;
-    p.M = (int32_t)M; p.N = (int32_t)N;
-    p.vec_d = aligned16(d, ldd * 4) && seg_pitch % 4 == 0;
-    return launch_i8<1, 256, I8_GATED_BWD>(p, {a, gate, up, lda, ldg, ldu, K, K}, (cudaStream_t)stream);
-}
-
-int ima_int8_digit_gemm(const int8_t* a_planes, int planes, int64_t lda, const float* row_scale, const int8_t* b,
-                        int64_t ldb, const int8_t* b2, int64_t ldb2, int64_t M, int64_t N, int64_t K, void* y,
-                        int y_dtype, int64_t ldy, void* stream) {
-    if (planes != 2 && planes != 3) return IMA_ERR_UNSUPPORTED;
-    // with a second B the planes hold two segments of K columns, the second on a k-tile boundary
-    const int64_t seg = b2 ? (K + I8_KT - 1) / I8_KT * I8_KT : 0;
-    int rc = check_i8_operand(a_planes, M, seg + K, lda);
-    if (rc == IMA_OK) rc = check_i8_operand(b, N, K, ldb);
-    if (rc == IMA_OK && b2) rc = check_i8_operand(b2, N, K, ldb2);
-    if (rc != IMA_OK) return rc;
-    if (M == 0 || N == 0) return IMA_OK;
-    if (!y || !row_scale || (ldy < N && M > 1) || !known_dtype(y_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    I8Params p;
-    memset(&p, 0, sizeof(p));
-    p.y = y; p.xs = row_scale; p.ldy = ldy; p.y_dtype = y_dtype;
-    p.M = (int32_t)M; p.N = (int32_t)N;
-    p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
-    p.seg_tiles = (int32_t)((K + I8_KT - 1) / I8_KT);
-    const I8Operands o = {a_planes, b, b2, lda, ldb, ldb2, seg + K, K};
-    if (planes == 2) return run_digits<2, 256>(p, o, (cudaStream_t)stream);
-    return run_digits<3, 128>(p, o, (cudaStream_t)stream);
-}
-
 // Operator entries: floating activations in.  Few tokens: one launch, quantiser inside.  Otherwise the row
 // quantiser into q and scale, then the product.
+int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated) {
+    SkPlan plan;
+    return K >= 0 && K <= I8_MAX_K && fused_plan(M, N, K, gated ? 2 : 1, plan) ? 1 : 0;
+}
+
 int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                     int keep_codes, const int8_t* w, int64_t ldw, int64_t N, const float* w_scale, const void* bias,
                     int bias_dtype, void* y, int64_t ldy, void* stream) {
@@ -171,16 +131,16 @@ int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld
     int rc = check_i8_operand(w, N, K, ldw);
     if (rc != IMA_OK) return rc;
     if (M > 0 && K > 0 && (!x || (M > 1 && ldx < K))) return IMA_ERR_INVALID_ARGUMENT;
-    if (M > 0 && M <= 16 && N > 0 && !keep_codes) {
-        const SkPlan plan = sk_plan(M, N, i8_steps(K), 1, 1, true);
-        if (fused_wanted(M, plan)) {
+    {
+        SkPlan plan;
+        if (!keep_codes && fused_plan(M, N, K, 1, plan)) {
             if (!y || !w_scale || (ldy < N && M > 1) || (bias && !known_dtype(bias_dtype))) return IMA_ERR_INVALID_ARGUMENT;
             SkParams p;
             memset(&p, 0, sizeof(p));
             p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
             p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
             p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
-            rc = sk_weight_maps(p, {nullptr, w, nullptr, 0, ldw, 0, K, K});
+            rc = sk_weight_maps(p, {nullptr, w, nullptr, 0, ldw, 0, K, K, 0});
             if (rc != IMA_OK) return rc;
             return run_fused<I8_LINEAR>(p, x_dtype, plan, (cudaStream_t)stream);
         }
@@ -200,9 +160,9 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
     if (rc != IMA_OK) return rc;
     if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
     if (M > 0 && K > 0 && (!x || (M > 1 && ldx < K))) return IMA_ERR_INVALID_ARGUMENT;
-    if (M > 0 && M <= 16 && N > 0 && !keep_codes) {
-        const SkPlan plan = sk_plan(M, N, i8_steps(K), 1, 2, true);
-        if (fused_wanted(M, plan)) {
+    {
+        SkPlan plan;
+        if (!keep_codes && fused_plan(M, N, K, 2, plan)) {
             if (!y || !gate_scale || !up_scale || (ldy < N && M > 1) || ((gate_bias || up_bias) && !known_dtype(bias_dtype)))
                 return IMA_ERR_INVALID_ARGUMENT;
             SkParams p;
@@ -211,7 +171,7 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
             p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.act = activation;
             p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias; p.bias_dtype = bias_dtype;
             p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
-            rc = sk_weight_maps(p, {nullptr, gate, up, 0, ldg, ldu, K, K});
+            rc = sk_weight_maps(p, {nullptr, gate, up, 0, ldg, ldu, K, K, 0});
             if (rc != IMA_OK) return rc;
             return run_fused<I8_GATED>(p, x_dtype, plan, (cudaStream_t)stream);
         }
@@ -220,6 +180,254 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
     if (rc != IMA_OK) return rc;
     return int8_gated_entry(q, ldq, gate, ldg, up, ldu, M, N, K, scale, gate_scale, up_scale, gate_bias, up_bias,
                             bias_dtype, activation, y, x_dtype, ldy, 1, stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Backward passes.  Launches, in order: [g and u again, their gradients D and D's maxima | D's maxima],
+// the digits of D by rows and by columns with the partial bias sums, [W transposed], dx, q transposed,
+// dW, bias sums.
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr int BWD_DX = 1, BWD_DW = 2, BWD_DB = 4, BWD_OWN_WT = 8;
+
+struct BwdPlan {
+    int64_t pitch, W, ldm, ldwt;
+    int64_t maxima, maxima_bytes, d, rows, row_scale, cols, col_scale, q_t, w_t, partial, total;   // offsets
+};
+
+BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int segs, int planes, int want) {
+    BwdPlan b = {};
+    // segments of a pair start on a k-tile of the dx product and on a row tile of the dW product
+    b.pitch = segs == 2 ? (N + 127) / 128 * 128 : (N + 15) / 16 * 16;
+    b.W = segs * b.pitch;
+    b.ldm = (M + 15) / 16 * 16;
+    b.ldwt = (N + 15) / 16 * 16;
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t o = at;
+        at += (bytes + 255) / 256 * 256;
+        return o;
+    };
+    const bool dx = want & BWD_DX, dw = want & BWD_DW;
+    b.maxima_bytes = (M + b.W) * 4;
+    b.maxima = take(b.maxima_bytes);
+    if (segs == 2) b.d = take(M * b.W * 4);
+    if (dx) {
+        b.rows = take(planes * M * b.W);
+        b.row_scale = take(M * 4);
+    }
+    if (dw) {
+        b.cols = take(planes * b.W * b.ldm);
+        b.col_scale = take(b.W * 4);
+        b.q_t = take(K * b.ldm);
+    }
+    if (want & BWD_OWN_WT) b.w_t = take(segs * K * b.ldwt);
+    if (want & BWD_DB) b.partial = take((M + 127) / 128 * b.W * 4);
+    b.total = at;
+    return b;
+}
+
+struct BwdArgs {
+    const void* grad;
+    int grad_dtype;
+    int64_t ldg, M, N, K;
+    const int8_t* q;
+    int64_t ldq;
+    const float* scale;
+    int segs;
+    const int8_t* w[2];
+    int64_t ldw[2];
+    const int8_t* w_t[2];          // [K, N] (NULL: made in the workspace)
+    int64_t ldwt[2];
+    const float* w_scale[2];
+    const void* bias[2];
+    int bias_dtype, activation, planes;
+    void* dx;
+    int dx_dtype;
+    void* dw[2];
+    int dw_dtype;
+    void* db[2];
+    int db_dtype;
+    void* workspace;
+};
+
+int zero_out(void* p, int64_t n, int dtype, cudaStream_t st) {
+    if (!p || n == 0) return IMA_OK;
+    return ima_note_cuda(cudaMemsetAsync(p, 0, (size_t)(n * dtype_bytes(dtype)), st));
+}
+
+template <int P, int BN>
+int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStream_t st) {
+    int rc = IMA_OK;
+    if (a.dx) {
+        const int8_t* wt[2] = {a.w_t[0], a.w_t[1]};
+        int64_t ldwt[2] = {a.ldwt[0], a.ldwt[1]};
+        for (int i = 0; i < a.segs; ++i)
+            if (!wt[i]) {
+                int8_t* t = reinterpret_cast<int8_t*>(ws + b.w_t) + i * a.K * b.ldwt;
+                rc = ima_int8_transpose(a.w[i], a.N, a.K, a.ldw[i], t, b.ldwt, st);
+                if (rc != IMA_OK) return rc;
+                wt[i] = t;
+                ldwt[i] = b.ldwt;
+            }
+        I8Params p;
+        memset(&p, 0, sizeof(p));
+        p.y = a.dx; p.ldy = a.K; p.y_dtype = a.dx_dtype; p.xs = reinterpret_cast<const float*>(ws + b.row_scale);
+        p.M = (int32_t)a.M; p.N = (int32_t)a.K;
+        p.vec_y = aligned16(a.dx, a.K * dtype_bytes(a.dx_dtype));
+        p.seg_tiles = (int32_t)i8_steps(a.N);
+        const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.rows), wt[0], a.segs == 2 ? wt[1] : nullptr, b.W,
+                              ldwt[0], ldwt[1], (a.segs - 1) * b.pitch + a.N, a.N, a.M * b.W};
+        if (a.K > 0) rc = run_digits<P, BN>(p, o, st);
+        if (rc != IMA_OK) return rc;
+    }
+    if ((a.dw[0] || a.dw[1]) && a.K > 0) {
+        int8_t* qt = reinterpret_cast<int8_t*>(ws + b.q_t);
+        rc = ima_int8_transpose(a.q, a.M, a.K, a.ldq, qt, b.ldm, st);
+        if (rc != IMA_OK) return rc;
+        const int first = a.dw[0] ? 0 : 1;
+        const bool both = a.dw[0] && a.dw[1];
+        I8Params p;
+        memset(&p, 0, sizeof(p));
+        p.y = a.dw[first]; p.ldy = a.K; p.y_dtype = a.dw_dtype;
+        p.xs = reinterpret_cast<const float*>(ws + b.col_scale) + first * b.pitch;
+        p.M = (int32_t)(both ? b.pitch + a.N : a.N); p.N = (int32_t)a.K;
+        p.vec_y = aligned16(p.y, a.K * dtype_bytes(a.dw_dtype));
+        if (both) {
+            p.y2 = a.dw[1]; p.split_row = b.pitch; p.seg_rows = a.N;
+            p.vec_y = p.vec_y && aligned16(p.y2, a.K * dtype_bytes(a.dw_dtype));
+        }
+        p.seg_tiles = (int32_t)i8_steps(a.M);
+        const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.cols) + first * b.pitch * b.ldm, qt, nullptr, b.ldm,
+                              b.ldm, 0, a.M, a.M, b.W * b.ldm};
+        rc = run_digits<P, BN>(p, o, st);
+    }
+    return rc;
+}
+
+int run_backward(const BwdArgs& a, cudaStream_t st) {
+    const bool want_dw = a.dw[0] || a.dw[1], want_db = a.db[0] || a.db[1];
+    if (a.M < 0 || a.N < 0 || a.K < 0 || !known_dtype(a.grad_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    if (a.planes != 2 && a.planes != 3) return IMA_ERR_UNSUPPORTED;
+    if ((a.dx && !known_dtype(a.dx_dtype)) || (want_dw && !known_dtype(a.dw_dtype)) || (want_db && !known_dtype(a.db_dtype)))
+        return IMA_ERR_INVALID_ARGUMENT;
+    int rc = check_i8_operand(a.q, a.M, a.K, a.ldq);
+    for (int i = 0; i < a.segs && rc == IMA_OK; ++i) {
+        rc = check_i8_operand(a.w[i], a.N, a.K, a.ldw[i]);
+        if (rc == IMA_OK && a.dx && a.w_t[i]) rc = check_i8_operand(a.w_t[i], a.K, a.N, a.ldwt[i]);
+    }
+    if (rc != IMA_OK) return rc;
+    const bool own = a.dx && (!a.w_t[0] || (a.segs == 2 && !a.w_t[1]));
+    const BwdPlan b = bwd_plan(a.M, a.N, a.K, a.segs, a.planes,
+                               (a.dx ? BWD_DX : 0) | (want_dw ? BWD_DW : 0) | (want_db ? BWD_DB : 0) | (own ? BWD_OWN_WT : 0));
+    if ((a.dx && (a.segs - 1) * b.pitch + a.N > I8_MAX_K) || (want_dw && a.M > I8_MAX_K)) return IMA_ERR_UNSUPPORTED;
+    if (b.W > INT32_MAX / 2 || (a.M + 63) / 64 > 65535 || (a.N + 127) / 128 > 65535) return IMA_ERR_UNSUPPORTED;
+    if (a.M == 0 || a.N == 0) {   // empty sums
+        if (a.dx) rc = zero_out(a.dx, a.M * a.K, a.dx_dtype, st);
+        for (int i = 0; i < a.segs && rc == IMA_OK; ++i) {
+            rc = zero_out(a.dw[i], a.N * a.K, a.dw_dtype, st);
+            if (rc == IMA_OK) rc = zero_out(a.db[i], a.N, a.db_dtype, st);
+        }
+        return rc;
+    }
+    if (!a.dx && !want_dw && !want_db) return IMA_OK;
+    if (!a.grad || !a.scale || !a.workspace || (a.M > 1 && a.ldg < a.N)) return IMA_ERR_INVALID_ARGUMENT;
+    for (int i = 0; i < a.segs; ++i)
+        if (!a.w_scale[i]) return IMA_ERR_INVALID_ARGUMENT;
+    unsigned char* ws = reinterpret_cast<unsigned char*>(a.workspace);
+    uint32_t* row_max = reinterpret_cast<uint32_t*>(ws + b.maxima);
+    GradDigits d;
+    memset(&d, 0, sizeof(d));
+    GradSrc& g = d.g;
+    g.src = a.grad; g.ld = a.ldg; g.M = a.M; g.n = a.N; g.pitch = b.pitch; g.W = b.W; g.xs = a.scale;
+    g.ws[0] = a.w_scale[0]; g.ws[1] = a.w_scale[1];
+    g.row_max = a.dx ? row_max : nullptr;
+    g.col_max = want_dw ? row_max + a.M : nullptr;
+    if (a.dx || want_dw) {
+        rc = ima_note_cuda(cudaMemsetAsync(row_max, 0, (size_t)b.maxima_bytes, st));
+        if (rc != IMA_OK) return rc;
+    }
+    int src_dtype = a.grad_dtype;
+    if (a.segs == 2) {
+        I8Params p;
+        memset(&p, 0, sizeof(p));
+        p.xs = a.scale; p.ws[0] = a.w_scale[0]; p.ws[1] = a.w_scale[1]; p.bias[0] = a.bias[0]; p.bias[1] = a.bias[1];
+        p.bias_dtype = a.bias_dtype; p.act = a.activation; p.dh = a.grad; p.dh_dtype = a.grad_dtype; p.ldh = a.ldg;
+        p.d = reinterpret_cast<float*>(ws + b.d); p.ldd = b.W; p.seg_pitch = b.pitch;
+        p.row_max = g.row_max; p.col_max = g.col_max;
+        p.M = (int32_t)a.M; p.N = (int32_t)a.N;
+        p.vec_d = 1;
+        rc = launch_i8<1, 256, I8_GATED_BWD>(p, {a.q, a.w[0], a.w[1], a.ldq, a.ldw[0], a.ldw[1], a.K, a.K, a.M * a.ldq}, st);
+        if (rc != IMA_OK) return rc;
+        g.src = p.d;
+        g.ld = b.W;
+        src_dtype = IMA_DTYPE_F32;
+    } else if (a.dx || want_dw) {
+        rc = run_grad_max(g, src_dtype, st);
+        if (rc != IMA_OK) return rc;
+    }
+    if (a.dx) {
+        d.rows = reinterpret_cast<int8_t*>(ws + b.rows);
+        d.row_scale = reinterpret_cast<float*>(ws + b.row_scale);
+    }
+    if (want_dw) {
+        d.cols = reinterpret_cast<int8_t*>(ws + b.cols);
+        d.col_scale = reinterpret_cast<float*>(ws + b.col_scale);
+    }
+    if (want_db) d.partial = reinterpret_cast<float*>(ws + b.partial);
+    d.ldm = b.ldm;
+    rc = run_grad_digits(d, src_dtype, a.planes, st);
+    if (rc != IMA_OK) return rc;
+    rc = a.planes == 2 ? bwd_products<2, 256>(a, b, ws, st) : bwd_products<3, 128>(a, b, ws, st);
+    for (int i = 0; i < a.segs && rc == IMA_OK; ++i)
+        if (a.db[i]) {
+            int8_col_sum_kernel<<<(unsigned)((a.N + 255) / 256), 256, 0, st>>>(d.partial + i * b.pitch, (a.M + 127) / 128, b.W,
+                                                                             a.N, a.db[i], a.db_dtype);
+            rc = IMA_LAUNCH_STATUS();
+        }
+    return rc;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ima_int8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int planes, int dx, int dw, int db,
+                                          int own_transposed) {
+    if (M < 0 || N < 0 || K < 0) return 0;
+    const int want = (dx ? BWD_DX : 0) | (dw ? BWD_DW : 0) | (db ? BWD_DB : 0) | (dx && own_transposed ? BWD_OWN_WT : 0);
+    return bwd_plan(M, N, K, gated ? 2 : 1, planes, want).total;
+}
+
+int ima_int8_linear_backward(const void* grad, int grad_dtype, int64_t ldg, int64_t M, int64_t N, int64_t K,
+                             const int8_t* q, int64_t ldq, const float* scale, const int8_t* w, int64_t ldw,
+                             const int8_t* w_t, int64_t ldwt, const float* w_scale, int planes, void* dx, int dx_dtype,
+                             void* dw, int dw_dtype, void* db, int db_dtype, void* workspace, void* stream) {
+    BwdArgs a;
+    memset(&a, 0, sizeof(a));
+    a.grad = grad; a.grad_dtype = grad_dtype; a.ldg = ldg; a.M = M; a.N = N; a.K = K; a.q = q; a.ldq = ldq; a.scale = scale;
+    a.segs = 1; a.w[0] = w; a.ldw[0] = ldw; a.w_t[0] = w_t; a.ldwt[0] = ldwt; a.w_scale[0] = w_scale; a.planes = planes;
+    a.dx = dx; a.dx_dtype = dx_dtype; a.dw[0] = dw; a.dw_dtype = dw_dtype; a.db[0] = db; a.db_dtype = db_dtype;
+    a.workspace = workspace;
+    return run_backward(a, (cudaStream_t)stream);
+}
+
+int ima_int8_gated_backward(const void* grad, int grad_dtype, int64_t ldg, int64_t M, int64_t N, int64_t K,
+                            const int8_t* q, int64_t ldq, const float* scale, const int8_t* gate, int64_t ldgate,
+                            const int8_t* up, int64_t ldup, const int8_t* gate_t, int64_t ldgate_t, const int8_t* up_t,
+                            int64_t ldup_t, const float* gate_scale, const float* up_scale, const void* gate_bias,
+                            const void* up_bias, int bias_dtype, int activation, int planes, void* dx, int dx_dtype,
+                            void* dgate, void* dup, int dw_dtype, void* dgate_bias, void* dup_bias, int db_dtype,
+                            void* workspace, void* stream) {
+    if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
+    if ((gate_bias || up_bias) && !known_dtype(bias_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    const BwdArgs a = {grad, grad_dtype, ldg, M, N, K, q, ldq, scale, 2, {gate, up}, {ldgate, ldup}, {gate_t, up_t},
+                       {ldgate_t, ldup_t}, {gate_scale, up_scale}, {gate_bias, up_bias}, bias_dtype, activation, planes,
+                       dx, dx_dtype, {dgate, dup}, dw_dtype, {dgate_bias, dup_bias}, db_dtype, workspace};
+    return run_backward(a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

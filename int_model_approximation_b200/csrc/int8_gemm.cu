@@ -26,6 +26,7 @@
 #pragma once
 #include <cudaTypedefs.h>
 #include <algorithm>
+#include <atomic>
 #include "sm100_primitives.cuh"
 
 namespace {
@@ -64,6 +65,9 @@ struct __align__(64) I8Params {
     const void* bias[2];
     const void* dh;
     float* d;                       // I8_GATED_BWD: D^g, and D^u seg_pitch columns further
+    uint32_t *row_max, *col_max;    // I8_GATED_BWD: maxima of |D t| by rows and |D s| by columns (NULL: none)
+    void* y2;                       // I8_DIGIT: rows from split_row on go here (NULL: all to y)
+    int64_t split_row, seg_rows;    // and of each part only seg_rows exist
     int64_t ldc, ldy, ldh, ldd, seg_pitch;
     int32_t M, N, m_tiles, n_tiles, k_tiles, group_m;
     int32_t y_dtype, bias_dtype, dh_dtype, act, vec_c, vec_y, vec_d;
@@ -160,8 +164,8 @@ IMA_DEVINL void stage_store(unsigned char* st, int lane, const uint32_t (&w)[16]
 
 // 32 fp32 values of this lane's row at column `col` of y, in y's type.
 IMA_DEVINL void store_y32(const I8Params& p, unsigned char* st, int lane, const float (&v)[32], int64_t row0, int rows,
-                          int32_t col) {
-    unsigned char* y = reinterpret_cast<unsigned char*>(p.y);
+                          int32_t col, void* y_base) {
+    unsigned char* y = reinterpret_cast<unsigned char*>(y_base);
     uint32_t w[16];
     if (p.y_dtype == IMA_DTYPE_F32) {
 #pragma unroll
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                             v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)r[j]), xs), cols[c0 + j]);
                             if (p.bias[0]) v[j] = __fadd_rn(v[j], cols[HALF + c0 + j]);
                         }
-                        store_y32(p, st, lane, v, row0, rows, n0 + c0);
+                        store_y32(p, st, lane, v, row0, rows, n0 + c0, p.y);
                     }
                 }
             } else if constexpr (EPI == I8_GATED) {
@@ -403,13 +407,14 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                                                       cols[3 * HALF + c0 + j]);
                             v[j] = act_value<ACT>(g) * u;
                         }
-                        store_y32(p, st, lane, v, row0, rows, n0 + c0);
+                        store_y32(p, st, lane, v, row0, rows, n0 + c0, p.y);
                     }
                 };
                 if (p.act == IMA_ACT_SILU) chunks(std::integral_constant<int, IMA_ACT_SILU>{});
                 else if (p.act == IMA_ACT_GELU) chunks(std::integral_constant<int, IMA_ACT_GELU>{});
                 else chunks(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
             } else if constexpr (EPI == I8_GATED_BWD) {
+                uint32_t rm = 0;
                 auto chunks = [&](auto tag) {
                     constexpr int ACT = decltype(tag)::value;
 #pragma unroll 1
@@ -434,7 +439,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                         }
                         tmem_wait_ld();
                         if (n >= p.N || rows == 0) continue;
-                        uint32_t wg[16], wu[16];
+                        uint32_t wg[16], wu[16], cm = 0;
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             const float g0 = zero ? 0.0f : __int2float_rn((int32_t)rg[j]);
@@ -444,9 +449,20 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                                                       cols[3 * HALF + c0 + j]);
                             float a, da;
                             act_both<ACT>(g, a, da);
-                            wg[j] = __float_as_uint(dh[j] * u * da);
-                            wu[j] = __float_as_uint(dh[j] * a);
+                            const float dg = dh[j] * u * da, du = dh[j] * a;
+                            wg[j] = __float_as_uint(dg);
+                            wu[j] = __float_as_uint(du);
+                            // maxima of the bit patterns of magnitudes: order like the values, NaN above all
+                            rm = max(rm, max(__float_as_uint(fabsf(__fmul_rn(dg, cols[c0 + j]))),
+                                             __float_as_uint(fabsf(__fmul_rn(du, cols[2 * HALF + c0 + j])))));
+                            if (p.col_max) {
+                                const uint32_t mg = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fabsf(__fmul_rn(dg, xs))));
+                                const uint32_t mu = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fabsf(__fmul_rn(du, xs))));
+                                cm = lane == j ? mg : (lane == 16 + j ? mu : cm);
+                            }
                         }
+                        if (p.col_max && n + (lane & 15) < p.N)
+                            atomicMax(p.col_max + n + (lane & 15) + (lane >= 16 ? p.seg_pitch : 0), cm);
                         float* d = p.d + row0 * p.ldd + n;
                         stage_store(st, lane, wg, reinterpret_cast<unsigned char*>(d), p.ldd * 4, rows, (p.N - n) * 4,
                                     p.vec_d, 4);
@@ -457,14 +473,20 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                 if (p.act == IMA_ACT_SILU) chunks(std::integral_constant<int, IMA_ACT_SILU>{});
                 else if (p.act == IMA_ACT_GELU) chunks(std::integral_constant<int, IMA_ACT_GELU>{});
                 else chunks(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
+                if (p.row_max && lane < rows) atomicMax(p.row_max + row0 + lane, rm);
             } else {
+                // the second part's rows start on a multiple of 128: a warp's 32 rows lie in one part
+                const bool second = p.y2 && row0 >= p.split_row;
+                const int64_t out_row = second ? row0 - p.split_row : row0;
+                const int out_rows = p.y2 ? (int)max((int64_t)0, min((int64_t)rows, p.seg_rows - out_row)) : rows;
+                void* out = second ? p.y2 : p.y;
 #pragma unroll 1
                 for (int c0 = 0; c0 < HALF; c0 += 32) {
                     uint32_t r[P][32];
 #pragma unroll
                     for (int i = 0; i < P; ++i) tmem_ld32(tq + i * BN + c0, r[i]);
                     tmem_wait_ld();
-                    if (n0 + c0 >= p.N || rows == 0) continue;
+                    if (n0 + c0 >= p.N || out_rows <= 0) continue;
                     float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
@@ -473,7 +495,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                         for (int i = 0; i < P; ++i) s += (int64_t)(int32_t)r[i][j] << (8 * i);
                         v[j] = zero ? __fmul_rn(0.0f, xs) : __fmul_rn(__ll2float_rn(s), xs);
                     }
-                    store_y32(p, st, lane, v, row0, rows, n0 + c0);
+                    store_y32(p, st, lane, v, out_row, out_rows, n0 + c0, out);
                 }
             }
             tc_fence_before();
@@ -498,19 +520,33 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// Map over [planes][rows][K] bytes (row pitch ld) with a {128 B, box_rows(, 1)} box, 128-byte swizzle.
-int make_i8_map(CUtensorMap* map, const int8_t* base, int64_t K, int64_t ld, int64_t rows, int planes, int box_rows,
-                bool three_d) {
+// Map over [planes][rows][K] bytes (row pitch ld, planes plane_stride apart; 0: a matrix) with a {128 B,
+// box_rows(, 1)} box, 128-byte swizzle.
+int make_i8_map(CUtensorMap* map, const int8_t* base, int64_t K, int64_t ld, int64_t rows, int planes,
+                int64_t plane_stride, int box_rows) {
+    const bool three_d = plane_stride != 0;
     auto enc = get_encode_fn();
     if (!enc) return IMA_ERR_CUDA;
     cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)planes};
-    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(ld * rows)};
+    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)plane_stride};
     cuuint32_t box[3] = {(cuuint32_t)I8_KT, (cuuint32_t)box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, three_d ? 3 : 2, const_cast<int8_t*>(base), dims, strides, box,
                      estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? IMA_OK : IMA_ERR_INVALID_ARGUMENT;
+}
+
+// Allow `kern` its dynamic shared memory, once per device (a bit each for the first 64).
+int set_smem_once(std::atomic<uint64_t>& ready, const void* kern, int bytes) {
+    int dev = 0;
+    int rc = ima_note_cuda(cudaGetDevice(&dev));
+    if (rc != IMA_OK) return rc;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (ready.load(std::memory_order_acquire) & bit) return IMA_OK;
+    rc = ima_note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (rc == IMA_OK) ready.fetch_or(bit, std::memory_order_release);
+    return rc;
 }
 
 // An int8 operand as the loads need it: 16-byte aligned rows of at least K bytes.
@@ -531,6 +567,7 @@ constexpr int i8_box_rows() { return EPI == I8_GATED || EPI == I8_GATED_BWD ? BN
 struct I8Operands {
     const int8_t *a, *b, *b2;
     int64_t lda, ldb, ldb2, Ka, K;   // A has Ka columns per plane, B and b2 K
+    int64_t a_planes;                // bytes between the planes of A
 };
 
 template <int P, int BN, int EPI, int CG>
@@ -545,13 +582,14 @@ int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
     p.stall_ns = g_gemm_stall_ns;
     int rc = IMA_OK;
     if (o.K > 0) {   // K == 0 loads nothing
-        rc = make_i8_map(&p.ma, o.a, o.Ka, o.lda, p.M, P, I8_BM, true);
-        if (rc == IMA_OK) rc = make_i8_map(&p.mb, o.b, o.K, o.ldb, p.N, 1, BOX, false);
-        if (rc == IMA_OK && o.b2) rc = make_i8_map(&p.mb2, o.b2, o.K, o.ldb2, p.N, 1, BOX, false);
+        rc = make_i8_map(&p.ma, o.a, o.Ka, o.lda, p.M, P, o.a_planes, I8_BM);
+        if (rc == IMA_OK) rc = make_i8_map(&p.mb, o.b, o.K, o.ldb, p.N, 1, 0, BOX);
+        if (rc == IMA_OK && o.b2) rc = make_i8_map(&p.mb2, o.b2, o.K, o.ldb2, p.N, 1, 0, BOX);
         if (rc != IMA_OK) return rc;
     }
     auto kern = int8_gemm_kernel<P, BN, EPI, CG>;
-    rc = ima_note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+    static std::atomic<uint64_t> ready{0};
+    rc = set_smem_once(ready, (const void*)kern, L::ALLOC);
     if (rc != IMA_OK) return rc;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     cudaLaunchConfig_t cfg = {};

@@ -8,8 +8,8 @@
 //
 // Gradient digits.  A gradient product has one integer factor (codes) and one real factor D.  D
 // is written against its row maximum as v = rint(D / s), s = amax / V_P, in P balanced base-256
-// digits, v = sum_p 256^p d_p with d_p in [-128, 127] (V_2 = 127 * 256 + 127, V_3 = 127 * 65536 +
-// 127 * 256 + 127), so the product runs on the int8 tensor cores exactly.  The rounding is the
+// digits, v = sum_p 256^p d_p with d_p in [-128, 127] (V_2 = 127 * 256 + 127, V_3 = 8355000, a little
+// below 127 * 65536 + 127 * 256 + 127), so the product runs on the int8 tensor cores exactly.  The rounding is the
 // one place where a gradient loses bits: half a step of amax / V_P, i.e. at most 2^-16 (P = 2, for
 // bf16) or 2^-24 (P = 3, for fp16 and fp32) of the row's largest element.  Against the rms of
 // the row's products that is at most sqrt(L / 3) 2^-16 for L summands, reached only when one
@@ -65,11 +65,6 @@ IMA_DEVINL float i8_row_scale(float amax, bool nan) {
     if (nan) return __int_as_float(0x7FC00000);
     const float s = __fdiv_rn(amax, 127.0f);
     return s < 1e-12f ? 1e-12f : s;
-}
-
-IMA_DEVINL uint32_t pack4(const int32_t* v) {
-    return __byte_perm(__byte_perm((uint32_t)v[0], (uint32_t)v[1], 0x0040),
-                       __byte_perm((uint32_t)v[2], (uint32_t)v[3], 0x0040), 0x5410);
 }
 
 // Eight consecutive elements as loaded (16 bytes of a 16-bit type, 32 of fp32).  max_bits() is the fp32
@@ -198,237 +193,251 @@ __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* 
 // Digits
 // ---------------------------------------------------------------------------
 template <int P>
-IMA_DEVINL float digit_limit() { return P == 2 ? 32639.0f : 8355711.0f; }
+IMA_DEVINL float digit_limit() { return P == 2 ? 32639.0f : 8355000.0f; }
 
 // Scale of a row (or column) with largest magnitude `amax`: never zero, so that a row of zeros has
-// codes 0, and never so small that its reciprocal overflows.
+// codes 0, and never so small that its reciprocal overflows; NaN where an element is NaN or infinite,
+// so that its products are NaN.
 template <int P>
-IMA_DEVINL float digit_scale(float amax, bool nan) {
-    if (nan) return __int_as_float(0x7FC00000);
+IMA_DEVINL float digit_scale(float amax) {
+    if (!(amax <= 3.402823466e38f)) return __int_as_float(0x7FC00000);
     return fmaxf(__fdiv_rn(amax, digit_limit<P>()), 1.17549435e-38f);
 }
 
-// Balanced base-256 digits of rint(x * inv): |rint| <= V_P + 1 after rounding, clamped to V_P.
+// The P digit bytes of eight values x * inv, packed.  Two digits: fma(x, inv, 1.5 * 2^23) holds v in its
+// low mantissa bits; its lowest byte is d_0 and (v + 128) >> 8 is d_1.  |x * inv| <= V_P (1 + 2^-22):
+// 32639.01, and 8355002 where the digits end at 8355711, so no rounding leaves the range.
 template <int P>
-IMA_DEVINL void digits_of(float x, float inv, int32_t (&d)[P]) {
-    const int32_t lim = P == 2 ? 32639 : 8355711;
-    int32_t v = min(max(__float2int_rn(__fmul_rn(x, inv)), -lim), lim);
+IMA_DEVINL void digits8(const float (&x)[8], float inv, uint2 (&out)[P]) {
+    uint32_t v[8];
 #pragma unroll
-    for (int p = 0; p < P - 1; ++p) {
-        d[p] = (int32_t)(int8_t)(v & 255);
-        v = (v - d[p]) >> 8;
+    for (int j = 0; j < 8; ++j)
+        v[j] = P == 2 ? __float_as_uint(__fmaf_rn(x[j], inv, 12582912.0f)) : (uint32_t)__float2int_rn(__fmul_rn(x[j], inv));
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        out[p] = make_uint2(__byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410),
+                            __byte_perm(__byte_perm(v[4], v[5], 0x0040), __byte_perm(v[6], v[7], 0x0040), 0x5410));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (uint32_t)((int32_t)(v[j] + 128u) >> 8);
     }
-    d[P - 1] = v;
 }
 
-// Row digits of D[m, j] = src[m, j] * col_scale[j].  The row is `segs` segments of `seg_len`
-// columns, segment i starting at column i * seg_pitch of the source, of col_scale and of the
-// planes; columns between segments are zero in the planes.
-struct DigitRows {
+// A gradient D [M, W]: `segs` segments of n columns, `pitch` columns apart (W = segs * pitch; columns
+// between segments hold nothing).  Its row form is D ws (channel scales, one vector per segment), its
+// column form D xs (token scales), each with its own maxima, as bit patterns of non-negative fp32.
+struct GradSrc {
     const void* src;
-    const float* col_scale;   // NULL: 1
-    int8_t* planes;           // plane p at planes + p * plane_stride
-    float* row_scale;
-    int64_t ld, M, seg_len, seg_pitch, ldp, plane_stride;
-    int32_t segs, pad;
+    const float* ws[2];
+    const float* xs;
+    uint32_t* row_max;        // [M]
+    uint32_t* col_max;        // [W]
+    int64_t ld, M, n, pitch, W;
+};
+
+// Maxima of both forms.  A block takes 64 rows by 256 columns: a warp has one row's 256 columns at a
+// time, so the row maximum is one warp reduction and the column maxima stay in registers.
+template <int DT>
+__global__ void __launch_bounds__(256) int8_grad_max_kernel(const GradSrc a) {
+    __shared__ uint32_t s_max[8][256];
+    const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int64_t j0 = (int64_t)blockIdx.x * 256 + cg * 8;
+    const int64_t m0 = (int64_t)blockIdx.y * 64;
+    uint32_t mx[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    float w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = a.row_max && j0 + j < a.n ? __ldg(a.ws[0] + j0 + j) : 0.0f;
+    Raw8<DT> r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t m = m0 + rl + i * 8;
+        const unsigned char* row = reinterpret_cast<const unsigned char*>(a.src) + m * a.ld * dtype_bytes(DT);
+        r[i].clear();
+        if (m < a.M && j0 < a.n) r[i].load(row, j0, a.n, (reinterpret_cast<uintptr_t>(row) & 15) == 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t m = m0 + rl + i * 8;
+        if (m >= a.M) break;
+        float v[8];
+        r[i].unpack(v);
+        const float xs = a.col_max ? __ldg(a.xs + m) : 0.0f;
+        uint32_t rm = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            rm = max(rm, __float_as_uint(fabsf(__fmul_rn(v[j], w[j]))));
+            mx[j] = max(mx[j], __float_as_uint(fabsf(__fmul_rn(v[j], xs))));
+        }
+        if (a.row_max) {
+            rm = __reduce_max_sync(0xFFFFFFFFu, rm);
+            if (cg == 0) atomicMax(a.row_max + m, rm);
+        }
+    }
+    if (!a.col_max) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s_max[rl][cg * 8 + j] = mx[j];
+    __syncthreads();
+    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, s_max[i][threadIdx.x]);
+    if (col < a.n) atomicMax(a.col_max + col, m);
+}
+
+// Digit planes of both forms, and partial column sums of D, in one pass over D.  A block takes 128 rows
+// by 64 columns; the transposed form goes through shared memory (element (r, c) at column c ^ 4 (r / 16),
+// so that eight 16-row groups of four columns read without bank conflicts).  Every plane row is written
+// in pieces of 64 (rows) or 128 (columns) contiguous bytes.  Either form and the sums may be absent.
+struct GradDigits {
+    GradSrc g;
+    int8_t* rows;             // [P][M][W]
+    float* row_scale;         // [M]
+    int8_t* cols;             // [P][W][ldm]
+    float* col_scale;         // [W]
+    float* partial;           // [ceil(M / 128)][W]
+    int64_t ldm;
 };
 
 template <int DT, int P>
-__global__ void __launch_bounds__(256) int8_digit_rows_kernel(const DigitRows a) {
-    __shared__ uint32_t s_max[8];
-    const int tid = threadIdx.x;
-    for (int64_t m = blockIdx.x; m < a.M; m += gridDim.x) {
-        const unsigned char* row = reinterpret_cast<const unsigned char*>(a.src) + m * a.ld * dtype_bytes(DT);
+__global__ void __launch_bounds__(256) int8_grad_digits_kernel(const GradDigits a) {
+    __shared__ float tile[128 * 64];
+    const GradSrc& g = a.g;
+    const int64_t m0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 64;
+    const int seg = c0 >= g.pitch ? 1 : 0;
+    const int64_t valid = g.n - (c0 - seg * g.pitch);           // columns of this tile that hold something
+    const int ch = threadIdx.x & 7, r0 = threadIdx.x >> 3;      // eight columns of rows r0 + 32 i
+    Raw8<DT> raw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + r0 + i * 32;
+        raw[i].clear();
+        if (m < g.M && ch * 8 < valid) {
+            const unsigned char* p = reinterpret_cast<const unsigned char*>(g.src) + (m * g.ld + c0) * dtype_bytes(DT);
+            raw[i].load(p, ch * 8, valid, (reinterpret_cast<uintptr_t>(p) & 15) == 0);
+        }
+    }
+    float w[8];
+    if (a.rows) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = ch * 8 + j < valid ? __ldg(g.ws[seg] + (c0 - seg * g.pitch) + ch * 8 + j) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = r0 + i * 32;
+        const int64_t m = m0 + r;
         float v[8];
-        uint32_t mx = 0;
-        auto scaled = [&](int sg, int64_t j0, float (&o)[8]) {
-            const unsigned char* base = row + sg * a.seg_pitch * dtype_bytes(DT);
-            Raw8<DT> r;
-            r.load(base, j0, a.seg_len, (reinterpret_cast<uintptr_t>(base) & 15) == 0);
-            r.unpack(o);
-            if (a.col_scale) {
-                const float* cs = a.col_scale + sg * a.seg_pitch;
+        raw[i].unpack(v);
+        if (a.rows && m < g.M && c0 + ch * 8 < g.W) {
+            const float amax = __uint_as_float(g.row_max[m]);
+            const float s = digit_scale<P>(amax);
+            if (c0 == 0 && ch == 0) a.row_scale[m] = s;
+            const float inv = __frcp_rn(s);
+            float x[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j0 + j < a.seg_len) o[j] = __fmul_rn(o[j], __ldg(cs + j0 + j));
-            }
-        };
-        for (int sg = 0; sg < a.segs; ++sg)
-            for (int64_t j0 = (int64_t)tid * 8; j0 < a.seg_len; j0 += 2048) {
-                scaled(sg, j0, v);
+            for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(v[j], w[j]);
+            uint2 d[P];
+            digits8<P>(x, inv, d);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) mx = max(mx, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-            }
-        const float amax = __uint_as_float(row_max<256>(mx, s_max));
-        const float s = digit_scale<P>(amax, amax != amax);
-        const float inv = __frcp_rn(s);
-        if (tid == 0) a.row_scale[m] = s;
-        for (int sg = 0; sg < a.segs; ++sg) {
-            const int64_t width = sg + 1 < a.segs ? a.seg_pitch : a.ldp - sg * a.seg_pitch;
-            for (int64_t j0 = (int64_t)tid * 8; j0 < width; j0 += 2048) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-                if (j0 < a.seg_len) scaled(sg, j0, v);
-                int32_t d[P][8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    int32_t t[P];
-                    digits_of<P>(v[j], inv, t);
-#pragma unroll
-                    for (int p = 0; p < P; ++p) d[p][j] = t[p];
-                }
-#pragma unroll
-                for (int p = 0; p < P; ++p)
-                    *reinterpret_cast<uint2*>(a.planes + p * a.plane_stride + m * a.ldp + sg * a.seg_pitch + j0) =
-                        make_uint2(pack4(d[p]), pack4(d[p] + 4));
-            }
+            for (int p = 0; p < P; ++p)
+                *reinterpret_cast<uint2*>(a.rows + ((int64_t)p * g.M + m) * g.W + c0 + ch * 8) = d[p];
+        }
+        if (a.cols || a.partial) {
+            const int x = (r >> 4) << 2;
+            *reinterpret_cast<float4*>(tile + r * 64 + ((ch * 8) ^ x)) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(tile + r * 64 + ((ch * 8 + 4) ^ x)) = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
-}
-
-// Column statistics of src [M, L]: col_max[j] = bits of max_m |src[m, j] * row_scale[m]| (unsigned
-// order equals float order for non-negative floats, and NaN is above everything), and the partial
-// column sums of src itself over chunks of rows.  Both are independent of the order of execution.
-struct DigitCols {
-    const void* src;
-    const float* row_scale;   // [M]
-    uint32_t* col_max;        // [L], zeroed before
-    float* partial;           // [chunks][L] (NULL: no sums)
-    int8_t* planes;           // [P][L][ldp]
-    float* col_scale;         // [L] written by the digit pass
-    int64_t ld, M, L, ldp, plane_stride, rows_per_chunk;
-};
-
-template <int DT>
-__global__ void __launch_bounds__(256) int8_col_stats_kernel(const DigitCols a) {
-    // 32 groups of 8 columns by 8 row lanes
-    __shared__ float s_amax[8][256], s_sum[8][256];
-    const int cg = threadIdx.x & 31, rl = threadIdx.x >> 5;
-    const int64_t j0 = ((int64_t)blockIdx.x * 32 + cg) * 8;
-    const int64_t m0 = (int64_t)blockIdx.y * a.rows_per_chunk;
-    const int64_t m1 = min(a.M, m0 + a.rows_per_chunk);
-    uint32_t mx[8];
-    float sum[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { mx[j] = 0; sum[j] = 0.0f; }
-    if (j0 < a.L) {
-        for (int64_t m = m0 + rl; m < m1; m += 8) {
-            const unsigned char* row = reinterpret_cast<const unsigned char*>(a.src) + m * a.ld * dtype_bytes(DT);
-            Raw8<DT> r;
-            float v[8];
-            r.load(row, j0, a.L, (reinterpret_cast<uintptr_t>(row) & 15) == 0);
-            r.unpack(v);
-            const float rs = a.row_scale ? __ldg(a.row_scale + m) : 1.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum[j] += v[j];
-                mx[j] = max(mx[j], __float_as_uint(fabsf(__fmul_rn(v[j], rs))));
-            }
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        s_amax[rl][cg * 8 + j] = __uint_as_float(mx[j]);
-        s_sum[rl][cg * 8 + j] = sum[j];
-    }
+    if (!a.cols && !a.partial) return;
     __syncthreads();
-    const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (col >= a.L) return;
-    uint32_t m = 0;
-    float t = 0.0f;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sg = lane >> 2;                                   // rows 16 sg .. + 15
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        m = max(m, __float_as_uint(s_amax[i][threadIdx.x]));
-        t += s_sum[i][threadIdx.x];
+    for (int it = 0; it < 2; ++it) {
+        const int c = warp * 8 + it * 4 + (lane & 3);
+        float v[16];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            v[i] = tile[(sg * 16 + i) * 64 + (c ^ (sg << 2))];
+            sum += v[i];
+        }
+        if (a.partial) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            if (lane < 4 && c < valid) a.partial[(int64_t)blockIdx.y * g.W + c0 + c] = sum;
+        }
+        if (a.cols && c < valid && m0 + sg * 16 < a.ldm) {
+            const float amax = __uint_as_float(g.col_max[c0 + c]);
+            const float s = digit_scale<P>(amax);
+            if (m0 == 0 && sg == 0) a.col_scale[c0 + c] = s;
+            const float inv = __frcp_rn(s);
+            uint2 d[2][P];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t m = m0 + sg * 16 + hf * 8 + i;
+                    x[i] = m < g.M ? __fmul_rn(v[hf * 8 + i], __ldg(g.xs + m)) : 0.0f;
+                }
+                digits8<P>(x, inv, d[hf]);
+            }
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                *reinterpret_cast<uint4*>(a.cols + ((int64_t)p * g.W + c0 + c) * a.ldm + m0 + sg * 16) =
+                    make_uint4(d[0][p].x, d[0][p].y, d[1][p].x, d[1][p].y);
+        }
     }
-    if (a.col_max) atomicMax(a.col_max + col, m);
-    if (a.partial) a.partial[(int64_t)blockIdx.y * a.L + col] = t;
 }
 
 // out[j] = sum over chunks of partial[chunk][j], in the type of the bias.
-__global__ void __launch_bounds__(256) int8_col_sum_kernel(const float* partial, int64_t chunks, int64_t L, void* out,
-                                                           int dtype) {
+__global__ void __launch_bounds__(256) int8_col_sum_kernel(const float* partial, int64_t chunks, int64_t W, int64_t n,
+                                                           void* out, int dtype) {
     const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= L) return;
+    if (j >= n) return;
     double t = 0.0;
-    for (int64_t c = 0; c < chunks; ++c) t += (double)partial[c * L + j];
+    for (int64_t c = 0; c < chunks; ++c) t += (double)partial[c * W + j];
     const float f = (float)t;
     if (dtype == IMA_DTYPE_F32) reinterpret_cast<float*>(out)[j] = f;
     else if (dtype == IMA_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(out)[j] = __float2bfloat16_rn(f);
     else reinterpret_cast<__half*>(out)[j] = __float2half_rn(f);
 }
 
-// Transposed digits: planes[p][j][m] of src[m, j] * row_scale[m] against the column maximum.
-// A block turns 128 rows by 32 columns through shared memory: it reads 64 or 128 bytes of a row
-// and writes 128 bytes of a plane row at a time.
-template <int DT, int P>
-__global__ void __launch_bounds__(256) int8_digit_cols_kernel(const DigitCols a) {
-    __shared__ float tile[128][33];
-    const int64_t m0 = (int64_t)blockIdx.y * 128, j0 = (int64_t)blockIdx.x * 32;
-    for (int i = threadIdx.x; i < 128 * 32; i += 256) {
-        const int r = i >> 5, c = i & 31;
-        float v = 0.0f;
-        if (m0 + r < a.M && j0 + c < a.L) {
-            v = load_as_f32(a.src, DT, (m0 + r) * a.ld + j0 + c);
-            if (a.row_scale) v = __fmul_rn(v, __ldg(a.row_scale + m0 + r));
-        }
-        tile[r][c] = v;
-    }
-    __syncthreads();
-    const int c = threadIdx.x >> 3, r0 = (threadIdx.x & 7) * 16;
-    const int64_t j = j0 + c;
-    if (j >= a.L) return;
-    const float mx = __uint_as_float(a.col_max[j]);
-    const float s = digit_scale<P>(mx, mx != mx);
-    const float inv = __frcp_rn(s);
-    if (blockIdx.y == 0 && r0 == 0) a.col_scale[j] = s;
-    if (m0 + r0 >= a.ldp) return;   // ldp is a multiple of 16
-    uint32_t w[P][4];
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        int32_t d[P][4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            int32_t t[P];
-            digits_of<P>(tile[r0 + g * 4 + e][c], inv, t);
-#pragma unroll
-            for (int p = 0; p < P; ++p) d[p][e] = t[p];
-        }
-#pragma unroll
-        for (int p = 0; p < P; ++p) w[p][g] = pack4(d[p]);
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-        *reinterpret_cast<uint4*>(a.planes + p * a.plane_stride + j * a.ldp + m0 + r0) =
-            make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
-}
-
-// dst[c][r] = src[r][c], int8; columns rows..round16(rows) of dst are zero.
+// dst[c][r] = src[r][c], int8; columns rows..round16(rows) of dst are zero.  A block turns 128 x 128
+// bytes: 16-byte loads, 4 x 4 byte blocks turned in registers, 128 contiguous bytes out per row.
 __global__ void __launch_bounds__(256) int8_transpose_kernel(const int8_t* src, int64_t rows, int64_t cols, int64_t ld,
                                                              int8_t* dst, int64_t ldd, int vec) {
     __shared__ uint32_t tile[128][33];   // 128 rows of 128 bytes
     const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
-    for (int i = threadIdx.x; i < 128 * 32; i += 256) {
-        const int r = i >> 5, w = i & 31;
-        uint32_t v = 0;
-        if (r0 + r < rows) {
-            const int8_t* p = src + (r0 + r) * ld + c0 + w * 4;
-            if (vec && c0 + w * 4 + 4 <= cols) {
-                v = *reinterpret_cast<const uint32_t*>(p);
-            } else {
+    uint4 v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c0 + w * 4 + e < cols) v |= (uint32_t)(uint8_t)p[e] << (8 * e);
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + (threadIdx.x >> 3), b = (threadIdx.x & 7) * 16;
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (r0 + r < rows && c0 + b < cols) {
+            const int8_t* p = src + (r0 + r) * ld + c0 + b;
+            if (vec && c0 + b + 16 <= cols) {
+                v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+            } else {
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (c0 + b + e < cols) w[e >> 2] |= (uint32_t)(uint8_t)p[e] << (8 * (e & 3));
+                v[i] = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
-        tile[r][w] = v;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + (threadIdx.x >> 3), w = (threadIdx.x & 7) * 4;
+        tile[r][w] = v[i].x; tile[r][w + 1] = v[i].y; tile[r][w + 2] = v[i].z; tile[r][w + 3] = v[i].w;
     }
     __syncthreads();
-    // each thread turns 4 x 4 blocks: rows 4 rr .. + 3, columns 4 cw .. + 3
     const int64_t width = (rows + 15) / 16 * 16;
-    for (int i = threadIdx.x; i < 32 * 32; i += 256) {
-        const int rr = i & 31, cw = i >> 5;
-        if (r0 + rr * 4 >= width) continue;
+    const int rr = threadIdx.x & 31;     // rows 4 rr .. + 3: a warp writes 128 contiguous bytes
+    if (r0 + rr * 4 >= width) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int cw = i * 8 + (threadIdx.x >> 5);
         const uint32_t a = tile[rr * 4][cw], b = tile[rr * 4 + 1][cw], c = tile[rr * 4 + 2][cw], d = tile[rr * 4 + 3][cw];
         const uint32_t ab = __byte_perm(a, b, 0x5140), AB = __byte_perm(a, b, 0x7362);
         const uint32_t cd = __byte_perm(c, d, 0x5140), CD = __byte_perm(c, d, 0x7362);
@@ -462,28 +471,30 @@ int launch_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, int8_t* q,
 }
 
 template <int DT>
-int launch_digit_rows(const DigitRows& a, int planes, cudaStream_t st) {
-    const unsigned grid = (unsigned)std::min<int64_t>(a.M, 148 * 32);
-    if (planes == 2) int8_digit_rows_kernel<DT, 2><<<grid, 256, 0, st>>>(a);
-    else int8_digit_rows_kernel<DT, 3><<<grid, 256, 0, st>>>(a);
-    return IMA_LAUNCH_STATUS();
-}
-
-constexpr int64_t I8_COL_CHUNK = 256;   // rows per partial column sum
-
-template <int DT>
-int launch_col_stats(const DigitCols& a, cudaStream_t st) {
-    const dim3 grid((unsigned)((a.L + 255) / 256), (unsigned)((a.M + a.rows_per_chunk - 1) / a.rows_per_chunk));
-    int8_col_stats_kernel<DT><<<grid, 256, 0, st>>>(a);
+int launch_grad_max(const GradSrc& a, cudaStream_t st) {
+    const dim3 grid((unsigned)((a.n + 255) / 256), (unsigned)((a.M + 63) / 64));
+    int8_grad_max_kernel<DT><<<grid, 256, 0, st>>>(a);
     return IMA_LAUNCH_STATUS();
 }
 
 template <int DT>
-int launch_digit_cols(const DigitCols& a, int planes, cudaStream_t st) {
-    const dim3 grid((unsigned)((a.L + 31) / 32), (unsigned)((a.ldp + 127) / 128));
-    if (planes == 2) int8_digit_cols_kernel<DT, 2><<<grid, 256, 0, st>>>(a);
-    else int8_digit_cols_kernel<DT, 3><<<grid, 256, 0, st>>>(a);
+int launch_grad_digits(const GradDigits& a, int planes, cudaStream_t st) {
+    const dim3 grid((unsigned)((a.g.W + 63) / 64), (unsigned)((a.g.M + 127) / 128));
+    if (planes == 2) int8_grad_digits_kernel<DT, 2><<<grid, 256, 0, st>>>(a);
+    else int8_grad_digits_kernel<DT, 3><<<grid, 256, 0, st>>>(a);
     return IMA_LAUNCH_STATUS();
+}
+
+int run_grad_max(const GradSrc& a, int dtype, cudaStream_t st) {
+    if (dtype == IMA_DTYPE_BF16) return launch_grad_max<IMA_DTYPE_BF16>(a, st);
+    if (dtype == IMA_DTYPE_F16) return launch_grad_max<IMA_DTYPE_F16>(a, st);
+    return launch_grad_max<IMA_DTYPE_F32>(a, st);
+}
+
+int run_grad_digits(const GradDigits& a, int dtype, int planes, cudaStream_t st) {
+    if (dtype == IMA_DTYPE_BF16) return launch_grad_digits<IMA_DTYPE_BF16>(a, planes, st);
+    if (dtype == IMA_DTYPE_F16) return launch_grad_digits<IMA_DTYPE_F16>(a, planes, st);
+    return launch_grad_digits<IMA_DTYPE_F32>(a, planes, st);
 }
 
 }  // namespace
@@ -509,71 +520,10 @@ int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld
     if (!src || !dst || ld < cols || ldd < rows || ldd % 16 || (reinterpret_cast<uintptr_t>(dst) & 15))
         return IMA_ERR_INVALID_ARGUMENT;
     if ((rows + 127) / 128 > 65535) return IMA_ERR_UNSUPPORTED;
-    const int vec = !((reinterpret_cast<uintptr_t>(src) | (uintptr_t)ld) & 3);
+    const int vec = !((reinterpret_cast<uintptr_t>(src) | (uintptr_t)ld) & 15);
     const dim3 grid((unsigned)((cols + 127) / 128), (unsigned)((rows + 127) / 128));
     int8_transpose_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(src, rows, cols, ld, dst, ldd, vec);
     return IMA_LAUNCH_STATUS();
-}
-
-int ima_int8_digits_rows(const void* src, int src_dtype, int64_t M, int64_t seg_len, int64_t seg_pitch, int segs,
-                         int64_t ld, const float* col_scale, int planes, int8_t* out, int64_t ldp, float* row_scale,
-                         void* stream) {
-    if (M < 0 || seg_len < 0 || segs < 1 || segs > 2 || !known_dtype(src_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    if (planes != 2 && planes != 3) return IMA_ERR_UNSUPPORTED;
-    if (M == 0) return IMA_OK;
-    if (!row_scale || !out || (seg_len > 0 && !src)) return IMA_ERR_INVALID_ARGUMENT;
-    if (seg_pitch < seg_len || ldp % 16 || (segs > 1 && seg_pitch % 16)) return IMA_ERR_INVALID_ARGUMENT;
-    const int64_t width = (segs - 1) * seg_pitch + seg_len;
-    if (ldp < width || (M > 1 && ld < width) || (reinterpret_cast<uintptr_t>(out) & 15)) return IMA_ERR_INVALID_ARGUMENT;
-    const DigitRows a = {src, col_scale, out, row_scale, ld, M, seg_len, seg_pitch, ldp, M * ldp, segs, 0};
-    cudaStream_t st = (cudaStream_t)stream;
-    if (src_dtype == IMA_DTYPE_BF16) return launch_digit_rows<IMA_DTYPE_BF16>(a, planes, st);
-    if (src_dtype == IMA_DTYPE_F16) return launch_digit_rows<IMA_DTYPE_F16>(a, planes, st);
-    return launch_digit_rows<IMA_DTYPE_F32>(a, planes, st);
-}
-
-int64_t ima_int8_cols_workspace_bytes(int64_t M, int64_t L) {
-    if (M < 0 || L < 0) return 0;
-    return ((M + I8_COL_CHUNK - 1) / I8_COL_CHUNK + 1) * L * 4;
-}
-
-int ima_int8_digits_cols(const void* src, int src_dtype, int64_t M, int64_t L, int64_t ld, const float* row_scale,
-                         int planes, int8_t* out, int64_t ldp, float* col_scale, void* sum_out, int sum_dtype,
-                         void* workspace, void* stream) {
-    if (M < 0 || L < 0 || !known_dtype(src_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    if (planes != 0 && planes != 2 && planes != 3) return IMA_ERR_UNSUPPORTED;
-    if (L == 0) return IMA_OK;
-    if (!workspace || (M > 0 && (!src || (M > 1 && ld < L)))) return IMA_ERR_INVALID_ARGUMENT;
-    if (planes && (!out || !col_scale || ldp < M || ldp % 16 || (reinterpret_cast<uintptr_t>(out) & 15)))
-        return IMA_ERR_INVALID_ARGUMENT;
-    if (sum_out && !known_dtype(sum_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    if ((ldp + 127) / 128 > 65535 || (M + I8_COL_CHUNK - 1) / I8_COL_CHUNK > 65535) return IMA_ERR_UNSUPPORTED;
-    cudaStream_t st = (cudaStream_t)stream;
-    uint32_t* col_max = reinterpret_cast<uint32_t*>(workspace);
-    float* partial = reinterpret_cast<float*>(workspace) + L;
-    int rc = IMA_OK;
-    if (planes) {
-        rc = ima_note_cuda(cudaMemsetAsync(col_max, 0, (size_t)L * 4, st));
-        if (rc != IMA_OK) return rc;
-    }
-    DigitCols a = {src, row_scale, planes ? col_max : nullptr, sum_out ? partial : nullptr, out, col_scale, ld, M, L,
-                   ldp, L * ldp, I8_COL_CHUNK};
-    if (M > 0) {
-        if (src_dtype == IMA_DTYPE_BF16) rc = launch_col_stats<IMA_DTYPE_BF16>(a, st);
-        else if (src_dtype == IMA_DTYPE_F16) rc = launch_col_stats<IMA_DTYPE_F16>(a, st);
-        else rc = launch_col_stats<IMA_DTYPE_F32>(a, st);
-        if (rc != IMA_OK) return rc;
-    }
-    if (sum_out) {
-        int8_col_sum_kernel<<<(unsigned)((L + 255) / 256), 256, 0, st>>>(partial, (M + I8_COL_CHUNK - 1) / I8_COL_CHUNK,
-                                                                        L, sum_out, sum_dtype);
-        rc = IMA_LAUNCH_STATUS();
-        if (rc != IMA_OK) return rc;
-    }
-    if (!planes || M == 0) return IMA_OK;
-    if (src_dtype == IMA_DTYPE_BF16) return launch_digit_cols<IMA_DTYPE_BF16>(a, planes, st);
-    if (src_dtype == IMA_DTYPE_F16) return launch_digit_cols<IMA_DTYPE_F16>(a, planes, st);
-    return launch_digit_cols<IMA_DTYPE_F32>(a, planes, st);
 }
 
 }  // extern "C"

@@ -36,7 +36,8 @@ struct __align__(64) SkParams {
     const float* xs;               // [M] token scales (not fused)
     const float* ws[2];            // [N] channel scales
     const void* bias[2];
-    int64_t ldx, ldc, ldy, K;
+    void* y2;                      // I8_DIGIT: rows from split_row on, seg_rows of each part (NULL: all to y)
+    int64_t ldx, ldc, ldy, K, split_row, seg_rows;
     int32_t M, N, tm, k_steps, seg_steps, splits, stages, codes_bytes, partial_bytes, tmem_cols;
     int32_t y_dtype, bias_dtype, act, vec_c, vec_y, dependent;
     uint64_t stall_ns;             // test knob (ima_set_gemm_wait_test); 0 in normal use
@@ -275,6 +276,10 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
             __syncwarp();
             if (lane == 0) mbar_arrive(&tok_ready);
         }
+        if (!FUSED) {   // the token scales
+            if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (int t = threadIdx.x - 64; t < rows; t += SK_WORKERS * 32) s_scale[t] = p.xs ? p.xs[m0 + t] : 0.0f;
+        }
         // push the partial sums to the owners: TMEM lane = weight row, column = (operand, plane, token)
         const bool ok = mbar_wait_or_abort(&acc_full, 0u, &abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_SKINNY, 200);
         __syncwarp();
@@ -308,26 +313,40 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
         __syncthreads();
     }
 
-    // ---- phase 3: the outputs this CTA owns, four consecutive columns at a time ----
-    if (!abort_flag) {
-        if (!FUSED && p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");   // the token scales
+    // ---- phase 3: the outputs this CTA owns; a thread keeps its four columns and walks the tokens ----
+    if (!abort_flag && threadIdx.x < 256) {
         const int own = SK_ROWS / S, per = own / 4;
-        for (int i = threadIdx.x; i < rows * per; i += SK_THREADS) {
-            const int t = i / per, j = (i % per) * 4;
-            const int32_t n = n0 + (int32_t)rank * own + j;
-            if (n >= p.N) continue;
-            const int valid = min(4, p.N - n);
-            const int64_t m = m0 + t;
-            auto gather = [&](int col) {   // sum over the cluster of 4 partial sums of one column
-                int4 a = make_int4(0, 0, 0, 0);
-                for (int r = 0; r < S; ++r) {
-                    const int4 b = *reinterpret_cast<const int4*>(part + (r * OPS * P * p.tm + col) * own + j);
-                    a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-                }
-                return a;
-            };
+        const int j = (threadIdx.x % per) * 4;
+        const int32_t n = n0 + (int32_t)rank * own + j;
+        const int valid = min(4, p.N - n);
+        float ws[OPS][4], bias[OPS][4];
+#pragma unroll
+        for (int o = 0; o < OPS; ++o)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? __ldg(p.ws[o] + n + e) : 0.0f;
+                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, n + e) : 0.0f;
+            }
+        auto gather = [&](int col) {   // sum over the cluster of 4 partial sums of one column
+            int4 a = make_int4(0, 0, 0, 0);
+            for (int r = 0; r < S; ++r) {
+                const int4 b = *reinterpret_cast<const int4*>(part + (r * OPS * P * p.tm + col) * own + j);
+                a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+            }
+            return a;
+        };
+#pragma unroll 2
+        for (int t = threadIdx.x / per; t < rows && valid > 0; t += 256 / per) {
+            int64_t m = m0 + t;
+            const float xs = s_scale[t];
             float v[4];
+            void* y = p.y;
             if constexpr (EPI == I8_DIGIT) {
+                if (p.y2) {
+                    const bool second = m >= p.split_row;
+                    if (second) { m -= p.split_row; y = p.y2; }
+                    if (m >= p.seg_rows) continue;
+                }
                 int64_t s[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < P; ++d) {
@@ -337,11 +356,9 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
                     s[2] += (int64_t)a.z << (8 * d);
                     s[3] += (int64_t)a.w << (8 * d);
                 }
-                const float xs = p.xs[m];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__ll2float_rn(s[e]), xs);
             } else {
-                const float xs = FUSED ? s_scale[t] : (p.xs ? p.xs[m] : 0.0f);
                 const int4 a = gather(t);
                 const int32_t av[4] = {a.x, a.y, a.z, a.w};
                 if constexpr (EPI == I8_GATED) {
@@ -349,12 +366,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
                     const int32_t bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[e] = 0.0f;
-                        if (e >= valid) continue;
-                        const float gb = p.bias[0] ? load_as_f32(p.bias[0], p.bias_dtype, n + e) : 0.0f;
-                        const float ub = p.bias[1] ? load_as_f32(p.bias[1], p.bias_dtype, n + e) : 0.0f;
-                        const float g = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(av[e]), xs), p.ws[0][n + e]), gb);
-                        const float u = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(bv[e]), xs), p.ws[1][n + e]), ub);
+                        const float g = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(av[e]), xs), ws[0][e]), bias[0][e]);
+                        const float u = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(bv[e]), xs), ws[OPS - 1][e]), bias[OPS - 1][e]);
                         v[e] = gated_value(p.act, g, u);
                     }
                 } else {
@@ -367,14 +380,12 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
                     if (!p.y) continue;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[e] = 0.0f;
-                        if (e >= valid) continue;
-                        v[e] = __fmul_rn(__fmul_rn(__int2float_rn(av[e]), xs), p.ws[0][n + e]);
-                        if (p.bias[0]) v[e] = __fadd_rn(v[e], load_as_f32(p.bias[0], p.bias_dtype, n + e));
+                        v[e] = __fmul_rn(__fmul_rn(__int2float_rn(av[e]), xs), ws[0][e]);
+                        if (p.bias[0]) v[e] = __fadd_rn(v[e], bias[0][e]);
                     }
                 }
             }
-            store_quad(p.y, p.y_dtype, m * p.ldy + n, v, valid, p.vec_y);
+            store_quad(y, p.y_dtype, m * p.ldy + n, v, valid, p.vec_y);
         }
     }
     if (warp == 1) {
@@ -432,7 +443,8 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, bool 
 template <int EPI, int P, int DT>
 int launch_skinny(SkParams& p, const SkPlan& q, cudaStream_t stream) {
     auto kern = int8_skinny_kernel<EPI, P, DT>;
-    int rc = ima_note_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_SMEM));
+    static std::atomic<uint64_t> ready{0};
+    const int rc = set_smem_once(ready, (const void*)kern, SK_SMEM);
     if (rc != IMA_OK) return rc;
     p.tm = q.tm;
     p.k_steps = q.k_steps;
@@ -470,8 +482,8 @@ int launch_skinny(SkParams& p, const SkPlan& q, cudaStream_t stream) {
 // Weight maps of the split form: o.b (and o.b2) in boxes of a tile's rows.
 int sk_weight_maps(SkParams& p, const I8Operands& o) {
     if (o.K == 0) return IMA_OK;
-    int rc = make_i8_map(&p.mw, o.b, o.K, o.ldb, p.N, 1, SK_ROWS, false);
-    if (rc == IMA_OK && o.b2) rc = make_i8_map(&p.mw2, o.b2, o.K, o.ldb2, p.N, 1, SK_ROWS, false);
+    int rc = make_i8_map(&p.mw, o.b, o.K, o.ldb, p.N, 1, 0, SK_ROWS);
+    if (rc == IMA_OK && o.b2) rc = make_i8_map(&p.mw2, o.b2, o.K, o.ldb2, p.N, 1, 0, SK_ROWS);
     return rc;
 }
 
@@ -481,11 +493,12 @@ int run_skinny_codes(const I8Params& g, const I8Operands& o, const SkPlan& q, cu
     SkParams p;
     memset(&p, 0, sizeof(p));
     p.c = g.c; p.y = g.y; p.xs = g.xs; p.ws[0] = g.ws[0]; p.ws[1] = g.ws[1]; p.bias[0] = g.bias[0]; p.bias[1] = g.bias[1];
+    p.y2 = g.y2; p.split_row = g.split_row; p.seg_rows = g.seg_rows;
     p.ldc = g.ldc; p.ldy = g.ldy; p.M = g.M; p.N = g.N; p.K = o.K; p.y_dtype = g.y_dtype; p.bias_dtype = g.bias_dtype;
     p.act = g.act; p.vec_c = g.vec_c; p.vec_y = g.vec_y; p.dependent = g.dependent;
     p.seg_steps = g.seg_tiles;
     int rc = sk_weight_maps(p, o);
-    if (rc == IMA_OK && o.K > 0) rc = make_i8_map(&p.mt, o.a, o.Ka, o.lda, p.M, P, q.tm, true);
+    if (rc == IMA_OK && o.K > 0) rc = make_i8_map(&p.mt, o.a, o.Ka, o.lda, p.M, P, o.a_planes, q.tm);
     if (rc != IMA_OK) return rc;
     return launch_skinny<EPI, P, -1>(p, q, stream);
 }

@@ -43,15 +43,23 @@ ACTIVATIONS = {"silu": nat.IMA_ACT_SILU, "gelu": nat.IMA_ACT_GELU, "gelu_tanh": 
 _DTYPE_CODES = {torch.float32: nat.IMA_DTYPE_F32, torch.bfloat16: nat.IMA_DTYPE_BF16, torch.float16: nat.IMA_DTYPE_F16}
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(dev: torch.device, fn: str, *args) -> None:
     """A C entry whose last argument is the stream, on `dev` and its current stream."""
     if torch.cuda.current_device() == dev.index:
-        status = getattr(nat.lib(), fn)(*args, torch.cuda.current_stream(dev).cuda_stream)
+        status = getattr(nat.lib(), fn)(*args, _raw_stream(dev.index))
     else:
         with torch.cuda.device(dev):
-            status = getattr(nat.lib(), fn)(*args, torch.cuda.current_stream(dev).cuda_stream)
+            status = getattr(nat.lib(), fn)(*args, _raw_stream(dev.index))
     if status:
         raise nat.NativeError(fn, status)
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _round_up(v: int, to: int) -> int:
@@ -148,6 +156,7 @@ class Int8Weight:
         self.codes = _aligned_codes(codes.detach(), "int8 weight")
         nat.require_device(codes.device, ("weight scale", scale))
         self.scale = _scales(scale, codes.shape[0], "weight scale")
+        self.shape, self.device, self.ld = self.codes.shape, self.codes.device, _code_ld(self.codes)
         self._transposed: tuple | None = None
 
     @classmethod
@@ -157,14 +166,6 @@ class Int8Weight:
             raise RuntimeError(f"int8 weight source must be 2-D, got {tuple(weight.shape)}")
         _require_cuda(weight, "int8 weight source")
         return cls(*per_token_int8(weight))
-
-    @property
-    def shape(self) -> torch.Size:
-        return self.codes.shape
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
 
     def transposed(self) -> torch.Tensor:
         version = nat.tensor_version(self.codes)
@@ -185,25 +186,23 @@ def _check_out(t: torch.Tensor, shape: tuple[int, int], dtypes: tuple, label: st
         raise RuntimeError(f"{label} must have contiguous rows that do not overlap")
 
 
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
-
-
 def _bias_args(n: int, *biases: torch.Tensor | None) -> tuple[list[torch.Tensor | None], int]:
     """Biases as contiguous vectors of one floating type, and that type's code."""
-    given = [b for b in biases if b is not None]
-    if not given:
+    dtype = None
+    for b in biases:
+        if b is not None:
+            dtype = b.dtype if dtype in (None, b.dtype) and b.dtype in _DTYPE_CODES else torch.float32
+    if dtype is None:
         return list(biases), 0
-    dtype = given[0].dtype if all(b.dtype == given[0].dtype for b in given) else torch.float32
-    if dtype not in _FLOATS:
-        dtype = torch.float32
     out = []
     for b in biases:
         if b is not None:
-            b = b.detach().reshape(-1).to(dtype).contiguous()
-            if b.numel() != n:
+            if b.ndim != 1 or b.dtype != dtype or not b.is_contiguous():
+                b = b.detach().reshape(-1).to(dtype).contiguous()
+            if b.shape[0] != n:
                 raise RuntimeError(f"bias has {b.numel()} entries, expected {n}")
         out.append(b)
-    return out, nat.dtype_code(dtype)
+    return out, _DTYPE_CODES[dtype]
 
 
 def int8_gemm(
@@ -237,7 +236,7 @@ def int8_gemm(
         if x_scale is None or w_scale is None:
             raise RuntimeError("int8_gemm needs x_scale and w_scale for the rescaled output")
         y = y_out if y_out is not None else torch.empty((m, n), dtype=y_dtype, device=dev)
-        _check_out(y, (m, n), _FLOATS, "output")
+        _check_out(y, (m, n), tuple(_DTYPE_CODES), "output")
         nat.require_device(dev, ("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias))
         x_scale = _scales(x_scale, m, "x_scale")
         w_scale = _scales(w_scale, n, "w_scale")
@@ -247,50 +246,44 @@ def int8_gemm(
     if c is None and y is None:
         raise RuntimeError("int8_gemm has no output to compute: want_c, y_dtype or y_out")
     nat.require_device(dev, ("B matrix", b), ("int32 output", c), ("output", y))
-    _call(dev, "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, nat.ptr(c),
-          _ld(c) if c is not None else n, nat.ptr(x_scale), nat.ptr(w_scale), nat.ptr(bias), bias_dtype, nat.ptr(y),
+    _call(dev, "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, _ptr(c),
+          _ld(c) if c is not None else n, _ptr(x_scale), _ptr(w_scale), _ptr(bias), bias_dtype, _ptr(y),
           nat.dtype_code(y.dtype) if y is not None else 0, _ld(y) if y is not None else n)
     return c, y
+
+
+def _code_buffers(rows: torch.Tensor, n: int, gated: bool, keep: bool):
+    """Room for the codes and scales of x rows (None, None when the product quantises them itself)."""
+    m, k = rows.shape
+    if not keep and nat.lib().ima_int8_fused(m, n, k, gated):
+        return None, None
+    return (rows.new_empty((m, _round_up(max(k, 1), 16)), dtype=torch.int8),
+            rows.new_empty((m,), dtype=torch.float32))
 
 
 def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None, keep: bool = False):
     """(y [M, N], codes, scale) of x rows; codes and scale hold something only with keep."""
     m, k = rows.shape
     n = weight.shape[0]
-    dev = rows.device
-    y = torch.empty((m, n), dtype=rows.dtype, device=dev)
-    ld = _round_up(max(k, 1), 16)
-    q = torch.empty((m, ld), dtype=torch.int8, device=dev)
-    scale = torch.empty((m,), dtype=torch.float32, device=dev)
+    y = rows.new_empty((m, n))
+    q, scale = _code_buffers(rows, n, False, keep)
     (bias,), bias_dtype = _bias_args(n, bias)
-    codes = weight.codes
-    _call(dev, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q.data_ptr(), ld,
-          scale.data_ptr(), keep, codes.data_ptr(), _code_ld(codes), n, weight.scale.data_ptr(), nat.ptr(bias),
-          bias_dtype, y.data_ptr(), max(n, 1))
+    _call(rows.device, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), _ptr(q),
+          _round_up(max(k, 1), 16), _ptr(scale), keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(),
+          _ptr(bias), bias_dtype, y.data_ptr(), max(n, 1))
     return y, q[:, :k] if keep else None, scale
-
-
-def _gated_args(q: torch.Tensor, scale: torch.Tensor, gate: Int8Weight, up: Int8Weight, biases, bias_dtype: int,
-                activation: str) -> tuple:
-    m, k = q.shape
-    return (q.data_ptr(), _code_ld(q), gate.codes.data_ptr(), _code_ld(gate.codes), up.codes.data_ptr(),
-            _code_ld(up.codes), m, gate.shape[0], k, scale.data_ptr(), gate.scale.data_ptr(), up.scale.data_ptr(),
-            nat.ptr(biases[0]), nat.ptr(biases[1]), bias_dtype, ACTIVATIONS[activation])
 
 
 def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bias, up_bias, activation: str,
                    keep: bool = False):
     m, k = rows.shape
     n = gate.shape[0]
-    dev = rows.device
-    h = torch.empty((m, n), dtype=rows.dtype, device=dev)
-    ld = _round_up(max(k, 1), 16)
-    q = torch.empty((m, ld), dtype=torch.int8, device=dev)
-    scale = torch.empty((m,), dtype=torch.float32, device=dev)
+    h = rows.new_empty((m, n))
+    q, scale = _code_buffers(rows, n, True, keep)
     (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(dev, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q.data_ptr(), ld,
-          scale.data_ptr(), keep, gate.codes.data_ptr(), _code_ld(gate.codes), up.codes.data_ptr(), _code_ld(up.codes),
-          n, gate.scale.data_ptr(), up.scale.data_ptr(), nat.ptr(gate_bias), nat.ptr(up_bias), bias_dtype,
+    _call(rows.device, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), _ptr(q),
+          _round_up(max(k, 1), 16), _ptr(scale), keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n,
+          gate.scale.data_ptr(), up.scale.data_ptr(), _ptr(gate_bias), _ptr(up_bias), bias_dtype,
           ACTIVATIONS[activation], h.data_ptr(), max(n, 1))
     return h, q[:, :k] if keep else None, scale
 
@@ -298,48 +291,11 @@ def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bi
 # ---------------------------------------------------------------------------
 # gradients
 # ---------------------------------------------------------------------------
-def _digit_count(*dtypes: torch.dtype) -> int:
+def _digit_count(*dtypes: torch.dtype | None) -> int:
     """Digits of a gradient: two reach 2^-16 of its row maximum, three 2^-24.  Over rows whose elements
     differ a lot (a column of token gradients) two are off by up to 6e-4 of the result's norm: below
     bf16's own rounding (2e-3), above fp16's (2e-4)."""
     return 2 if all(t in (None, torch.bfloat16) for t in dtypes) else 3
-
-
-def _digits_rows(src: torch.Tensor, seg_len: int, seg_pitch: int, segs: int, col_scale: torch.Tensor, planes: int):
-    m = src.shape[0]
-    dev = src.device
-    width = _round_up(max((segs - 1) * seg_pitch + seg_len, 1), 16)
-    out = torch.empty((planes, m, width), dtype=torch.int8, device=dev)
-    scale = torch.empty((m,), dtype=torch.float32, device=dev)
-    _call(dev, "ima_int8_digits_rows", src.data_ptr(), nat.dtype_code(src.dtype), m, seg_len, seg_pitch, segs, _ld(src),
-          col_scale.data_ptr(), planes, out.data_ptr(), width, scale.data_ptr())
-    return out, scale
-
-
-def _digits_cols(src: torch.Tensor, row_scale: torch.Tensor, planes: int, sum_dtype: torch.dtype | None):
-    """Transposed digits of src [M, L] (planes == 0: none) and its column sums (sum_dtype None: none)."""
-    m, length = src.shape
-    dev = src.device
-    width = _round_up(max(m, 1), 16)
-    out = torch.empty((planes, length, width), dtype=torch.int8, device=dev) if planes else None
-    scale = torch.empty((length,), dtype=torch.float32, device=dev) if planes else None
-    sums = torch.empty((length,), dtype=sum_dtype, device=dev) if sum_dtype is not None else None
-    ws = torch.empty((int(nat.lib().ima_int8_cols_workspace_bytes(m, length)),), dtype=torch.uint8, device=dev)
-    _call(dev, "ima_int8_digits_cols", src.data_ptr(), nat.dtype_code(src.dtype), m, length, _ld(src),
-          row_scale.data_ptr(), planes, nat.ptr(out), width, nat.ptr(scale), nat.ptr(sums),
-          nat.dtype_code(sum_dtype) if sums is not None else 0, ws.data_ptr())
-    return out, scale, sums
-
-
-def _digit_gemm(planes: torch.Tensor, row_scale: torch.Tensor, b: torch.Tensor, b2: torch.Tensor | None, m: int,
-                k: int, dtype: torch.dtype) -> torch.Tensor:
-    n = b.shape[0]
-    dev = planes.device
-    y = torch.empty((m, n), dtype=dtype, device=dev)
-    _call(dev, "ima_int8_digit_gemm", planes.data_ptr(), planes.shape[0], planes.shape[2], row_scale.data_ptr(),
-          b.data_ptr(), _code_ld(b), nat.ptr(b2), _code_ld(b2) if b2 is not None else 0, m, n, k, y.data_ptr(),
-          nat.dtype_code(dtype), max(n, 1))
-    return y
 
 
 def _check_backward(m: int, contraction: int, want_dw: bool) -> None:
@@ -352,27 +308,24 @@ def _check_backward(m: int, contraction: int, want_dw: bool) -> None:
 def _grad_rows(grad: torch.Tensor, m: int, n: int, dev: torch.device) -> torch.Tensor:
     if grad.shape[-1] != n or grad.numel() != m * n:
         raise RuntimeError(f"output gradient has shape {tuple(grad.shape)}, expected {m} rows of {n}")
-    nat.require_device(dev, ("output gradient", grad))
+    if grad.device != dev:
+        nat.require_device(dev, ("output gradient", grad))
     nat.dtype_code(grad.dtype)
     return _rows(grad.detach().reshape(m, n))
 
 
-def _weight_gradient(d: torch.Tensor, codes_t: torch.Tensor | None, scale: torch.Tensor, g_dtype: torch.dtype,
-                     w_dtype: torch.dtype | None, b_dtype: torch.dtype | None):
-    """(dW, db) of one projection from its output gradient d [M, N]; g_dtype: the type d came from."""
-    want_dw = w_dtype is not None
-    if not want_dw and b_dtype is None:
-        return None, None
-    m, n = d.shape
-    planes = _digit_count(g_dtype, w_dtype) if want_dw else 0
-    digits, digit_scale, db = _digits_cols(d, scale, planes, b_dtype)
-    dw = None
-    if want_dw:
-        if m == 0:
-            dw = torch.zeros((n, codes_t.shape[0]), dtype=w_dtype, device=d.device)
-        else:
-            dw = _digit_gemm(digits, digit_scale, codes_t, None, n, m, w_dtype)
-    return dw, db
+def _one_type(*dtypes: torch.dtype | None) -> torch.dtype | None:
+    """The type of gradients that come out together: theirs if they agree, else fp32."""
+    given = {t for t in dtypes if t is not None}
+    return None if not given else given.pop() if len(given) == 1 else torch.float32
+
+
+def _out(like: torch.Tensor, shape: tuple, dtype: torch.dtype | None, wanted: bool = True) -> torch.Tensor | None:
+    return like.new_empty(shape, dtype=dtype) if wanted and dtype is not None else None
+
+
+def _code(t: torch.Tensor | None) -> int:
+    return 0 if t is None else _DTYPE_CODES[t.dtype]
 
 
 def int8_linear_backward(
@@ -384,26 +337,32 @@ def int8_linear_backward(
     dx_dtype: torch.dtype | None = None,
     dw_dtype: torch.dtype | None = None,
     db_dtype: torch.dtype | None = None,
+    keep_transposed: bool = True,
 ):
     """Gradients of int8_linear as (dx [M, K], dw [N, K], db [N]); None where no type is given.
 
-    grad: output gradient [..., N]; codes, scale: per_token_int8 of the activations.  Launches only,
-    on the current stream."""
+    grad: output gradient [..., N]; codes, scale: per_token_int8 of the activations.  keep_transposed:
+    the transposed weight that dx needs stays with `weight` for the next call (one more byte per
+    weight), else it is temporary.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
-    m, n = codes.shape[0], weight.shape[0]
+    (m, k), n = codes.shape, weight.shape[0]
     dev = codes.device
-    if weight.shape[1] != codes.shape[1]:
-        raise RuntimeError(f"int8 matmul shape mismatch: K={codes.shape[1]} vs K={weight.shape[1]}")
+    if weight.shape[1] != k:
+        raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={weight.shape[1]}")
     nat.require_device(dev, ("weight", weight.codes), ("scale", scale))
     scale = _scales(scale, m, "scale")
     d = _grad_rows(grad, m, n, dev)
     _check_backward(m, n if dx_dtype is not None else 0, dw_dtype is not None)
-    dx = None
-    if dx_dtype is not None:
-        digits, digit_scale = _digits_rows(d, n, n, 1, weight.scale, _digit_count(d.dtype, dx_dtype))
-        dx = _digit_gemm(digits, digit_scale, weight.transposed(), None, m, n, dx_dtype)
-    codes_t = _transpose(codes) if dw_dtype is not None else None
-    dw, db = _weight_gradient(d, codes_t, scale, d.dtype, dw_dtype, db_dtype)
+    planes = _digit_count(d.dtype, dx_dtype, dw_dtype)
+    dx, dw, db = _out(scale, (m, k), dx_dtype), _out(scale, (n, k), dw_dtype), _out(scale, (n,), db_dtype)
+    wt = weight.transposed() if dx is not None and keep_transposed else None
+    nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 0, planes, dx is not None, dw is not None,
+                                                         db is not None, wt is None)
+    ws = scale.new_empty((nbytes,), dtype=torch.uint8)
+    _call(dev, "ima_int8_linear_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, codes.data_ptr(),
+          _code_ld(codes), scale.data_ptr(), weight.codes.data_ptr(), weight.ld, _ptr(wt),
+          _code_ld(wt) if wt is not None else 0, weight.scale.data_ptr(), planes, _ptr(dx), _code(dx), _ptr(dw),
+          _code(dw), _ptr(db), _code(db), ws.data_ptr())
     return dx, dw, db
 
 
@@ -422,41 +381,44 @@ def int8_gated_backward(
     dup_dtype: torch.dtype | None = None,
     gate_db_dtype: torch.dtype | None = None,
     up_db_dtype: torch.dtype | None = None,
+    keep_transposed: bool = True,
 ):
     """Gradients of int8_gated as (dx, dgate, dup, dgate_bias, dup_bias); None where no type is given.
 
-    grad: gradient of h [..., N]; codes, scale: per_token_int8 of the activations.  Both projections
-    are formed again from the codes, so a forward pass keeps one byte per activation and nothing
-    of width N.  Launches only, on the current stream."""
+    grad: gradient of h [..., N]; codes, scale: per_token_int8 of the activations; keep_transposed as in
+    int8_linear_backward.  Both projections are formed again from the codes, so a forward pass keeps
+    one byte per activation and nothing of width N.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
-    m, k = codes.shape
-    n = gate.shape[0]
+    (m, k), n = codes.shape, gate.shape[0]
     dev = codes.device
     _check_gated(k, gate, up, activation)
     nat.require_device(dev, ("gate weight", gate.codes), ("up weight", up.codes), ("scale", scale),
                        ("gate bias", gate_bias), ("up bias", up_bias))
     scale = _scales(scale, m, "scale")
-    dh = _grad_rows(grad, m, n, dev)
-    pitch = _round_up(max(n, 1), 128)
+    d = _grad_rows(grad, m, n, dev)
     want_dw = dgate_dtype is not None or dup_dtype is not None
-    _check_backward(m, pitch + n if dx_dtype is not None else 0, want_dw)
-    # one tensor for the gradients of both projections, fp32: their digits are taken against row
-    # and column maxima that are known only once it is complete
-    d = torch.empty((m, 2 * pitch), dtype=torch.float32, device=dev)
-    biases, bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(dev, "ima_int8_gated_backward_gemm", *_gated_args(codes, scale, gate, up, biases, bias_dtype, activation),
-          dh.data_ptr(), nat.dtype_code(dh.dtype), _ld(dh), d.data_ptr(), 2 * pitch, pitch)
-    dx = None
-    if dx_dtype is not None:
-        channel = torch.zeros((2, pitch), dtype=torch.float32, device=dev)
-        channel[0, :n] = gate.scale
-        channel[1, :n] = up.scale
-        digits, digit_scale = _digits_rows(d, n, pitch, 2, channel, _digit_count(dh.dtype, dx_dtype))
-        dx = _digit_gemm(digits, digit_scale, gate.transposed(), up.transposed(), m, n, dx_dtype)
-    codes_t = _transpose(codes) if want_dw else None
-    dg, dgb = _weight_gradient(d[:, :n], codes_t, scale, dh.dtype, dgate_dtype, gate_db_dtype)
-    du, dub = _weight_gradient(d[:, pitch:pitch + n], codes_t, scale, dh.dtype, dup_dtype, up_db_dtype)
-    return dx, dg, du, dgb, dub
+    _check_backward(m, _round_up(n, 128) + n if dx_dtype is not None else 0, want_dw)
+    planes = _digit_count(d.dtype, dx_dtype, dgate_dtype, dup_dtype)
+    w_type, b_type = _one_type(dgate_dtype, dup_dtype), _one_type(gate_db_dtype, up_db_dtype)
+    dx = _out(scale, (m, k), dx_dtype)
+    dgate, dup = _out(scale, (n, k), w_type, dgate_dtype is not None), _out(scale, (n, k), w_type, dup_dtype is not None)
+    dgb, dub = _out(scale, (n,), b_type, gate_db_dtype is not None), _out(scale, (n,), b_type, up_db_dtype is not None)
+    gt = ut = None
+    if dx is not None and keep_transposed:
+        gt, ut = gate.transposed(), up.transposed()
+    nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 1, planes, dx is not None, want_dw, b_type is not None,
+                                                         gt is None)
+    ws = scale.new_empty((nbytes,), dtype=torch.uint8)
+    (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
+    _call(dev, "ima_int8_gated_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, codes.data_ptr(),
+          _code_ld(codes), scale.data_ptr(), gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(),
+          up.ld, _ptr(gt), _code_ld(gt) if gt is not None else 0, _ptr(ut),
+          _code_ld(ut) if ut is not None else 0, gate.scale.data_ptr(), up.scale.data_ptr(), _ptr(gate_bias),
+          _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], planes, _ptr(dx), _code(dx), _ptr(dgate), _ptr(dup),
+          _code(dgate if dgate is not None else dup), _ptr(dgb), _ptr(dub), _code(dgb if dgb is not None else dub),
+          ws.data_ptr())
+    outs = zip((dx, dgate, dup, dgb, dub), (dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype))
+    return tuple(None if t is None else t.to(dtype) for t, dtype in outs)
 
 
 # ---------------------------------------------------------------------------
@@ -485,7 +447,7 @@ class _LinearFunction(torch.autograd.Function):
         w = handle if handle is not None else Int8Weight.from_float(weight)
         y, q, scale = _linear_forward(_rows(x.detach()), w, bias, keep=True)
         ctx.save_for_backward(q, scale)
-        ctx.weight = w
+        ctx.weight, ctx.frozen = w, handle is not None
         ctx.types = tuple(t.dtype if t is not None and need else None
                           for t, need in zip((x, weight, bias), ctx.needs_input_grad))
         ctx.shapes = (x.shape, None if bias is None else bias.shape)
@@ -496,7 +458,7 @@ class _LinearFunction(torch.autograd.Function):
     def backward(ctx, grad):
         q, scale = ctx.saved_tensors
         dx, dw, db = int8_linear_backward(grad, q, scale, ctx.weight, dx_dtype=ctx.types[0], dw_dtype=ctx.types[1],
-                                          db_dtype=ctx.types[2])
+                                          db_dtype=ctx.types[2], keep_transposed=ctx.frozen)
         return (None if dx is None else dx.reshape(ctx.shapes[0]), dw, None if db is None else db.reshape(ctx.shapes[1]),
                 None)
 
@@ -509,6 +471,7 @@ class _GatedFunction(torch.autograd.Function):
         h, q, scale = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation, keep=True)
         ctx.save_for_backward(q, scale, gate_bias, up_bias)
         ctx.gate, ctx.up, ctx.activation = g, u, activation
+        ctx.frozen = gate is not None and up is not None
         inputs = (x, gate_weight, up_weight, gate_bias, up_bias)
         ctx.types = tuple(t.dtype if t is not None and need else None for t, need in zip(inputs, ctx.needs_input_grad))
         ctx.shapes = tuple(None if t is None else t.shape for t in inputs)
@@ -520,22 +483,31 @@ class _GatedFunction(torch.autograd.Function):
         q, scale, gate_bias, up_bias = ctx.saved_tensors
         tx, tg, tu, tgb, tub = ctx.types
         grads = int8_gated_backward(grad, q, scale, ctx.gate, ctx.up, gate_bias, up_bias, activation=ctx.activation,
-                                    dx_dtype=tx, dgate_dtype=tg, dup_dtype=tu, gate_db_dtype=tgb, up_db_dtype=tub)
+                                    dx_dtype=tx, dgate_dtype=tg, dup_dtype=tu, gate_db_dtype=tgb, up_db_dtype=tub,
+                                    keep_transposed=ctx.frozen)
         return (*(None if g is None else g.reshape(shape) for g, shape in zip(grads, ctx.shapes)), None, None, None)
 
 
-def _check_linear_inputs(x: torch.Tensor, *named) -> None:
-    _require_cuda(x, "int8 input")
+def _check_inputs(x: torch.Tensor, *named) -> None:
+    if not x.is_cuda:
+        _require_cuda(x, "int8 input")
     if x.ndim < 1:
         raise RuntimeError("int8 input must have at least one dimension")
-    nat.dtype_code(x.dtype)
+    if x.dtype not in _DTYPE_CODES:
+        nat.dtype_code(x.dtype)
+    dev = x.device
     for label, t in named:
-        if isinstance(t, torch.Tensor):
-            nat.require_device(x.device, (label, t))
-            nat.dtype_code(t.dtype)
-        elif isinstance(t, Int8Weight):
-            nat.require_device(x.device, (label, t.codes))
-        elif t is not None:
+        if t is None:
+            continue
+        if type(t) is Int8Weight:
+            if t.device != dev:
+                nat.require_device(dev, (label, t.codes))
+        elif isinstance(t, torch.Tensor):
+            if t.device != dev:
+                nat.require_device(dev, (label, t))
+            if t.dtype not in _DTYPE_CODES:
+                nat.dtype_code(t.dtype)
+        else:
             raise RuntimeError(f"{label} must be a tensor or an Int8Weight, got {type(t).__name__}")
 
 
@@ -544,7 +516,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
 
     weight: an Int8Weight (frozen) or a floating tensor, quantised in the call and differentiable.
     """
-    _check_linear_inputs(x, ("weight", weight), ("bias", bias))
+    _check_inputs(x, ("weight", weight), ("bias", bias))
     if weight.shape[-1] != x.shape[-1]:
         raise RuntimeError(f"int8 matmul shape mismatch: K={x.shape[-1]} vs K={weight.shape[-1]}")
     if _wants_grad(x, weight, bias):
@@ -553,8 +525,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
                         not frozen and weight.requires_grad)
         return _LinearFunction.apply(x, None if frozen else weight, bias, weight if frozen else None)
     w = _weight_of(weight)
-    y, _q, _s = _linear_forward(_rows(x.detach()), w, bias)
-    return y.reshape(*x.shape[:-1], w.shape[0])
+    y, _q, _s = _linear_forward(_rows(x), w, bias)
+    return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 
 def int8_gated(
@@ -570,7 +542,7 @@ def int8_gated(
 
     Both projections, the activation ("silu", "gelu" with the error function, or "gelu_tanh") and the
     product run in one kernel; g and u never reach memory.  Weights as in int8_linear."""
-    _check_linear_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
+    _check_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
     _check_gated(x.shape[-1], gate, up, activation)
     if _wants_grad(x, gate, up, gate_bias, up_bias):
         frozen = [isinstance(w, Int8Weight) for w in (gate, up)]
@@ -580,5 +552,5 @@ def int8_gated(
         return _GatedFunction.apply(x, None if frozen[0] else gate, None if frozen[1] else up, gate_bias, up_bias,
                                     gate if frozen[0] else None, up if frozen[1] else None, activation)
     g, u = _weight_of(gate), _weight_of(up)
-    h, _q, _s = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation)
-    return h.reshape(*x.shape[:-1], g.shape[0])
+    h, _q, _s = _gated_forward(_rows(x), g, u, gate_bias, up_bias, activation)
+    return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])

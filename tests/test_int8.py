@@ -135,10 +135,15 @@ def test_c_entries_refuse_bad_arguments_before_any_launch():
     assert lib.ima_int8_gemm(24, 32, 16, 32, 2, 2, 32, 16, 2, None, None, None, 0, None, 0, 2, None) == bad
     assert lib.ima_int8_gemm(16, 24, 16, 32, 2, 2, 24, 16, 2, None, None, None, 0, None, 0, 2, None) == bad
     assert lib.ima_int8_gemm(16, 32, 16, 32, 2, 2, 32, 16, 1, None, None, None, 0, None, 0, 2, None) == bad
-    # gated: unknown activation; digits: only 2 or 3 planes
+    # gated: unknown activation
     assert lib.ima_int8_gated_gemm(16, 32, 16, 32, 16, 32, 2, 2, 32, 16, 16, 16, None, None, 0, 7, 16, 1, 2, None) == uns
-    assert lib.ima_int8_digits_rows(16, 1, 2, 32, 32, 1, 32, None, 4, 16, 32, 16, None) == uns
-    assert lib.ima_int8_digit_gemm(16, 1, 32, 16, 16, 32, None, 0, 2, 2, 32, 16, 1, 2, None) == uns
+    # backward: only 2 or 3 digits, contractions too long, no workspace
+    def backward(m=2, n=32, k=32, planes=2, dx=256, dw=None, ws=256):
+        ld = (max(n, k) + 15) // 16 * 16
+        return lib.ima_int8_linear_backward(16, 1, n, m, n, k, 16, ld, 16, 16, ld, 16, ld, 16, planes, dx, 1, dw, 1, None,
+                                            1, ws, None)
+    assert backward(planes=1) == uns and backward(n=131072) == uns and backward(m=131072, dx=None, dw=256) == uns
+    assert backward(ws=None) == bad
 
 
 @pytest.mark.gpu
