@@ -376,7 +376,7 @@ int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_
  * int8 and scale [M] are workspace; with keep_codes != 0 they hold the codes and scales of x
  * afterwards (what a backward pass needs), otherwise a product of few tokens quantises them in
  * its own launch and leaves both alone. */
-int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated); /* 1: q and scale may be NULL (keep_codes == 0) */
+int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated, int x_dtype); /* 1: without keep_codes, q and scale may be NULL */
 int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                     int keep_codes, const int8_t* w, int64_t ldw, int64_t N, const float* w_scale, const void* bias,
                     int bias_dtype, void* y, int64_t ldy, void* stream);

@@ -7,13 +7,13 @@ namespace {
 
 int64_t i8_steps(int64_t Ka) { return (Ka + I8_KT - 1) / I8_KT; }
 
-// Time of the tiled form in ns: rounds of 128 x BN tiles over the machine at the tensor core's rate (8192
+// Time of the tiled form in ns: rounds of 128 x bn tiles over the machine at the tensor core's rate (8192
 // multiplications per clock and SM at 1.6 GHz), two thirds of it while a stage's loads limit it, and
-// the fill and drain of its pipeline.
+// 8 us from launch to the end of the last epilogue.
 double tiled_ns(int64_t M, int64_t N, int64_t k_steps, int planes, int bn) {
     const int64_t tiles = ((M + I8_BM - 1) / I8_BM) * ((N + bn - 1) / bn);
     const int64_t rounds = (tiles + gemm_grid_limit() - 1) / gemm_grid_limit();
-    return (double)rounds * (double)k_steps * planes * bn * 128.0 * 128.0 / (8192.0 * 1.6 * 0.67) + 3000.0;
+    return (double)rounds * (double)k_steps * planes * bn * 128.0 * 128.0 / (8192.0 * 1.6 * 0.67) + 8000.0;
 }
 
 // The form with the shorter estimate.
@@ -46,10 +46,10 @@ int run_fused(SkParams& p, int x_dtype, const SkPlan& q, cudaStream_t st) {
 
 // Whether the tokens are quantised inside the product: every cluster then does it for itself, which
 // pays while the workers hold a CTA's share in one batch of loads.
-bool fused_plan(int64_t M, int64_t N, int64_t K, int ops, SkPlan& q) {
+bool fused_plan(int64_t M, int64_t N, int64_t K, int ops, int x_dtype, SkPlan& q) {
     if (M < 1 || M > 16 || N < 1) return false;
     q = sk_plan(M, N, i8_steps(K), 1, ops, true);
-    return q.ok && M * ((q.k_steps + q.splits - 1) / q.splits) * I8_KT <= SK_WORKERS * 32 * SK_BATCH * 8;
+    return q.ok && M * ((q.k_steps + q.splits - 1) / q.splits) * I8_KT <= SK_WORKERS * 32 * sk_batch(x_dtype) * 8;
 }
 
 }  // namespace
@@ -119,9 +119,9 @@ int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_
 
 // Operator entries: floating activations in.  Few tokens: one launch, quantiser inside.  Otherwise the row
 // quantiser into q and scale, then the product.
-int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated) {
+int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated, int x_dtype) {
     SkPlan plan;
-    return K >= 0 && K <= I8_MAX_K && fused_plan(M, N, K, gated ? 2 : 1, plan) ? 1 : 0;
+    return K >= 0 && K <= I8_MAX_K && fused_plan(M, N, K, gated ? 2 : 1, x_dtype, plan) ? 1 : 0;
 }
 
 int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
@@ -133,7 +133,7 @@ int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld
     if (M > 0 && K > 0 && (!x || (M > 1 && ldx < K))) return IMA_ERR_INVALID_ARGUMENT;
     {
         SkPlan plan;
-        if (!keep_codes && fused_plan(M, N, K, 1, plan)) {
+        if (!keep_codes && fused_plan(M, N, K, 1, x_dtype, plan)) {
             if (!y || !w_scale || (ldy < N && M > 1) || (bias && !known_dtype(bias_dtype))) return IMA_ERR_INVALID_ARGUMENT;
             SkParams p;
             memset(&p, 0, sizeof(p));
@@ -162,7 +162,7 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
     if (M > 0 && K > 0 && (!x || (M > 1 && ldx < K))) return IMA_ERR_INVALID_ARGUMENT;
     {
         SkPlan plan;
-        if (!keep_codes && fused_plan(M, N, K, 2, plan)) {
+        if (!keep_codes && fused_plan(M, N, K, 2, x_dtype, plan)) {
             if (!y || !gate_scale || !up_scale || (ldy < N && M > 1) || ((gate_bias || up_bias) && !known_dtype(bias_dtype)))
                 return IMA_ERR_INVALID_ARGUMENT;
             SkParams p;

@@ -26,7 +26,9 @@ constexpr int SK_THREADS = 64 + SK_WORKERS * 32;
 constexpr int SK_MAX_STAGES = 12;
 constexpr int SK_SMEM = 221 * 1024;              // with 5 KB static and 1 KB of the system: one CTA per SM at most
 constexpr int SK_MAX_TM = 128;
-constexpr int SK_BATCH = 8;                        // loads in flight per lane of the fused quantiser
+
+// Groups of eight elements that a lane of the fused quantiser has in flight (32 registers).
+__host__ __device__ constexpr int sk_batch(int dtype) { return dtype == IMA_DTYPE_F32 ? 4 : 8; }
 
 struct __align__(64) SkParams {
     CUtensorMap mw, mw2, mt;       // weight rows (or G), U (or the second segment's rows), token codes
@@ -79,10 +81,11 @@ IMA_DEVINL float gated_value(int act, float g, float u) {
 // EPI: I8_LINEAR, I8_GATED or I8_DIGIT; P digit planes (1 otherwise); DT: type of the activations when
 // the quantiser is fused, -1 when the tokens come as codes.
 template <int EPI, int P, int DT>
-__global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid_constant__ SkParams p) {
+__global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid_constant__ SkParams p) {
     constexpr bool FUSED = DT >= 0;
     constexpr int OPS = EPI == I8_GATED ? 2 : 1;
     constexpr int XT = FUSED ? DT : IMA_DTYPE_F32;
+    constexpr int BATCH = sk_batch(XT);
     extern __shared__ unsigned char sk_raw[];
     __shared__ uint64_t full[SK_MAX_STAGES], empty[SK_MAX_STAGES], tok_ready, acc_full, drained;
     __shared__ uint32_t tmem_slot;
@@ -106,6 +109,15 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
     unsigned char* tiles = smem + p.codes_bytes;
     int32_t* part = reinterpret_cast<int32_t*>(tiles + p.stages * stage_bytes);   // [S][OPS][P][tm][128 / S]
 
+    auto load_weights = [&](int i) {   // i-th k-step of this CTA
+        const int st = i % p.stages, ks = s0 + i;
+        unsigned char* sb = tiles + st * stage_bytes;
+        mbar_arrive_expect_tx(&full[st], (uint32_t)stage_bytes);
+        if (EPI == I8_DIGIT && ks >= p.seg_steps) tma_load_2d(sb, &p.mw2, &full[st], (ks - p.seg_steps) * I8_KT, n0);
+        else tma_load_2d(sb, &p.mw, &full[st], ks * I8_KT, n0);
+        if (EPI == I8_GATED) tma_load_2d(sb + W_BYTES, &p.mw2, &full[st], ks * I8_KT, n0);
+    };
+    const int first = min(steps, p.stages);
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
             mbar_init(&full[s], 1);
@@ -116,6 +128,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
+        for (int i = 0; i < first; ++i) load_weights(i);        // on their way before anything else is set up
     }
     if (FUSED)
         for (int i = threadIdx.x; i < 8 * SK_MAX_TM; i += SK_THREADS) s_amax[i] = 0;
@@ -128,14 +141,6 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    auto load_weights = [&](int i) {   // i-th k-step of this CTA
-        const int st = i % p.stages, ks = s0 + i;
-        unsigned char* sb = tiles + st * stage_bytes;
-        mbar_arrive_expect_tx(&full[st], (uint32_t)stage_bytes);
-        if (EPI == I8_DIGIT && ks >= p.seg_steps) tma_load_2d(sb, &p.mw2, &full[st], (ks - p.seg_steps) * I8_KT, n0);
-        else tma_load_2d(sb, &p.mw, &full[st], ks * I8_KT, n0);
-        if (EPI == I8_GATED) tma_load_2d(sb + W_BYTES, &p.mw2, &full[st], ks * I8_KT, n0);
-    };
     auto load_tokens = [&](int i) {
         const int st = i % p.stages;
         unsigned char* sb = tiles + st * stage_bytes + OPS * W_BYTES;
@@ -143,23 +148,22 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
         for (int d = 0; d < P; ++d) tma_load_3d(sb + d * p.tm * I8_KT, &p.mt, &full[st], (s0 + i) * I8_KT, m0, d);
     };
 
-    // ---- phase 1: first weight tiles on their way; row maxima of this CTA's slice ----
-    const int first = min(steps, p.stages);
+    // ---- phase 1: row maxima of this CTA's slice ----
     const int64_t kbeg = (int64_t)s0 * I8_KT, kend = min(p.K, (int64_t)s1 * I8_KT);
     // eight warps over the tokens, or several warps per token when there are fewer
     const int wpt = rows >= 8 || !FUSED ? 1 : (rows > 4 ? 1 : (rows > 2 ? 2 : (rows > 1 ? 4 : 8)));
     const int tok0 = (warp - 2) / wpt, tok_step = SK_WORKERS / wpt;
     const int chunk0 = ((warp - 2) % wpt) * 32 + lane, chunk_step = wpt * 32;
     const int chunks = FUSED ? (int)((kend - kbeg + 7) / 8) : 0;
-    const bool resident = FUSED && chunks <= SK_BATCH * chunk_step && rows <= tok_step;   // one batch holds it all
-    Raw8<XT> batch[FUSED ? SK_BATCH : 1];
+    const bool resident = FUSED && chunks <= BATCH * chunk_step && rows <= tok_step;   // one batch holds it all
+    Raw8<XT> batch[FUSED ? BATCH : 1];
     auto x_row = [&](int t) {
         return reinterpret_cast<const unsigned char*>(p.x) + (int64_t)(m0 + t) * p.ldx * dtype_bytes(XT);
     };
     auto load_batch = [&](const unsigned char* row, int c0) {
         const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
 #pragma unroll
-        for (int i = 0; i < (FUSED ? SK_BATCH : 0); ++i) {
+        for (int i = 0; i < (FUSED ? BATCH : 0); ++i) {
             const int64_t k = kbeg + (int64_t)(c0 + i * chunk_step) * 8;
             if (vec && k + 8 <= kend) batch[i].load_whole(row, k);
             else if (k < kend) batch[i].load(row, k, kend, false);
@@ -167,7 +171,6 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
         }
     };
     if (warp == 0 && lane == 0) {
-        for (int i = 0; i < first; ++i) load_weights(i);
         if (!FUSED) {
             if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int i = 0; i < first; ++i) load_tokens(i);
@@ -176,10 +179,10 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
         for (int t = tok0; t < rows; t += tok_step) {
             const unsigned char* row = x_row(t);
             uint32_t mx = 0;
-            for (int c0 = chunk0; c0 < chunks; c0 += SK_BATCH * chunk_step) {
+            for (int c0 = chunk0; c0 < chunks; c0 += BATCH * chunk_step) {
                 load_batch(row, c0);
 #pragma unroll
-                for (int i = 0; i < (FUSED ? SK_BATCH : 0); ++i) mx = max(mx, batch[i].max_bits());
+                for (int i = 0; i < (FUSED ? BATCH : 0); ++i) mx = max(mx, batch[i].max_bits());
             }
             mx = __reduce_max_sync(0xFFFFFFFFu, mx);
             if (lane == 0) atomicMax(&s_amax[rank * SK_MAX_TM + t], mx);
@@ -257,10 +260,10 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
                 const unsigned char* row = x_row(t);
                 const float s = s_scale[t];
                 const I8Inv inv = i8_inv(s);
-                for (int c0 = chunk0; c0 < chunks; c0 += SK_BATCH * chunk_step) {
+                for (int c0 = chunk0; c0 < chunks; c0 += BATCH * chunk_step) {
                     if (!resident) load_batch(row, c0);
 #pragma unroll
-                    for (int i = 0; i < SK_BATCH; ++i) {
+                    for (int i = 0; i < BATCH; ++i) {
                         const int off = (c0 + i * chunk_step) * 8;      // element of the slice
                         if (off >= chunks * 8) break;
                         float v[8];
@@ -279,115 +282,145 @@ __global__ void __launch_bounds__(SK_THREADS, 1) int8_skinny_kernel(const __grid
         if (!FUSED) {   // the token scales
             if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
             for (int t = threadIdx.x - 64; t < rows; t += SK_WORKERS * 32) s_scale[t] = p.xs ? p.xs[m0 + t] : 0.0f;
+            named_barrier_sync(1, SK_WORKERS * 32);
         }
-        // push the partial sums to the owners: TMEM lane = weight row, column = (operand, plane, token)
-        const bool ok = mbar_wait_or_abort(&acc_full, 0u, &abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_SKINNY, 200);
-        __syncwarp();
-        const bool all_ok = __all_sync(0xFFFFFFFFu, ok);
-        tc_fence_after();
-        if (all_ok) {
-            const int q = warp & 3, hw = (warp - 2) >> 2;
-            const int own = SK_ROWS / S, n = q * 32 + lane;
-            const uint32_t base = S > 1 ? cluster_addr(smem_u32(part), (uint32_t)(n / own)) : smem_u32(part);
-            for (int c0 = hw * 8; c0 < OPS * P * p.tm; c0 += 16) {
-                if (c0 % p.tm >= rows) continue;                // tokens beyond the last one
-                uint32_t r[8];
-                tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c0, r);
-                tmem_wait_ld();
-                const uint32_t at = base + (uint32_t)((((int)rank * OPS * P * p.tm + c0) * own + n % own) * 4);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t v = steps > 0 ? r[j] : 0u;
-                    if (S > 1) st_cluster_u32(at + (uint32_t)(j * own * 4), v);
-                    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + (uint32_t)(j * own * 4)), "r"(v) : "memory");
-                }
-            }
-        }
-        tc_fence_before();
-    }
-    __syncwarp();
-    if (S > 1) {
-        cluster_arrive();                                       // C: all partial sums are with their owners
-        cluster_wait();
-    } else {
-        __syncthreads();
-    }
-
-    // ---- phase 3: the outputs this CTA owns; a thread keeps its four columns and walks the tokens ----
-    if (!abort_flag && threadIdx.x < 256) {
-        const int own = SK_ROWS / S, per = own / 4;
-        const int j = (threadIdx.x % per) * 4;
-        const int32_t n = n0 + (int32_t)rank * own + j;
-        const int valid = min(4, p.N - n);
+        // scales and biases while the products run: of the lane's weight row (one CTA), or of the four
+        // columns that the thread will own (a cluster)
+        const int q = warp & 3, hw = (warp - 2) >> 2, wt = threadIdx.x - 64;
+        const int own = SK_ROWS / S, per = own / 4, j4 = (wt % per) * 4;
+        const int32_t nq = S > 1 ? n0 + (int32_t)rank * own + j4 : n0 + q * 32 + lane;
+        const int valid = max(0, min(S > 1 ? 4 : 1, p.N - nq));
         float ws[OPS][4], bias[OPS][4];
 #pragma unroll
         for (int o = 0; o < OPS; ++o)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? __ldg(p.ws[o] + n + e) : 0.0f;
-                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, n + e) : 0.0f;
+                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? __ldg(p.ws[o] + nq + e) : 0.0f;
+                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, nq + e) : 0.0f;
             }
-        auto gather = [&](int col) {   // sum over the cluster of 4 partial sums of one column
-            int4 a = make_int4(0, 0, 0, 0);
-            for (int r = 0; r < S; ++r) {
-                const int4 b = *reinterpret_cast<const int4*>(part + (r * OPS * P * p.tm + col) * own + j);
-                a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-            }
-            return a;
-        };
-#pragma unroll 2
-        for (int t = threadIdx.x / per; t < rows && valid > 0; t += 256 / per) {
-            int64_t m = m0 + t;
-            const float xs = s_scale[t];
-            float v[4];
-            void* y = p.y;
+        // the value of one output from its exact sums: a[plane], or a[0] of the operand(s)
+        auto value = [&](const int32_t (&a)[P], int32_t b, float xs, int e) {
             if constexpr (EPI == I8_DIGIT) {
-                if (p.y2) {
-                    const bool second = m >= p.split_row;
-                    if (second) { m -= p.split_row; y = p.y2; }
-                    if (m >= p.seg_rows) continue;
-                }
-                int64_t s[4] = {0, 0, 0, 0};
+                int64_t sum = 0;
 #pragma unroll
-                for (int d = 0; d < P; ++d) {
-                    const int4 a = gather(d * p.tm + t);
-                    s[0] += (int64_t)a.x << (8 * d);
-                    s[1] += (int64_t)a.y << (8 * d);
-                    s[2] += (int64_t)a.z << (8 * d);
-                    s[3] += (int64_t)a.w << (8 * d);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(__ll2float_rn(s[e]), xs);
+                for (int d = 0; d < P; ++d) sum += (int64_t)a[d] << (8 * d);
+                return __fmul_rn(__ll2float_rn(sum), xs);
             } else {
-                const int4 a = gather(t);
-                const int32_t av[4] = {a.x, a.y, a.z, a.w};
-                if constexpr (EPI == I8_GATED) {
-                    const int4 b = gather(p.tm + t);
-                    const int32_t bv[4] = {b.x, b.y, b.z, b.w};
+                float v = __fmul_rn(__fmul_rn(__int2float_rn(a[0]), xs), ws[0][e]);
+                if (EPI == I8_GATED) {
+                    const float u = __fmul_rn(__fmul_rn(__int2float_rn(b), xs), ws[OPS - 1][e]);
+                    return gated_value(p.act, __fadd_rn(v, bias[0][e]), __fadd_rn(u, bias[OPS - 1][e]));
+                }
+                return p.bias[0] ? __fadd_rn(v, bias[0][e]) : v;
+            }
+        };
+        // row of y that token t of the tile goes to (false: none)
+        auto place = [&](int t, void*& y, int64_t& m) {
+            y = p.y;
+            m = m0 + t;
+            if (EPI == I8_DIGIT && p.y2) {
+                if (m >= p.split_row) { m -= p.split_row; y = p.y2; }
+                return m < p.seg_rows;
+            }
+            return true;
+        };
+        const bool ok = mbar_wait_or_abort(&acc_full, 0u, &abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_SKINNY, 200);
+        __syncwarp();
+        const bool all_ok = __all_sync(0xFFFFFFFFu, ok);
+        tc_fence_after();
+        const uint32_t tq = tmem + ((uint32_t)(q * 32) << 16);   // TMEM lane = weight row, column = (operand, plane, token)
+        if (all_ok && S == 1) {
+            // straight from tensor memory: a warp stores 32 consecutive outputs of a token
+            for (int c0 = hw * 8; c0 < rows; c0 += 16) {
+                uint32_t r[OPS * P][8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float g = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(av[e]), xs), ws[0][e]), bias[0][e]);
-                        const float u = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(bv[e]), xs), ws[OPS - 1][e]), bias[OPS - 1][e]);
-                        v[e] = gated_value(p.act, g, u);
+                for (int o = 0; o < OPS * P; ++o) tmem_ld8(tq + (uint32_t)(o * p.tm + c0), r[o]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    void* y;
+                    int64_t m;
+                    if (c0 + i >= rows || valid == 0 || !place(c0 + i, y, m)) continue;
+                    int32_t a[P];
+#pragma unroll
+                    for (int d = 0; d < P; ++d) a[d] = steps > 0 ? (int32_t)r[d][i] : 0;
+                    const int32_t b = steps > 0 ? (int32_t)r[OPS * P - 1][i] : 0;
+                    if (EPI == I8_LINEAR && p.c) p.c[m * p.ldc + nq] = a[0];
+                    if (!p.y) continue;
+                    const float v = value(a, b, s_scale[c0 + i], 0);
+                    const int64_t at = m * p.ldy + nq;
+                    if (p.y_dtype == IMA_DTYPE_F32) reinterpret_cast<float*>(y)[at] = v;
+                    else if (p.y_dtype == IMA_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+                    else reinterpret_cast<__half*>(y)[at] = __float2half_rn(v);
+                }
+            }
+        } else if (all_ok) {
+            // push the partial sums to the owners
+            const int n = q * 32 + lane;
+            const uint32_t base = cluster_addr(smem_u32(part), (uint32_t)(n / own));
+            for (int c0 = hw * 8; c0 < OPS * P * p.tm; c0 += 16) {
+                if (c0 % p.tm >= rows) continue;                // tokens beyond the last one
+                uint32_t r[8];
+                tmem_ld8(tq + (uint32_t)c0, r);
+                tmem_wait_ld();
+                const uint32_t at = base + (uint32_t)((((int)rank * OPS * P * p.tm + c0) * own + n % own) * 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) st_cluster_u32(at + (uint32_t)(j * own * 4), steps > 0 ? r[j] : 0u);
+            }
+        }
+        tc_fence_before();
+        if (S > 1) {
+            __syncwarp();
+            cluster_arrive();                                   // C: all partial sums are with their owners
+            cluster_wait();
+            // the outputs this CTA owns: a thread keeps its four columns and walks the tokens
+            if (all_ok && valid > 0) {
+                auto gather = [&](int col) {   // sum over the cluster of 4 partial sums of one column
+                    int4 a = make_int4(0, 0, 0, 0);
+                    for (int r = 0; r < S; ++r) {
+                        const int4 b = *reinterpret_cast<const int4*>(part + (r * OPS * P * p.tm + col) * own + j4);
+                        a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
                     }
-                } else {
-                    if (p.c) {
-                        int32_t* dst = p.c + m * p.ldc + n;
-                        if (p.vec_c && valid == 4) *reinterpret_cast<int4*>(dst) = a;
-                        else
+                    return a;
+                };
+#pragma unroll 2
+                for (int t = wt / per; t < rows; t += 256 / per) {
+                    void* y;
+                    int64_t m;
+                    if (!place(t, y, m)) continue;
+                    int4 a[P], b = make_int4(0, 0, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < P; ++d) a[d] = gather(d * p.tm + t);
+                    if (EPI == I8_GATED) b = gather(p.tm + t);
+                    if (EPI == I8_LINEAR && p.c) {
+                        int32_t* dst = p.c + m * p.ldc + nq;
+                        if (p.vec_c && valid == 4) *reinterpret_cast<int4*>(dst) = a[0];
+                        else {
+                            const int32_t av[4] = {a[0].x, a[0].y, a[0].z, a[0].w};
                             for (int e = 0; e < valid; ++e) dst[e] = av[e];
+                        }
                     }
                     if (!p.y) continue;
+                    float v[4];
+                    const float xs = s_scale[t];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        v[e] = __fmul_rn(__fmul_rn(__int2float_rn(av[e]), xs), ws[0][e]);
-                        if (p.bias[0]) v[e] = __fadd_rn(v[e], bias[0][e]);
+                        int32_t ae[P];
+#pragma unroll
+                        for (int d = 0; d < P; ++d) ae[d] = e == 0 ? a[d].x : e == 1 ? a[d].y : e == 2 ? a[d].z : a[d].w;
+                        v[e] = value(ae, e == 0 ? b.x : e == 1 ? b.y : e == 2 ? b.z : b.w, xs, e);
                     }
+                    store_quad(y, p.y_dtype, m * p.ldy + nq, v, valid, p.vec_y);
                 }
             }
-            store_quad(y, p.y_dtype, m * p.ldy + n, v, valid, p.vec_y);
         }
     }
+    if (S > 1 && warp < 2) {
+        __syncwarp();
+        cluster_arrive();                                       // C, of the two warps without outputs
+        cluster_wait();
+    }
+    __syncthreads();
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -405,9 +438,9 @@ struct SkPlan {
 };
 
 // The split form of a product of M tokens by N outputs over k_steps k-steps: tokens per tile, split,
-// stages and an estimate of its time.  A CTA streams its weight tiles at up to 90 bytes/ns, the machine
-// at 6000; a cluster barrier exchange costs about 1.5 us, which a split has to earn; CTAs that do
-// not fit the machine at once wait for a round.
+// stages and an estimate of its time, from measurements: 6 us for a round of CTAs from launch to exit and
+// 12 ns per token column of its epilogue, a stream of 45 bytes/ns into an SM and 5800 into the machine
+// (a kernel that only loads 68 MB takes 15.0 us), 1 us for the exchange of a cluster.
 SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, bool fused) {
     const int max_tm = planes == 3 ? 32 : (planes == 2 || ops == 2 ? 64 : SK_MAX_TM);
     SkPlan best = {};
@@ -420,7 +453,7 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, bool 
         const int64_t tok = (int64_t)planes * tm * I8_KT;
         const int64_t codes = fused ? steps * tok : 0;
         const int64_t stage = (int64_t)ops * SK_ROWS * I8_KT + (fused ? 0 : tok);
-        const int64_t partial = (int64_t)ops * planes * tm * SK_ROWS * 4;
+        const int64_t partial = s > 1 ? (int64_t)ops * planes * tm * SK_ROWS * 4 : 0;
         const int64_t fit = (SK_SMEM - 1024 - codes - partial) / stage;
         const int64_t stages = std::min<int64_t>(std::min<int64_t>(fit, SK_MAX_STAGES), std::max<int64_t>(steps, 1));
         if (stages < std::min<int64_t>(3, std::max<int64_t>(steps, 1))) continue;
@@ -431,9 +464,9 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, bool 
         const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(2, 227 * 1024 / (q.smem + 8192)));
         const int64_t room = gemm_grid_limit() * per_sm * (s == 8 ? 7 : 8) / 8;
         const double rounds = (double)((ctas + room - 1) / room);
-        const double stream = std::max((double)(steps * stage) / 90.0 * rounds,
-                                       (double)(N * k_steps * I8_KT * ops * m_tiles) / 6000.0);
-        q.ns = stream + (s > 1 ? 1500.0 : 0.0);
+        const double stream = std::max((double)(steps * stage) / 45.0 * rounds,
+                                       (double)(N * k_steps * I8_KT * ops * m_tiles) / 5800.0);
+        q.ns = rounds * (6000.0 + 12.0 * (double)(ops * planes * tm)) + stream + (s > 1 ? 1000.0 : 0.0);
         q.ok = true;
         if (!best.ok || q.ns < best.ns) best = q;
     }

@@ -255,7 +255,7 @@ def int8_gemm(
 def _code_buffers(rows: torch.Tensor, n: int, gated: bool, keep: bool):
     """Room for the codes and scales of x rows (None, None when the product quantises them itself)."""
     m, k = rows.shape
-    if not keep and nat.lib().ima_int8_fused(m, n, k, gated):
+    if not keep and nat.lib().ima_int8_fused(m, n, k, gated, _DTYPE_CODES[rows.dtype]):
         return None, None
     return (rows.new_empty((m, _round_up(max(k, 1), 16)), dtype=torch.int8),
             rows.new_empty((m,), dtype=torch.float32))
