@@ -16,44 +16,68 @@
 // element carries the whole row; 4e-5 for Gaussian rows, 6e-4 measured for columns of token
 // gradients of very different sizes, where a bf16 result is off by 2e-3 and an fp16 one by 2e-4.
 #include <algorithm>
-#include "ima_common.cuh"
+#include <type_traits>
+#include "sm100_primitives.cuh"
 
 namespace {
 
 // Reciprocals of a scale that bracket it: x * lo and x * hi lie on either side of RN32(x / s), which is off
 // by at most 2^-24 of the quotient, as are the products.
 struct I8Inv {
-    float lo, hi;
+    float mid, lo, hi;
 };
 IMA_DEVINL I8Inv i8_inv(float s) {
     const float inv = __frcp_rn(s);
-    return {__fmul_rn(inv, 1.0f - 0x1p-21f), __fmul_rn(inv, 1.0f + 0x1p-21f)};
+    return {inv, __fmul_rn(inv, 1.0f - 0x1p-21f), __fmul_rn(inv, 1.0f + 0x1p-21f)};
 }
 
-// Codes of eight elements, rint(RN32(x / s)) each, without a division per element: fma(x, inv, 1.5 *
-// 2^23) holds rint(x * inv) in its low mantissa bits, and rounding is monotonic, so where both
-// brackets round to the same integer the quotient does too.  Where they differ (a quotient within
-// 2^-20 of itself of a half-integer, some 3 in 10^5) the division decides.  A scale that is NaN or
-// inf gives codes 0.
+// rint(RN32(x / s)) where x * inv rounds to a on one side of its bracket and to c on the other, without
+// dividing.  h = (a + c) / 2 is the half-integer between; e = x - h s is exact (h has 8 bits, s 24, and
+// the difference few).  RN32(x / s) equals h, a tie, when |x / s - h| is below half a step of fp32 at
+// h (a quotient of two fp32 numbers is never exactly on that boundary); otherwise e's sign decides.
+IMA_DEVINL uint32_t i8_near_tie(float x, float s, float a, float c) {
+    const float h = 0.5f * (a + c);
+    const float e = __fmaf_rn(-h, s, x);
+    const float half_step = __uint_as_float((__float_as_uint(h) & 0x7F800000u) - (24u << 23));
+    const float even = __fmul_rn(2.0f, rintf(__fmul_rn(0.5f, h)));   // the even one of a and c
+    const float k = fabsf(e) < __fmul_rn(s, half_step) ? even : (e > 0.0f ? fmaxf(a, c) : fminf(a, c));
+    return (uint32_t)(int32_t)k;
+}
+
+// Codes of eight elements, rint(RN32(x / s)) each, without a division per element.  A scale that is NaN
+// or inf gives codes 0.  1.5 * 2^23 is added to have the rounded integer in the low mantissa bits.
+//   16-bit inputs: Markstein's correction (see the fp8 quantiser), q0 = x y, q = q0 + (x - s q0) y with y =
+//     RN(1/s), which is RN32(x / s) to the last bit or at least rounds like it for every pair of a bf16
+//     or fp16 maximum and element (powers of two apart, 128^2 and 1024^2 pairs of significands times ten
+//     binades; a GPU test goes through them).  No branch: these inputs have few bits, and near-ties
+//     are common (0.2 % of bf16 elements).
+//   fp32: fma(x, inv, 1.5 * 2^23) for both brackets; rounding is monotonic, so where they agree the
+//     quotient rounds alike, and elsewhere (3 in 10^5) i8_near_tie decides.
+template <int DT>
 IMA_DEVINL uint2 i8_codes8(const float (&v)[8], float s, I8Inv inv) {
     constexpr float kRound = 12582912.0f;
-    uint32_t b[8], differ = 0;
+    uint32_t b[8];
+    if (DT != IMA_DTYPE_F32) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        b[j] = __float_as_uint(__fmaf_rn(v[j], inv.lo, kRound));
-        differ |= b[j] ^ __float_as_uint(__fmaf_rn(v[j], inv.hi, kRound));
-    }
-    if (differ) {
-#pragma unroll 1
         for (int j = 0; j < 8; ++j) {
-            float x = v[0];
+            const float q0 = __fmul_rn(v[j], inv.mid);
+            const float q = __fmaf_rn(__fmaf_rn(-q0, s, v[j]), inv.mid, q0);
+            b[j] = __float_as_uint(__fadd_rn(q, kRound));
+        }
+    } else {
+        float lo[8], hi[8];
+        uint32_t differ = 0;
 #pragma unroll
-            for (int e = 1; e < 8; ++e) x = j == e ? v[e] : x;
-            if (__fmaf_rn(x, inv.lo, kRound) != __fmaf_rn(x, inv.hi, kRound)) {
-                const uint32_t k = (uint32_t)__float2int_rn(__fdiv_rn(x, s));
+        for (int j = 0; j < 8; ++j) {
+            lo[j] = __fmaf_rn(v[j], inv.lo, kRound);
+            hi[j] = __fmaf_rn(v[j], inv.hi, kRound);
+            b[j] = __float_as_uint(lo[j]);
+            differ |= b[j] ^ __float_as_uint(hi[j]);
+        }
+        if (differ) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) b[e] = j == e ? k : b[e];
-            }
+            for (int j = 0; j < 8; ++j)
+                if (lo[j] != hi[j]) b[j] = i8_near_tie(v[j], s, lo[j] - kRound, hi[j] - kRound);
         }
     }
     if (!(s <= 3.402823466e38f)) return make_uint2(0, 0);
@@ -120,16 +144,17 @@ struct Raw8<IMA_DTYPE_F16> : RawHalf8<false> {};
 
 __host__ __device__ __forceinline__ int dtype_bytes(int dtype) { return dtype == IMA_DTYPE_F32 ? 4 : 2; }
 
-// Maximum over the TPR threads of a row (TPR == 32, or the block).
+// Maximum over the TPR threads of a row (whole warps of a block of 256).
 template <int TPR>
 IMA_DEVINL uint32_t row_max(uint32_t m, uint32_t* s_max) {
     m = __reduce_max_sync(0xFFFFFFFFu, m);
     if (TPR > 32) {
-        if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-        __syncthreads();
+        const int warp = threadIdx.x >> 5, group = threadIdx.x / TPR;
+        if ((threadIdx.x & 31) == 0) s_max[warp] = m;
+        named_barrier_sync(1 + group, TPR);
 #pragma unroll
-        for (int i = 0; i < TPR / 32; ++i) m = max(m, s_max[i]);
-        __syncthreads();
+        for (int i = 0; i < TPR / 32; ++i) m = max(m, s_max[group * (TPR / 32) + i]);
+        named_barrier_sync(1 + group, TPR);
     }
     return m;
 }
@@ -175,7 +200,7 @@ __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* 
         auto emit = [&](const Raw8<DT>& r, int64_t k0) {
             float v[8];
             r.unpack(v);
-            *reinterpret_cast<uint2*>(qr + k0) = i8_codes8(v, s, inv);
+            *reinterpret_cast<uint2*>(qr + k0) = i8_codes8<DT>(v, s, inv);
         };
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -455,18 +480,21 @@ bool known_dtype(int d) { return d == IMA_DTYPE_F32 || d == IMA_DTYPE_BF16 || d 
 template <int DT>
 int launch_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
                     cudaStream_t st) {
-    // A warp per row where the row fits its registers and the rows fill the machine (no barrier across the
-    // block), else a block per row: all of a long row's loads in flight at once.
-    constexpr int W = DT == IMA_DTYPE_F32 ? 8 : 16;
-    if (K <= 32 * 8 * 4 || (K <= 32 * 8 * W && M >= 148 * 8)) {
-        const unsigned grid = (unsigned)std::min<int64_t>((M + 7) / 8, 148 * 32);
-        if (K <= 1024) int8_quantize_rows_kernel<DT, 32, 4><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
-        else int8_quantize_rows_kernel<DT, 32, W><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
-    } else {
-        const unsigned grid = (unsigned)std::min<int64_t>(M, 148 * 32);
-        if (K <= 4096) int8_quantize_rows_kernel<DT, 256, 2><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
-        else int8_quantize_rows_kernel<DT, 256, 10><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
-    }
+    // As few threads per row as hold it in registers, when the rows fill the machine: 8 KB of a row in flight
+    // per warp and no barrier, or a barrier of two to eight warps.  Few rows: a block each, for latency.
+    constexpr bool F = DT == IMA_DTYPE_F32;
+    const bool many = M >= 148 * 8;
+    auto run = [&](auto tpr, auto v) {
+        constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
+        const unsigned grid = (unsigned)std::min<int64_t>((M * TPR + 255) / 256, 148 * 32);
+        int8_quantize_rows_kernel<DT, TPR, V><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+    };
+    if (K <= 1024) run(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
+    else if (many && K <= (F ? 2048 : 4096)) run(std::integral_constant<int, 32>{}, std::integral_constant<int, F ? 8 : 16>{});
+    else if (many && K <= 5120) run(std::integral_constant<int, 64>{}, std::integral_constant<int, 10>{});
+    else if (many && K <= 10240) run(std::integral_constant<int, 128>{}, std::integral_constant<int, 10>{});
+    else if (K <= 4096) run(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    else run(std::integral_constant<int, 256>{}, std::integral_constant<int, 10>{});
     return IMA_LAUNCH_STATUS();
 }
 

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
                         // k-step off / 128, token t, 16-byte piece (off % 128) / 16 at its swizzled place
                         unsigned char* dst = codes + (off >> 7) * tok_bytes + t * I8_KT +
                                              ((((off >> 4) & 7) ^ (t & 7)) << 4) + (off & 8);
-                        *reinterpret_cast<uint2*>(dst) = i8_codes8(v, s, inv);
+                        *reinterpret_cast<uint2*>(dst) = i8_codes8<XT>(v, s, inv);
                     }
                 }
             }

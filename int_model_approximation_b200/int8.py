@@ -47,13 +47,17 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _call(dev: torch.device, fn: str, *args) -> None:
     """A C entry whose last argument is the stream, on `dev` and its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        status = getattr(nat.lib(), fn)(*args, _raw_stream(dev.index))
+    index = dev.index
+    if _current_device() == index:
+        status = getattr(nat.lib(), fn)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            status = getattr(nat.lib(), fn)(*args, _raw_stream(dev.index))
+            status = getattr(nat.lib(), fn)(*args, _raw_stream(index))
     if status:
         raise nat.NativeError(fn, status)
 
@@ -438,7 +442,10 @@ def _check_gated(k: int, gate, up, activation: str) -> None:
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    for t in tensors:
+        if t is not None and type(t) is not Int8Weight and t.requires_grad:
+            return True
+    return False
 
 
 class _LinearFunction(torch.autograd.Function):
@@ -519,7 +526,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
     _check_inputs(x, ("weight", weight), ("bias", bias))
     if weight.shape[-1] != x.shape[-1]:
         raise RuntimeError(f"int8 matmul shape mismatch: K={x.shape[-1]} vs K={weight.shape[-1]}")
-    if _wants_grad(x, weight, bias):
+    if torch.is_grad_enabled() and _wants_grad(x, weight, bias):
         frozen = isinstance(weight, Int8Weight)
         _check_backward(x.numel() // max(x.shape[-1], 1), weight.shape[0] if x.requires_grad else 0,
                         not frozen and weight.requires_grad)
@@ -544,7 +551,7 @@ def int8_gated(
     product run in one kernel; g and u never reach memory.  Weights as in int8_linear."""
     _check_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
     _check_gated(x.shape[-1], gate, up, activation)
-    if _wants_grad(x, gate, up, gate_bias, up_bias):
+    if torch.is_grad_enabled() and _wants_grad(x, gate, up, gate_bias, up_bias):
         frozen = [isinstance(w, Int8Weight) for w in (gate, up)]
         _check_backward(x.numel() // max(x.shape[-1], 1),
                         _round_up(gate.shape[0], 128) + gate.shape[0] if x.requires_grad else 0,

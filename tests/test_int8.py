@@ -201,6 +201,30 @@ def test_quantiser_matches_its_definition(cuda_device, dtype, m, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 7), (torch.float16, 10)])
+@pytest.mark.parametrize("k_pad", [0, 5])
+def test_quantiser_every_pair_of_significands(cuda_device, dtype, bits, k_pad):
+    """Codes against torch's fp32 division for every significand of the row maximum and of the
+    element, over the ten binades in which the code is not 0 whatever the rounding.  Other rows
+    differ by powers of two, which scale every step exactly.  k_pad 5: rows off the 16-byte grid."""
+    n = 2**bits
+    maxima = (1.0 + torch.arange(n, device=cuda_device) / n) * 2.0
+    binades = 2.0 ** torch.arange(1, -9, -1, device=cuda_device).float()
+    elements = ((1.0 + torch.arange(n, device=cuda_device) / n)[None] * binades[:, None]).reshape(-1)
+    for chunk in maxima.split(128):
+        x = torch.zeros((chunk.numel(), elements.numel() + 1 + k_pad), device=cuda_device, dtype=dtype)
+        x[:, 0] = chunk.to(dtype)
+        rest = elements[None].expand(chunk.numel(), -1) * (elements[None] <= chunk[:, None])
+        sign = torch.where(torch.arange(elements.numel(), device=cuda_device) % 3 == 0, -1.0, 1.0)
+        x[:, 1:1 + elements.numel()] = (rest * sign).to(dtype)
+        q, s = int8.per_token_int8(x)
+        x32 = x.float()
+        s32 = x32.abs().amax(dim=1, keepdim=True) / torch.full_like(s, 127.0)
+        assert torch.equal(s, s32)
+        assert torch.equal(q.float(), (x32 / s32).round())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_quantiser_ties_and_special_rows(cuda_device, dtype):
     rows = torch.zeros((9, 40), dtype=torch.float32)
