@@ -195,7 +195,8 @@ constexpr int BWD_DX = 1, BWD_DW = 2, BWD_DB = 4, BWD_OWN_WT = 8;
 
 struct BwdPlan {
     int64_t pitch, W, ldm, ldwt;
-    int64_t maxima, maxima_bytes, d, rows, row_scale, cols, col_scale, q_t, w_t, partial, total;   // offsets
+    int64_t maxima, maxima_bytes, d, rows, row_scale, cols, col_scale, q_t, w_t, partial, tail, total;   // offsets
+    bool has_tail;
 };
 
 BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int segs, int planes, int want) {
@@ -226,6 +227,10 @@ BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int segs, int planes, int want
     }
     if (want & BWD_OWN_WT) b.w_t = take(segs * K * b.ldwt);
     if (want & BWD_DB) b.partial = take((M + 127) / 128 * b.W * 4);
+    // more 128 x 128 blocks than workers: the tiled form may have a tail to split
+    const int64_t kb = (K + 127) / 128;
+    b.has_tail = (dx && (M + 127) / 128 * kb > 74) || (dw && (b.W + 127) / 128 * kb > 74);
+    if (b.has_tail) b.tail = take(I8_TAIL_BYTES);
     b.total = at;
     return b;
 }
@@ -279,6 +284,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         p.M = (int32_t)a.M; p.N = (int32_t)a.K;
         p.vec_y = aligned16(a.dx, a.K * dtype_bytes(a.dx_dtype));
         p.seg_tiles = (int32_t)i8_steps(a.N);
+        p.tail = b.has_tail ? reinterpret_cast<int32_t*>(ws + b.tail) : nullptr;
         const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.rows), wt[0], a.segs == 2 ? wt[1] : nullptr, b.W,
                               ldwt[0], ldwt[1], (a.segs - 1) * b.pitch + a.N, a.N, a.M * b.W};
         if (a.K > 0) rc = run_digits<P, BN>(p, o, st);
@@ -301,6 +307,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
             p.vec_y = p.vec_y && aligned16(p.y2, a.K * dtype_bytes(a.dw_dtype));
         }
         p.seg_tiles = (int32_t)i8_steps(a.M);
+        p.tail = b.has_tail ? reinterpret_cast<int32_t*>(ws + b.tail) : nullptr;
         const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.cols) + first * b.pitch * b.ldm, qt, nullptr, b.ldm,
                               b.ldm, 0, a.M, a.M, b.W * b.ldm};
         rc = run_digits<P, BN>(p, o, st);

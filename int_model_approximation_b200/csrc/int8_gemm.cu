@@ -10,12 +10,12 @@
 // int32 accumulators are exact; the digits' accumulators are joined in int64 and rounded to fp32
 // once.
 //
-// Tile and roles (persistent, 10 warps per CTA): a tile is 128 rows of A by BN rows of B.  A stage
+// Tile and roles (persistent, 10 or 18 warps per CTA): a tile is 128 rows of A by BN rows of B.  A stage
 // holds 128 bytes of K of the P planes of A and of the tile's rows of B, 128-byte swizzled.
 //   warp 0    TMA producer;
 //   warp 1    allocates tensor memory and issues the MMAs (one thread);
-//   warps 2-9 epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 (one output row per thread) and
-//             half of the tile's columns, and stores 64-byte row pieces through shared memory, so
+//   warps 2.. epilogue: warp w reads TMEM lanes 32 (w % 4) .. + 31 (one output row per thread) and
+//             half (of 8 warps) or a quarter (of 16) of the tile's columns, and stores 64-byte row pieces through shared memory, so
 //             that a warp store covers 8 rows of 64 contiguous bytes.
 // With one plane there are two accumulators, so the epilogue of a tile runs under the MMAs of
 // the next.  The gated forms put 128 rows of G and 128 rows of U into one B tile: a single MMA of
@@ -33,24 +33,29 @@ namespace {
 
 constexpr int I8_BM = 128;      // rows of A per CTA
 constexpr int I8_KT = 128;      // bytes of K per stage: one 128-byte swizzle row
-constexpr int I8_EPI_WARPS = 8;
-constexpr int I8_THREADS = 64 + I8_EPI_WARPS * 32;
 constexpr int64_t I8_MAX_K = 131071;
 
 enum I8Epi { I8_LINEAR = 0, I8_GATED = 1, I8_GATED_BWD = 2, I8_DIGIT = 3 };
+// Epilogue warps: the gradients of the gated block do 45 instructions per column where the others do 10 to
+// 25, waiting for loads in between; with 8 warps they would take longer than the tile's MMAs.
+constexpr int i8_epi_warps(int epi) { return epi == I8_GATED_BWD ? 16 : 8; }
 
-template <int P, int BN, int CG>
+template <int P, int BN, int CG, int EPI>
 struct I8Cfg {
+    static constexpr int EW = i8_epi_warps(EPI);
+    static constexpr int THREADS = 64 + EW * 32;
     static constexpr int A_PLANE = I8_BM * I8_KT;
     static constexpr int B_BYTES = BN / CG * I8_KT;          // a CTA pair holds half of B each
     static constexpr int STAGE_BYTES = P * A_PLANE + B_BYTES;
-    static constexpr int STAGES = 200 * 1024 / STAGE_BYTES < 6 ? 200 * 1024 / STAGE_BYTES : 6;
+    static constexpr int EPI_BYTES = EW * 2048 + EW * 128 * 8;   // output staging; scales and biases
+    static constexpr int ROOM = (225 * 1024 - EPI_BYTES) / STAGE_BYTES;
+    static constexpr int STAGES = ROOM < 6 ? ROOM : 6;
     static constexpr int ACC = P * BN;                       // tensor-memory columns of one tile
     static constexpr int BUFS = 2 * ACC <= 512 ? 2 : 1;
     static_assert(ACC <= 512, "accumulators exceed tensor memory");
     static constexpr int STG_OFFSET = STAGES * STAGE_BYTES;  // 2 KB of output staging per epilogue warp
-    static constexpr int COL_OFFSET = STG_OFFSET + I8_EPI_WARPS * 2048;   // 256 floats per epilogue warp
-    static constexpr int BAR_OFFSET = COL_OFFSET + I8_EPI_WARPS * 1024;
+    static constexpr int COL_OFFSET = STG_OFFSET + EW * 2048;    // 256 floats per epilogue warp (128 of 16 warps)
+    static constexpr int BAR_OFFSET = STG_OFFSET + EPI_BYTES;
     static constexpr int TOTAL = BAR_OFFSET + (2 * STAGES + 2 * BUFS + 1) * 8 + 16;
     static constexpr int ALLOC = TOTAL + 1024;               // slack to align the base to 1024 B
     static_assert(ALLOC <= 227 * 1024, "shared memory per CTA");
@@ -69,6 +74,10 @@ struct __align__(64) I8Params {
     void* y2;                       // I8_DIGIT: rows from split_row on go here (NULL: all to y)
     int64_t split_row, seg_rows;    // and of each part only seg_rows exist
     int64_t ldc, ldy, ldh, ldd, seg_pitch;
+    int32_t* tail;                  // I8_DIGIT: sums of the tail tiles, [tile][plane][BN][rows], and their counters
+    uint32_t* tail_count;           // [tile][CTA of the pair][epilogue warp]; both zero at launch
+    int64_t full_tiles;             // tiles taken whole; each of the rest is split over tail_splits workers
+    int32_t tail_splits;
     int32_t M, N, m_tiles, n_tiles, k_tiles, group_m;
     int32_t y_dtype, bias_dtype, dh_dtype, act, vec_c, vec_y, vec_d;
     int32_t dependent;              // launched while the kernel before it (a quantiser) still runs
@@ -86,6 +95,30 @@ IMA_DEVINL void i8_tile(const I8Params& p, int64_t t, int32_t& mt, int32_t& nt) 
     mt = g * p.group_m + within % gm;
     nt = within / gm;
 }
+
+// The work of one worker (a CTA, or a pair): whole tiles first, first + step, ..., then at most one part of
+// the k-range of a tail tile.
+struct I8Work {
+    int64_t t;
+    int32_t k0, k1;       // k-tiles
+    bool split;
+    IMA_DEVINL bool get(const I8Params& p, int64_t i, int64_t first, int64_t step) {
+        t = first + i * step;
+        k0 = 0;
+        k1 = p.k_tiles;
+        split = false;
+        if (t < p.full_tiles) return true;
+        // the worker's item after its last whole tile
+        if (p.tail_splits == 0 || (i > 0 && t - step >= p.full_tiles)) return false;
+        const int64_t tail = first / p.tail_splits, part = first % p.tail_splits;
+        t = p.full_tiles + tail;
+        if (t >= (int64_t)p.m_tiles * p.n_tiles) return false;
+        k0 = (int32_t)(part * p.k_tiles / p.tail_splits);
+        k1 = (int32_t)((part + 1) * p.k_tiles / p.tail_splits);
+        split = true;
+        return true;
+    }
+};
 
 // ---------------------------------------------------------------------------
 // activations and their derivatives, fp32
@@ -183,11 +216,13 @@ IMA_DEVINL void store_y32(const I8Params& p, unsigned char* st, int lane, const 
 }
 
 template <int P, int BN, int EPI, int CG>
-__global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_constant__ I8Params p) {
-    using L = I8Cfg<P, BN, CG>;
+__global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kernel(const __grid_constant__ I8Params p) {
+    using L = I8Cfg<P, BN, CG, EPI>;
     constexpr bool PAIR = EPI == I8_GATED || EPI == I8_GATED_BWD;   // B tile = BN / 2 rows of G, then of U
     constexpr int TN = PAIR ? BN / 2 : BN;                          // output columns of a tile
-    constexpr int HALF = TN / 2;                                    // output columns of an epilogue warp
+    constexpr int HALF = TN / (L::EW / 4);                          // output columns of an epilogue warp
+    constexpr int COLS = L::EW == 16 ? 128 : 256;                   // its scales and biases
+    static_assert((PAIR ? 4 : 2) * HALF <= COLS, "scales and biases of an epilogue warp");
     extern __shared__ unsigned char i8_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);
@@ -199,7 +234,6 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t num_tiles = (int64_t)p.m_tiles * p.n_tiles;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;   // CTA of the pair; 0 issues its MMAs
     const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -210,7 +244,7 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         }
         for (int b = 0; b < L::BUFS; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], I8_EPI_WARPS * CG);
+            mbar_init(&acc_empty[b], L::EW * CG);
         }
         mbar_init(drained, 1);
         *abort_flag = 0;
@@ -235,10 +269,11 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         // ---------------- TMA producer ----------------
         uint32_t stage = 0, phase = 0;
         uint64_t issued = 0;
-        for (int64_t t = first; t < num_tiles && !*abort_flag; t += step) {
+        I8Work w;
+        for (int64_t i = 0; !*abort_flag && w.get(p, i, first, step); ++i) {
             int32_t mt, nt;
-            i8_tile(p, t, mt, nt);
-            for (int kt = 0; kt < p.k_tiles; ++kt) {
+            i8_tile(p, w.t, mt, nt);
+            for (int kt = w.k0; kt < w.k1; ++kt) {
                 if (!mbar_wait_or_abort(&empty[stage], phase ^ 1u, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM,
                                         (int)stage))
                     break;
@@ -250,8 +285,8 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                 if constexpr (CG == 1) {
                     mbar_arrive_expect_tx(&full[stage], (uint32_t)L::STAGE_BYTES);
 #pragma unroll
-                    for (int i = 0; i < P; ++i)
-                        tma_load_3d(sb + i * L::A_PLANE, &p.ma, &full[stage], kt * I8_KT, mt * I8_BM, i);
+                    for (int pl = 0; pl < P; ++pl)
+                        tma_load_3d(sb + pl * L::A_PLANE, &p.ma, &full[stage], kt * I8_KT, mt * I8_BM, pl);
                     tma_load_2d(bb, second ? &p.mb2 : &p.mb, &full[stage], bx, nt * TN);
                     if (PAIR) tma_load_2d(bb + TN * I8_KT, &p.mb2, &full[stage], bx, nt * TN);
                 } else {
@@ -260,8 +295,8 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                     const uint32_t bar = cluster_map(&full[stage], 0);
                     if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2u * (uint32_t)L::STAGE_BYTES);
 #pragma unroll
-                    for (int i = 0; i < P; ++i)
-                        tma_load_3d_pair(sb + i * L::A_PLANE, &p.ma, bar, kt * I8_KT, (mt * 2 + (int)rank) * I8_BM, i);
+                    for (int pl = 0; pl < P; ++pl)
+                        tma_load_3d_pair(sb + pl * L::A_PLANE, &p.ma, bar, kt * I8_KT, (mt * 2 + (int)rank) * I8_BM, pl);
                     if (PAIR)
                         tma_load_2d_pair(bb, rank ? &p.mb2 : &p.mb, bar, bx, nt * TN);
                     else
@@ -286,13 +321,14 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         uint32_t stage = 0, phase = 0, buf = 0, bphase = 0;
         if (p.stall_ns)   // test knob: a wait that nothing ends runs out
             mbar_wait_or_abort(drained, 0u, abort_flag, p.stall_ns, IMA_WHERE_INT8_GEMM, -2);
-        for (int64_t t = first; t < num_tiles && !*abort_flag; t += step) {
+        I8Work w;
+        for (int64_t i = 0; !*abort_flag && w.get(p, i, first, step); ++i) {
             if (!mbar_wait_or_abort(&acc_empty[buf], bphase ^ 1u, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM, -1))
                 break;
             tc_fence_after();
             const uint32_t acc = tmem_base + buf * L::ACC;
             bool fed = true;
-            for (int kt = 0; kt < p.k_tiles; ++kt) {
+            for (int kt = w.k0; kt < w.k1; ++kt) {
                 if (!mbar_wait_or_abort(&full[stage], phase, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM,
                                         50 + (int)stage)) {
                     fed = false;
@@ -304,11 +340,11 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
 #pragma unroll
                 for (int ks = 0; ks < I8_KT / 32; ++ks)
 #pragma unroll
-                    for (int i = 0; i < P; ++i) {
-                        const uint64_t da = umma_desc_sw128_kmajor(sa + i * L::A_PLANE + ks * 32);
+                    for (int pl = 0; pl < P; ++pl) {
+                        const uint64_t da = umma_desc_sw128_kmajor(sa + pl * L::A_PLANE + ks * 32);
                         const uint64_t db = umma_desc_sw128_kmajor(sb + ks * 32);
-                        if (CG == 2) mma_i8_pair(acc + i * BN, da, db, idesc, (kt | ks) ? 1u : 0u);
-                        else mma_i8(acc + i * BN, da, db, idesc, (kt | ks) ? 1u : 0u);
+                        if (CG == 2) mma_i8_pair(acc + pl * BN, da, db, idesc, (kt > w.k0 || ks) ? 1u : 0u);
+                        else mma_i8(acc + pl * BN, da, db, idesc, (kt > w.k0 || ks) ? 1u : 0u);
                     }
                 if (CG == 2) mma_commit_pair(&empty[stage]);
                 else mma_commit(&empty[stage]);
@@ -327,11 +363,12 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
         // ---------------- epilogue ----------------
         const int ew = warp - 2, q = warp & 3, h = ew >> 2;
         unsigned char* st = smem + L::STG_OFFSET + ew * 2048;
-        float* cols = reinterpret_cast<float*>(smem + L::COL_OFFSET) + ew * 256;
+        float* cols = reinterpret_cast<float*>(smem + L::COL_OFFSET) + ew * COLS;
         uint32_t buf = 0, bphase = 0;
-        for (int64_t t = first; t < num_tiles; t += step) {
+        I8Work wk;
+        for (int64_t item = 0; wk.get(p, item, first, step); ++item) {
             int32_t mt, nt;
-            i8_tile(p, t, mt, nt);
+            i8_tile(p, wk.t, mt, nt);
             const int64_t row0 = ((int64_t)mt * CG + rank) * I8_BM + q * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, (int64_t)p.M - row0));
             const int32_t n0 = nt * TN + h * HALF;
@@ -480,12 +517,44 @@ __global__ void __launch_bounds__(I8_THREADS, 1) int8_gemm_kernel(const __grid_c
                 const int64_t out_row = second ? row0 - p.split_row : row0;
                 const int out_rows = p.y2 ? (int)max((int64_t)0, min((int64_t)rows, p.seg_rows - out_row)) : rows;
                 void* out = second ? p.y2 : p.y;
+                bool store = true;
+                int32_t* sums = nullptr;   // this warp's rows and columns of a split tile: [plane][column][row]
+                if (wk.split) {
+                    // exact sums in any order; the last worker to add to this warp's part writes it out
+                    sums = p.tail + (((wk.t - p.full_tiles) * P * BN + h * HALF) * CG + rank) * I8_BM + q * 32 + lane;
 #pragma unroll 1
-                for (int c0 = 0; c0 < HALF; c0 += 32) {
-                    uint32_t r[P][32];
+                    for (int c0 = 0; c0 < HALF; c0 += 32)
+#pragma unroll 1
+                        for (int i = 0; i < P; ++i) {
+                            uint32_t r[32];
+                            tmem_ld32(tq + i * BN + c0, r);
+                            tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < P; ++i) tmem_ld32(tq + i * BN + c0, r[i]);
-                    tmem_wait_ld();
+                            for (int j = 0; j < 32; ++j)
+                                atomicAdd(sums + (int64_t)(i * BN + c0 + j) * CG * I8_BM, (int32_t)r[j]);
+                        }
+                    __threadfence();
+                    __syncwarp();
+                    uint32_t before = 0;
+                    if (lane == 0)
+                        before = atomicAdd(p.tail_count + ((wk.t - p.full_tiles) * CG + rank) * L::EW + ew, 1u);
+                    store = __shfl_sync(0xFFFFFFFFu, before, 0) + 1 == (uint32_t)p.tail_splits;
+                    __threadfence();
+                }
+#pragma unroll 1
+                for (int c0 = 0; c0 < HALF && store; c0 += 32) {
+                    uint32_t r[P][32];
+                    if (wk.split) {
+#pragma unroll
+                        for (int i = 0; i < P; ++i)
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                r[i][j] = (uint32_t)__ldcg(sums + (int64_t)(i * BN + c0 + j) * CG * I8_BM);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < P; ++i) tmem_ld32(tq + i * BN + c0, r[i]);
+                        tmem_wait_ld();
+                    }
                     if (n0 + c0 >= p.N || out_rows <= 0) continue;
                     float v[32];
 #pragma unroll
@@ -570,9 +639,17 @@ struct I8Operands {
     int64_t a_planes;                // bytes between the planes of A
 };
 
+// Tail tiles of a digit product that the workspace of a backward pass has room for (I8_TAIL_BYTES), and
+// the bytes that `tiles` of them take: their sums and counters.
+constexpr int64_t I8_TAIL_BYTES = 24ll << 20;
+template <int P, int BN>
+int64_t tail_bytes(int cg, int64_t tiles) { return tiles * cg * ((int64_t)P * BN * I8_BM * 4 + i8_epi_warps(I8_DIGIT) * 4); }
+template <int P, int BN>
+int64_t tail_tiles(int cg) { return I8_TAIL_BYTES / tail_bytes<P, BN>(cg, 1); }
+
 template <int P, int BN, int EPI, int CG>
 int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
-    using L = I8Cfg<P, BN, CG>;
+    using L = I8Cfg<P, BN, CG, EPI>;
     constexpr int TN = EPI == I8_GATED || EPI == I8_GATED_BWD ? BN / 2 : BN;
     constexpr int BOX = i8_box_rows<BN, EPI, CG>();
     p.m_tiles = (p.M + CG * I8_BM - 1) / (CG * I8_BM);
@@ -587,14 +664,29 @@ int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
         if (rc == IMA_OK && o.b2) rc = make_i8_map(&p.mb2, o.b2, o.K, o.ldb2, p.N, 1, 0, BOX);
         if (rc != IMA_OK) return rc;
     }
+    const int64_t all = (int64_t)p.m_tiles * p.n_tiles, workers = std::max<int64_t>(1, gemm_grid_limit() / CG);
+    p.full_tiles = all;
+    p.tail_splits = 0;
+    if (EPI == I8_DIGIT && p.tail && all > workers) {
+        // a last round that fills less than 5/8 of the machine: its tiles split over all workers (at least 8 k-tiles
+        // each, and at most 16 of them per tile, whose sums meet in L2)
+        const int64_t rest = all % workers;
+        const int64_t splits = rest ? std::min<int64_t>(std::min<int64_t>(workers / rest, 16), p.k_tiles / 8) : 0;
+        if (rest * 8 <= workers * 5 && splits >= 2 && rest <= tail_tiles<P, BN>(CG)) {
+            p.full_tiles = all - rest;
+            p.tail_splits = (int32_t)splits;
+            rc = ima_note_cuda(cudaMemsetAsync(p.tail, 0, tail_bytes<P, BN>(CG, rest), stream));
+            if (rc != IMA_OK) return rc;
+            p.tail_count = reinterpret_cast<uint32_t*>(p.tail + rest * P * BN * CG * I8_BM);
+        }
+    }
     auto kern = int8_gemm_kernel<P, BN, EPI, CG>;
     static std::atomic<uint64_t> ready{0};
     rc = set_smem_once(ready, (const void*)kern, L::ALLOC);
     if (rc != IMA_OK) return rc;
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(tiles, gemm_grid_limit() / CG) * CG));
-    cfg.blockDim = dim3(I8_THREADS);
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(all, workers) * CG));
+    cfg.blockDim = dim3(L::THREADS);
     cfg.dynamicSmemBytes = L::ALLOC;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];

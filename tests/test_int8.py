@@ -448,7 +448,7 @@ def grad_bound(d, d_err, factor, codes, limit, dtype, want):
 
 
 GRAD_SHAPES = [(1, 1, 1), (1, 300, 64), (5, 17, 33), (64, 130, 250), (130, 257, 129), (300, 64, 896), (257, 896, 128),
-               (300, 64, 10250), (2000, 96, 4000)]
+               (300, 64, 10250), (2000, 96, 4000), (2000, 2100, 2500)]
 
 
 @pytest.mark.gpu
