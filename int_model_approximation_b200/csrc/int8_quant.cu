@@ -309,8 +309,9 @@ __global__ void __launch_bounds__(256) int8_grad_max_kernel(const GradSrc a) {
 }
 
 // Digit planes of both forms, and partial column sums of D, in one pass over D.  A block takes 128 rows
-// by 64 columns; the transposed form goes through shared memory (element (r, c) at column c ^ 4 (r / 16),
-// so that eight 16-row groups of four columns read without bank conflicts).  Every plane row is written
+// by 64 columns; the transposed form goes through shared memory.  There a row is 16 quads of columns, the
+// two of its thread t at t ^ (row / 16) and (t + 8) ^ (row / 16): eight threads that write a row, and eight
+// 16-row groups that read a quad, meet no bank conflicts.  Every plane row is written
 // in pieces of 64 (rows) or 128 (columns) contiguous bytes.  Either form and the sums may be absent.
 struct GradDigits {
     GradSrc g;
@@ -324,51 +325,99 @@ struct GradDigits {
 
 template <int DT, int P>
 __global__ void __launch_bounds__(256) int8_grad_digits_kernel(const GradDigits a) {
-    __shared__ float tile[128 * 64];
+    __shared__ float4 tile[128 * 16];                           // four columns each
+    __shared__ float4 s_xs[32];                                 // token scales of the 128 rows, 0 beyond the last
+    __shared__ float s_row_inv[128], s_col_inv[64];             // reciprocals of the digit scales
     const GradSrc& g = a.g;
     const int64_t m0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 64;
     const int seg = c0 >= g.pitch ? 1 : 0;
-    const int64_t valid = g.n - (c0 - seg * g.pitch);           // columns of this tile that hold something
-    const int ch = threadIdx.x & 7, r0 = threadIdx.x >> 3;      // eight columns of rows r0 + 32 i
+    const int valid = (int)min((int64_t)64, g.n - (c0 - seg * g.pitch));   // columns of this tile that hold something
+    const int rows = (int)min((int64_t)128, g.M - m0);
+    // eight columns of rows r0 + 32 i, in two quads: neighbours of 16 bits, 32 columns apart of fp32, so that eight
+    // threads load 128 contiguous bytes either way
+    constexpr bool F32 = DT == IMA_DTYPE_F32;
+    const int ch = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+    const int ca = F32 ? 4 * ch : 8 * ch, cb = F32 ? 4 * ch + 32 : 8 * ch + 4;
     Raw8<DT> raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int64_t m = m0 + r0 + i * 32;
+        const int r = r0 + i * 32;
         raw[i].clear();
-        if (m < g.M && ch * 8 < valid) {
-            const unsigned char* p = reinterpret_cast<const unsigned char*>(g.src) + (m * g.ld + c0) * dtype_bytes(DT);
-            raw[i].load(p, ch * 8, valid, (reinterpret_cast<uintptr_t>(p) & 15) == 0);
+        if (r < rows && ca < valid) {
+            const unsigned char* p = reinterpret_cast<const unsigned char*>(g.src) + ((m0 + r) * g.ld + c0) * dtype_bytes(DT);
+            const bool vec = (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+            if constexpr (F32) {
+                const float* f = reinterpret_cast<const float*>(p);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int c = hf ? cb : ca;
+                    if (vec && c + 4 <= valid) {
+                        const float4 q = __ldg(reinterpret_cast<const float4*>(f + c));
+                        raw[i].v[4 * hf] = q.x; raw[i].v[4 * hf + 1] = q.y; raw[i].v[4 * hf + 2] = q.z; raw[i].v[4 * hf + 3] = q.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) raw[i].v[4 * hf + e] = c + e < valid ? __ldg(f + c + e) : 0.0f;
+                    }
+                }
+            } else {
+                if (vec && ca + 8 <= valid) raw[i].load_whole(p, ca);
+                else raw[i].load(p, ca, valid, false);
+            }
+        }
+    }
+    if (threadIdx.x < 128) {
+        const int r = threadIdx.x;
+        if (a.cols) reinterpret_cast<float*>(s_xs)[r] = r < rows ? __ldg(g.xs + m0 + r) : 0.0f;
+        if (a.rows && r < rows) {
+            const float s = digit_scale<P>(__uint_as_float(g.row_max[m0 + r]));
+            if (blockIdx.x == 0) a.row_scale[m0 + r] = s;
+            s_row_inv[r] = __frcp_rn(s);
+        }
+    } else if (a.cols && threadIdx.x < 192) {
+        const int c = threadIdx.x - 128;
+        if (c < valid) {
+            const float s = digit_scale<P>(__uint_as_float(g.col_max[c0 + c]));
+            if (blockIdx.y == 0) a.col_scale[c0 + c] = s;
+            s_col_inv[c] = __frcp_rn(s);
         }
     }
     float w[8];
     if (a.rows) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = ch * 8 + j < valid ? __ldg(g.ws[seg] + (c0 - seg * g.pitch) + ch * 8 + j) : 0.0f;
+        for (int j = 0; j < 8; ++j) {
+            const int c = j < 4 ? ca + j : cb + j - 4;
+            w[j] = c < valid ? __ldg(g.ws[seg] + (c0 - seg * g.pitch) + c) : 0.0f;
+        }
     }
+    __syncthreads();
+    const bool in_a = a.rows && c0 + ca < g.W, in_b = a.rows && c0 + cb < g.W;
+    int8_t* row_out = a.rows + (m0 + r0) * g.W + c0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = r0 + i * 32;
-        const int64_t m = m0 + r;
         float v[8];
         raw[i].unpack(v);
-        if (a.rows && m < g.M && c0 + ch * 8 < g.W) {
-            const float amax = __uint_as_float(g.row_max[m]);
-            const float s = digit_scale<P>(amax);
-            if (c0 == 0 && ch == 0) a.row_scale[m] = s;
-            const float inv = __frcp_rn(s);
+        if (in_a && r < rows) {
+            const float inv = s_row_inv[r];
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(v[j], w[j]);
             uint2 d[P];
             digits8<P>(x, inv, d);
 #pragma unroll
-            for (int p = 0; p < P; ++p)
-                *reinterpret_cast<uint2*>(a.rows + ((int64_t)p * g.M + m) * g.W + c0 + ch * 8) = d[p];
+            for (int p = 0; p < P; ++p) {
+                int8_t* out = row_out + (int64_t)p * g.M * g.W + (int64_t)i * 32 * g.W;
+                if (F32) {
+                    *reinterpret_cast<uint32_t*>(out + ca) = d[p].x;
+                    if (in_b) *reinterpret_cast<uint32_t*>(out + cb) = d[p].y;
+                } else {
+                    *reinterpret_cast<uint2*>(out + ca) = d[p];
+                }
+            }
         }
         if (a.cols || a.partial) {
-            const int x = (r >> 4) << 2;
-            *reinterpret_cast<float4*>(tile + r * 64 + ((ch * 8) ^ x)) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(tile + r * 64 + ((ch * 8 + 4) ^ x)) = make_float4(v[4], v[5], v[6], v[7]);
+            tile[r * 16 + (ch ^ (r >> 4))] = make_float4(v[0], v[1], v[2], v[3]);
+            tile[r * 16 + ((ch + 8) ^ (r >> 4))] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
     if (!a.cols && !a.partial) return;
@@ -377,33 +426,29 @@ __global__ void __launch_bounds__(256) int8_grad_digits_kernel(const GradDigits 
     const int sg = lane >> 2;                                   // rows 16 sg .. + 15
 #pragma unroll
     for (int it = 0; it < 2; ++it) {
-        const int c = warp * 8 + it * 4 + (lane & 3);
+        const int c = (F32 ? it * 32 + warp * 4 : warp * 8 + it * 4) + (lane & 3);
+        const float* from = reinterpret_cast<const float*>(tile + sg * 256 + ((warp + it * 8) ^ sg)) + (lane & 3);
         float v[16];
-        float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            v[i] = tile[(sg * 16 + i) * 64 + (c ^ (sg << 2))];
-            sum += v[i];
-        }
+        for (int i = 0; i < 16; ++i) v[i] = from[i * 64];
         if (a.partial) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += v[i];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             if (lane < 4 && c < valid) a.partial[(int64_t)blockIdx.y * g.W + c0 + c] = sum;
         }
         if (a.cols && c < valid && m0 + sg * 16 < a.ldm) {
-            const float amax = __uint_as_float(g.col_max[c0 + c]);
-            const float s = digit_scale<P>(amax);
-            if (m0 == 0 && sg == 0) a.col_scale[c0 + c] = s;
-            const float inv = __frcp_rn(s);
+            const float inv = s_col_inv[c];
             uint2 d[2][P];
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int64_t m = m0 + sg * 16 + hf * 8 + i;
-                    x[i] = m < g.M ? __fmul_rn(v[hf * 8 + i], __ldg(g.xs + m)) : 0.0f;
-                }
+                const float4 x0 = s_xs[sg * 4 + hf * 2], x1 = s_xs[sg * 4 + hf * 2 + 1];
+                const float* u = v + hf * 8;
+                const float x[8] = {__fmul_rn(u[0], x0.x), __fmul_rn(u[1], x0.y), __fmul_rn(u[2], x0.z),
+                                    __fmul_rn(u[3], x0.w), __fmul_rn(u[4], x1.x), __fmul_rn(u[5], x1.y),
+                                    __fmul_rn(u[6], x1.z), __fmul_rn(u[7], x1.w)};
                 digits8<P>(x, inv, d[hf]);
             }
 #pragma unroll
