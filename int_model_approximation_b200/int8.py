@@ -14,7 +14,8 @@ There is no counterpart in the reference.
                     in one kernel
   int8_linear_backward, int8_gated_backward   their gradients as plain calls
 
-int8_linear and int8_gated take part in autograd.  Gradients pass straight through the
+int8_linear and int8_gated take part in autograd (a whole training step can be captured into a CUDA
+graph if no eager autograd graph of the same leaves is alive; the *_backward calls can always).  Gradients pass straight through the
 rounding: they are the derivatives at the dequantised activations and weights, with the
 scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
 gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
@@ -88,9 +89,11 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-def _empty_codes(rows: int, k: int, device: torch.device) -> torch.Tensor:
-    """int8 [rows, k] whose rows start on 16 bytes."""
-    return torch.empty((rows, _round_up(max(k, 1), 16)), dtype=torch.int8, device=device)[:, :k]
+def _empty_codes(rows: int, k: int, like: torch.Tensor) -> torch.Tensor:
+    """int8 [rows, k] whose rows start on 16 bytes, on the device of `like`."""
+    ld = _round_up(max(k, 1), 16)
+    t = like.new_empty((rows, ld), dtype=torch.int8)
+    return t if ld == k else t[:, :k]
 
 
 def _aligned_codes(t: torch.Tensor, label: str) -> torch.Tensor:
@@ -104,7 +107,7 @@ def _aligned_codes(t: torch.Tensor, label: str) -> torch.Tensor:
     one_row = t.shape[0] <= 1
     if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or t.data_ptr() % 16 or
                       not one_row and (t.stride(0) % 16 or t.stride(0) < t.shape[1])):
-        out = _empty_codes(t.shape[0], t.shape[1], t.device)
+        out = _empty_codes(t.shape[0], t.shape[1], t)
         out.copy_(t)
         return out
     return t
@@ -133,20 +136,25 @@ def per_token_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _quantise(rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     m, k = rows.shape
-    dev = rows.device
-    q = _empty_codes(m, k, dev)
-    scale = torch.empty((m, 1), dtype=torch.float32, device=dev)
-    _call(dev, "ima_int8_quantize_rows", rows.data_ptr(), nat.dtype_code(rows.dtype), m, k, _ld(rows), q.data_ptr(),
-          _code_ld(q), scale.data_ptr())
+    if rows.dtype not in _DTYPE_CODES:
+        nat.dtype_code(rows.dtype)
+    q = _empty_codes(m, k, rows)
+    scale = rows.new_empty((m, 1), dtype=torch.float32)
+    _call(rows.device, "ima_int8_quantize_rows", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows),
+          q.data_ptr(), _code_ld(q), scale.data_ptr())
     return q, scale
 
 
 def _transpose(t: torch.Tensor) -> torch.Tensor:
     """int8 [rows, cols] (aligned) -> [cols, rows]."""
     rows, cols = t.shape
-    out = _empty_codes(cols, rows, t.device)
+    out = _empty_codes(cols, rows, t)
     _call(t.device, "ima_int8_transpose", t.data_ptr(), rows, cols, _code_ld(t), out.data_ptr(), _code_ld(out))
     return out
+
+
+def _capturing() -> bool:
+    return torch.cuda.is_current_stream_capturing()
 
 
 class Int8Weight:
@@ -157,11 +165,14 @@ class Int8Weight:
     one and kept until the codes change."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
-        self.codes = _aligned_codes(codes.detach(), "int8 weight")
+        codes = _aligned_codes(codes.detach(), "int8 weight")
         nat.require_device(codes.device, ("weight scale", scale))
-        self.scale = _scales(scale, codes.shape[0], "weight scale")
-        self.shape, self.device, self.ld = self.codes.shape, self.codes.device, _code_ld(self.codes)
-        self._transposed: tuple | None = None
+        self._set(codes, _scales(scale, codes.shape[0], "weight scale"))
+
+    def _set(self, codes: torch.Tensor, scale: torch.Tensor) -> None:
+        self.codes, self.scale = codes, scale
+        self.shape, self.device, self.ld = codes.shape, codes.device, _code_ld(codes)
+        self._transposed: tuple | None = None   # (codes [K, N], version of self.codes, stream, event until it has passed)
 
     @classmethod
     def from_float(cls, weight: torch.Tensor) -> "Int8Weight":
@@ -169,14 +180,40 @@ class Int8Weight:
         if weight.ndim != 2:
             raise RuntimeError(f"int8 weight source must be 2-D, got {tuple(weight.shape)}")
         _require_cuda(weight, "int8 weight source")
-        return cls(*per_token_int8(weight))
+        if weight.shape[1] > MAX_K:
+            raise RuntimeError(f"int8 weight: contraction of {weight.shape[1]} exceeds {MAX_K} (exact int32 sums)")
+        codes, scale = _quantise(_rows(weight.detach()))
+        made = cls.__new__(cls)
+        made._set(codes, scale.view(-1))
+        return made
 
-    def transposed(self) -> torch.Tensor:
+    def transposed(self) -> torch.Tensor | None:
+        """The transposed codes [K, N], made once.  None where the kept copy cannot be used (codes without
+        a version counter; a capture before it exists or is complete): the caller makes its own."""
         version = nat.tensor_version(self.codes)
-        if self._transposed is not None and version is not None and self._transposed[1] == version:
-            return self._transposed[0]
-        t = _transpose(self.codes)
-        self._transposed = (t, version)
+        kept = self._transposed
+        if version is None:
+            return None
+        stream = torch.cuda.current_stream(self.device)
+        if kept is None or kept[1] != version:
+            if _capturing():    # what a capture writes is not there before its replay
+                return None
+            with torch.inference_mode(False):
+                t = _transpose(self.codes)
+            event = torch.cuda.Event()
+            event.record(stream)
+            self._transposed = (t, version, stream, event)
+            return t
+        t, _version, maker, event = kept
+        if event is not None and stream != maker:
+            if _capturing():
+                return None
+            if event.query():
+                self._transposed = (t, version, maker, None)
+            else:
+                stream.wait_event(event)
+        if stream != maker and not _capturing():
+            t.record_stream(stream)
         return t
 
 
@@ -309,13 +346,20 @@ def _check_backward(m: int, contraction: int, want_dw: bool) -> None:
         raise RuntimeError(f"int8 weight gradient over {m} tokens exceeds {MAX_K} (exact int32 sums); split the batch")
 
 
+def _check_types(*dtypes: torch.dtype | None) -> None:
+    for dtype in dtypes:
+        if dtype is not None:
+            nat.dtype_code(dtype)
+
+
 def _grad_rows(grad: torch.Tensor, m: int, n: int, dev: torch.device) -> torch.Tensor:
     if grad.shape[-1] != n or grad.numel() != m * n:
         raise RuntimeError(f"output gradient has shape {tuple(grad.shape)}, expected {m} rows of {n}")
     if grad.device != dev:
         nat.require_device(dev, ("output gradient", grad))
-    nat.dtype_code(grad.dtype)
-    return _rows(grad.detach().reshape(m, n))
+    if grad.dtype not in _DTYPE_CODES:
+        nat.dtype_code(grad.dtype)
+    return _rows(grad if grad.ndim == 2 else grad.reshape(m, n))
 
 
 def _one_type(*dtypes: torch.dtype | None) -> torch.dtype | None:
@@ -350,21 +394,25 @@ def int8_linear_backward(
     weight), else it is temporary.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
     (m, k), n = codes.shape, weight.shape[0]
-    dev = codes.device
     if weight.shape[1] != k:
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={weight.shape[1]}")
-    nat.require_device(dev, ("weight", weight.codes), ("scale", scale))
-    scale = _scales(scale, m, "scale")
-    d = _grad_rows(grad, m, n, dev)
+    nat.require_device(codes.device, ("weight", weight.codes), ("scale", scale))
+    _check_types(dx_dtype, dw_dtype, db_dtype)
     _check_backward(m, n if dx_dtype is not None else 0, dw_dtype is not None)
+    return _linear_backward(grad, codes, _scales(scale, m, "scale"), weight, dx_dtype, dw_dtype, db_dtype, keep_transposed)
+
+
+def _linear_backward(grad, codes, scale, weight, dx_dtype, dw_dtype, db_dtype, keep_transposed):
+    (m, k), n = codes.shape, weight.shape[0]
+    d = _grad_rows(grad, m, n, codes.device)
     planes = _digit_count(d.dtype, dx_dtype, dw_dtype)
     dx, dw, db = _out(scale, (m, k), dx_dtype), _out(scale, (n, k), dw_dtype), _out(scale, (n,), db_dtype)
     wt = weight.transposed() if dx is not None and keep_transposed else None
     nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 0, planes, dx is not None, dw is not None,
                                                          db is not None, wt is None)
     ws = scale.new_empty((nbytes,), dtype=torch.uint8)
-    _call(dev, "ima_int8_linear_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, codes.data_ptr(),
-          _code_ld(codes), scale.data_ptr(), weight.codes.data_ptr(), weight.ld, _ptr(wt),
+    _call(codes.device, "ima_int8_linear_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k,
+          codes.data_ptr(), _code_ld(codes), scale.data_ptr(), weight.codes.data_ptr(), weight.ld, _ptr(wt),
           _code_ld(wt) if wt is not None else 0, weight.scale.data_ptr(), planes, _ptr(dx), _code(dx), _ptr(dw),
           _code(dw), _ptr(db), _code(db), ws.data_ptr())
     return dx, dw, db
@@ -394,14 +442,22 @@ def int8_gated_backward(
     one byte per activation and nothing of width N.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
     (m, k), n = codes.shape, gate.shape[0]
-    dev = codes.device
     _check_gated(k, gate, up, activation)
-    nat.require_device(dev, ("gate weight", gate.codes), ("up weight", up.codes), ("scale", scale),
+    nat.require_device(codes.device, ("gate weight", gate.codes), ("up weight", up.codes), ("scale", scale),
                        ("gate bias", gate_bias), ("up bias", up_bias))
-    scale = _scales(scale, m, "scale")
-    d = _grad_rows(grad, m, n, dev)
+    types = (dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype)
+    _check_types(*types)
+    _check_backward(m, _round_up(n, 128) + n if dx_dtype is not None else 0,
+                    dgate_dtype is not None or dup_dtype is not None)
+    return _gated_backward(grad, codes, _scales(scale, m, "scale"), gate, up, gate_bias, up_bias, activation, types,
+                           keep_transposed)
+
+
+def _gated_backward(grad, codes, scale, gate, up, gate_bias, up_bias, activation, types, keep_transposed):
+    dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype = types
+    (m, k), n = codes.shape, gate.shape[0]
+    d = _grad_rows(grad, m, n, codes.device)
     want_dw = dgate_dtype is not None or dup_dtype is not None
-    _check_backward(m, _round_up(n, 128) + n if dx_dtype is not None else 0, want_dw)
     planes = _digit_count(d.dtype, dx_dtype, dgate_dtype, dup_dtype)
     w_type, b_type = _one_type(dgate_dtype, dup_dtype), _one_type(gate_db_dtype, up_db_dtype)
     dx = _out(scale, (m, k), dx_dtype)
@@ -411,18 +467,18 @@ def int8_gated_backward(
     if dx is not None and keep_transposed:
         gt, ut = gate.transposed(), up.transposed()
     nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 1, planes, dx is not None, want_dw, b_type is not None,
-                                                         gt is None)
+                                                         gt is None or ut is None)
     ws = scale.new_empty((nbytes,), dtype=torch.uint8)
     (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(dev, "ima_int8_gated_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, codes.data_ptr(),
+    _call(codes.device, "ima_int8_gated_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, codes.data_ptr(),
           _code_ld(codes), scale.data_ptr(), gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(),
           up.ld, _ptr(gt), _code_ld(gt) if gt is not None else 0, _ptr(ut),
           _code_ld(ut) if ut is not None else 0, gate.scale.data_ptr(), up.scale.data_ptr(), _ptr(gate_bias),
           _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], planes, _ptr(dx), _code(dx), _ptr(dgate), _ptr(dup),
           _code(dgate if dgate is not None else dup), _ptr(dgb), _ptr(dub), _code(dgb if dgb is not None else dub),
           ws.data_ptr())
-    outs = zip((dx, dgate, dup, dgb, dub), (dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype))
-    return tuple(None if t is None else t.to(dtype) for t, dtype in outs)
+    return tuple(None if t is None else t if t.dtype == dtype else t.to(dtype)
+                 for t, dtype in zip((dx, dgate, dup, dgb, dub), types))
 
 
 # ---------------------------------------------------------------------------
@@ -448,26 +504,62 @@ def _wants_grad(*tensors) -> bool:
     return False
 
 
+_STREAM_MARK = "int8_recorded_on"
+
+
+def _record(function, leaves, *args):
+    """function.apply(*args), keeping captures safe.  The node that accumulates a leaf's gradient works on
+    the stream it was made on, and lives as long as any graph with the leaf.  A capture that records a
+    backward pass through a node of another stream ends the process when it runs that pass: eager
+    recordings leave a mark on the nodes, and a capture that finds one is refused before it records."""
+    leaves = [t for t in leaves if t is not None and t.requires_grad and t.is_leaf]
+    stream = _raw_stream(_current_device())
+    if not _capturing():
+        out = function.apply(*args)
+        for t in leaves:
+            torch.autograd.graph.get_gradient_edge(t).node.metadata.setdefault(_STREAM_MARK, stream)
+        return out
+    for t in leaves:
+        if torch.autograd.graph.get_gradient_edge(t).node.metadata.get(_STREAM_MARK, stream) != stream:
+            raise RuntimeError("an eager autograd graph of this leaf tensor is alive on another stream: release it before "
+                               "capturing a backward pass, or capture int8_linear_backward / int8_gated_backward, which "
+                               "record nothing")
+    return function.apply(*args)
+
+
+def _versions(*weights: Int8Weight) -> tuple:
+    return tuple(nat.tensor_version(w.codes) for w in weights)
+
+
+def _check_versions(before: tuple, *weights: Int8Weight) -> None:
+    if before != _versions(*weights):
+        raise RuntimeError("int8 weight codes were modified in place between the forward and the backward pass")
+
+
+def _wanted_types(ctx, inputs) -> tuple:
+    return tuple(t.dtype if need else None for t, need in zip(inputs, ctx.needs_input_grad))
+
+
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, handle):
         w = handle if handle is not None else Int8Weight.from_float(weight)
         y, q, scale = _linear_forward(_rows(x.detach()), w, bias, keep=True)
         ctx.save_for_backward(q, scale)
-        ctx.weight, ctx.frozen = w, handle is not None
-        ctx.types = tuple(t.dtype if t is not None and need else None
-                          for t, need in zip((x, weight, bias), ctx.needs_input_grad))
+        ctx.weight, ctx.frozen, ctx.version = w, handle is not None, _versions(w)
+        ctx.types = _wanted_types(ctx, (x, weight, bias))
         ctx.shapes = (x.shape, None if bias is None else bias.shape)
-        return y.reshape(*x.shape[:-1], w.shape[0])
+        return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         q, scale = ctx.saved_tensors
-        dx, dw, db = int8_linear_backward(grad, q, scale, ctx.weight, dx_dtype=ctx.types[0], dw_dtype=ctx.types[1],
-                                          db_dtype=ctx.types[2], keep_transposed=ctx.frozen)
-        return (None if dx is None else dx.reshape(ctx.shapes[0]), dw, None if db is None else db.reshape(ctx.shapes[1]),
-                None)
+        _check_versions(ctx.version, ctx.weight)
+        dx, dw, db = _linear_backward(grad, q, scale, ctx.weight, *ctx.types, ctx.frozen)
+        if dx is not None and len(ctx.shapes[0]) != 2:
+            dx = dx.reshape(ctx.shapes[0])
+        return dx, dw, None if db is None else db.reshape(ctx.shapes[1]), None
 
 
 class _GatedFunction(torch.autograd.Function):
@@ -477,21 +569,20 @@ class _GatedFunction(torch.autograd.Function):
         u = up if up is not None else Int8Weight.from_float(up_weight)
         h, q, scale = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation, keep=True)
         ctx.save_for_backward(q, scale, gate_bias, up_bias)
-        ctx.gate, ctx.up, ctx.activation = g, u, activation
+        ctx.gate, ctx.up, ctx.activation, ctx.version = g, u, activation, _versions(g, u)
         ctx.frozen = gate is not None and up is not None
         inputs = (x, gate_weight, up_weight, gate_bias, up_bias)
-        ctx.types = tuple(t.dtype if t is not None and need else None for t, need in zip(inputs, ctx.needs_input_grad))
+        ctx.types = _wanted_types(ctx, inputs)
         ctx.shapes = tuple(None if t is None else t.shape for t in inputs)
-        return h.reshape(*x.shape[:-1], g.shape[0])
+        return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         q, scale, gate_bias, up_bias = ctx.saved_tensors
-        tx, tg, tu, tgb, tub = ctx.types
-        grads = int8_gated_backward(grad, q, scale, ctx.gate, ctx.up, gate_bias, up_bias, activation=ctx.activation,
-                                    dx_dtype=tx, dgate_dtype=tg, dup_dtype=tu, gate_db_dtype=tgb, up_db_dtype=tub,
-                                    keep_transposed=ctx.frozen)
+        _check_versions(ctx.version, ctx.gate, ctx.up)
+        grads = _gated_backward(grad, q, scale, ctx.gate, ctx.up, gate_bias, up_bias, ctx.activation, ctx.types,
+                                ctx.frozen)
         return (*(None if g is None else g.reshape(shape) for g, shape in zip(grads, ctx.shapes)), None, None, None)
 
 
@@ -530,7 +621,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
         frozen = isinstance(weight, Int8Weight)
         _check_backward(x.numel() // max(x.shape[-1], 1), weight.shape[0] if x.requires_grad else 0,
                         not frozen and weight.requires_grad)
-        return _LinearFunction.apply(x, None if frozen else weight, bias, weight if frozen else None)
+        w = None if frozen else weight
+        return _record(_LinearFunction, (x, w, bias), x, w, bias, weight if frozen else None)
     w = _weight_of(weight)
     y, _q, _s = _linear_forward(_rows(x), w, bias)
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
@@ -556,8 +648,9 @@ def int8_gated(
         _check_backward(x.numel() // max(x.shape[-1], 1),
                         _round_up(gate.shape[0], 128) + gate.shape[0] if x.requires_grad else 0,
                         any(not f and w.requires_grad for f, w in zip(frozen, (gate, up))))
-        return _GatedFunction.apply(x, None if frozen[0] else gate, None if frozen[1] else up, gate_bias, up_bias,
-                                    gate if frozen[0] else None, up if frozen[1] else None, activation)
+        inputs = (x, None if frozen[0] else gate, None if frozen[1] else up, gate_bias, up_bias)
+        return _record(_GatedFunction, inputs, *inputs, gate if frozen[0] else None, up if frozen[1] else None,
+                       activation)
     g, u = _weight_of(gate), _weight_of(up)
     h, _q, _s = _gated_forward(_rows(x), g, u, gate_bias, up_bias, activation)
     return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])

@@ -656,6 +656,72 @@ def test_captured_and_replayed_calls_follow_their_inputs(cuda_device, m):
 
 
 @pytest.mark.gpu
+def test_captured_training_step_and_live_eager_graphs(cuda_device):
+    """A captured forward and backward pass; refused while an eager graph of the same leaves lives (its
+    accumulation node belongs to another stream), fine once it is gone."""
+    m, n, k = 40, 64, 96
+    x, w, b = make(m, n, k, torch.float32, 31, cuda_device, bias=True)
+    for t in (x, w, b):
+        t.requires_grad_()
+    dy = torch.randn((m, n), device=cuda_device)
+
+    def step():
+        return torch.autograd.grad(int8.int8_gated(x, w, w, b, None), (x, w, b), dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    alive = int8.int8_linear(x, w, b)
+    with pytest.raises(RuntimeError, match="eager autograd graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            int8.int8_gated(x, w, w, b, None)
+    torch.autograd.grad(alive, (x, w, b), dy)   # the eager graph is unharmed
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    with torch.no_grad():
+        x.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, step()))
+    status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+def test_codes_edited_between_forward_and_backward_are_refused(cuda_device):
+    x, w, _ = make(8, 16, 32, torch.float32, 32, cuda_device)
+    x.requires_grad_()
+    wt = int8.Int8Weight.from_float(w)
+    y = int8.int8_linear(x, wt)
+    wt.codes.zero_()
+    with pytest.raises(RuntimeError, match="modified in place"):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_kept_transposed_codes_on_another_stream(cuda_device):
+    """The transposed copy a first backward pass makes is waited for by a pass on another stream."""
+    x, w, _ = make(64, 3584, 4096, torch.bfloat16, 33, cuda_device)
+    dy = torch.randn((64, 3584), device=cuda_device).to(torch.bfloat16)
+    q, s = int8.per_token_int8(x)
+    fresh = int8.Int8Weight.from_float(w)
+    want = int8.int8_linear_backward(dy, q, s, fresh, dx_dtype=torch.bfloat16, keep_transposed=False)[0]
+    for _ in range(5):
+        wt = int8.Int8Weight.from_float(w)
+        a, b = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            first = int8.int8_linear_backward(dy, q, s, wt, dx_dtype=torch.bfloat16)[0]
+        with torch.cuda.stream(b):
+            second = int8.int8_linear_backward(dy, q, s, wt, dx_dtype=torch.bfloat16)[0]
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and torch.equal(second, want)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(cuda_device):
     x, w, _ = make(300, 500, 1024, torch.bfloat16, 14, cuda_device)
     wt = int8.Int8Weight.from_float(w)
