@@ -9,22 +9,23 @@ int64_t i8_steps(int64_t Ka) { return (Ka + I8_KT - 1) / I8_KT; }
 
 // Time of the tiled form in ns: rounds of 128 x bn tiles over the machine at the tensor core's rate (8192
 // multiplications per clock and SM at 1.6 GHz), two thirds of it while a stage's loads limit it, and
-// 8 us from launch to the end of the last epilogue.
+// 8 us from launch to the end of the last epilogue; at least the time that B takes to arrive.
 double tiled_ns(int64_t M, int64_t N, int64_t k_steps, int planes, int bn) {
     const int64_t tiles = ((M + I8_BM - 1) / I8_BM) * ((N + bn - 1) / bn);
     const int64_t rounds = (tiles + gemm_grid_limit() - 1) / gemm_grid_limit();
-    return (double)rounds * (double)k_steps * planes * bn * 128.0 * 128.0 / (8192.0 * 1.6 * 0.67) + 8000.0;
+    const double mma = (double)rounds * (double)k_steps * planes * bn * 128.0 * 128.0 / (8192.0 * 1.6 * 0.67);
+    return std::max(mma, (double)(N * k_steps * I8_KT) / 5000.0) + 8000.0;
 }
 
 // The form with the shorter estimate.
 int run_linear(I8Params& p, const I8Operands& o, cudaStream_t st) {
-    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.K), 1, 1, false);
+    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.K), 1, 1, -1);
     if (q.ok && q.ns < tiled_ns(p.M, p.N, i8_steps(o.K), 1, 256)) return run_skinny_codes<I8_LINEAR, 1>(p, o, q, st);
     return launch_i8<1, 256, I8_LINEAR>(p, o, st);
 }
 
 int run_gated(I8Params& p, const I8Operands& o, cudaStream_t st) {
-    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.K), 1, 2, false);
+    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.K), 1, 2, -1);
     if (q.ok && q.ns < tiled_ns(p.M, 2 * (int64_t)p.N, i8_steps(o.K), 1, 256))
         return run_skinny_codes<I8_GATED, 1>(p, o, q, st);
     return launch_i8<1, 256, I8_GATED>(p, o, st);
@@ -32,7 +33,7 @@ int run_gated(I8Params& p, const I8Operands& o, cudaStream_t st) {
 
 template <int P, int BN>
 int run_digits(I8Params& p, const I8Operands& o, cudaStream_t st) {
-    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.Ka), P, 1, false);
+    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.Ka), P, 1, -1);
     if (q.ok && q.ns < tiled_ns(p.M, p.N, i8_steps(o.Ka), P, BN)) return run_skinny_codes<I8_DIGIT, P>(p, o, q, st);
     return launch_i8<P, BN, I8_DIGIT>(p, o, st);
 }
@@ -44,12 +45,15 @@ int run_fused(SkParams& p, int x_dtype, const SkPlan& q, cudaStream_t st) {
     return launch_skinny<EPI, 1, IMA_DTYPE_F32>(p, q, st);
 }
 
-// Whether the tokens are quantised inside the product: every cluster then does it for itself, which
-// pays while the workers hold a CTA's share in one batch of loads.
+// Whether the tokens are quantised inside the product: if it can, and a split that allows it costs no more
+// than the 3.5 us that the row quantiser and its launch add.
 bool fused_plan(int64_t M, int64_t N, int64_t K, int ops, int x_dtype, SkPlan& q) {
-    if (M < 1 || M > 16 || N < 1) return false;
-    q = sk_plan(M, N, i8_steps(K), 1, ops, true);
-    return q.ok && M * ((q.k_steps + q.splits - 1) / q.splits) * I8_KT <= SK_WORKERS * 32 * sk_batch(x_dtype) * 8;
+    if (M < 1 || M > SK_MAX_TM || N < 1) return false;
+    q = sk_plan(M, N, i8_steps(K), 1, ops, x_dtype);
+    if (!q.ok) return false;
+    const SkPlan codes = sk_plan(M, N, i8_steps(K), 1, ops, -1);
+    const double tiled = tiled_ns(M, ops * N, i8_steps(K), 1, 256);
+    return q.ns <= std::min(codes.ok ? codes.ns : tiled, tiled) + 3500.0;
 }
 
 }  // namespace

@@ -150,24 +150,24 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
 
     // ---- phase 1: row maxima of this CTA's slice ----
     const int64_t kbeg = (int64_t)s0 * I8_KT, kend = min(p.K, (int64_t)s1 * I8_KT);
-    // eight warps over the tokens, or several warps per token when there are fewer
-    const int wpt = rows >= 8 || !FUSED ? 1 : (rows > 4 ? 1 : (rows > 2 ? 2 : (rows > 1 ? 4 : 8)));
-    const int tok0 = (warp - 2) / wpt, tok_step = SK_WORKERS / wpt;
-    const int chunk0 = ((warp - 2) % wpt) * 32 + lane, chunk_step = wpt * 32;
-    const int chunks = FUSED ? (int)((kend - kbeg + 7) / 8) : 0;
-    const bool resident = FUSED && chunks <= BATCH * chunk_step && rows <= tok_step;   // one batch holds it all
+    // units of 256 elements of a token's slice, dealt to the warps in turn, at most BATCH each (sk_plan): loaded
+    // once, kept until the scales are known
+    const int per_tok = FUSED ? max(1, (int)((kend - kbeg + 255) / 256)) : 1;
+    const int units = FUSED && kend > kbeg ? rows * per_tok : 0;
     Raw8<XT> batch[FUSED ? BATCH : 1];
-    auto x_row = [&](int t) {
-        return reinterpret_cast<const unsigned char*>(p.x) + (int64_t)(m0 + t) * p.ldx * dtype_bytes(XT);
-    };
-    auto load_batch = [&](const unsigned char* row, int c0) {
-        const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
+    auto load_batch = [&](int u0) {
 #pragma unroll
         for (int i = 0; i < (FUSED ? BATCH : 0); ++i) {
-            const int64_t k = kbeg + (int64_t)(c0 + i * chunk_step) * 8;
-            if (vec && k + 8 <= kend) batch[i].load_whole(row, k);
-            else if (k < kend) batch[i].load(row, k, kend, false);
-            else batch[i].clear();
+            const int u = u0 + i * SK_WORKERS;
+            batch[i].clear();
+            if (u < units) {
+                const int t = u / per_tok;
+                const int64_t k = kbeg + (int64_t)(u - t * per_tok) * 256 + lane * 8;
+                const unsigned char* row =
+                    reinterpret_cast<const unsigned char*>(p.x) + (int64_t)(m0 + t) * p.ldx * dtype_bytes(XT);
+                if ((reinterpret_cast<uintptr_t>(row) & 15) == 0 && k + 8 <= kend) batch[i].load_whole(row, k);
+                else if (k < kend) batch[i].load(row, k, kend, false);
+            }
         }
     };
     if (warp == 0 && lane == 0) {
@@ -176,16 +176,13 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
             for (int i = 0; i < first; ++i) load_tokens(i);
         }
     } else if (FUSED && warp >= 2) {
-        for (int t = tok0; t < rows; t += tok_step) {
-            const unsigned char* row = x_row(t);
-            uint32_t mx = 0;
-            for (int c0 = chunk0; c0 < chunks; c0 += BATCH * chunk_step) {
-                load_batch(row, c0);
+        load_batch(warp - 2);
 #pragma unroll
-                for (int i = 0; i < (FUSED ? BATCH : 0); ++i) mx = max(mx, batch[i].max_bits());
-            }
-            mx = __reduce_max_sync(0xFFFFFFFFu, mx);
-            if (lane == 0) atomicMax(&s_amax[rank * SK_MAX_TM + t], mx);
+        for (int i = 0; i < (FUSED ? BATCH : 0); ++i) {
+            const int u = warp - 2 + i * SK_WORKERS;
+            if (u >= units) break;
+            const uint32_t mx = __reduce_max_sync(0xFFFFFFFFu, batch[i].max_bits());
+            if (lane == 0) atomicMax(&s_amax[rank * SK_MAX_TM + u / per_tok], mx);
         }
     }
     if (S > 1) {
@@ -256,24 +253,20 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
                 s_scale[t] = i8_row_scale(a, a != a);
             }
             named_barrier_sync(1, SK_WORKERS * 32);
-            for (int t = tok0; t < rows; t += tok_step) {
-                const unsigned char* row = x_row(t);
-                const float s = s_scale[t];
-                const I8Inv inv = i8_inv(s);
-                for (int c0 = chunk0; c0 < chunks; c0 += BATCH * chunk_step) {
-                    if (!resident) load_batch(row, c0);
 #pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        const int off = (c0 + i * chunk_step) * 8;      // element of the slice
-                        if (off >= chunks * 8) break;
-                        float v[8];
-                        batch[i].unpack(v);
-                        // k-step off / 128, token t, 16-byte piece (off % 128) / 16 at its swizzled place
-                        unsigned char* dst = codes + (off >> 7) * tok_bytes + t * I8_KT +
-                                             ((((off >> 4) & 7) ^ (t & 7)) << 4) + (off & 8);
-                        *reinterpret_cast<uint2*>(dst) = i8_codes8<XT>(v, s, inv);
-                    }
-                }
+            for (int i = 0; i < BATCH; ++i) {
+                const int u = warp - 2 + i * SK_WORKERS;
+                if (u >= units) break;
+                const int t = u / per_tok;
+                const int off = (u - t * per_tok) * 256 + lane * 8;     // element of the slice
+                if (kbeg + off >= kend) continue;
+                const float s = s_scale[t];
+                float v[8];
+                batch[i].unpack(v);
+                // k-step off / 128, token t, 16-byte piece (off % 128) / 16 at its swizzled place
+                unsigned char* dst = codes + (off >> 7) * tok_bytes + t * I8_KT +
+                                     ((((off >> 4) & 7) ^ (t & 7)) << 4) + (off & 8);
+                *reinterpret_cast<uint2*>(dst) = i8_codes8<XT>(v, s, i8_inv(s));
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -441,15 +434,19 @@ struct SkPlan {
 // stages and an estimate of its time, from measurements: 6 us for a round of CTAs from launch to exit and
 // 12 ns per token column of its epilogue, a stream of 45 bytes/ns into an SM and 5800 into the machine
 // (a kernel that only loads 68 MB takes 15.0 us), 1 us for the exchange of a cluster.
-SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, bool fused) {
+// The fused quantiser (x_dtype >= 0) takes what its workers hold in registers at once: another pass over the
+// activations costs 6 us (64 tokens, K = 3584), more than the row quantiser and its launch.
+SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x_dtype) {
+    const bool fused = x_dtype >= 0;
     const int max_tm = planes == 3 ? 32 : (planes == 2 || ops == 2 ? 64 : SK_MAX_TM);
     SkPlan best = {};
     const int64_t m_tiles = (M + max_tm - 1) / max_tm, n_tiles = (N + SK_ROWS - 1) / SK_ROWS;
     const int64_t tm = ((M + m_tiles - 1) / m_tiles + 15) / 16 * 16;
-    if (m_tiles > 65535) return best;
+    if (m_tiles > 65535 || (fused && m_tiles > 1)) return best;
     for (int s = 1; s <= 8 && s <= std::max<int64_t>(k_steps, 1); s *= 2) {
         SkPlan q = {};
         const int64_t steps = (k_steps + s - 1) / s;
+        if (fused && M * ((steps * I8_KT + 255) / 256) > SK_WORKERS * sk_batch(x_dtype)) continue;
         const int64_t tok = (int64_t)planes * tm * I8_KT;
         const int64_t codes = fused ? steps * tok : 0;
         const int64_t stage = (int64_t)ops * SK_ROWS * I8_KT + (fused ? 0 : tok);

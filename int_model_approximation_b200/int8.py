@@ -118,10 +118,11 @@ def _code_ld(t: torch.Tensor) -> int:
 
 
 def _scales(t: torch.Tensor, n: int, label: str) -> torch.Tensor:
-    s = t.detach().reshape(-1).to(torch.float32).contiguous()
-    if s.numel() != n:
-        raise RuntimeError(f"{label} has {s.numel()} entries, expected {n}")
-    return s
+    if t.numel() != n:
+        raise RuntimeError(f"{label} has {t.numel()} entries, expected {n}")
+    if t.dtype == torch.float32 and t.is_contiguous():
+        return t
+    return t.detach().reshape(-1).to(torch.float32).contiguous()
 
 
 def per_token_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -167,6 +168,8 @@ class Int8Weight:
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
         codes = _aligned_codes(codes.detach(), "int8 weight")
         nat.require_device(codes.device, ("weight scale", scale))
+        if scale.requires_grad:
+            raise RuntimeError("the scales of an Int8Weight are constants; give int8_linear a floating weight to train it")
         self._set(codes, _scales(scale, codes.shape[0], "weight scale"))
 
     def _set(self, codes: torch.Tensor, scale: torch.Tensor) -> None:
@@ -264,21 +267,29 @@ def int8_gemm(
     Returns (c int32 [M, N] or None, y [M, N] or None)."""
     a = _aligned_codes(a, "int8 activation matrix")
     b = _aligned_codes(b, "int8 weight matrix")
-    m, k = a.shape
-    n = b.shape[0]
+    (m, k), n = a.shape, b.shape[0]
     if b.shape[1] != k:
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={b.shape[1]}")
     dev = a.device
-    c = c_out if c_out is not None else (torch.empty((m, n), dtype=torch.int32, device=dev) if want_c else None)
-    if c is not None:
-        _check_out(c, (m, n), (torch.int32,), "int8 product")
+    for label, t in (("B matrix", b), ("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias), ("int32 output", c_out),
+                     ("output", y_out)):
+        if t is not None and t.device != dev:
+            nat.require_device(dev, (label, t))
+    if c_out is not None:
+        _check_out(c_out, (m, n), (torch.int32,), "int8 product")
+        c = c_out
+    else:
+        c = a.new_empty((m, n), dtype=torch.int32) if want_c else None
     y, bias_dtype = None, 0
     if y_dtype is not None or y_out is not None:
         if x_scale is None or w_scale is None:
             raise RuntimeError("int8_gemm needs x_scale and w_scale for the rescaled output")
-        y = y_out if y_out is not None else torch.empty((m, n), dtype=y_dtype, device=dev)
-        _check_out(y, (m, n), tuple(_DTYPE_CODES), "output")
-        nat.require_device(dev, ("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias))
+        if y_out is not None:
+            _check_out(y_out, (m, n), tuple(_DTYPE_CODES), "output")
+            y = y_out
+        else:
+            _check_types(y_dtype)
+            y = a.new_empty((m, n), dtype=y_dtype)
         x_scale = _scales(x_scale, m, "x_scale")
         w_scale = _scales(w_scale, n, "w_scale")
         (bias,), bias_dtype = _bias_args(n, bias)
@@ -286,33 +297,40 @@ def int8_gemm(
         x_scale = w_scale = bias = None
     if c is None and y is None:
         raise RuntimeError("int8_gemm has no output to compute: want_c, y_dtype or y_out")
-    nat.require_device(dev, ("B matrix", b), ("int32 output", c), ("output", y))
     _call(dev, "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, _ptr(c),
-          _ld(c) if c is not None else n, _ptr(x_scale), _ptr(w_scale), _ptr(bias), bias_dtype, _ptr(y),
-          nat.dtype_code(y.dtype) if y is not None else 0, _ld(y) if y is not None else n)
+          _ld(c) if c is not None else n, _ptr(x_scale), _ptr(w_scale), _ptr(bias), bias_dtype, _ptr(y), _code(y),
+          _ld(y) if y is not None else n)
     return c, y
 
 
 def _code_buffers(rows: torch.Tensor, n: int, gated: bool, keep: bool):
-    """Room for the codes and scales of x rows (None, None when the product quantises them itself)."""
+    """Room for the codes and scales of x rows: (codes, scale, their addresses); the tensors are kept by the
+    caller if it wants them, and all is None when the product quantises the rows itself."""
     m, k = rows.shape
-    if not keep and nat.lib().ima_int8_fused(m, n, k, gated, _DTYPE_CODES[rows.dtype]):
-        return None, None
-    return (rows.new_empty((m, _round_up(max(k, 1), 16)), dtype=torch.int8),
-            rows.new_empty((m,), dtype=torch.float32))
+    ld = _round_up(max(k, 1), 16)
+    if keep:
+        q, scale = rows.new_empty((m, ld), dtype=torch.int8), rows.new_empty((m,), dtype=torch.float32)
+        return q, scale, q.data_ptr(), ld, scale.data_ptr()
+    if nat.lib().ima_int8_fused(m, n, k, gated, _DTYPE_CODES[rows.dtype]):
+        return None, None, None, ld, None
+    ws = rows.new_empty((m * (ld + 4),), dtype=torch.uint8)
+    at = ws.data_ptr()
+    return ws, None, at, ld, at + m * ld
 
 
 def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None, keep: bool = False):
-    """(y [M, N], codes, scale) of x rows; codes and scale hold something only with keep."""
+    """(y [M, N], codes, scale) of x rows; codes and scale only with keep."""
     m, k = rows.shape
     n = weight.shape[0]
     y = rows.new_empty((m, n))
-    q, scale = _code_buffers(rows, n, False, keep)
-    (bias,), bias_dtype = _bias_args(n, bias)
-    _call(rows.device, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), _ptr(q),
-          _round_up(max(k, 1), 16), _ptr(scale), keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(),
-          _ptr(bias), bias_dtype, y.data_ptr(), max(n, 1))
-    return y, q[:, :k] if keep else None, scale
+    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, n, False, keep)
+    bias_dtype = 0
+    if bias is not None:
+        (bias,), bias_dtype = _bias_args(n, bias)
+    _call(rows.device, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q_ptr, ld, scale_ptr,
+          keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(), _ptr(bias), bias_dtype, y.data_ptr(),
+          n or 1)
+    return y, q[:, :k] if keep and ld != k else q, scale
 
 
 def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bias, up_bias, activation: str,
@@ -320,13 +338,14 @@ def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bi
     m, k = rows.shape
     n = gate.shape[0]
     h = rows.new_empty((m, n))
-    q, scale = _code_buffers(rows, n, True, keep)
-    (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(rows.device, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), _ptr(q),
-          _round_up(max(k, 1), 16), _ptr(scale), keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n,
-          gate.scale.data_ptr(), up.scale.data_ptr(), _ptr(gate_bias), _ptr(up_bias), bias_dtype,
-          ACTIVATIONS[activation], h.data_ptr(), max(n, 1))
-    return h, q[:, :k] if keep else None, scale
+    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, n, True, keep)
+    bias_dtype = 0
+    if gate_bias is not None or up_bias is not None:
+        (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
+    _call(rows.device, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q_ptr, ld, scale_ptr,
+          keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n, gate.scale.data_ptr(),
+          up.scale.data_ptr(), _ptr(gate_bias), _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], h.data_ptr(), n or 1)
+    return h, q[:, :k] if keep and ld != k else q, scale
 
 
 # ---------------------------------------------------------------------------
