@@ -23,8 +23,9 @@ namespace {
 constexpr int SK_ROWS = 128;                       // weight rows per tile and operand
 constexpr int SK_WORKERS = 8;
 constexpr int SK_THREADS = 64 + SK_WORKERS * 32;
-constexpr int SK_MAX_STAGES = 12;
+constexpr int SK_MAX_STAGES = 8;
 constexpr int SK_SMEM = 221 * 1024;              // with 5 KB static and 1 KB of the system: one CTA per SM at most
+constexpr int SK_SMEM_HALF = 107 * 1024;           // two CTAs per SM
 constexpr int SK_MAX_TM = 128;
 
 // Groups of eight elements that a lane of the fused quantiser has in flight (32 registers).
@@ -430,10 +431,12 @@ struct SkPlan {
     double ns;   // estimate
 };
 
-// The split form of a product of M tokens by N outputs over k_steps k-steps: tokens per tile, split,
-// stages and an estimate of its time, from measurements: 6 us for a round of CTAs from launch to exit and
-// 12 ns per token column of its epilogue, a stream of 45 bytes/ns into an SM and 5800 into the machine
-// (a kernel that only loads 68 MB takes 15.0 us), 1 us for the exchange of a cluster.
+// The split form of a product of M tokens by N outputs over k_steps k-steps: tokens per tile, split and
+// stages with the shortest estimate, which follows measurements.  A CTA streams its tiles at 34 bytes/ns
+// whatever its stages beyond three (a kernel that only loads 68 MB with one CTA per SM takes 15.0 us), the
+// machine at 5500; so two CTAs of four stages per SM beat one of eight (3584 x 18944 with 16 tokens: 18.9 us
+// with 224 CTAs, 24.6 with 112).  A round of CTAs takes 6 us from launch to exit besides, its epilogue 12
+// ns per token column, the exchange in a cluster 1 us.
 // The fused quantiser (x_dtype >= 0) takes what its workers hold in registers at once: another pass over the
 // activations costs 6 us (64 tokens, K = 3584), more than the row quantiser and its launch.
 SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x_dtype) {
@@ -451,18 +454,23 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x
         const int64_t codes = fused ? steps * tok : 0;
         const int64_t stage = (int64_t)ops * SK_ROWS * I8_KT + (fused ? 0 : tok);
         const int64_t partial = s > 1 ? (int64_t)ops * planes * tm * SK_ROWS * 4 : 0;
-        const int64_t fit = (SK_SMEM - 1024 - codes - partial) / stage;
-        const int64_t stages = std::min<int64_t>(std::min<int64_t>(fit, SK_MAX_STAGES), std::max<int64_t>(steps, 1));
-        if (stages < std::min<int64_t>(3, std::max<int64_t>(steps, 1))) continue;
+        const int64_t least = std::min<int64_t>(3, std::max<int64_t>(steps, 1));
+        const int64_t fixed = 1024 + codes + partial;
+        int64_t per_sm = 2, stages = std::min<int64_t>((SK_SMEM_HALF - fixed) / stage, 4);
+        if (stages < least) {
+            per_sm = 1;
+            stages = std::min<int64_t>((SK_SMEM - fixed) / stage, SK_MAX_STAGES);
+        }
+        if (stages < least) continue;
+        stages = std::min<int64_t>(stages, std::max<int64_t>(steps, 1));
         q.tm = (int)tm; q.m_tiles = (int)m_tiles; q.n_tiles = (int)n_tiles; q.k_steps = (int)k_steps;
         q.splits = s; q.stages = (int)stages; q.codes_bytes = (int)codes; q.partial_bytes = (int)partial;
-        q.smem = (int)(codes + stages * stage + partial + 1024);
+        q.smem = (int)(fixed + stages * stage);
         const int64_t ctas = m_tiles * n_tiles * s;
-        const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(2, 227 * 1024 / (q.smem + 8192)));
-        const int64_t room = gemm_grid_limit() * per_sm * (s == 8 ? 7 : 8) / 8;
+        const int64_t room = gemm_grid_limit() * per_sm * (s == 8 ? 7 : 8) / 8;   // clusters of 8 leave some SMs out
         const double rounds = (double)((ctas + room - 1) / room);
-        const double stream = std::max((double)(steps * stage) / 45.0 * rounds,
-                                       (double)(N * k_steps * I8_KT * ops * m_tiles) / 5800.0);
+        const double stream = std::max((double)(steps * stage) / 34.0 * rounds,
+                                       (double)(N * k_steps * I8_KT * ops * m_tiles) / 5500.0);
         q.ns = rounds * (6000.0 + 12.0 * (double)(ops * planes * tm)) + stream + (s > 1 ? 1000.0 : 0.0);
         q.ok = true;
         if (!best.ok || q.ns < best.ns) best = q;

@@ -531,14 +531,16 @@ def _record(function, leaves, *args):
     the stream it was made on, and lives as long as any graph with the leaf.  A capture that records a
     backward pass through a node of another stream ends the process when it runs that pass: eager
     recordings leave a mark on the nodes, and a capture that finds one is refused before it records."""
-    leaves = [t for t in leaves if t is not None and t.requires_grad and t.is_leaf]
     stream = _raw_stream(_current_device())
     if not _capturing():
         out = function.apply(*args)
-        for t in leaves:
-            torch.autograd.graph.get_gradient_edge(t).node.metadata.setdefault(_STREAM_MARK, stream)
+        for node, _ in out.grad_fn.next_functions:
+            if type(node).__name__ == "AccumulateGrad":
+                node.metadata.setdefault(_STREAM_MARK, stream)
         return out
     for t in leaves:
+        if t is None or not (t.requires_grad and t.is_leaf):
+            continue
         if torch.autograd.graph.get_gradient_edge(t).node.metadata.get(_STREAM_MARK, stream) != stream:
             raise RuntimeError("an eager autograd graph of this leaf tensor is alive on another stream: release it before "
                                "capturing a backward pass, or capture int8_linear_backward / int8_gated_backward, which "
