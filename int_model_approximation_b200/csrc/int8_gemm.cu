@@ -206,12 +206,12 @@ IMA_DEVINL void store_y32(const I8Params& p, unsigned char* st, int lane, const 
 #pragma unroll
             for (int j = 0; j < 16; ++j) w[j] = __float_as_uint(v[hf * 16 + j]);
             const int32_t c = col + hf * 16;
-            stage_store(st, lane, w, y + (row0 * p.ldy + c) * 4, p.ldy * 4, rows, (p.N - c) * 4, p.vec_y, 4);
+            stage_store(st, lane, w, y + (row0 * p.ldy + c) * 4, p.ldy * 4, rows, min(p.N - c, 16) * 4, p.vec_y, 4);
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) w[j] = pack_half2(v[2 * j], v[2 * j + 1], p.y_dtype);
-        stage_store(st, lane, w, y + (row0 * p.ldy + col) * 2, p.ldy * 2, rows, (p.N - col) * 2, p.vec_y, 2);
+        stage_store(st, lane, w, y + (row0 * p.ldy + col) * 2, p.ldy * 2, rows, min(p.N - col, 32) * 2, p.vec_y, 2);
     }
 }
 
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                             for (int j = 0; j < 16; ++j) w[j] = r[hf * 16 + j];
                             const int32_t c = n0 + c0 + hf * 16;
                             stage_store(st, lane, w, reinterpret_cast<unsigned char*>(p.c + row0 * p.ldc + c),
-                                        p.ldc * 4, rows, (p.N - c) * 4, p.vec_c, 4);
+                                        p.ldc * 4, rows, min(p.N - c, 16) * 4, p.vec_c, 4);
                         }
                     }
                     if (p.y) {
@@ -501,10 +501,10 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                         if (p.col_max && n + (lane & 15) < p.N)
                             atomicMax(p.col_max + n + (lane & 15) + (lane >= 16 ? p.seg_pitch : 0), cm);
                         float* d = p.d + row0 * p.ldd + n;
-                        stage_store(st, lane, wg, reinterpret_cast<unsigned char*>(d), p.ldd * 4, rows, (p.N - n) * 4,
+                        stage_store(st, lane, wg, reinterpret_cast<unsigned char*>(d), p.ldd * 4, rows, min(p.N - n, 16) * 4,
                                     p.vec_d, 4);
                         stage_store(st, lane, wu, reinterpret_cast<unsigned char*>(d + p.seg_pitch), p.ldd * 4, rows,
-                                    (p.N - n) * 4, p.vec_d, 4);
+                                    min(p.N - n, 16) * 4, p.vec_d, 4);
                     }
                 };
                 if (p.act == IMA_ACT_SILU) chunks(std::integral_constant<int, IMA_ACT_SILU>{});

@@ -467,7 +467,8 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x
         q.splits = s; q.stages = (int)stages; q.codes_bytes = (int)codes; q.partial_bytes = (int)partial;
         q.smem = (int)(fixed + stages * stage);
         const int64_t ctas = m_tiles * n_tiles * s;
-        const int64_t room = gemm_grid_limit() * per_sm * (s == 8 ? 7 : 8) / 8;   // clusters of 8 leave some SMs out
+        // clusters of 8 leave some SMs out
+        const int64_t room = std::max<int64_t>(1, gemm_grid_limit() * per_sm * (s == 8 ? 7 : 8) / 8);
         const double rounds = (double)((ctas + room - 1) / room);
         const double stream = std::max((double)(steps * stage) / 34.0 * rounds,
                                        (double)(N * k_steps * I8_KT * ops * m_tiles) / 5500.0);

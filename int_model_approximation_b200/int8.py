@@ -177,6 +177,12 @@ class Int8Weight:
         self.shape, self.device, self.ld = codes.shape, codes.device, _code_ld(codes)
         self._transposed: tuple | None = None   # (codes [K, N], version of self.codes, stream, event until it has passed)
 
+    def __getstate__(self):
+        return self.codes, self.scale   # copies make their own transposed codes
+
+    def __setstate__(self, state) -> None:
+        self._set(*state)
+
     @classmethod
     def from_float(cls, weight: torch.Tensor) -> "Int8Weight":
         """Quantise a floating weight [N, K], one scale per row."""
@@ -531,7 +537,7 @@ def _record(function, leaves, *args):
     the stream it was made on, and lives as long as any graph with the leaf.  A capture that records a
     backward pass through a node of another stream ends the process when it runs that pass: eager
     recordings leave a mark on the nodes, and a capture that finds one is refused before it records."""
-    stream = _raw_stream(_current_device())
+    stream = _raw_stream(args[0].device.index)
     if not _capturing():
         out = function.apply(*args)
         for node, _ in out.grad_fn.next_functions:

@@ -9,6 +9,7 @@ contraction.  Every bound below is formed element by element from these, in 64 b
 
 from __future__ import annotations
 
+import copy
 import math
 
 import pytest
@@ -320,6 +321,47 @@ def test_int8_product_strides_outputs_and_neighbours(cuda_device, m):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda_device):
+    """Outputs and activations of more than 2^31 elements, compared on rows at both ends."""
+    m, n, k = 66_000, 33_000, 48
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    a = torch.randint(-127, 128, (m, k), generator=g, device=cuda_device, dtype=torch.int8)
+    b = torch.randint(-127, 128, (n, k), generator=g, device=cuda_device, dtype=torch.int8)
+    ones_m, ones_n = torch.ones((m,), device=cuda_device), torch.ones((n,), device=cuda_device)
+    _c, y = int8.int8_gemm(a, b, want_c=False, x_scale=ones_m, w_scale=ones_n, y_dtype=torch.float16)
+    pick = torch.tensor([0, 1, 32_999, 65_076, 65_077, m - 2, m - 1], device=cuda_device)
+    # 127^2 * 48 exceeds fp16's range: the same rounding, to infinity too
+    assert torch.equal(y[pick], int_product(a[pick], b).to(torch.float16))
+    q, s = int8.per_token_int8(y.nan_to_num_(posinf=60000.0, neginf=-60000.0))
+    q64, s64 = plain_codes(y[pick])
+    assert torch.equal(q[pick].double(), q64) and torch.equal(s[pick].flatten().double(), s64)
+    del y
+    status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+def test_results_under_an_sm_limit(cuda_device):
+    """Fewer SMs (left to collectives) give the same results, whatever form or split that selects."""
+    x, w, _ = make(700, 3000, 2100, torch.bfloat16, 41, cuda_device)
+    x.requires_grad_()
+    wt = int8.Int8Weight.from_float(w)
+    dy = torch.randn((700, 3000), device=cuda_device).to(torch.bfloat16)
+
+    def run():
+        y = int8.int8_linear(x, wt)
+        return y, torch.autograd.grad(y, x, dy)[0], int8.int8_linear(x.detach()[:5], wt)
+
+    want = run()
+    try:
+        for limit in (1, 7, 100):
+            nat.call("ima_set_gemm_sm_limit", limit)
+            assert all(torch.equal(a, b) for a, b in zip(run(), want))
+    finally:
+        nat.call("ima_set_gemm_sm_limit", 0)
+    status_clean(cuda_device)
+
+
+@pytest.mark.gpu
 def test_int8_product_verifies_under_freivalds(cuda_device):
     x, w, _ = make(50, 96, 300, torch.bfloat16, 3, cuda_device)
     (q, _s), wt = int8.per_token_int8(x), int8.Int8Weight.from_float(w)
@@ -584,6 +626,39 @@ def test_gradients_of_expanded_and_shared_tensors(cuda_device):
 
 
 @pytest.mark.gpu
+def test_gradients_of_mixed_types(cuda_device):
+    """bf16 activations against fp32 master weights: each gradient in its tensor's type."""
+    m, n, k = 50, 70, 90
+    x, _w, _ = make(m, n, k, torch.bfloat16, 5, cuda_device)
+    _x, w, b = make(m, n, k, torch.float32, 6, cuda_device, bias=True)
+    _x, w2, _ = make(m, n, k, torch.bfloat16, 7, cuda_device)
+    b2 = b.detach().half()
+    for t in (x, w, b, w2, b2):
+        t.requires_grad_()
+    dy = torch.randn((m, n), device=cuda_device).to(torch.bfloat16)
+    got = torch.autograd.grad(int8.int8_linear(x, w, b), (x, w, b), dy)
+    assert [g.dtype for g in got] == [torch.bfloat16, torch.float32, torch.float32]
+    (q, s), (wq, t) = plain_codes(x), plain_codes(w)
+    want = (dy.double() * s[:, None]).T @ q
+    none = torch.zeros((n, m), dtype=torch.float64, device=cuda_device)
+    assert_within(got[1], want, grad_bound(dy.double().T, none, s, q, 8355000.0, torch.float32, want))
+    got = torch.autograd.grad(int8.int8_gated(x, w, w2, b, b2), (x, w, w2, b, b2), dy)
+    assert [g.dtype for g in got] == [t.dtype for t in (x, w, w2, b, b2)]
+    assert all(bool(torch.isfinite(g).all()) for g in got)
+    # one frozen projection beside a trained one: the trained one's gradient alone
+    up = int8.Int8Weight.from_float(w2)
+    alone = torch.autograd.grad(int8.int8_gated(x, w, up, b, b2), (x, w), dy)
+    assert torch.equal(alone[0], got[0]) and torch.equal(alone[1], got[1])
+    alone = torch.autograd.grad(int8.int8_gated(x, int8.Int8Weight.from_float(w), w2, b, b2), w2, dy)[0]
+    # (its types are all bf16: two digits where the pass above took three)
+    ref = gated_reference(x, w, w2, b, b2, "silu")
+    d, err = dy.double() * ref["a"], dy.double().abs() * act_slack(ref)
+    want = (d * ref["s"][:, None]).T @ ref["q"]
+    for digits, g in ((32639.0, alone), (8355000.0, got[2])):
+        assert_within(g, want, grad_bound(d.T, err.T, ref["s"], ref["q"], digits, torch.bfloat16, want))
+
+
+@pytest.mark.gpu
 def test_gradient_rows_with_nan_and_zero_rows(cuda_device):
     m, n, k = 20, 48, 64
     x, w, _ = make(m, n, k, torch.float32, 6, cuda_device)
@@ -811,6 +886,11 @@ def test_int8_student_model(cuda_device, monkeypatch, act, tokens):
         p = torch.relu(g(h)) * u(h)
     z = int8.int8_linear(h + mlp.down_proj(p), model.head.int8_weight())
     assert torch.equal(z, y)
+    # a copy of the model, also after a backward pass (which leaves the transposed codes with the weights)
+    model(x.clone().requires_grad_()).sum().backward()
+    twin = copy.deepcopy(model)
+    with torch.inference_mode():
+        assert torch.equal(twin(x), y)
     # gradients reach the input through the frozen model
     xg = x.clone().requires_grad_()
     model(xg).square().sum().backward()
