@@ -363,27 +363,29 @@ int ima_int8_gemm(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, in
                   int32_t* c, int64_t ldc, const float* x_scale, const float* w_scale, const void* bias, int bias_dtype,
                   void* y, int y_dtype, int64_t ldy, void* stream);
 
-/* Gated feed-forward block in one kernel: y [M,N] = act(g) * u with g = (fp32(a gate^T) *
- * x_scale[m]) * gate_scale[n] (+ gate_bias[n]) and u the same of up. */
 #define IMA_ACT_SILU 0
 #define IMA_ACT_GELU 1      /* with the error function */
 #define IMA_ACT_GELU_TANH 2 /* with its tanh approximation */
-int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
-                        int64_t M, int64_t N, int64_t K, const float* x_scale, const float* gate_scale,
-                        const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype,
-                        int activation, void* y, int y_dtype, int64_t ldy, void* stream);
-/* The two operators on floating activations x [M,K] (row stride ldx): y [M,N] in x's type.  q [M,ldq]
+
+/* The two operators on floating activations x [M,K] (row stride ldx): y [M,N] in x's type.
+ *   linear: y = (fp32(q w^T) * scale[m]) * w_scale[n] (+ bias[n])
+ *   gated:  y = act(g) * u, both projections, activation and product in one kernel, with
+ *           g = (fp32(q gate^T) * scale[m]) * gate_scale[n] (+ gate_bias[n]) and u the same of up
+ * q [M,ldq]
  * int8 and scale [M] are workspace; with keep_codes != 0 they hold the codes and scales of x
  * afterwards (what a backward pass needs), otherwise a product of few tokens quantises them in
- * its own launch and leaves both alone. */
+ * its own launch and leaves both alone.  w_src (gate_src, up_src): the weight [N,K] as a floating
+ * tensor of w_src_dtype, quantised first into w and w_scale; NULL when those hold it already. */
 int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated, int x_dtype); /* 1: without keep_codes, q and scale may be NULL */
 int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
-                    int keep_codes, const int8_t* w, int64_t ldw, int64_t N, const float* w_scale, const void* bias,
-                    int bias_dtype, void* y, int64_t ldy, void* stream);
+                    int keep_codes, int8_t* w, int64_t ldw, int64_t N, float* w_scale, const void* w_src,
+                    int w_src_dtype, int64_t ldw_src, const void* bias, int bias_dtype, void* y, int64_t ldy,
+                    void* stream);
 int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
-                   int keep_codes, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu, int64_t N,
-                   const float* gate_scale, const float* up_scale, const void* gate_bias, const void* up_bias,
-                   int bias_dtype, int activation, void* y, int64_t ldy, void* stream);
+                   int keep_codes, int8_t* gate, int64_t ldg, int8_t* up, int64_t ldu, int64_t N, float* gate_scale,
+                   float* up_scale, const void* gate_src, int64_t ldgate_src, const void* up_src, int64_t ldup_src,
+                   int w_src_dtype, const void* gate_bias, const void* up_bias, int bias_dtype, int activation, void* y,
+                   int64_t ldy, void* stream);
 
 /* dst [cols, rows] (row stride ldd, a multiple of 16; columns rows..round_up(rows, 16) zero) = src
  * [rows, cols] transposed. */

@@ -143,19 +143,16 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         _I32,
         [_VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _I64, _VP, _VP, _VP, _I32, _VP, _I32, _I64, _VP],
     ),
-    "ima_int8_gated_gemm": (
-        _I32,
-        [_VP, _I64, _VP, _I64, _VP, _I64, _I64, _I64, _I64, _VP, _VP, _VP, _VP, _VP, _I32, _I32, _VP, _I32, _I64, _VP],
-    ),
     "ima_int8_fused": (_I32, [_I64, _I64, _I64, _I32, _I32]),
     "ima_int8_linear": (
         _I32,
-        [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _I32, _VP, _I64, _I64, _VP, _VP, _I32, _VP, _I64, _VP],
+        [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _I32, _VP, _I64, _I64, _VP, _VP, _I32, _I64, _VP, _I32, _VP, _I64,
+         _VP],
     ),
     "ima_int8_gated": (
         _I32,
-        [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _I32, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _VP, _VP, _I32, _I32,
-         _VP, _I64, _VP],
+        [_VP, _I32, _I64, _I64, _I64, _VP, _I64, _VP, _I32, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _VP, _I64, _VP, _I64,
+         _I32, _VP, _VP, _I32, _I32, _VP, _I64, _VP],
     ),
     "ima_int8_transpose": (_I32, [_VP, _I64, _I64, _I64, _VP, _I64, _VP]),
     "ima_int8_backward_workspace_bytes": (_I64, [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]),

@@ -60,6 +60,35 @@ bool fused_plan(int64_t M, int64_t N, int64_t K, int ops, int x_dtype, SkPlan& q
 
 namespace {
 
+// What the launch before a product wrote of its operands: nothing, its activations, or weights too.
+constexpr int AFTER_NOTHING = 0, AFTER_TOKENS = 1, AFTER_WEIGHTS = 2;
+
+struct Pair8 { int8_t* p[2]; };
+struct PairL { int64_t v[2]; };
+struct PairF { float* p[2]; };
+struct PairV { const void* p[2]; };
+
+// The quantisers before a product: of the activations unless it quantises them itself, and of the weights that are
+// given as floating tensors; one launch where the types agree.  `after`: see above.
+int quantise_all(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
+                 bool fused, Pair8 w, PairL ldw, PairF w_scale, PairV src, PairL ldsrc, int src_dtype, int64_t N, int& after,
+                 cudaStream_t st) {
+    QuantRows weights = {}, tokens = {};
+    weights.K = tokens.K = K;
+    int nw = 0, nt = 0, rc = IMA_OK;
+    const bool any = src.p[0] || src.p[1];
+    if (any && !known_dtype(src_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    const bool together = any && !fused && src_dtype == x_dtype;
+    if (!fused) rc = add_quantize(together ? weights : tokens, together ? nw : nt, x, M, ldx, q, ldq, scale);
+    for (int i = 0; i < 2 && rc == IMA_OK; ++i)
+        if (src.p[i]) rc = add_quantize(weights, nw, src.p[i], N, ldsrc.v[i], w.p[i], ldw.v[i], w_scale.p[i]);
+    if (rc == IMA_OK && nw > 0) rc = run_quantize(weights, src_dtype, st);
+    if (rc == IMA_OK && nt > 0) rc = run_quantize(tokens, x_dtype, st);
+    // a product that starts early may read weights before it waits unless the launch right before it wrote them
+    after = fused || M == 0 ? AFTER_NOTHING : together ? AFTER_WEIGHTS : AFTER_TOKENS;
+    return rc;
+}
+
 int int8_gemm_entry(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, int64_t M, int64_t N, int64_t K,
                   int32_t* c, int64_t ldc, const float* x_scale, const float* w_scale, const void* bias, int bias_dtype,
                   void* y, int y_dtype, int64_t ldy, int dependent, void* stream) {
@@ -113,14 +142,6 @@ int ima_int8_gemm(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, in
     return int8_gemm_entry(a, lda, b, ldb, M, N, K, c, ldc, x_scale, w_scale, bias, bias_dtype, y, y_dtype, ldy, 0, stream);
 }
 
-int ima_int8_gated_gemm(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
-                        int64_t M, int64_t N, int64_t K, const float* x_scale, const float* gate_scale,
-                        const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype,
-                        int activation, void* y, int y_dtype, int64_t ldy, void* stream) {
-    return int8_gated_entry(a, lda, gate, ldg, up, ldu, M, N, K, x_scale, gate_scale, up_scale, gate_bias, up_bias,
-                            bias_dtype, activation, y, y_dtype, ldy, 0, stream);
-}
-
 // Operator entries: floating activations in.  Few tokens: one launch, quantiser inside.  Otherwise the row
 // quantiser into q and scale, then the product.
 int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated, int x_dtype) {
@@ -129,69 +150,75 @@ int ima_int8_fused(int64_t M, int64_t N, int64_t K, int gated, int x_dtype) {
 }
 
 int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
-                    int keep_codes, const int8_t* w, int64_t ldw, int64_t N, const float* w_scale, const void* bias,
-                    int bias_dtype, void* y, int64_t ldy, void* stream) {
+                    int keep_codes, int8_t* w, int64_t ldw, int64_t N, float* w_scale, const void* w_src,
+                    int w_src_dtype, int64_t ldw_src, const void* bias, int bias_dtype, void* y, int64_t ldy,
+                    void* stream) {
     if (M < 0 || K < 0 || !known_dtype(x_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    cudaStream_t st = (cudaStream_t)stream;
     int rc = check_i8_operand(w, N, K, ldw);
     if (rc != IMA_OK) return rc;
     if (M > 0 && K > 0 && (!x || (M > 1 && ldx < K))) return IMA_ERR_INVALID_ARGUMENT;
-    {
-        SkPlan plan;
-        if (!keep_codes && fused_plan(M, N, K, 1, x_dtype, plan)) {
-            if (!y || !w_scale || (ldy < N && M > 1) || (bias && !known_dtype(bias_dtype))) return IMA_ERR_INVALID_ARGUMENT;
-            SkParams p;
-            memset(&p, 0, sizeof(p));
-            p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
-            p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
-            p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
-            rc = sk_weight_maps(p, {nullptr, w, nullptr, 0, ldw, 0, K, K, 0});
-            if (rc != IMA_OK) return rc;
-            return run_fused<I8_LINEAR>(p, x_dtype, plan, (cudaStream_t)stream);
-        }
-    }
-    rc = ima_int8_quantize_rows(x, x_dtype, M, K, ldx, q, ldq, scale, stream);
+    SkPlan plan;
+    const bool fused = !keep_codes && fused_plan(M, N, K, 1, x_dtype, plan);
+    int after = AFTER_NOTHING;
+    rc = quantise_all(x, x_dtype, M, K, ldx, q, ldq, scale, fused, {w, nullptr}, {ldw, 0}, {w_scale, nullptr},
+                      {w_src, nullptr}, {ldw_src, 0}, w_src_dtype, N, after, st);
     if (rc != IMA_OK) return rc;
-    return int8_gemm_entry(q, ldq, w, ldw, M, N, K, nullptr, N, scale, w_scale, bias, bias_dtype, y, x_dtype, ldy, 1, stream);
+    if (fused) {
+        if (!y || !w_scale || (ldy < N && M > 1) || (bias && !known_dtype(bias_dtype))) return IMA_ERR_INVALID_ARGUMENT;
+        SkParams p;
+        memset(&p, 0, sizeof(p));
+        p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
+        p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
+        p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
+        rc = sk_weight_maps(p, {nullptr, w, nullptr, 0, ldw, 0, K, K, 0});
+        if (rc != IMA_OK) return rc;
+        return run_fused<I8_LINEAR>(p, x_dtype, plan, st);
+    }
+    return int8_gemm_entry(q, ldq, w, ldw, M, N, K, nullptr, N, scale, w_scale, bias, bias_dtype, y, x_dtype, ldy, after, stream);
 }
 
 int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
-                   int keep_codes, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu, int64_t N,
-                   const float* gate_scale, const float* up_scale, const void* gate_bias, const void* up_bias,
-                   int bias_dtype, int activation, void* y, int64_t ldy, void* stream) {
+                   int keep_codes, int8_t* gate, int64_t ldg, int8_t* up, int64_t ldu, int64_t N, float* gate_scale,
+                   float* up_scale, const void* gate_src, int64_t ldgate_src, const void* up_src, int64_t ldup_src,
+                   int w_src_dtype, const void* gate_bias, const void* up_bias, int bias_dtype, int activation, void* y,
+                   int64_t ldy, void* stream) {
     if (M < 0 || K < 0 || !known_dtype(x_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    cudaStream_t st = (cudaStream_t)stream;
     int rc = check_i8_operand(gate, N, K, ldg);
     if (rc == IMA_OK) rc = check_i8_operand(up, N, K, ldu);
     if (rc != IMA_OK) return rc;
     if (activation != IMA_ACT_SILU && activation != IMA_ACT_GELU && activation != IMA_ACT_GELU_TANH) return IMA_ERR_UNSUPPORTED;
     if (M > 0 && K > 0 && (!x || (M > 1 && ldx < K))) return IMA_ERR_INVALID_ARGUMENT;
-    {
-        SkPlan plan;
-        if (!keep_codes && fused_plan(M, N, K, 2, x_dtype, plan)) {
-            if (!y || !gate_scale || !up_scale || (ldy < N && M > 1) || ((gate_bias || up_bias) && !known_dtype(bias_dtype)))
-                return IMA_ERR_INVALID_ARGUMENT;
-            SkParams p;
-            memset(&p, 0, sizeof(p));
-            p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
-            p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.act = activation;
-            p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias; p.bias_dtype = bias_dtype;
-            p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
-            rc = sk_weight_maps(p, {nullptr, gate, up, 0, ldg, ldu, K, K, 0});
-            if (rc != IMA_OK) return rc;
-            return run_fused<I8_GATED>(p, x_dtype, plan, (cudaStream_t)stream);
-        }
-    }
-    rc = ima_int8_quantize_rows(x, x_dtype, M, K, ldx, q, ldq, scale, stream);
+    SkPlan plan;
+    const bool fused = !keep_codes && fused_plan(M, N, K, 2, x_dtype, plan);
+    int after = AFTER_NOTHING;
+    rc = quantise_all(x, x_dtype, M, K, ldx, q, ldq, scale, fused, {gate, up}, {ldg, ldu}, {gate_scale, up_scale},
+                      {gate_src, up_src}, {ldgate_src, ldup_src}, w_src_dtype, N, after, st);
     if (rc != IMA_OK) return rc;
+    if (fused) {
+        if (!y || !gate_scale || !up_scale || (ldy < N && M > 1) || ((gate_bias || up_bias) && !known_dtype(bias_dtype)))
+            return IMA_ERR_INVALID_ARGUMENT;
+        SkParams p;
+        memset(&p, 0, sizeof(p));
+        p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
+        p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.act = activation;
+        p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias; p.bias_dtype = bias_dtype;
+        p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
+        rc = sk_weight_maps(p, {nullptr, gate, up, 0, ldg, ldu, K, K, 0});
+        if (rc != IMA_OK) return rc;
+        return run_fused<I8_GATED>(p, x_dtype, plan, st);
+    }
     return int8_gated_entry(q, ldq, gate, ldg, up, ldu, M, N, K, scale, gate_scale, up_scale, gate_bias, up_bias,
-                            bias_dtype, activation, y, x_dtype, ldy, 1, stream);
+                            bias_dtype, activation, y, x_dtype, ldy, after, stream);
 }
 
 }  // extern "C"
 
 // ---------------------------------------------------------------------------
-// Backward passes.  Launches, in order: [g and u again, their gradients D and D's maxima | D's maxima],
-// the digits of D by rows and by columns with the partial bias sums, [W transposed], dx, q transposed,
-// dW, bias sums.
+// Backward passes.  Launches, in order: W and q transposed (and the maxima zeroed), [g and u again, their
+// gradients D and D's maxima | D's maxima], the digits of D by rows and by columns with the partial bias
+// sums, dx, dW, bias sums.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -276,10 +303,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         int64_t ldwt[2] = {a.ldwt[0], a.ldwt[1]};
         for (int i = 0; i < a.segs; ++i)
             if (!wt[i]) {
-                int8_t* t = reinterpret_cast<int8_t*>(ws + b.w_t) + i * a.K * b.ldwt;
-                rc = ima_int8_transpose(a.w[i], a.N, a.K, a.ldw[i], t, b.ldwt, st);
-                if (rc != IMA_OK) return rc;
-                wt[i] = t;
+                wt[i] = reinterpret_cast<const int8_t*>(ws + b.w_t) + i * a.K * b.ldwt;
                 ldwt[i] = b.ldwt;
             }
         I8Params p;
@@ -295,9 +319,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         if (rc != IMA_OK) return rc;
     }
     if ((a.dw[0] || a.dw[1]) && a.K > 0) {
-        int8_t* qt = reinterpret_cast<int8_t*>(ws + b.q_t);
-        rc = ima_int8_transpose(a.q, a.M, a.K, a.ldq, qt, b.ldm, st);
-        if (rc != IMA_OK) return rc;
+        const int8_t* qt = reinterpret_cast<const int8_t*>(ws + b.q_t);
         const int first = a.dw[0] ? 0 : 1;
         const bool both = a.dw[0] && a.dw[1];
         I8Params p;
@@ -357,8 +379,18 @@ int run_backward(const BwdArgs& a, cudaStream_t st) {
     g.ws[0] = a.w_scale[0]; g.ws[1] = a.w_scale[1];
     g.row_max = a.dx ? row_max : nullptr;
     g.col_max = want_dw ? row_max + a.M : nullptr;
-    if (a.dx || want_dw) {
-        rc = ima_note_cuda(cudaMemsetAsync(row_max, 0, (size_t)b.maxima_bytes, st));
+    if (a.dx || want_dw) {   // the transposed operands, and the maxima at zero
+        TransposeJobs t = {};
+        int n = 0;
+        t.zero = row_max;
+        t.zero_words = b.maxima_bytes / 4;
+        if (a.K > 0) {
+            for (int i = 0; i < a.segs && a.dx; ++i)
+                if (!a.w_t[i])
+                    add_transpose(t, n, a.w[i], a.N, a.K, a.ldw[i], reinterpret_cast<int8_t*>(ws + b.w_t) + i * a.K * b.ldwt, b.ldwt);
+            if (want_dw) add_transpose(t, n, a.q, a.M, a.K, a.ldq, reinterpret_cast<int8_t*>(ws + b.q_t), b.ldm);
+        }
+        rc = run_transposes(t, st);
         if (rc != IMA_OK) return rc;
     }
     int src_dtype = a.grad_dtype;
@@ -393,12 +425,12 @@ int run_backward(const BwdArgs& a, cudaStream_t st) {
     rc = run_grad_digits(d, src_dtype, a.planes, st);
     if (rc != IMA_OK) return rc;
     rc = a.planes == 2 ? bwd_products<2, 256>(a, b, ws, st) : bwd_products<3, 128>(a, b, ws, st);
-    for (int i = 0; i < a.segs && rc == IMA_OK; ++i)
-        if (a.db[i]) {
-            int8_col_sum_kernel<<<(unsigned)((a.N + 255) / 256), 256, 0, st>>>(d.partial + i * b.pitch, (a.M + 127) / 128, b.W,
-                                                                             a.N, a.db[i], a.db_dtype);
-            rc = IMA_LAUNCH_STATUS();
-        }
+    if (rc == IMA_OK && want_db) {
+        const dim3 grid((unsigned)((a.N + 255) / 256), (unsigned)a.segs);
+        int8_col_sum_kernel<<<grid, 256, 0, st>>>(d.partial, (a.M + 127) / 128, b.W, a.N, b.pitch, a.db[0], a.db[1],
+                                                  a.db_dtype);
+        rc = IMA_LAUNCH_STATUS();
+    }
     return rc;
 }
 

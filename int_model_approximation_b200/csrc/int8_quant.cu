@@ -164,16 +164,27 @@ IMA_DEVINL uint32_t row_max(uint32_t m, uint32_t* s_max) {
 // and kept in registers between the maximum and the codes, a longer one is read again (from
 // L2).  Bound by memory: 2 or 4 bytes in and 1 out per element.
 // ---------------------------------------------------------------------------
+struct QuantRows {           // up to three matrices of K columns, one after the other (activations, weights)
+    const void* x[3];
+    int8_t* q[3];
+    float* scale[3];
+    int64_t ldx[3], ldq[3], end[3];   // end: rows of this and the matrices before it
+    int64_t K;
+};
+
 template <int DT, int TPR, int V>
-__global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* x, int64_t M, int64_t K, int64_t ldx,
-                                                                    int8_t* q, int64_t ldq, float* scale) {
+__global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const __grid_constant__ QuantRows a) {
     // a product launched to follow this kernel may start now; it waits for this kernel's end before it reads
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ uint32_t s_max[8];
     constexpr int ROWS = 256 / TPR;
     const int tid = threadIdx.x % TPR;
-    for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; m < M; m += (int64_t)gridDim.x * ROWS) {
-        const unsigned char* row = reinterpret_cast<const unsigned char*>(x) + m * ldx * dtype_bytes(DT);
+    const int64_t K = a.K;
+    for (int64_t row_at = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR; row_at < a.end[2];
+         row_at += (int64_t)gridDim.x * ROWS) {
+        const int which = (row_at >= a.end[0]) + (row_at >= a.end[1]);
+        const int64_t m = row_at - (which ? a.end[which - 1] : 0);
+        const unsigned char* row = reinterpret_cast<const unsigned char*>(a.x[which]) + m * a.ldx[which] * dtype_bytes(DT);
         const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
         // whole aligned groups of eight that this thread keeps; the rest is loaded twice
         const int64_t whole = vec ? min(K / 8 * 8, (int64_t)V * TPR * 8) : 0;
@@ -195,8 +206,8 @@ __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const void* 
         const float amax = __uint_as_float(row_max<TPR>(mx, s_max));
         const float s = i8_row_scale(amax, amax != amax);
         const I8Inv inv = i8_inv(s);
-        if (tid == 0) scale[m] = s;
-        int8_t* qr = q + m * ldq;
+        if (tid == 0) a.scale[which][m] = s;
+        int8_t* qr = a.q[which] + m * a.ldq[which];
         auto emit = [&](const Raw8<DT>& r, int64_t k0) {
             float v[8];
             r.unpack(v);
@@ -459,13 +470,15 @@ __global__ void __launch_bounds__(256) int8_grad_digits_kernel(const GradDigits 
     }
 }
 
-// out[j] = sum over chunks of partial[chunk][j], in the type of the bias.
+// out[j] = sum over chunks of partial[chunk][j], in the type of the bias; blockIdx.y: which of two
+// segments, `pitch` columns apart (out NULL: not wanted).
 __global__ void __launch_bounds__(256) int8_col_sum_kernel(const float* partial, int64_t chunks, int64_t W, int64_t n,
-                                                           void* out, int dtype) {
+                                                           int64_t pitch, void* out0, void* out1, int dtype) {
     const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (j >= n) return;
+    void* out = blockIdx.y ? out1 : out0;
+    if (j >= n || !out) return;
     double t = 0.0;
-    for (int64_t c = 0; c < chunks; ++c) t += (double)partial[c * W + j];
+    for (int64_t c = 0; c < chunks; ++c) t += (double)partial[c * W + blockIdx.y * pitch + j];
     const float f = (float)t;
     if (dtype == IMA_DTYPE_F32) reinterpret_cast<float*>(out)[j] = f;
     else if (dtype == IMA_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(out)[j] = __float2bfloat16_rn(f);
@@ -473,11 +486,28 @@ __global__ void __launch_bounds__(256) int8_col_sum_kernel(const float* partial,
 }
 
 // dst[c][r] = src[r][c], int8; columns rows..round16(rows) of dst are zero.  A block turns 128 x 128
-// bytes: 16-byte loads, 4 x 4 byte blocks turned in registers, 128 contiguous bytes out per row.
-__global__ void __launch_bounds__(256) int8_transpose_kernel(const int8_t* src, int64_t rows, int64_t cols, int64_t ld,
-                                                             int8_t* dst, int64_t ldd, int vec) {
+// bytes: 16-byte loads, 4 x 4 byte blocks turned in registers, 128 contiguous bytes out per row.  Up to three
+// matrices in one launch, and words to be zeroed.
+struct TransposeJobs {
+    const int8_t* src[3];
+    int8_t* dst[3];
+    int64_t rows[3], cols[3], ld[3], ldd[3], end[3];   // end: blocks of this and the matrices before it
+    uint32_t* zero;
+    int64_t zero_words;
+};
+
+__global__ void __launch_bounds__(256) int8_transpose_kernel(const __grid_constant__ TransposeJobs a) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.zero_words; i += (int64_t)gridDim.x * 256) a.zero[i] = 0;
+    const int64_t block = blockIdx.x;
+    if (block >= a.end[2]) return;
+    const int which = (block >= a.end[0]) + (block >= a.end[1]);
+    const int64_t rows = a.rows[which], cols = a.cols[which], ld = a.ld[which], ldd = a.ldd[which];
+    const int8_t* src = a.src[which];
+    int8_t* dst = a.dst[which];
+    const bool vec = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)ld) & 15) == 0;
+    const int64_t across = (cols + 127) / 128, at = block - (which ? a.end[which - 1] : 0);
+    const int64_t r0 = at / across * 128, c0 = at % across * 128;
     __shared__ uint32_t tile[128][33];   // 128 rows of 128 bytes
-    const int64_t r0 = (int64_t)blockIdx.y * 128, c0 = (int64_t)blockIdx.x * 128;
     uint4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -523,8 +553,9 @@ __global__ void __launch_bounds__(256) int8_transpose_kernel(const int8_t* src, 
 bool known_dtype(int d) { return d == IMA_DTYPE_F32 || d == IMA_DTYPE_BF16 || d == IMA_DTYPE_F16; }
 
 template <int DT>
-int launch_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq, float* scale,
-                    cudaStream_t st) {
+int launch_quantize(const QuantRows& a, cudaStream_t st) {
+    const int64_t M = a.end[2], K = a.K;
+    if (M == 0) return IMA_OK;
     // As few threads per row as hold it in registers, when the rows fill the machine: 8 KB of a row in flight
     // per warp and no barrier, or a barrier of two to eight warps.  Few rows: a block each, for latency.
     constexpr bool F = DT == IMA_DTYPE_F32;
@@ -532,7 +563,7 @@ int launch_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, int8_t* q,
     auto run = [&](auto tpr, auto v) {
         constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
         const unsigned grid = (unsigned)std::min<int64_t>((M * TPR + 255) / 256, 148 * 32);
-        int8_quantize_rows_kernel<DT, TPR, V><<<grid, 256, 0, st>>>(x, M, K, ldx, q, ldq, scale);
+        int8_quantize_rows_kernel<DT, TPR, V><<<grid, 256, 0, st>>>(a);
     };
     if (K <= 1024) run(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
     else if (many && K <= (F ? 2048 : 4096)) run(std::integral_constant<int, 32>{}, std::integral_constant<int, F ? 8 : 16>{});
@@ -570,20 +601,55 @@ int run_grad_digits(const GradDigits& a, int dtype, int planes, cudaStream_t st)
     return launch_grad_digits<IMA_DTYPE_F32>(a, planes, st);
 }
 
+void add_transpose(TransposeJobs& a, int& n, const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst,
+                   int64_t ldd) {
+    a.src[n] = src; a.dst[n] = dst; a.rows[n] = rows; a.cols[n] = cols; a.ld[n] = ld; a.ldd[n] = ldd;
+    const int64_t before = n ? a.end[n - 1] : 0;
+    for (int i = n; i < 3; ++i) a.end[i] = before + (rows + 127) / 128 * ((cols + 127) / 128);
+    ++n;
+}
+
+int run_transposes(const TransposeJobs& a, cudaStream_t st) {
+    const int64_t blocks = std::max(a.end[2], std::min<int64_t>((a.zero_words + 255) / 256, 296));
+    if (blocks == 0) return IMA_OK;
+    if (blocks > INT32_MAX) return IMA_ERR_UNSUPPORTED;
+    int8_transpose_kernel<<<(unsigned)blocks, 256, 0, st>>>(a);
+    return IMA_LAUNCH_STATUS();
+}
+
+int run_quantize(const QuantRows& a, int dtype, cudaStream_t st) {
+    if (dtype == IMA_DTYPE_BF16) return launch_quantize<IMA_DTYPE_BF16>(a, st);
+    if (dtype == IMA_DTYPE_F16) return launch_quantize<IMA_DTYPE_F16>(a, st);
+    return launch_quantize<IMA_DTYPE_F32>(a, st);
+}
+
+// Append a matrix to `a` (fewer than three so far, `n` of them).
+int add_quantize(QuantRows& a, int& n, const void* x, int64_t M, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
+    const int64_t K = a.K;
+    if (M < 0 || K < 0) return IMA_ERR_INVALID_ARGUMENT;
+    if (M > 0) {
+        if (!scale || (K > 0 && (!x || !q || (M > 1 && ldx < K)))) return IMA_ERR_INVALID_ARGUMENT;
+        if (ldq < K || ldq % 16 || (reinterpret_cast<uintptr_t>(q) & 15)) return IMA_ERR_INVALID_ARGUMENT;
+    }
+    a.x[n] = x; a.q[n] = q; a.scale[n] = scale; a.ldx[n] = ldx; a.ldq[n] = ldq;
+    const int64_t before = n ? a.end[n - 1] : 0;
+    for (int i = n; i < 3; ++i) a.end[i] = before + M;
+    ++n;
+    return IMA_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
 int ima_int8_quantize_rows(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx, int8_t* q, int64_t ldq,
                            float* scale, void* stream) {
-    if (M < 0 || K < 0 || !known_dtype(x_dtype)) return IMA_ERR_INVALID_ARGUMENT;
-    if (M == 0) return IMA_OK;
-    if (!scale || (K > 0 && (!x || !q || (M > 1 && ldx < K)))) return IMA_ERR_INVALID_ARGUMENT;
-    if (ldq < K || ldq % 16 || (reinterpret_cast<uintptr_t>(q) & 15)) return IMA_ERR_INVALID_ARGUMENT;
-    cudaStream_t st = (cudaStream_t)stream;
-    if (x_dtype == IMA_DTYPE_BF16) return launch_quantize<IMA_DTYPE_BF16>(x, M, K, ldx, q, ldq, scale, st);
-    if (x_dtype == IMA_DTYPE_F16) return launch_quantize<IMA_DTYPE_F16>(x, M, K, ldx, q, ldq, scale, st);
-    return launch_quantize<IMA_DTYPE_F32>(x, M, K, ldx, q, ldq, scale, st);
+    if (!known_dtype(x_dtype)) return IMA_ERR_INVALID_ARGUMENT;
+    QuantRows a = {};
+    a.K = K;
+    int n = 0;
+    const int rc = add_quantize(a, n, x, M, ldx, q, ldq, scale);
+    return rc != IMA_OK ? rc : run_quantize(a, x_dtype, (cudaStream_t)stream);
 }
 
 int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst, int64_t ldd,
@@ -592,11 +658,10 @@ int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld
     if (rows == 0 || cols == 0) return IMA_OK;
     if (!src || !dst || ld < cols || ldd < rows || ldd % 16 || (reinterpret_cast<uintptr_t>(dst) & 15))
         return IMA_ERR_INVALID_ARGUMENT;
-    if ((rows + 127) / 128 > 65535) return IMA_ERR_UNSUPPORTED;
-    const int vec = !((reinterpret_cast<uintptr_t>(src) | (uintptr_t)ld) & 15);
-    const dim3 grid((unsigned)((cols + 127) / 128), (unsigned)((rows + 127) / 128));
-    int8_transpose_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(src, rows, cols, ld, dst, ldd, vec);
-    return IMA_LAUNCH_STATUS();
+    TransposeJobs a = {};
+    int n = 0;
+    add_transpose(a, n, src, rows, cols, ld, dst, ldd);
+    return run_transposes(a, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -42,7 +42,8 @@ struct __align__(64) SkParams {
     void* y2;                      // I8_DIGIT: rows from split_row on, seg_rows of each part (NULL: all to y)
     int64_t ldx, ldc, ldy, K, split_row, seg_rows;
     int32_t M, N, tm, k_steps, seg_steps, splits, stages, codes_bytes, partial_bytes, tmem_cols;
-    int32_t y_dtype, bias_dtype, act, vec_c, vec_y, dependent;
+    int32_t y_dtype, bias_dtype, act, vec_c, vec_y;
+    int32_t dependent;             // launched while the kernel before it still runs: 1: it writes the tokens, 2: weights too
     uint64_t stall_ns;             // test knob (ima_set_gemm_wait_test); 0 in normal use
 };
 
@@ -129,6 +130,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
+        if (p.dependent == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // the weights come from there too
         for (int i = 0; i < first; ++i) load_weights(i);        // on their way before anything else is set up
     }
     if (FUSED)

@@ -146,6 +146,12 @@ def _quantise(rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
+def _quantise_into(weight: "Int8Weight", src: torch.Tensor) -> None:
+    n, k = src.shape
+    _call(src.device, "ima_int8_quantize_rows", src.data_ptr(), _DTYPE_CODES[src.dtype], n, k, _ld(src),
+          weight.codes.data_ptr(), weight.ld, weight.scale.data_ptr())
+
+
 def _transpose(t: torch.Tensor) -> torch.Tensor:
     """int8 [rows, cols] (aligned) -> [cols, rows]."""
     rows, cols = t.shape
@@ -324,8 +330,22 @@ def _code_buffers(rows: torch.Tensor, n: int, gated: bool, keep: bool):
     return ws, None, at, ld, at + m * ld
 
 
-def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor | None, keep: bool = False):
-    """(y [M, N], codes, scale) of x rows; codes and scale only with keep."""
+def _weight_args(weight) -> tuple[Int8Weight, torch.Tensor | None]:
+    """(handle, rows to quantise into it or None) of a weight as the operators take it."""
+    if isinstance(weight, Int8Weight):
+        return weight, None
+    if weight.ndim != 2:
+        raise RuntimeError(f"int8 weight source must be 2-D, got {tuple(weight.shape)}")
+    src = _rows(weight.detach())
+    n, k = src.shape
+    made = Int8Weight.__new__(Int8Weight)
+    made._set(_empty_codes(n, k, src), src.new_empty((n,), dtype=torch.float32))
+    return made, src
+
+
+def _linear_forward(rows: torch.Tensor, weight: Int8Weight, src: torch.Tensor | None, bias: torch.Tensor | None,
+                    keep: bool = False):
+    """(y [M, N], codes, scale) of x rows; codes and scale only with keep.  src: weight rows to be quantised."""
     m, k = rows.shape
     n = weight.shape[0]
     y = rows.new_empty((m, n))
@@ -334,15 +354,18 @@ def _linear_forward(rows: torch.Tensor, weight: Int8Weight, bias: torch.Tensor |
     if bias is not None:
         (bias,), bias_dtype = _bias_args(n, bias)
     _call(rows.device, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q_ptr, ld, scale_ptr,
-          keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(), _ptr(bias), bias_dtype, y.data_ptr(),
-          n or 1)
+          keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(), _ptr(src), _code(src),
+          0 if src is None else _ld(src), _ptr(bias), bias_dtype, y.data_ptr(), n or 1)
     return y, q[:, :k] if keep and ld != k else q, scale
 
 
-def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bias, up_bias, activation: str,
-                   keep: bool = False):
+def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_src, up_src, gate_bias, up_bias,
+                   activation: str, keep: bool = False):
     m, k = rows.shape
     n = gate.shape[0]
+    if gate_src is not None and up_src is not None and gate_src.dtype != up_src.dtype:
+        _quantise_into(up, up_src)   # weights of two types: the second on its own
+        up_src = None
     h = rows.new_empty((m, n))
     q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, n, True, keep)
     bias_dtype = 0
@@ -350,8 +373,14 @@ def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_bi
         (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
     _call(rows.device, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q_ptr, ld, scale_ptr,
           keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n, gate.scale.data_ptr(),
-          up.scale.data_ptr(), _ptr(gate_bias), _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], h.data_ptr(), n or 1)
+          up.scale.data_ptr(), _ptr(gate_src), 0 if gate_src is None else _ld(gate_src), _ptr(up_src),
+          0 if up_src is None else _ld(up_src), _code(gate_src if gate_src is not None else up_src), _ptr(gate_bias),
+          _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], h.data_ptr(), n or 1)
     return h, q[:, :k] if keep and ld != k else q, scale
+
+
+def _code(t: torch.Tensor | None) -> int:
+    return 0 if t is None else _DTYPE_CODES[t.dtype]
 
 
 # ---------------------------------------------------------------------------
@@ -395,10 +424,6 @@ def _one_type(*dtypes: torch.dtype | None) -> torch.dtype | None:
 
 def _out(like: torch.Tensor, shape: tuple, dtype: torch.dtype | None, wanted: bool = True) -> torch.Tensor | None:
     return like.new_empty(shape, dtype=dtype) if wanted and dtype is not None else None
-
-
-def _code(t: torch.Tensor | None) -> int:
-    return 0 if t is None else _DTYPE_CODES[t.dtype]
 
 
 def int8_linear_backward(
@@ -509,10 +534,6 @@ def _gated_backward(grad, codes, scale, gate, up, gate_bias, up_bias, activation
 # ---------------------------------------------------------------------------
 # the operators
 # ---------------------------------------------------------------------------
-def _weight_of(weight) -> Int8Weight:
-    return weight if isinstance(weight, Int8Weight) else Int8Weight.from_float(weight)
-
-
 def _check_gated(k: int, gate, up, activation: str) -> None:
     if activation not in ACTIVATIONS:
         raise RuntimeError(f"unknown activation {activation!r}; choose one of: {', '.join(sorted(ACTIVATIONS))}")
@@ -570,8 +591,8 @@ def _wanted_types(ctx, inputs) -> tuple:
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, handle):
-        w = handle if handle is not None else Int8Weight.from_float(weight)
-        y, q, scale = _linear_forward(_rows(x.detach()), w, bias, keep=True)
+        w, src = _weight_args(handle if handle is not None else weight)
+        y, q, scale = _linear_forward(_rows(x.detach()), w, src, bias, keep=True)
         ctx.save_for_backward(q, scale)
         ctx.weight, ctx.frozen, ctx.version = w, handle is not None, _versions(w)
         ctx.types = _wanted_types(ctx, (x, weight, bias))
@@ -592,9 +613,9 @@ class _LinearFunction(torch.autograd.Function):
 class _GatedFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, gate, up, activation):
-        g = gate if gate is not None else Int8Weight.from_float(gate_weight)
-        u = up if up is not None else Int8Weight.from_float(up_weight)
-        h, q, scale = _gated_forward(_rows(x.detach()), g, u, gate_bias, up_bias, activation, keep=True)
+        g, g_src = _weight_args(gate if gate is not None else gate_weight)
+        u, u_src = _weight_args(up if up is not None else up_weight)
+        h, q, scale = _gated_forward(_rows(x.detach()), g, u, g_src, u_src, gate_bias, up_bias, activation, keep=True)
         ctx.save_for_backward(q, scale, gate_bias, up_bias)
         ctx.gate, ctx.up, ctx.activation, ctx.version = g, u, activation, _versions(g, u)
         ctx.frozen = gate is not None and up is not None
@@ -641,17 +662,21 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
 
     weight: an Int8Weight (frozen) or a floating tensor, quantised in the call and differentiable.
     """
-    _check_inputs(x, ("weight", weight), ("bias", bias))
-    if weight.shape[-1] != x.shape[-1]:
-        raise RuntimeError(f"int8 matmul shape mismatch: K={x.shape[-1]} vs K={weight.shape[-1]}")
+    frozen = type(weight) is Int8Weight
+    if not (frozen and x.is_cuda and bias is None and x.dtype in _DTYPE_CODES and x.device == weight.device):
+        _check_inputs(x, ("weight", weight), ("bias", bias))
+    k = x.shape[-1]
+    if weight.shape[-1] != k:
+        raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={weight.shape[-1]}")
+    if k > MAX_K:
+        raise RuntimeError(f"int8 linear: contraction of {k} exceeds {MAX_K} (exact int32 sums)")
     if torch.is_grad_enabled() and _wants_grad(x, weight, bias):
-        frozen = isinstance(weight, Int8Weight)
-        _check_backward(x.numel() // max(x.shape[-1], 1), weight.shape[0] if x.requires_grad else 0,
+        _check_backward(x.numel() // max(k, 1), weight.shape[0] if x.requires_grad else 0,
                         not frozen and weight.requires_grad)
         w = None if frozen else weight
         return _record(_LinearFunction, (x, w, bias), x, w, bias, weight if frozen else None)
-    w = _weight_of(weight)
-    y, _q, _s = _linear_forward(_rows(x), w, bias)
+    w, src = (weight, None) if frozen else _weight_args(weight)
+    y = _linear_forward(_rows(x), w, src, bias)[0]
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 
@@ -669,15 +694,18 @@ def int8_gated(
     Both projections, the activation ("silu", "gelu" with the error function, or "gelu_tanh") and the
     product run in one kernel; g and u never reach memory.  Weights as in int8_linear."""
     _check_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
-    _check_gated(x.shape[-1], gate, up, activation)
+    k = x.shape[-1]
+    _check_gated(k, gate, up, activation)
+    if k > MAX_K:
+        raise RuntimeError(f"int8 gated block: contraction of {k} exceeds {MAX_K} (exact int32 sums)")
     if torch.is_grad_enabled() and _wants_grad(x, gate, up, gate_bias, up_bias):
         frozen = [isinstance(w, Int8Weight) for w in (gate, up)]
-        _check_backward(x.numel() // max(x.shape[-1], 1),
+        _check_backward(x.numel() // max(k, 1),
                         _round_up(gate.shape[0], 128) + gate.shape[0] if x.requires_grad else 0,
                         any(not f and w.requires_grad for f, w in zip(frozen, (gate, up))))
         inputs = (x, None if frozen[0] else gate, None if frozen[1] else up, gate_bias, up_bias)
         return _record(_GatedFunction, inputs, *inputs, gate if frozen[0] else None, up if frozen[1] else None,
                        activation)
-    g, u = _weight_of(gate), _weight_of(up)
-    h, _q, _s = _gated_forward(_rows(x), g, u, gate_bias, up_bias, activation)
+    (g, g_src), (u, u_src) = _weight_args(gate), _weight_args(up)
+    h = _gated_forward(_rows(x), g, u, g_src, u_src, gate_bias, up_bias, activation)[0]
     return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])

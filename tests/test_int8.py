@@ -137,7 +137,8 @@ def test_c_entries_refuse_bad_arguments_before_any_launch():
     assert lib.ima_int8_gemm(16, 24, 16, 32, 2, 2, 24, 16, 2, None, None, None, 0, None, 0, 2, None) == bad
     assert lib.ima_int8_gemm(16, 32, 16, 32, 2, 2, 32, 16, 1, None, None, None, 0, None, 0, 2, None) == bad
     # gated: unknown activation
-    assert lib.ima_int8_gated_gemm(16, 32, 16, 32, 16, 32, 2, 2, 32, 16, 16, 16, None, None, 0, 7, 16, 1, 2, None) == uns
+    assert lib.ima_int8_gated(16, 1, 2, 32, 32, 16, 32, 16, 0, 16, 32, 16, 32, 2, 16, 16, None, 0, None, 0, 0, None, None, 0,
+                              7, 16, 2, None) == uns
     # backward: only 2 or 3 digits, contractions too long, no workspace
     def backward(m=2, n=32, k=32, planes=2, dx=256, dw=None, ws=256):
         ld = (max(n, k) + 15) // 16 * 16
