@@ -27,7 +27,7 @@
 #include <cudaTypedefs.h>
 #include <algorithm>
 #include <atomic>
-#include "sm100_primitives.cuh"
+#include "sm100_pair.cuh"
 
 namespace {
 
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
     if (CG == 2) cluster_sync_all();   // both CTAs' barriers exist before either signals the other's
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");   // codes and scales are complete
+    if (p.dependent) wait_previous_kernel();   // codes and scales are complete
 
     if (warp == 0 && lane == 0) {
         // ---------------- TMA producer ----------------

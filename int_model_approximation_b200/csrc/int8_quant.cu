@@ -17,7 +17,7 @@
 // gradients of very different sizes, where a bf16 result is off by 2e-3 and an fp16 one by 2e-4.
 #include <algorithm>
 #include <type_traits>
-#include "sm100_primitives.cuh"
+#include "sm100_pair.cuh"
 
 namespace {
 
@@ -175,7 +175,7 @@ struct QuantRows {           // up to three matrices of K columns, one after the
 template <int DT, int TPR, int V>
 __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const __grid_constant__ QuantRows a) {
     // a product launched to follow this kernel may start now; it waits for this kernel's end before it reads
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    allow_next_kernel();
     __shared__ uint32_t s_max[8];
     constexpr int ROWS = 256 / TPR;
     const int tid = threadIdx.x % TPR;

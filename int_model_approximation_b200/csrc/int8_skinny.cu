@@ -16,7 +16,7 @@
 // layout that the MMA reads, in shared memory, while the first weight tiles are on their way.  This
 // saves a launch and a round trip of the codes.  Otherwise the row quantiser runs before, and this
 // kernel is launched so that it starts, and loads its first weight tiles, while that one finishes.
-#include "sm100_primitives.cuh"
+#include "sm100_pair.cuh"
 
 namespace {
 
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
         mbar_init(&drained, 1);
         abort_flag = 0;
         mbar_fence_init();
-        if (p.dependent == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // the weights come from there too
+        if (p.dependent == 2) wait_previous_kernel();   // the weights come from there too
         for (int i = 0; i < first; ++i) load_weights(i);        // on their way before anything else is set up
     }
     if (FUSED)
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
     };
     if (warp == 0 && lane == 0) {
         if (!FUSED) {
-            if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (p.dependent) wait_previous_kernel();
             for (int i = 0; i < first; ++i) load_tokens(i);
         }
     } else if (FUSED && warp >= 2) {
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
             if (lane == 0) mbar_arrive(&tok_ready);
         }
         if (!FUSED) {   // the token scales
-            if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (p.dependent) wait_previous_kernel();
             for (int t = threadIdx.x - 64; t < rows; t += SK_WORKERS * 32) s_scale[t] = p.xs ? p.xs[m0 + t] : 0.0f;
             named_barrier_sync(1, SK_WORKERS * 32);
         }
