@@ -392,6 +392,11 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
 int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld, int8_t* dst, int64_t ldd,
                        void* stream);
 
+/* Int8 rows moved to rows that start on 16 bytes: dst_a [rows_a, cols] = a (row stride lda) and dst_b = b
+ * (NULL and 0 rows: none), both with row stride ldd, a multiple of 16; columns cols..round_up(cols, 16) zero. */
+int ima_int8_pack_rows(const int8_t* a, int64_t rows_a, int64_t lda, int8_t* dst_a, const int8_t* b, int64_t rows_b,
+                       int64_t ldb, int8_t* dst_b, int64_t cols, int64_t ldd, void* stream);
+
 /* Gradients of the two operators from grad [M,N] (row stride ldg), straight through the rounding; q [M,K]
  * and scale [M] are the codes of the activations.
  *   linear: dx = (grad * w_scale) w, dw = (grad * scale)^T q, db = sum_m grad

@@ -155,6 +155,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
          _I32, _VP, _VP, _I32, _I32, _VP, _I64, _VP],
     ),
     "ima_int8_transpose": (_I32, [_VP, _I64, _I64, _I64, _VP, _I64, _VP]),
+    "ima_int8_pack_rows": (_I32, [_VP, _I64, _I64, _VP, _VP, _I64, _I64, _VP, _I64, _I64, _VP]),
     "ima_int8_backward_workspace_bytes": (_I64, [_I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]),
     "ima_int8_linear_backward": (
         _I32,

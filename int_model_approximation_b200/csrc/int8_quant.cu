@@ -550,6 +550,38 @@ __global__ void __launch_bounds__(256) int8_transpose_kernel(const __grid_consta
     }
 }
 
+// Rows of int8 codes moved to rows that start on 16 bytes, as the tile loads need them: dst[r][c] = src[r][c], and zeros in
+// columns cols..round16(cols).  Up to two matrices of one width in a launch.  A thread makes 16 bytes from the
+// aligned 4-byte words that hold them, shifted into place.
+struct PackRows {
+    const int8_t* src[2];
+    int8_t* dst[2];
+    int64_t ld[2], end[2];   // end: rows of this and the matrix before it
+    int64_t cols, ldd;
+};
+
+__global__ void __launch_bounds__(256) int8_pack_rows_kernel(const __grid_constant__ PackRows a) {
+    const int64_t chunks = (a.cols + 15) / 16, total = a.end[1] * chunks;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / chunks, c = (i - row * chunks) * 16;
+        const int which = row >= a.end[0];
+        const int64_t r = row - (which ? a.end[0] : 0);
+        const uintptr_t from = reinterpret_cast<uintptr_t>(a.src[which] + r * a.ld[which] + c);
+        const int n = (int)min((int64_t)16, a.cols - c), shift = (int)(from & 3);
+        const uint32_t* p = reinterpret_cast<const uint32_t*>(from - shift);
+        uint32_t w[5], o[4];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) w[j] = j * 4 < n + shift ? __ldg(p + j) : 0;   // words with a wanted byte
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[j] = __funnelshift_r(w[j], w[j + 1], shift * 8);
+            const int left = n - j * 4;
+            if (left < 4) o[j] = left > 0 ? o[j] & ((1u << (left * 8)) - 1) : 0;
+        }
+        *reinterpret_cast<uint4*>(a.dst[which] + r * a.ldd + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
 bool known_dtype(int d) { return d == IMA_DTYPE_F32 || d == IMA_DTYPE_BF16 || d == IMA_DTYPE_F16; }
 
 template <int DT>
@@ -662,6 +694,22 @@ int ima_int8_transpose(const int8_t* src, int64_t rows, int64_t cols, int64_t ld
     int n = 0;
     add_transpose(a, n, src, rows, cols, ld, dst, ldd);
     return run_transposes(a, (cudaStream_t)stream);
+}
+
+int ima_int8_pack_rows(const int8_t* a, int64_t rows_a, int64_t lda, int8_t* dst_a, const int8_t* b, int64_t rows_b,
+                       int64_t ldb, int8_t* dst_b, int64_t cols, int64_t ldd, void* stream) {
+    if (rows_a < 0 || rows_b < 0 || cols < 0) return IMA_ERR_INVALID_ARGUMENT;
+    if (cols == 0 || rows_a + rows_b == 0) return IMA_OK;
+    if (ldd % 16 || ldd < cols) return IMA_ERR_INVALID_ARGUMENT;
+    if (rows_a > 0 && (!a || !dst_a || (rows_a > 1 && lda < cols) || (reinterpret_cast<uintptr_t>(dst_a) & 15)))
+        return IMA_ERR_INVALID_ARGUMENT;
+    if (rows_b > 0 && (!b || !dst_b || (rows_b > 1 && ldb < cols) || (reinterpret_cast<uintptr_t>(dst_b) & 15)))
+        return IMA_ERR_INVALID_ARGUMENT;
+    const PackRows p = {{a, b}, {dst_a, dst_b}, {lda, ldb}, {rows_a, rows_a + rows_b}, cols, ldd};
+    const int64_t total = (rows_a + rows_b) * ((cols + 15) / 16);
+    const unsigned grid = (unsigned)std::min<int64_t>((total + 255) / 256, 148 * 32);
+    int8_pack_rows_kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+    return IMA_LAUNCH_STATUS();
 }
 
 }  // extern "C"

@@ -96,21 +96,44 @@ def _empty_codes(rows: int, k: int, like: torch.Tensor) -> torch.Tensor:
     return t if ld == k else t[:, :k]
 
 
-def _aligned_codes(t: torch.Tensor, label: str) -> torch.Tensor:
-    """An int8 matrix as the kernels load it: contiguous rows that start on 16 bytes (a copy
-    only if it is not)."""
+def _check_codes(t: torch.Tensor, label: str) -> None:
     if t.dtype != torch.int8 or t.ndim != 2:
         raise RuntimeError(f"{label} must be a 2-D int8 tensor, got {t.dtype} {tuple(t.shape)}")
     _require_cuda(t, label)
     if t.shape[1] > MAX_K:
         raise RuntimeError(f"{label}: contraction of {t.shape[1]} exceeds {MAX_K} (exact int32 sums)")
-    one_row = t.shape[0] <= 1
-    if t.numel() and (t.stride(1) != 1 and t.shape[1] > 1 or t.data_ptr() % 16 or
-                      not one_row and (t.stride(0) % 16 or t.stride(0) < t.shape[1])):
-        out = _empty_codes(t.shape[0], t.shape[1], t)
-        out.copy_(t)
-        return out
-    return t
+
+
+def _is_aligned(t: torch.Tensor) -> bool:
+    if t.stride(1) != 1 and t.shape[1] > 1 or t.data_ptr() % 16:
+        return t.numel() == 0
+    return t.shape[0] <= 1 or t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] or t.numel() == 0
+
+
+def _aligned_codes(t: torch.Tensor, label: str) -> torch.Tensor:
+    """An int8 matrix as the kernels load it: contiguous rows that start on 16 bytes (a copy
+    only if it is not)."""
+    _check_codes(t, label)
+    return t if _is_aligned(t) else _packed_codes(t)[0]
+
+
+def _packed_codes(*given: torch.Tensor) -> list[torch.Tensor]:
+    """Copies of one or two int8 matrices of one width and device, in rows that start on 16 bytes; one
+    launch where their columns are contiguous."""
+    k = given[0].shape[1]
+    out = [_empty_codes(t.shape[0], k, t) for t in given]
+    args = []
+    for t, o in zip(given, out):
+        if (t.stride(1) == 1 or k == 1) and (t.shape[0] <= 1 or t.stride(0) >= k):
+            args += [t.data_ptr(), t.shape[0], _ld(t), o.data_ptr()]
+        elif t.stride(0) == 1 and t.stride(1) >= t.shape[0]:
+            _call(t.device, "ima_int8_transpose", t.data_ptr(), k, t.shape[0], t.stride(1), o.data_ptr(), _code_ld(o))
+        else:
+            o.copy_(t)
+    if args:
+        args += [None, 0, 0, None] if len(args) == 4 else []
+        _call(out[0].device, "ima_int8_pack_rows", *args, k, _round_up(k, 16))
+    return out
 
 
 def _code_ld(t: torch.Tensor) -> int:
@@ -277,8 +300,8 @@ def int8_gemm(
 
     a: int8 [M, K]; b: int8 [N, K], any strides (rows that do not start on 16 bytes are copied).
     Returns (c int32 [M, N] or None, y [M, N] or None)."""
-    a = _aligned_codes(a, "int8 activation matrix")
-    b = _aligned_codes(b, "int8 weight matrix")
+    _check_codes(a, "int8 activation matrix")
+    _check_codes(b, "int8 weight matrix")
     (m, k), n = a.shape, b.shape[0]
     if b.shape[1] != k:
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={b.shape[1]}")
@@ -287,6 +310,10 @@ def int8_gemm(
                      ("output", y_out)):
         if t is not None and t.device != dev:
             nat.require_device(dev, (label, t))
+    pack_a, pack_b = not _is_aligned(a), not _is_aligned(b)
+    if pack_a or pack_b:
+        packed = _packed_codes(*(t for t, wanted in ((a, pack_a), (b, pack_b)) if wanted))
+        a, b = packed[0] if pack_a else a, packed[-1] if pack_b else b
     if c_out is not None:
         _check_out(c_out, (m, n), (torch.int32,), "int8 product")
         c = c_out

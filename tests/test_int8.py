@@ -941,3 +941,74 @@ def test_wait_that_runs_out_is_reported_and_the_next_call_is_exact(cuda_device, 
     c, _ = int8.int8_gemm(a, b)
     assert torch.equal(c, int_product(a, b))
     status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# operands whose rows do not start on 16 bytes
+# ---------------------------------------------------------------------------
+def test_pack_rows_refusals():
+    lib, bad = nat.lib(), nat.IMA_ERR_INVALID_ARGUMENT
+    assert lib.ima_int8_pack_rows(None, 0, 0, None, None, 0, 0, None, 7, 16, None) == 0
+    assert lib.ima_int8_pack_rows(17, 2, 7, 32, None, 0, 0, None, 0, 16, None) == 0
+    assert lib.ima_int8_pack_rows(17, -1, 7, 32, None, 0, 0, None, 7, 16, None) == bad
+    assert lib.ima_int8_pack_rows(17, 2, 7, 33, None, 0, 0, None, 7, 16, None) == bad      # destination off 16 bytes
+    assert lib.ima_int8_pack_rows(17, 2, 6, 32, None, 0, 0, None, 7, 16, None) == bad      # rows overlap
+    assert lib.ima_int8_pack_rows(17, 2, 17, 32, None, 0, 0, None, 17, 16, None) == bad    # narrower than its rows
+    assert lib.ima_int8_pack_rows(17, 2, 7, 32, None, 0, 0, None, 7, 24, None) == bad
+    assert lib.ima_int8_pack_rows(17, 2, 7, 32, None, 3, 7, 64, 7, 16, None) == bad
+
+
+def _laid_out(t, layout):
+    """t in another layout: the same values at odd addresses, odd row strides or other orders."""
+    r, c = t.shape
+    if layout.startswith("offset"):
+        at = int(layout[6:])
+        out = torch.zeros(r * c + at, dtype=t.dtype, device=t.device)[at:].view(r, c)
+    elif layout == "rows":
+        out = torch.zeros((r, c + 5), dtype=t.dtype, device=t.device)[:, 3:3 + c]
+    elif layout == "turned":
+        out = torch.zeros((c, r + 3), dtype=t.dtype, device=t.device)[:, 1:r + 1].t()
+    elif layout == "every second":
+        out = torch.zeros((r, 2 * c), dtype=t.dtype, device=t.device)[:, ::2]
+    else:
+        assert layout == "plain"
+        out = torch.zeros_like(t)
+    out.copy_(t)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("a_layout,b_layout", [("offset1", "plain"), ("plain", "offset2"), ("offset3", "rows"),
+                                               ("rows", "turned"), ("turned", "offset8"), ("every second", "rows"),
+                                               ("turned", "turned")])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 5, 3), (3, 2, 16), (2, 129, 17), (7, 40, 31), (130, 300, 1718),
+                                   (260, 65, 4099)])
+def test_packed_operands(cuda_device, m, n, k, a_layout, b_layout):
+    g = torch.Generator(device=cuda_device).manual_seed(m + n + k)
+    a = torch.randint(-128, 128, (m, k), generator=g, device=cuda_device, dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, k), generator=g, device=cuda_device, dtype=torch.int8)
+    c, _ = int8.int8_gemm(_laid_out(a, a_layout), _laid_out(b, b_layout))
+    assert torch.equal(c.double(), a.double() @ b.double().t())
+    w = int8.Int8Weight(_laid_out(b, b_layout), torch.ones(n, device=cuda_device))
+    assert torch.equal(w.codes, b)
+
+
+@pytest.mark.gpu
+def test_packed_rows_of_one_value(cuda_device):
+    a = torch.randint(-128, 128, (1, 37), device=cuda_device, dtype=torch.int8)
+    b = torch.randint(-128, 128, (4, 1), device=cuda_device, dtype=torch.int8)
+    c, _ = int8.int8_gemm(a.expand(9, 37), b.expand(4, 37))
+    assert torch.equal(c.double(), a.double().expand(9, 37) @ b.double().expand(4, 37).t())
+    one = torch.randint(-128, 128, (1, 1), device=cuda_device, dtype=torch.int8)
+    c, _ = int8.int8_gemm(one.expand(5, 1), b)
+    assert torch.equal(c.double(), one.double().expand(5, 1) @ b.double().t())
+
+
+@pytest.mark.gpu
+def test_packed_buffer_has_zeros_behind_its_rows(cuda_device):
+    src = torch.randint(-128, 128, (6 * 21 + 1,), device=cuda_device, dtype=torch.int8)[1:].view(6, 21)
+    dst = torch.full((8, 48), 77, dtype=torch.int8, device=cuda_device)
+    int8._call(torch.device("cuda", torch.cuda.current_device()), "ima_int8_pack_rows", src.data_ptr(), 6, 21,
+               dst.data_ptr(), None, 0, 0, None, 21, 48)
+    assert torch.equal(dst[:6, :21], src)
+    assert (dst[:6, 21:32] == 0).all() and (dst[:6, 32:] == 77).all() and (dst[6:] == 77).all()
