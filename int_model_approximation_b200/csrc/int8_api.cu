@@ -5,6 +5,14 @@
 
 namespace {
 
+// Bytes that a lane may store at once into rows of `ld` elements at p: the widest power of two up to 16 that
+// divides both the address and the row's bytes.
+int store_width(const void* p, int64_t ld, int esize) {
+    int w = 16;
+    while (w > esize && ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * esize)) & (w - 1))) w /= 2;
+    return w;
+}
+
 int64_t i8_steps(int64_t Ka) { return (Ka + I8_KT - 1) / I8_KT; }
 
 // Time of the tiled form in ns: rounds of 128 x bn tiles over the machine at the tensor core's rate (8192
@@ -105,8 +113,8 @@ int int8_gemm_entry(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, 
     p.c = c; p.y = y; p.xs = x_scale; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
     p.ldc = ldc; p.ldy = ldy; p.y_dtype = y_dtype;
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
-    p.vec_c = c && aligned16(c, ldc * 4);
-    p.vec_y = y && aligned16(y, ldy * dtype_bytes(y_dtype));
+    p.c_width = store_width(c, ldc, 4);
+    p.y_width = store_width(y, ldy, y ? dtype_bytes(y_dtype) : 4);
     return run_linear(p, {a, b, nullptr, lda, ldb, 0, K, K, M * lda}, (cudaStream_t)stream);
 }
 
@@ -128,7 +136,7 @@ int int8_gated_entry(const int8_t* a, int64_t lda, const int8_t* gate, int64_t l
     p.y = y; p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
     p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = activation;
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
-    p.vec_y = aligned16(y, ldy * dtype_bytes(y_dtype));
+    p.y_width = store_width(y, ldy, dtype_bytes(y_dtype));
     return run_gated(p, {a, gate, up, lda, ldg, ldu, K, K, M * lda}, (cudaStream_t)stream);
 }
 
@@ -170,7 +178,7 @@ int ima_int8_linear(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld
         memset(&p, 0, sizeof(p));
         p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
         p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.ws[0] = w_scale; p.bias[0] = bias; p.bias_dtype = bias_dtype;
-        p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
+        p.vec_y = store_width(y, ldy, dtype_bytes(x_dtype)) >= 4 * dtype_bytes(x_dtype);
         rc = sk_weight_maps(p, {nullptr, w, nullptr, 0, ldw, 0, K, K, 0});
         if (rc != IMA_OK) return rc;
         return run_fused<I8_LINEAR>(p, x_dtype, plan, st);
@@ -204,7 +212,7 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
         p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
         p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.act = activation;
         p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias; p.bias_dtype = bias_dtype;
-        p.vec_y = aligned16(y, ldy * dtype_bytes(x_dtype));
+        p.vec_y = store_width(y, ldy, dtype_bytes(x_dtype)) >= 4 * dtype_bytes(x_dtype);
         rc = sk_weight_maps(p, {nullptr, gate, up, 0, ldg, ldu, K, K, 0});
         if (rc != IMA_OK) return rc;
         return run_fused<I8_GATED>(p, x_dtype, plan, st);
@@ -310,7 +318,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         memset(&p, 0, sizeof(p));
         p.y = a.dx; p.ldy = a.K; p.y_dtype = a.dx_dtype; p.xs = reinterpret_cast<const float*>(ws + b.row_scale);
         p.M = (int32_t)a.M; p.N = (int32_t)a.K;
-        p.vec_y = aligned16(a.dx, a.K * dtype_bytes(a.dx_dtype));
+        p.y_width = store_width(a.dx, a.K, dtype_bytes(a.dx_dtype));
         p.seg_tiles = (int32_t)i8_steps(a.N);
         p.tail = b.has_tail ? reinterpret_cast<int32_t*>(ws + b.tail) : nullptr;
         const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.rows), wt[0], a.segs == 2 ? wt[1] : nullptr, b.W,
@@ -327,10 +335,10 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         p.y = a.dw[first]; p.ldy = a.K; p.y_dtype = a.dw_dtype;
         p.xs = reinterpret_cast<const float*>(ws + b.col_scale) + first * b.pitch;
         p.M = (int32_t)(both ? b.pitch + a.N : a.N); p.N = (int32_t)a.K;
-        p.vec_y = aligned16(p.y, a.K * dtype_bytes(a.dw_dtype));
+        p.y_width = store_width(p.y, a.K, dtype_bytes(a.dw_dtype));
         if (both) {
             p.y2 = a.dw[1]; p.split_row = b.pitch; p.seg_rows = a.N;
-            p.vec_y = p.vec_y && aligned16(p.y2, a.K * dtype_bytes(a.dw_dtype));
+            p.y_width = std::min(p.y_width, store_width(p.y2, a.K, dtype_bytes(a.dw_dtype)));
         }
         p.seg_tiles = (int32_t)i8_steps(a.M);
         p.tail = b.has_tail ? reinterpret_cast<int32_t*>(ws + b.tail) : nullptr;
@@ -402,7 +410,6 @@ int run_backward(const BwdArgs& a, cudaStream_t st) {
         p.d = reinterpret_cast<float*>(ws + b.d); p.ldd = b.W; p.seg_pitch = b.pitch;
         p.row_max = g.row_max; p.col_max = g.col_max;
         p.M = (int32_t)a.M; p.N = (int32_t)a.N;
-        p.vec_d = 1;
         rc = launch_i8<1, 256, I8_GATED_BWD>(p, {a.q, a.w[0], a.w[1], a.ldq, a.ldw[0], a.ldw[1], a.K, a.K, a.M * a.ldq}, st);
         if (rc != IMA_OK) return rc;
         g.src = p.d;

@@ -536,7 +536,7 @@ int run_skinny_codes(const I8Params& g, const I8Operands& o, const SkPlan& q, cu
     p.c = g.c; p.y = g.y; p.xs = g.xs; p.ws[0] = g.ws[0]; p.ws[1] = g.ws[1]; p.bias[0] = g.bias[0]; p.bias[1] = g.bias[1];
     p.y2 = g.y2; p.split_row = g.split_row; p.seg_rows = g.seg_rows;
     p.ldc = g.ldc; p.ldy = g.ldy; p.M = g.M; p.N = g.N; p.K = o.K; p.y_dtype = g.y_dtype; p.bias_dtype = g.bias_dtype;
-    p.act = g.act; p.vec_c = g.vec_c; p.vec_y = g.vec_y; p.dependent = g.dependent;
+    p.act = g.act; p.vec_c = g.c_width == 16; p.vec_y = g.y_width >= 4 * dtype_bytes(g.y_dtype); p.dependent = g.dependent;
     p.seg_steps = g.seg_tiles;
     int rc = sk_weight_maps(p, o);
     if (rc == IMA_OK && o.K > 0) rc = make_i8_map(&p.mt, o.a, o.Ka, o.lda, p.M, P, o.a_planes, q.tm);

@@ -1012,3 +1012,23 @@ def test_packed_buffer_has_zeros_behind_its_rows(cuda_device):
                dst.data_ptr(), None, 0, 0, None, 21, 48)
     assert torch.equal(dst[:6, :21], src)
     assert (dst[:6, 21:32] == 0).all() and (dst[:6, 32:] == 77).all() and (dst[6:] == 77).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k,pad", [(300, 260, 200, 0), (300, 260, 200, 2), (300, 262, 200, 1), (300, 261, 200, 0),
+                                       (40, 262, 2000, 0), (129, 33, 64, 3), (257, 1, 64, 0)])
+def test_outputs_of_every_alignment(cuda_device, dtype, m, n, k, pad):
+    g = torch.Generator(device=cuda_device).manual_seed(n + pad)
+    a = torch.randint(-128, 128, (m, k), generator=g, device=cuda_device, dtype=torch.int8)
+    b = torch.randint(-128, 128, (n, k), generator=g, device=cuda_device, dtype=torch.int8)
+    ones = torch.full((max(m, n),), 2.0**-6, device=cuda_device)
+    c_big = torch.full((m + 1, n + pad), 77, dtype=torch.int32, device=cuda_device)
+    y_big = torch.full((m + 1, n + pad), 77.0, dtype=dtype, device=cuda_device)
+    int8.int8_gemm(a, b, x_scale=ones[:m], w_scale=ones[:n], c_out=c_big[:m, pad:], y_out=y_big[:m, pad:])
+    want = int_product(a, b)
+    assert torch.equal(c_big[:m, pad:], want)
+    assert torch.equal(y_big[:m, pad:], (want.float() * 2.0**-12).to(dtype))
+    assert (c_big[m:] == 77).all() and (y_big[m:] == 77).all()
+    assert (c_big[:, :pad] == 77).all() and (y_big[:, :pad] == 77).all()
+    status_clean(cuda_device)
