@@ -76,7 +76,7 @@ struct __align__(64) I8Params {
     int64_t ldc, ldy, ldh, ldd, seg_pitch;
     int32_t* tail;                  // I8_DIGIT: sums of the tail tiles, [tile][plane][BN][rows], and their counters
     uint32_t* tail_count;           // [tile][CTA of the pair][epilogue warp]; both zero at launch
-    int64_t full_tiles;             // tiles taken whole; each of the rest is split over tail_splits workers
+    int32_t full_tiles;             // tiles taken whole; each of the rest is split over tail_splits workers
     int32_t tail_splits;
     int32_t M, N, m_tiles, n_tiles, k_tiles, group_m;
     int32_t y_dtype, bias_dtype, dh_dtype, act, c_width, y_width;   // width: see stage_store
@@ -87,10 +87,8 @@ struct __align__(64) I8Params {
 
 // Tile t -> (row tile, column tile): groups of group_m row tiles, rows fastest within a group, so
 // that the tiles in flight share their k-slices of both operands in L2.
-IMA_DEVINL void i8_tile(const I8Params& p, int64_t t, int32_t& mt, int32_t& nt) {
-    const int64_t per_group = (int64_t)p.group_m * p.n_tiles;
-    const int32_t g = (int32_t)(t / per_group);
-    const int32_t within = (int32_t)(t - (int64_t)g * per_group);
+IMA_DEVINL void i8_tile(const I8Params& p, int32_t t, int32_t& mt, int32_t& nt) {
+    const int32_t per_group = p.group_m * p.n_tiles, g = t / per_group, within = t - g * per_group;
     const int32_t gm = min(p.group_m, p.m_tiles - g * p.group_m);
     mt = g * p.group_m + within % gm;
     nt = within / gm;
@@ -99,10 +97,9 @@ IMA_DEVINL void i8_tile(const I8Params& p, int64_t t, int32_t& mt, int32_t& nt) 
 // The work of one worker (a CTA, or a pair): whole tiles first, first + step, ..., then at most one part of
 // the k-range of a tail tile.
 struct I8Work {
-    int64_t t;
-    int32_t k0, k1;       // k-tiles
+    int32_t t, k0, k1;    // tile, k-tiles
     bool split;
-    IMA_DEVINL bool get(const I8Params& p, int64_t i, int64_t first, int64_t step) {
+    IMA_DEVINL bool get(const I8Params& p, int32_t i, int32_t first, int32_t step) {
         t = first + i * step;
         k0 = 0;
         k1 = p.k_tiles;
@@ -110,11 +107,11 @@ struct I8Work {
         if (t < p.full_tiles) return true;
         // the worker's item after its last whole tile
         if (p.tail_splits == 0 || (i > 0 && t - step >= p.full_tiles)) return false;
-        const int64_t tail = first / p.tail_splits, part = first % p.tail_splits;
+        const int32_t tail = first / p.tail_splits, part = first % p.tail_splits;
         t = p.full_tiles + tail;
-        if (t >= (int64_t)p.m_tiles * p.n_tiles) return false;
-        k0 = (int32_t)(part * p.k_tiles / p.tail_splits);
-        k1 = (int32_t)((part + 1) * p.k_tiles / p.tail_splits);
+        if (t >= p.m_tiles * p.n_tiles) return false;
+        k0 = part * p.k_tiles / p.tail_splits;
+        k1 = (part + 1) * p.k_tiles / p.tail_splits;
         split = true;
         return true;
     }
@@ -149,13 +146,94 @@ IMA_DEVINL void act_both(float g, float& a, float& da) {
     }
 }
 
-IMA_DEVINL uint32_t pack_half2(float lo, float hi, int dtype) {
-    if (dtype == IMA_DTYPE_BF16) {
-        __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<uint32_t*>(&b);
+// Two fp32 values in one register pair, and arithmetic on both in one instruction; each rounds as the plain form does.
+IMA_DEVINL uint64_t pair2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+IMA_DEVINL float2 halves(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+IMA_DEVINL uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+IMA_DEVINL uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+IMA_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// Sums as fp32, rounded once.  A sum is written hi * 2^s + lo with parts that fp32 holds exactly, so that one fma rounds it.
+// 0x4B000000 and 0x4B400000 are the bits of 2^23 and 1.5 * 2^23: an integer of up to 23 bits, added to them as
+// bits, is a float after one subtraction.  The conversion instruction has an eighth of the multiplier's rate and
+// took half of the epilogue's time; this form takes 2 integer and 1.5 floating instructions per value.
+//   one plane:  s = 16
+//   two planes: r0 + 2^8 r1.  |r1| <= 127 * 128 * 131071 leaves room for r0 >> 8 in 32 bits: t = r1 + (r0 >> 8),
+//               the sum is 2^8 t + (r0 & 255); s = 17, and |t >> 9| < 2^22
+//   three:      in 64 bits, below 2^47; s = 23
+IMA_DEVINL void sum_parts(const int32_t (&r)[1], uint32_t& hi, uint32_t& lo) {
+    hi = (uint32_t)((r[0] >> 16) + 0x4B400000);
+    lo = __byte_perm((uint32_t)r[0], 0x4B000000u, 0x7610);
+}
+IMA_DEVINL void sum_parts(const int32_t (&r)[2], uint32_t& hi, uint32_t& lo) {
+    const int32_t t = r[1] + (r[0] >> 8);
+    hi = (uint32_t)((t >> 9) + 0x4B400000);
+    lo = (__byte_perm((uint32_t)t, (uint32_t)r[0], 0x1104) & 0x1FFFFu) | 0x4B000000u;
+}
+template <int P>
+IMA_DEVINL uint64_t sums_to_float2(const int32_t (&a)[P], const int32_t (&b)[P]) {
+    if constexpr (P <= 2) {
+        uint32_t ah, al, bh, bl;
+        sum_parts(a, ah, al);
+        sum_parts(b, bh, bl);
+        const uint64_t hi = add2(pair2(__uint_as_float(ah), __uint_as_float(bh)), pair2(-12582912.0f, -12582912.0f));
+        const uint64_t lo = add2(pair2(__uint_as_float(al), __uint_as_float(bl)), pair2(-8388608.0f, -8388608.0f));
+        constexpr float S = P == 1 ? 65536.0f : 131072.0f;
+        return fma2(hi, pair2(S, S), lo);
+    } else {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int32_t(&r)[P] = e ? b : a;
+            const int64_t s = ((int64_t)r[2] << 16) + ((int64_t)r[1] << 8) + r[0];
+            const float lo = __uint_as_float(((uint32_t)s & 0x7FFFFFu) | 0x4B000000u) - 8388608.0f;
+            f[e] = __fmaf_rn(__int2float_rn((int32_t)(s >> 23)), 8388608.0f, lo);
+        }
+        return pair2(f[0], f[1]);
     }
+}
+
+IMA_DEVINL uint64_t sum2(uint32_t a, uint32_t b) {
+    const int32_t x[1] = {(int32_t)a}, y[1] = {(int32_t)b};
+    return sums_to_float2<1>(x, y);
+}
+
+// (sum * x scale) * column scale + bias of two neighbouring columns; the biases lie `half` floats behind the scales
+IMA_DEVINL uint64_t projection(uint32_t a, uint32_t b, bool zero, uint64_t x2, const float* col, int half) {
+    const float2 w = *reinterpret_cast<const float2*>(col), t = *reinterpret_cast<const float2*>(col + half);
+    return add2(mul2(mul2(zero ? 0ull : sum2(a, b), x2), pair2(w.x, w.y)), pair2(t.x, t.y));
+}
+
+IMA_DEVINL uint32_t pack_bf16(float lo, float hi) {
+    __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&b);
+}
+IMA_DEVINL uint32_t pack_f16(float lo, float hi) {
     __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
+}
+IMA_DEVINL uint32_t pack_half2(float lo, float hi, int dtype) {
+    return dtype == IMA_DTYPE_BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
 }
 
 // Staged rows out, W bytes a lane: 64 / W neighbouring lanes write one row's 64 bytes together.
@@ -194,7 +272,17 @@ IMA_DEVINL void stage_store(unsigned char* st, int lane, const uint32_t (&w)[16]
         *reinterpret_cast<uint4*>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
             make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     __syncwarp();
-    if (width == 16) stage_out<16>(st, lane, base, pitch, rows, bytes, esize);
+    if (width == 16 && rows == 32 && bytes >= 64) {   // all of it
+        uint4 v[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+            const int r = it * 8 + (lane >> 2);
+            v[it] = *reinterpret_cast<const uint4*>(st + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+        }
+        unsigned char* dst = base + (lane >> 2) * pitch + (lane & 3) * 16;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) *reinterpret_cast<uint4*>(dst + it * 8 * pitch) = v[it];
+    } else if (width == 16) stage_out<16>(st, lane, base, pitch, rows, bytes, esize);
     else if (width == 8) stage_out<8>(st, lane, base, pitch, rows, bytes, esize);
     else if (width == 4) stage_out<4>(st, lane, base, pitch, rows, bytes, esize);
     else stage_out<2>(st, lane, base, pitch, rows, bytes, esize);
@@ -215,7 +303,11 @@ IMA_DEVINL void store_y32(const I8Params& p, unsigned char* st, int lane, const 
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_half2(v[2 * j], v[2 * j + 1], p.y_dtype);
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        if (p.y_dtype != IMA_DTYPE_BF16) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack_f16(v[2 * j], v[2 * j + 1]);
+        }
         stage_store(st, lane, w, y + (row0 * p.ldy + col) * 2, p.ldy * 2, rows, min(p.N - col, 32) * 2, p.y_width, 2);
     }
 }
@@ -240,7 +332,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;   // CTA of the pair; 0 issues its MMAs
-    const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+    const int32_t first = (int32_t)(blockIdx.x / CG), step = (int32_t)(gridDim.x / CG);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::STAGES; ++s) {
@@ -275,7 +367,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
         uint32_t stage = 0, phase = 0;
         uint64_t issued = 0;
         I8Work w;
-        for (int64_t i = 0; !*abort_flag && w.get(p, i, first, step); ++i) {
+        for (int32_t i = 0; !*abort_flag && w.get(p, i, first, step); ++i) {
             int32_t mt, nt;
             i8_tile(p, w.t, mt, nt);
             for (int kt = w.k0; kt < w.k1; ++kt) {
@@ -327,7 +419,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
         if (p.stall_ns)   // test knob: a wait that nothing ends runs out
             mbar_wait_or_abort(drained, 0u, abort_flag, p.stall_ns, IMA_WHERE_INT8_GEMM, -2);
         I8Work w;
-        for (int64_t i = 0; !*abort_flag && w.get(p, i, first, step); ++i) {
+        for (int32_t i = 0; !*abort_flag && w.get(p, i, first, step); ++i) {
             if (!mbar_wait_or_abort(&acc_empty[buf], bphase ^ 1u, abort_flag, IMA_WAIT_LIMIT_NS, IMA_WHERE_INT8_GEMM, -1))
                 break;
             tc_fence_after();
@@ -370,26 +462,38 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
         unsigned char* st = smem + L::STG_OFFSET + ew * 2048;
         float* cols = reinterpret_cast<float*>(smem + L::COL_OFFSET) + ew * COLS;
         uint32_t buf = 0, bphase = 0;
-        I8Work wk;
-        for (int64_t item = 0; wk.get(p, item, first, step); ++item) {
-            int32_t mt, nt;
-            i8_tile(p, wk.t, mt, nt);
+        // this warp's column scales and biases, [2 operands][scale, bias][HALF] in shared memory, and its lane's row
+        // scale: loaded one tile ahead
+        constexpr int OPS = PAIR ? 2 : 1, EACH = EPI == I8_DIGIT ? 0 : HALF / 32;
+        float ahead[OPS * 2 * EACH + 1], xs_ahead = 0.0f;
+        auto fetch = [&](const I8Work& w, int32_t& mt, int32_t& nt) {
+            i8_tile(p, w.t, mt, nt);
+            const int64_t row = ((int64_t)mt * CG + rank) * I8_BM + q * 32 + lane;
+            xs_ahead = row < p.M && p.xs ? p.xs[row] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int32_t n = nt * TN + h * HALF + i * 32 + lane;
+#pragma unroll
+                for (int o = 0; o < OPS; ++o) {
+                    ahead[(2 * o) * EACH + i] = n < p.N && p.ws[o] ? p.ws[o][n] : 0.0f;
+                    ahead[(2 * o + 1) * EACH + i] = n < p.N && p.bias[o] ? load_as_f32(p.bias[o], p.bias_dtype, n) : -0.0f;   // x + -0 is x
+                }
+            }
+        };
+        I8Work wk, next;
+        int32_t mt = 0, nt = 0, mt_next = 0, nt_next = 0;
+        bool more = wk.get(p, 0, first, step);
+        if (more) fetch(wk, mt, nt);
+        for (int32_t item = 0; more; ++item, wk = next, mt = mt_next, nt = nt_next) {
             const int64_t row0 = ((int64_t)mt * CG + rank) * I8_BM + q * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, (int64_t)p.M - row0));
             const int32_t n0 = nt * TN + h * HALF;
-            // this warp's column scales and biases: [2 operands][scale, bias][HALF]
-            if (EPI != I8_DIGIT) {
-                __syncwarp();
-                for (int i = lane; i < HALF; i += 32) {
-                    const int32_t n = n0 + i;
+            __syncwarp();
 #pragma unroll
-                    for (int o = 0; o < (PAIR ? 2 : 1); ++o) {
-                        cols[(2 * o) * HALF + i] = n < p.N && p.ws[o] ? p.ws[o][n] : 0.0f;
-                        cols[(2 * o + 1) * HALF + i] = n < p.N && p.bias[o] ? load_as_f32(p.bias[o], p.bias_dtype, n) : 0.0f;
-                    }
-                }
-            }
-            const float xs = lane < rows && p.xs ? p.xs[row0 + lane] : 0.0f;
+            for (int i = 0; i < OPS * 2 * EACH; ++i) cols[i * 32 + lane] = ahead[i];
+            const float xs = xs_ahead;
+            more = next.get(p, item + 1, first, step);
+            if (more) fetch(next, mt_next, nt_next);
             const bool ok = mbar_wait_or_abort(&acc_full[buf], bphase, abort_flag, IMA_WAIT_LIMIT_NS,
                                                IMA_WHERE_INT8_GEMM, 200);
             __syncwarp();
@@ -397,6 +501,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
             tc_fence_after();
             const uint32_t tq = tmem_base + ((uint32_t)(q * 32) << 16) + buf * L::ACC + h * HALF;
             const bool zero = p.k_tiles == 0;   // K == 0: no MMA wrote the accumulators
+            const uint64_t x2 = pair2(xs, xs);
             if constexpr (EPI == I8_LINEAR) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < HALF; c0 += 32) {
@@ -422,9 +527,13 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                     if (p.y) {
                         float v[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            v[j] = __fmul_rn(__fmul_rn(__int2float_rn((int32_t)r[j]), xs), cols[c0 + j]);
-                            if (p.bias[0]) v[j] = __fadd_rn(v[j], cols[HALF + c0 + j]);
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 w = *reinterpret_cast<const float4*>(cols + c0 + j);
+                            const uint64_t a = mul2(mul2(sum2(r[j], r[j + 1]), x2), pair2(w.x, w.y));
+                            const uint64_t b = mul2(mul2(sum2(r[j + 2], r[j + 3]), x2), pair2(w.z, w.w));
+                            const float4 t = *reinterpret_cast<const float4*>(cols + HALF + c0 + j);
+                            const float2 va = halves(add2(a, pair2(t.x, t.y))), vb = halves(add2(b, pair2(t.z, t.w)));
+                            v[j] = va.x; v[j + 1] = va.y; v[j + 2] = vb.x; v[j + 3] = vb.y;
                         }
                         store_y32(p, st, lane, v, row0, rows, n0 + c0, p.y);
                     }
@@ -441,13 +550,11 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                         if (n0 + c0 >= p.N || rows == 0) continue;
                         float v[32];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float g0 = zero ? 0.0f : __int2float_rn((int32_t)rg[j]);
-                            const float u0 = zero ? 0.0f : __int2float_rn((int32_t)ru[j]);
-                            const float g = __fadd_rn(__fmul_rn(__fmul_rn(g0, xs), cols[c0 + j]), cols[HALF + c0 + j]);
-                            const float u = __fadd_rn(__fmul_rn(__fmul_rn(u0, xs), cols[2 * HALF + c0 + j]),
-                                                      cols[3 * HALF + c0 + j]);
-                            v[j] = act_value<ACT>(g) * u;
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 g = halves(projection(rg[j], rg[j + 1], zero, x2, cols + c0 + j, HALF));
+                            const float2 u = halves(projection(ru[j], ru[j + 1], zero, x2, cols + 2 * HALF + c0 + j, HALF));
+                            v[j] = act_value<ACT>(g.x) * u.x;
+                            v[j + 1] = act_value<ACT>(g.y) * u.y;
                         }
                         store_y32(p, st, lane, v, row0, rows, n0 + c0, p.y);
                     }
@@ -482,13 +589,14 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                         tmem_wait_ld();
                         if (n >= p.N || rows == 0) continue;
                         uint32_t wg[16], wu[16], cm = 0;
+                        float2 g2 = {}, u2 = {};
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const float g0 = zero ? 0.0f : __int2float_rn((int32_t)rg[j]);
-                            const float u0 = zero ? 0.0f : __int2float_rn((int32_t)ru[j]);
-                            const float g = __fadd_rn(__fmul_rn(__fmul_rn(g0, xs), cols[c0 + j]), cols[HALF + c0 + j]);
-                            const float u = __fadd_rn(__fmul_rn(__fmul_rn(u0, xs), cols[2 * HALF + c0 + j]),
-                                                      cols[3 * HALF + c0 + j]);
+                            if (j % 2 == 0) {
+                                g2 = halves(projection(rg[j], rg[j + 1], zero, x2, cols + c0 + j, HALF));
+                                u2 = halves(projection(ru[j], ru[j + 1], zero, x2, cols + 2 * HALF + c0 + j, HALF));
+                            }
+                            const float g = j % 2 ? g2.y : g2.x, u = j % 2 ? u2.y : u2.x;
                             float a, da;
                             act_both<ACT>(g, a, da);
                             const float dg = dh[j] * u * da, du = dh[j] * a;
@@ -526,7 +634,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                 int32_t* sums = nullptr;   // this warp's rows and columns of a split tile: [plane][column][row]
                 if (wk.split) {
                     // exact sums in any order; the last worker to add to this warp's part writes it out
-                    sums = p.tail + (((wk.t - p.full_tiles) * P * BN + h * HALF) * CG + rank) * I8_BM + q * 32 + lane;
+                    sums = p.tail + (((int64_t)(wk.t - p.full_tiles) * P * BN + h * HALF) * CG + rank) * I8_BM + q * 32 + lane;
 #pragma unroll 1
                     for (int c0 = 0; c0 < HALF; c0 += 32)
 #pragma unroll 1
@@ -563,11 +671,12 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                     if (n0 + c0 >= p.N || out_rows <= 0) continue;
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        int64_t s = 0;
+                    for (int j = 0; j < 32; j += 2) {
+                        int32_t a[P], b[P];
 #pragma unroll
-                        for (int i = 0; i < P; ++i) s += (int64_t)(int32_t)r[i][j] << (8 * i);
-                        v[j] = zero ? __fmul_rn(0.0f, xs) : __fmul_rn(__ll2float_rn(s), xs);
+                        for (int i = 0; i < P; ++i) { a[i] = (int32_t)r[i][j]; b[i] = (int32_t)r[i][j + 1]; }
+                        const float2 f = halves(mul2(zero ? 0ull : sums_to_float2<P>(a, b), x2));
+                        v[j] = f.x; v[j + 1] = f.y;
                     }
                     store_y32(p, st, lane, v, out_row, out_rows, n0 + c0, out);
                 }
@@ -669,7 +778,8 @@ int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
         if (rc != IMA_OK) return rc;
     }
     const int64_t all = (int64_t)p.m_tiles * p.n_tiles, workers = std::max<int64_t>(1, gemm_grid_limit() / CG);
-    p.full_tiles = all;
+    if (all > INT32_MAX - workers) return IMA_ERR_UNSUPPORTED;   // tiles are counted in 32 bits
+    p.full_tiles = (int32_t)all;
     p.tail_splits = 0;
     if (EPI == I8_DIGIT && p.tail && all > workers) {
         // a last round that fills less than 5/8 of the machine: its tiles split over all workers (at least 8 k-tiles
@@ -677,7 +787,7 @@ int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
         const int64_t rest = all % workers;
         const int64_t splits = rest ? std::min<int64_t>(std::min<int64_t>(workers / rest, 16), p.k_tiles / 8) : 0;
         if (rest * 8 <= workers * 5 && splits >= 2 && rest <= tail_tiles<P, BN>(CG)) {
-            p.full_tiles = all - rest;
+            p.full_tiles = (int32_t)(all - rest);
             p.tail_splits = (int32_t)splits;
             rc = ima_note_cuda(cudaMemsetAsync(p.tail, 0, tail_bytes<P, BN>(CG, rest), stream));
             if (rc != IMA_OK) return rc;
