@@ -15,35 +15,14 @@ int store_width(const void* p, int64_t ld, int esize) {
 
 int64_t i8_steps(int64_t Ka) { return (Ka + I8_KT - 1) / I8_KT; }
 
-// Time of the tiled form in ns: rounds of 128 x bn tiles over the machine at the tensor core's rate (8192
-// multiplications per clock and SM at 1.6 GHz), two thirds of it while a stage's loads limit it, and
-// 8 us from launch to the end of the last epilogue; at least the time that B takes to arrive.
-double tiled_ns(int64_t M, int64_t N, int64_t k_steps, int planes, int bn) {
-    const int64_t tiles = ((M + I8_BM - 1) / I8_BM) * ((N + bn - 1) / bn);
-    const int64_t rounds = (tiles + gemm_grid_limit() - 1) / gemm_grid_limit();
-    const double mma = (double)rounds * (double)k_steps * planes * bn * 128.0 * 128.0 / (8192.0 * 1.6 * 0.67);
-    return std::max(mma, (double)(N * k_steps * I8_KT) / 5000.0) + 8000.0;
-}
-
 // The form with the shorter estimate.
-int run_linear(I8Params& p, const I8Operands& o, cudaStream_t st) {
-    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.K), 1, 1, -1);
-    if (q.ok && q.ns < tiled_ns(p.M, p.N, i8_steps(o.K), 1, 256)) return run_skinny_codes<I8_LINEAR, 1>(p, o, q, st);
-    return launch_i8<1, 256, I8_LINEAR>(p, o, st);
-}
-
-int run_gated(I8Params& p, const I8Operands& o, cudaStream_t st) {
-    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.K), 1, 2, -1);
-    if (q.ok && q.ns < tiled_ns(p.M, 2 * (int64_t)p.N, i8_steps(o.K), 1, 256))
-        return run_skinny_codes<I8_GATED, 1>(p, o, q, st);
-    return launch_i8<1, 256, I8_GATED>(p, o, st);
-}
-
-template <int P, int BN>
-int run_digits(I8Params& p, const I8Operands& o, cudaStream_t st) {
-    const SkPlan q = sk_plan(p.M, p.N, i8_steps(o.Ka), P, 1, -1);
-    if (q.ok && q.ns < tiled_ns(p.M, p.N, i8_steps(o.Ka), P, BN)) return run_skinny_codes<I8_DIGIT, P>(p, o, q, st);
-    return launch_i8<P, BN, I8_DIGIT>(p, o, st);
+template <int P, int EPI>
+int run_codes(I8Params& p, const I8Operands& o, int ops, cudaStream_t st) {
+    const int64_t k_steps = i8_steps(o.Ka);
+    const SkPlan q = sk_plan(p.M, p.N, k_steps, P, ops, -1);
+    const TilePlan t = tile_plan<P, EPI>(p.M, p.N, k_steps, EPI == I8_DIGIT && p.tail, p.dependent != 0);
+    if (q.ok && q.ns < t.ns) return run_skinny_codes<EPI, P>(p, o, q, st);
+    return launch_i8<P, EPI>(p, o, t, st);
 }
 
 template <int EPI>
@@ -53,15 +32,19 @@ int run_fused(SkParams& p, int x_dtype, const SkPlan& q, cudaStream_t st) {
     return launch_skinny<EPI, 1, IMA_DTYPE_F32>(p, q, st);
 }
 
-// Whether the tokens are quantised inside the product: if it can, and a split that allows it costs no more
-// than the 3.5 us that the row quantiser and its launch add.
+// Whether the tokens are quantised inside the product: if it can, and that costs no more than a launch of the row
+// quantiser, whose work the product's start hides in part.  A short product is over before the host has issued
+// the next call, so the launch counts by the host's 2 us; behind a longer one (from 10 us on) it counts half of one: 3584 x
+// 18944 with one token takes 19.5 us fused and 18.2 apart, 4864 x 896 8.8 and 7.7 but 12.7 and 15 issued one by one.
 bool fused_plan(int64_t M, int64_t N, int64_t K, int ops, int x_dtype, SkPlan& q) {
     if (M < 1 || M > SK_MAX_TM || N < 1) return false;
     q = sk_plan(M, N, i8_steps(K), 1, ops, x_dtype);
     if (!q.ok) return false;
     const SkPlan codes = sk_plan(M, N, i8_steps(K), 1, ops, -1);
-    const double tiled = tiled_ns(M, ops * N, i8_steps(K), 1, 256);
-    return q.ns <= std::min(codes.ok ? codes.ns : tiled, tiled) + 3500.0;
+    const double tiled = ops == 2 ? tile_plan<1, I8_GATED>(M, N, i8_steps(K), false, true).ns
+                                  : tile_plan<1, I8_LINEAR>(M, N, i8_steps(K), false, true).ns;
+    const double apart = std::min(codes.ok ? codes.ns : tiled, tiled);
+    return q.ns <= apart + (apart < 10000.0 ? 2000.0 : 500.0);
 }
 
 }  // namespace
@@ -115,7 +98,7 @@ int int8_gemm_entry(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, 
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
     p.c_width = store_width(c, ldc, 4);
     p.y_width = store_width(y, ldy, y ? dtype_bytes(y_dtype) : 4);
-    return run_linear(p, {a, b, nullptr, lda, ldb, 0, K, K, M * lda}, (cudaStream_t)stream);
+    return run_codes<1, I8_LINEAR>(p, {a, b, nullptr, lda, ldb, 0, K, K, M * lda}, 1, (cudaStream_t)stream);
 }
 
 int int8_gated_entry(const int8_t* a, int64_t lda, const int8_t* gate, int64_t ldg, const int8_t* up, int64_t ldu,
@@ -137,7 +120,7 @@ int int8_gated_entry(const int8_t* a, int64_t lda, const int8_t* gate, int64_t l
     p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = activation;
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
     p.y_width = store_width(y, ldy, dtype_bytes(y_dtype));
-    return run_gated(p, {a, gate, up, lda, ldg, ldu, K, K, M * lda}, (cudaStream_t)stream);
+    return run_codes<1, I8_GATED>(p, {a, gate, up, lda, ldg, ldu, K, K, M * lda}, 2, (cudaStream_t)stream);
 }
 
 }  // namespace
@@ -303,7 +286,7 @@ int zero_out(void* p, int64_t n, int dtype, cudaStream_t st) {
     return ima_note_cuda(cudaMemsetAsync(p, 0, (size_t)(n * dtype_bytes(dtype)), st));
 }
 
-template <int P, int BN>
+template <int P>
 int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStream_t st) {
     int rc = IMA_OK;
     if (a.dx) {
@@ -323,7 +306,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         p.tail = b.has_tail ? reinterpret_cast<int32_t*>(ws + b.tail) : nullptr;
         const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.rows), wt[0], a.segs == 2 ? wt[1] : nullptr, b.W,
                               ldwt[0], ldwt[1], (a.segs - 1) * b.pitch + a.N, a.N, a.M * b.W};
-        if (a.K > 0) rc = run_digits<P, BN>(p, o, st);
+        if (a.K > 0) rc = run_codes<P, I8_DIGIT>(p, o, 1, st);
         if (rc != IMA_OK) return rc;
     }
     if ((a.dw[0] || a.dw[1]) && a.K > 0) {
@@ -344,7 +327,7 @@ int bwd_products(const BwdArgs& a, const BwdPlan& b, unsigned char* ws, cudaStre
         p.tail = b.has_tail ? reinterpret_cast<int32_t*>(ws + b.tail) : nullptr;
         const I8Operands o = {reinterpret_cast<const int8_t*>(ws + b.cols) + first * b.pitch * b.ldm, qt, nullptr, b.ldm,
                               b.ldm, 0, a.M, a.M, b.W * b.ldm};
-        rc = run_digits<P, BN>(p, o, st);
+        rc = run_codes<P, I8_DIGIT>(p, o, 1, st);
     }
     return rc;
 }
@@ -410,7 +393,8 @@ int run_backward(const BwdArgs& a, cudaStream_t st) {
         p.d = reinterpret_cast<float*>(ws + b.d); p.ldd = b.W; p.seg_pitch = b.pitch;
         p.row_max = g.row_max; p.col_max = g.col_max;
         p.M = (int32_t)a.M; p.N = (int32_t)a.N;
-        rc = launch_i8<1, 256, I8_GATED_BWD>(p, {a.q, a.w[0], a.w[1], a.ldq, a.ldw[0], a.ldw[1], a.K, a.K, a.M * a.ldq}, st);
+        rc = launch_i8<1, I8_GATED_BWD>(p, {a.q, a.w[0], a.w[1], a.ldq, a.ldw[0], a.ldw[1], a.K, a.K, a.M * a.ldq},
+                                         tile_plan<1, I8_GATED_BWD>(a.M, a.N, i8_steps(a.K), false, false), st);
         if (rc != IMA_OK) return rc;
         g.src = p.d;
         g.ld = b.W;
@@ -431,7 +415,7 @@ int run_backward(const BwdArgs& a, cudaStream_t st) {
     d.ldm = b.ldm;
     rc = run_grad_digits(d, src_dtype, a.planes, st);
     if (rc != IMA_OK) return rc;
-    rc = a.planes == 2 ? bwd_products<2, 256>(a, b, ws, st) : bwd_products<3, 128>(a, b, ws, st);
+    rc = a.planes == 2 ? bwd_products<2>(a, b, ws, st) : bwd_products<3>(a, b, ws, st);
     if (rc == IMA_OK && want_db) {
         const dim3 grid((unsigned)((a.N + 255) / 256), (unsigned)a.segs);
         int8_col_sum_kernel<<<grid, 256, 0, st>>>(d.partial, (a.M + 127) / 128, b.W, a.N, b.pitch, a.db[0], a.db[1],

@@ -822,18 +822,66 @@ int launch_i8_tile(I8Params& p, const I8Operands& o, cudaStream_t stream) {
     return ima_note_cuda(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-// A CTA pair computes 256 rows by BN columns with half of B in each CTA, so a stage moves 2/3 of
-// the bytes of two single CTAs (P == 1), which is what the L2 -> SM path limits; one CTA halves the
-// tile.  The pair is taken when it needs no more than 4/3 of the single form's time in whole rounds of
-// tiles over the machine.
-template <int P, int BN, int EPI>
-int launch_i8(I8Params& p, const I8Operands& o, cudaStream_t stream) {
-    constexpr int TN = EPI == I8_GATED || EPI == I8_GATED_BWD ? BN / 2 : BN;
-    const int64_t sms = gemm_grid_limit(), nt = (p.N + TN - 1) / TN;
-    const int64_t one = ((p.M + I8_BM - 1) / I8_BM * nt + sms - 1) / sms;
-    const int64_t two = sms < 2 ? INT32_MAX : ((p.M + 2 * I8_BM - 1) / (2 * I8_BM) * nt + sms / 2 - 1) / (sms / 2);
-    if (two * 3 <= one * 4) return launch_i8_tile<P, BN, EPI, 2>(p, o, stream);
-    return launch_i8_tile<P, BN, EPI, 1>(p, o, stream);
+// Tile forms: a CTA pair (256 rows, each CTA holds half of B), one CTA, or one CTA with half the columns.  Per
+// unit of work the pair loads least (L2 to SM is 64 bytes a clock and SM), the small tile most; the small one fills the
+// machine with few tiles, ends a last round sooner, and with two digit planes has room for a second accumulator, so that
+// the epilogue of a tile runs during the products of the next.
+struct TilePlan {
+    double ns;
+    int bn, cg;
+};
+
+// Time of a form in ns, fitted to 160 measured times of 40 products of 128 to 16384 rows, and within 15 % of those
+// with one plane.  Clocks of a k-tile: 650 for the wide pair and 720 for the wide CTA with one plane, 850 with three, else
+// the tensor core's 2 per plane and column or the loads' bytes / 64, and 4 % more.  The epilogue of a tile takes 22 to 24
+// clocks per column (two planes 27, three 80, the gated gradients 35), behind the products of the next tile where two
+// accumulators fit.  3.5 us from launch to the first products, 0.6 more for a cluster; 1 more after a quantiser, whose
+// end the split form awaits with its weights already on their way.
+inline double tile_ns(int64_t M, int64_t N, int64_t k_steps, int planes, int epi, int bn, int cg, bool tail,
+                      bool dependent) {
+    const bool pair = epi == I8_GATED || epi == I8_GATED_BWD;
+    const int64_t tn = pair ? bn / 2 : bn, tiles = ((M + cg * I8_BM - 1) / (cg * I8_BM)) * ((N + tn - 1) / tn);
+    const int64_t workers = std::max<int64_t>(1, gemm_grid_limit() / cg);
+    const double mma = 2.0 * planes * bn, load = (planes * I8_BM + bn / cg) * I8_KT / 64.0;
+    const double step = planes == 1 && bn == 256 ? (cg == 2 ? 650.0 : 720.0) : planes == 3 ? 850.0 : 1.04 * std::max(mma, load);
+    const double products = (double)k_steps * step;
+    const double epilogue = (double)(std::min(tn, N) * (pair ? 2 : 1)) *
+                            (epi == I8_GATED_BWD ? 35.0 : planes == 1 ? 20.0 + 2.0 * cg : planes == 2 ? 27.0 : 80.0);
+    int64_t rounds = (tiles + workers - 1) / workers;
+    double extra = 0.0;
+    const int64_t rest = tiles % workers;
+    if (tail && rounds > 1 && rest && rest * 8 <= workers * 5) {   // the last round's tiles are split over all workers
+        rounds -= 1;
+        extra = products * (double)rest / (double)workers + 2.0 * epilogue;
+    }
+    const double clocks = 2 * planes * bn <= 512
+        ? products + (double)(rounds - 1) * std::max(products, epilogue) + epilogue
+        : (double)rounds * (products + epilogue);
+    const double streams = (double)((N * (pair ? 2 : 1) + M * planes) * k_steps * I8_KT) / 4700.0;
+    return std::max((clocks + extra) / 1.77, streams) + (cg == 2 ? 4100.0 : 3500.0) + (dependent ? 1000.0 : 0.0);
+}
+
+template <int P, int EPI>
+TilePlan tile_plan(int64_t M, int64_t N, int64_t k_steps, bool tail, bool dependent) {
+    constexpr int WIDE = P == 3 ? 128 : 256;
+    TilePlan best = {tile_ns(M, N, k_steps, P, EPI, WIDE, 1, tail, dependent), WIDE, 1};
+    auto consider = [&](int bn, int cg) {
+        const double ns = tile_ns(M, N, k_steps, P, EPI, bn, cg, tail, dependent);
+        if (ns < best.ns) best = {ns, bn, cg};
+    };
+    if (gemm_grid_limit() >= 2) consider(WIDE, 2);
+    if (P < 3 && EPI != I8_GATED_BWD) consider(128, 1);
+    return best;
+}
+
+template <int P, int EPI>
+int launch_i8(I8Params& p, const I8Operands& o, const TilePlan& t, cudaStream_t stream) {
+    constexpr int WIDE = P == 3 ? 128 : 256;
+    if (t.cg == 2) return launch_i8_tile<P, WIDE, EPI, 2>(p, o, stream);
+    if constexpr (P < 3 && EPI != I8_GATED_BWD) {
+        if (t.bn == 128) return launch_i8_tile<P, 128, EPI, 1>(p, o, stream);
+    }
+    return launch_i8_tile<P, WIDE, EPI, 1>(p, o, stream);
 }
 
 }  // namespace

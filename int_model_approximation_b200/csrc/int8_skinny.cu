@@ -434,11 +434,12 @@ struct SkPlan {
 };
 
 // The split form of a product of M tokens by N outputs over k_steps k-steps: tokens per tile, split and
-// stages with the shortest estimate, which follows measurements.  A CTA streams its tiles at 34 bytes/ns
-// whatever its stages beyond three (a kernel that only loads 68 MB with one CTA per SM takes 15.0 us), the
-// machine at 5500; so two CTAs of four stages per SM beat one of eight (3584 x 18944 with 16 tokens: 18.9 us
-// with 224 CTAs, 24.6 with 112).  A round of CTAs takes 6 us from launch to exit besides, its epilogue 12
-// ns per token column, the exchange in a cluster 1 us.
+// stages with the shortest estimate, which follows measurements.  A CTA streams its weights at 45 bytes/ns
+// whatever its stages beyond three (a kernel that only loads 68 MB with one CTA per SM takes 15.0 us), token codes,
+// which other CTAs read too, at 100 from L2, and the machine 5500; so two CTAs of four stages per SM beat one of
+// eight (3584 x 18944 with 16 tokens: 18.9 us with 224 CTAs, 24.6 with 112).  A round of CTAs takes 5 us from launch to
+// exit besides, the epilogue of the outputs that a CTA keeps 16 ns per token column (32 of two that share an SM), the
+// exchange in a cluster 4 ns per column and 1 us.
 // The fused quantiser (x_dtype >= 0) takes what its workers hold in registers at once: another pass over the
 // activations costs 6 us (64 tokens, K = 3584), more than the row quantiser and its launch.
 SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x_dtype) {
@@ -469,12 +470,12 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x
         q.splits = s; q.stages = (int)stages; q.codes_bytes = (int)codes; q.partial_bytes = (int)partial;
         q.smem = (int)(fixed + stages * stage);
         const int64_t ctas = m_tiles * n_tiles * s;
-        // clusters of 8 leave some SMs out
-        const int64_t room = std::max<int64_t>(1, gemm_grid_limit() * per_sm * (s == 8 ? 7 : 8) / 8);
+        // clusters of 8 leave some SMs out, and so do those of 4
+        const int64_t room = std::max<int64_t>(1, gemm_grid_limit() * per_sm * (s == 8 ? 14 : s == 4 ? 15 : 16) / 16);
         const double rounds = (double)((ctas + room - 1) / room);
-        const double stream = std::max((double)(steps * stage) / 34.0 * rounds,
+        const double stream = std::max(rounds * (double)steps * ((double)(ops * SK_ROWS * I8_KT) / 45.0 + (double)(stage - ops * SK_ROWS * I8_KT) / 100.0),
                                        (double)(N * k_steps * I8_KT * ops * m_tiles) / 5500.0);
-        q.ns = rounds * (6000.0 + 12.0 * (double)(ops * planes * tm)) + stream + (s > 1 ? 1000.0 : 0.0);
+        q.ns = rounds * ((fused ? 6000.0 + 100.0 * (double)M : 5000.0) + (4.0 + 16.0 * (double)per_sm / (double)s) * (double)(ops * planes * tm)) + stream + (s > 1 ? 1000.0 : 0.0);
         q.ok = true;
         if (!best.ok || q.ns < best.ns) best = q;
     }
