@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                         for (int i = 0; i < P; ++i)
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                r[i][j] = (uint32_t)__ldcg(sums + (int64_t)(i * BN + c0 + j) * CG * I8_BM);
+                                r[i][j] = load_l2(sums + (int64_t)(i * BN + c0 + j) * CG * I8_BM);
                     } else {
 #pragma unroll
                         for (int i = 0; i < P; ++i) tmem_ld32(tq + i * BN + c0, r[i]);

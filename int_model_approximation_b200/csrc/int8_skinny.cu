@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
         for (int o = 0; o < OPS; ++o)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? __ldg(p.ws[o] + nq + e) : 0.0f;
-                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, nq + e) : 0.0f;
+                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? p.ws[o][nq + e] : 0.0f;   // a kernel that still ran at this one's start may have written it: not __ldg
+                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, nq + e) : -0.0f;   // x + -0 is x
             }
         // the value of one output from its exact sums: a[plane], or a[0] of the operand(s)
         auto value = [&](const int32_t (&a)[P], int32_t b, float xs, int e) {
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
                     const float u = __fmul_rn(__fmul_rn(__int2float_rn(b), xs), ws[OPS - 1][e]);
                     return gated_value(p.act, __fadd_rn(v, bias[0][e]), __fadd_rn(u, bias[OPS - 1][e]));
                 }
-                return p.bias[0] ? __fadd_rn(v, bias[0][e]) : v;
+                return __fadd_rn(v, bias[0][e]);
             }
         };
         // row of y that token t of the tile goes to (false: none)

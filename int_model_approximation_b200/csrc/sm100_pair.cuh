@@ -86,6 +86,13 @@ IMA_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         : "r"(taddr));
 }
 
+// A word as it is in L2 now; stays behind the fences before it.
+IMA_DEVINL uint32_t load_l2(const int32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.cg.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
 // A kernel launched to start early (programmatic stream serialization): wait until the kernel before it has ended
 // and its writes are visible; and, in that kernel, allow the start.
 IMA_DEVINL void wait_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

@@ -366,6 +366,9 @@ def _weight_args(weight) -> tuple[Int8Weight, torch.Tensor | None]:
     src = _rows(weight.detach())
     n, k = src.shape
     made = Int8Weight.__new__(Int8Weight)
+    if k == 0:   # nothing to quantise: the scales of rows of zeros
+        made._set(_empty_codes(n, k, src), src.new_full((n,), 1e-12, dtype=torch.float32))
+        return made, None
     made._set(_empty_codes(n, k, src), src.new_empty((n,), dtype=torch.float32))
     return made, src
 

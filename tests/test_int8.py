@@ -1032,3 +1032,21 @@ def test_outputs_of_every_alignment(cuda_device, dtype, m, n, k, pad):
     assert (c_big[m:] == 77).all() and (y_big[m:] == 77).all()
     assert (c_big[:, :pad] == 77).all() and (y_big[:, :pad] == 77).all()
     status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+def test_empty_contraction_reads_no_stale_memory(cuda_device):
+    """Scales of weights without columns are those of zeros, whatever lay in their memory."""
+    for _ in range(4):
+        for n in (5, 300):
+            poison = [torch.full((n,), float("nan"), device=cuda_device) for _ in range(8)]
+            del poison
+            x, w = torch.randn((3, 0), device=cuda_device), torch.randn((n, 0), device=cuda_device)
+            b = torch.randn((n,), device=cuda_device)
+            for leaf in (x, w):
+                leaf.requires_grad_()
+            assert torch.equal(int8.int8_linear(x, w, b), b.expand(3, n))
+            assert float(int8.int8_gated(x, w, w, b, None).detach().abs().sum()) == 0.0
+            assert torch.equal(int8.int8_linear(x.detach(), w.detach(), b), b.expand(3, n))
+            assert float(int8.int8_gated(x.detach(), w.detach(), w.detach(), b, None).abs().sum()) == 0.0
+    status_clean(cuda_device)
