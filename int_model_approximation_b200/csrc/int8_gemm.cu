@@ -463,7 +463,8 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
         float* cols = reinterpret_cast<float*>(smem + L::COL_OFFSET) + ew * COLS;
         uint32_t buf = 0, bphase = 0;
         // this warp's column scales and biases, [2 operands][scale, bias][HALF] in shared memory, and its lane's row
-        // scale: loaded one tile ahead
+        // scale: loaded one tile ahead where registers allow (16 warps have 96 each, and hide the loads anyway)
+        constexpr bool AHEAD = EPI != I8_GATED_BWD;
         constexpr int OPS = PAIR ? 2 : 1, EACH = EPI == I8_DIGIT ? 0 : HALF / 32;
         float ahead[OPS * 2 * EACH + 1], xs_ahead = 0.0f;
         auto fetch = [&](const I8Work& w, int32_t& mt, int32_t& nt) {
@@ -483,8 +484,9 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
         I8Work wk, next;
         int32_t mt = 0, nt = 0, mt_next = 0, nt_next = 0;
         bool more = wk.get(p, 0, first, step);
-        if (more) fetch(wk, mt, nt);
-        for (int32_t item = 0; more; ++item, wk = next, mt = mt_next, nt = nt_next) {
+        if (AHEAD && more) fetch(wk, mt, nt);
+        for (int32_t item = 0; more; ++item) {
+            if (!AHEAD) fetch(wk, mt, nt);
             const int64_t row0 = ((int64_t)mt * CG + rank) * I8_BM + q * 32;
             const int rows = (int)max((int64_t)0, min((int64_t)32, (int64_t)p.M - row0));
             const int32_t n0 = nt * TN + h * HALF;
@@ -492,8 +494,10 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
 #pragma unroll
             for (int i = 0; i < OPS * 2 * EACH; ++i) cols[i * 32 + lane] = ahead[i];
             const float xs = xs_ahead;
-            more = next.get(p, item + 1, first, step);
-            if (more) fetch(next, mt_next, nt_next);
+            if (AHEAD) {
+                more = next.get(p, item + 1, first, step);
+                if (more) fetch(next, mt_next, nt_next);
+            }
             const bool ok = mbar_wait_or_abort(&acc_full[buf], bphase, abort_flag, IMA_WAIT_LIMIT_NS,
                                                IMA_WHERE_INT8_GEMM, 200);
             __syncwarp();
@@ -688,6 +692,11 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                 else mbar_arrive(&acc_empty[buf]);
             }
             if (++buf == (uint32_t)L::BUFS) { buf = 0; bphase ^= 1u; }
+            if (AHEAD) {
+                wk = next; mt = mt_next; nt = nt_next;
+            } else {
+                more = wk.get(p, item + 1, first, step);
+            }
         }
     }
     __syncthreads();
@@ -832,18 +841,18 @@ struct TilePlan {
 };
 
 // Time of a form in ns, fitted to 160 measured times of 40 products of 128 to 16384 rows, and within 15 % of those
-// with one plane.  Clocks of a k-tile: 650 for the wide pair and 720 for the wide CTA with one plane, 850 with three, else
-// the tensor core's 2 per plane and column or the loads' bytes / 64, and 4 % more.  The epilogue of a tile takes 22 to 24
-// clocks per column (two planes 27, three 80, the gated gradients 35), behind the products of the next tile where two
-// accumulators fit.  3.5 us from launch to the first products, 0.6 more for a cluster; 1 more after a quantiser, whose
-// end the split form awaits with its weights already on their way.
+// with one plane.  A k-tile takes the tensor core 2 clocks per plane and column, and its loads 1 per 64 bytes; measured,
+// the wide pair needs 650 and the wide CTA 720 clocks with one plane, 1065 and 1100 with two.  The epilogue of a tile
+// takes 22 to 24 clocks per column (two planes 27, three 80, the gated gradients 35), behind the products of the
+// next tile where two accumulators fit.  3.5 us from launch to the first products, 0.6 more for a cluster; 1 more after a
+// quantiser, whose end the split form awaits with its weights already on their way.
 inline double tile_ns(int64_t M, int64_t N, int64_t k_steps, int planes, int epi, int bn, int cg, bool tail,
                       bool dependent) {
     const bool pair = epi == I8_GATED || epi == I8_GATED_BWD;
     const int64_t tn = pair ? bn / 2 : bn, tiles = ((M + cg * I8_BM - 1) / (cg * I8_BM)) * ((N + tn - 1) / tn);
     const int64_t workers = std::max<int64_t>(1, gemm_grid_limit() / cg);
-    const double mma = 2.0 * planes * bn, load = (planes * I8_BM + bn / cg) * I8_KT / 64.0;
-    const double step = planes == 1 && bn == 256 ? (cg == 2 ? 650.0 : 720.0) : planes == 3 ? 850.0 : 1.04 * std::max(mma, load);
+    const double step = planes == 3 ? 850.0 : planes == 2 ? (bn == 128 ? 800.0 : cg == 2 ? 1065.0 : 1100.0)
+                                                          : (bn == 128 ? 530.0 : cg == 2 ? 650.0 : 720.0);
     const double products = (double)k_steps * step;
     const double epilogue = (double)(std::min(tn, N) * (pair ? 2 : 1)) *
                             (epi == I8_GATED_BWD ? 35.0 : planes == 1 ? 20.0 + 2.0 * cg : planes == 2 ? 27.0 : 80.0);
