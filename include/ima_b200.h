@@ -371,8 +371,7 @@ int ima_int8_gemm(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb, in
  *   linear: y = (fp32(q w^T) * scale[m]) * w_scale[n] (+ bias[n])
  *   gated:  y = act(g) * u, both projections, activation and product in one kernel, with
  *           g = (fp32(q gate^T) * scale[m]) * gate_scale[n] (+ gate_bias[n]) and u the same of up
- * q [M,ldq]
- * int8 and scale [M] are workspace; with keep_codes != 0 they hold the codes and scales of x
+ * q [M,ldq] int8 and scale [M] are workspace; with keep_codes != 0 they hold the codes and scales of x
  * afterwards (what a backward pass needs), otherwise a product of few tokens quantises them in
  * its own launch and leaves both alone.  w_src (gate_src, up_src): the weight [N,K] as a floating
  * tensor of w_src_dtype, quantised first into w and w_scale; NULL when those hold it already. */
@@ -405,7 +404,7 @@ int ima_int8_pack_rows(const int8_t* a, int64_t rows_a, int64_t lda, int8_t* dst
  * dx [M,K], dw [N,K], db [N] are contiguous, each optional (NULL).  w_t (gate_t, up_t): the transposed
  * codes [K,N] if the caller keeps them, else NULL and they are made in the workspace.  planes: base-256
  * digits of the real factor of each product against its row maximum, 2 (2^-16 of it) or 3 (2^-24).
- * Contractions are at most 131072 - 1: N (gated: round_up(N, 128) + N) for dx, M for dw
+ * Contractions are at most 131071: N (gated: round_up(N, 128) + N) for dx, M for dw
  * (IMA_ERR_UNSUPPORTED beyond).  workspace: ima_int8_backward_workspace_bytes(...), 256-byte aligned;
  * own_transposed != 0 when a w_t is NULL. */
 int64_t ima_int8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int planes, int dx, int dw, int db,

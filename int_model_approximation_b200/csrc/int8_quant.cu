@@ -162,7 +162,8 @@ IMA_DEVINL uint32_t row_max(uint32_t m, uint32_t* s_max) {
 // ---------------------------------------------------------------------------
 // Row quantiser.  TPR threads take one row; a row of up to TPR * 8 * V elements is read once
 // and kept in registers between the maximum and the codes, a longer one is read again (from
-// L2).  Bound by memory: 2 or 4 bytes in and 1 out per element.
+// L2).  Bound by memory: 2 or 4 bytes in and 1 out per element.  16384 x 3584 from bf16 takes 37 us (27 at the
+// measured copy rate), 16384 x 18944 177 (142); fp32 rows are at the copy rate.
 // ---------------------------------------------------------------------------
 struct QuantRows {           // up to three matrices of K columns, one after the other (activations, weights)
     const void* x[3];
@@ -323,7 +324,8 @@ __global__ void __launch_bounds__(256) int8_grad_max_kernel(const GradSrc a) {
 // by 64 columns; the transposed form goes through shared memory.  There a row is 16 quads of columns, the
 // two of its thread t at t ^ (row / 16) and (t + 8) ^ (row / 16): eight threads that write a row, and eight
 // 16-row groups that read a quad, meet no bank conflicts.  Every plane row is written
-// in pieces of 64 (rows) or 128 (columns) contiguous bytes.  Either form and the sums may be absent.
+// in pieces of 64 (rows) or 128 (columns) contiguous bytes.  Either form and the sums may be absent.  Bound by
+// memory: 4096 x 37888 from fp32 to two planes both ways (1.24 GB) takes 212 us, 189 at the measured copy rate.
 struct GradDigits {
     GradSrc g;
     int8_t* rows;             // [P][M][W]

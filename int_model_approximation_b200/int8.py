@@ -15,9 +15,9 @@ There is no counterpart in the reference.
   int8_linear_backward, int8_gated_backward   their gradients as plain calls
 
 int8_linear and int8_gated take part in autograd (a whole training step can be captured into a CUDA
-graph if no eager autograd graph of the same leaves is alive; the *_backward calls can always).  Gradients pass straight through the
-rounding: they are the derivatives at the dequantised activations and weights, with the
-scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
+graph if no eager autograd graph of the same leaves is alive; the *_backward calls can always).
+Gradients pass straight through the rounding: they are the derivatives at the dequantised
+activations and weights, with the scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
 gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
 products of a backward pass run on the int8 tensor cores too: the gradient is written in
 base-256 digits of its row maximum (two digits for bf16 tensors, three for fp16 and fp32; see

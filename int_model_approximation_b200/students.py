@@ -6,7 +6,8 @@ same student modules (CodebookLinear, HawkeyeLinear, HawkeyeClassCountsLinear an
 the non-FP8 Int32Linear, __main__.py:390-523), the same kernel wrappers
 (_int32_raw_matmul :228-253, _int32_matmul :301-333), the same probe
 (_Int32KernelProbe :667-678, bumped once per checkable integer product) and the
-same replacement pass (_replace_int32_linears :563-588).  Every integer product
+same replacement pass (_replace_int32_linears :563-588).  One kernel more: "int8",
+plain 8-bit linears and gated blocks (Int8Linear, Int8GatedMLP).  Every integer product
 runs on the sm_100a kernels of libima_b200.so; there is no CPU execution path.
 """
 
