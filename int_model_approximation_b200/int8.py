@@ -97,24 +97,31 @@ def _empty_codes(rows: int, k: int, like: torch.Tensor) -> torch.Tensor:
 
 
 def _check_codes(t: torch.Tensor, label: str) -> None:
-    if t.dtype != torch.int8 or t.ndim != 2:
+    if t.dtype is not torch.int8 or t.ndim != 2:
         raise RuntimeError(f"{label} must be a 2-D int8 tensor, got {t.dtype} {tuple(t.shape)}")
-    _require_cuda(t, label)
+    if not t.is_cuda:
+        _require_cuda(t, label)
     if t.shape[1] > MAX_K:
         raise RuntimeError(f"{label}: contraction of {t.shape[1]} exceeds {MAX_K} (exact int32 sums)")
 
 
-def _is_aligned(t: torch.Tensor) -> bool:
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.data_ptr() % 16:
-        return t.numel() == 0
-    return t.shape[0] <= 1 or t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1] or t.numel() == 0
+def _layout(t: torch.Tensor, rows: int, k: int) -> tuple[int, int] | None:
+    """(address, row stride) of an int8 matrix that the kernels can load, None if it has to be moved first."""
+    at, (ld, step) = t.data_ptr(), t.stride()
+    if rows <= 1 or k == 0:
+        ld = _round_up(max(k, 1), 16)
+    elif ld % 16 or ld < k:
+        return None
+    if at % 16 or step != 1 and k > 1:
+        return None if rows and k else (at, ld)
+    return at, ld
 
 
 def _aligned_codes(t: torch.Tensor, label: str) -> torch.Tensor:
     """An int8 matrix as the kernels load it: contiguous rows that start on 16 bytes (a copy
     only if it is not)."""
     _check_codes(t, label)
-    return t if _is_aligned(t) else _packed_codes(t)[0]
+    return t if _layout(t, *t.shape) else _packed_codes(t)[0]
 
 
 def _packed_codes(*given: torch.Tensor) -> list[torch.Tensor]:
@@ -137,7 +144,8 @@ def _packed_codes(*given: torch.Tensor) -> list[torch.Tensor]:
 
 
 def _code_ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else _round_up(max(t.shape[1], 1), 16)
+    rows, k = t.shape
+    return t.stride(0) if rows > 1 and k else _round_up(max(k, 1), 16)
 
 
 def _scales(t: torch.Tensor, n: int, label: str) -> torch.Tensor:
@@ -305,15 +313,18 @@ def int8_gemm(
     (m, k), n = a.shape, b.shape[0]
     if b.shape[1] != k:
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={b.shape[1]}")
-    dev = a.device
-    for label, t in (("B matrix", b), ("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias), ("int32 output", c_out),
-                     ("output", y_out)):
-        if t is not None and t.device != dev:
-            nat.require_device(dev, (label, t))
-    pack_a, pack_b = not _is_aligned(a), not _is_aligned(b)
-    if pack_a or pack_b:
-        packed = _packed_codes(*(t for t, wanted in ((a, pack_a), (b, pack_b)) if wanted))
-        a, b = packed[0] if pack_a else a, packed[-1] if pack_b else b
+    index = a.get_device()
+    for t in (b, x_scale, w_scale, bias, c_out, y_out):
+        if t is not None and t.get_device() != index:
+            nat.require_device(a.device, ("B matrix", b), ("x_scale", x_scale), ("w_scale", w_scale), ("bias", bias),
+                               ("int32 output", c_out), ("output", y_out))
+    a_at, b_at = _layout(a, m, k), _layout(b, n, k)
+    if a_at is None or b_at is None:
+        packed = _packed_codes(*(t for t, at in ((a, a_at), (b, b_at)) if at is None))
+        if a_at is None:
+            a_at = _layout(packed[0], m, k)
+        if b_at is None:
+            b_at = _layout(packed[-1], n, k)
     if c_out is not None:
         _check_out(c_out, (m, n), (torch.int32,), "int8 product")
         c = c_out
@@ -327,16 +338,18 @@ def int8_gemm(
             _check_out(y_out, (m, n), tuple(_DTYPE_CODES), "output")
             y = y_out
         else:
-            _check_types(y_dtype)
+            if y_dtype not in _DTYPE_CODES:
+                nat.dtype_code(y_dtype)
             y = a.new_empty((m, n), dtype=y_dtype)
         x_scale = _scales(x_scale, m, "x_scale")
         w_scale = _scales(w_scale, n, "w_scale")
-        (bias,), bias_dtype = _bias_args(n, bias)
+        if bias is not None:
+            (bias,), bias_dtype = _bias_args(n, bias)
     else:
         x_scale = w_scale = bias = None
     if c is None and y is None:
         raise RuntimeError("int8_gemm has no output to compute: want_c, y_dtype or y_out")
-    _call(dev, "ima_int8_gemm", a.data_ptr(), _code_ld(a), b.data_ptr(), _code_ld(b), m, n, k, _ptr(c),
+    _call(a.device, "ima_int8_gemm", *a_at, *b_at, m, n, k, _ptr(c),
           _ld(c) if c is not None else n, _ptr(x_scale), _ptr(w_scale), _ptr(bias), bias_dtype, _ptr(y), _code(y),
           _ld(y) if y is not None else n)
     return c, y

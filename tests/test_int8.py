@@ -1050,3 +1050,16 @@ def test_empty_contraction_reads_no_stale_memory(cuda_device):
             assert torch.equal(int8.int8_linear(x.detach(), w.detach(), b), b.expand(3, n))
             assert float(int8.int8_gated(x.detach(), w.detach(), w.detach(), b, None).abs().sum()) == 0.0
     status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+def test_codes_without_columns_as_they_come(cuda_device):
+    q = torch.empty((4, 0), dtype=torch.int8, device=cuda_device)
+    w = int8.Int8Weight(torch.empty((3, 0), dtype=torch.int8, device=cuda_device), torch.ones(3, device=cuda_device))
+    c, _ = int8.int8_gemm(q, w.codes)
+    assert c.shape == (4, 3) and not c.any()
+    dy = torch.ones((4, 3), device=cuda_device)
+    dx, _dw, db = int8.int8_linear_backward(dy, q, torch.ones(4, device=cuda_device), w, dx_dtype=torch.float32,
+                                            db_dtype=torch.float32)
+    assert dx.shape == (4, 0) and torch.equal(db, torch.full((3,), 4.0, device=cuda_device))
+    status_clean(cuda_device)
