@@ -79,7 +79,8 @@ def _require_cuda(t: torch.Tensor, label: str) -> None:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t [..., K] as a matrix whose rows are contiguous and do not overlap (a copy if need be)."""
     r = t if t.ndim == 2 else t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
-    if (r.stride(1) != 1 and r.shape[1] > 1) or (r.shape[0] > 1 and r.stride(0) < r.shape[1]):
+    (ld, step), (m, k) = r.stride(), r.shape
+    if (step != 1 and k > 1) or (m > 1 and ld < k):
         r = r.contiguous()
     return r
 
@@ -211,7 +212,7 @@ class Int8Weight:
 
     def _set(self, codes: torch.Tensor, scale: torch.Tensor) -> None:
         self.codes, self.scale = codes, scale
-        self.shape, self.device, self.ld = codes.shape, codes.device, _code_ld(codes)
+        self.shape, self.device, self.index, self.ld = codes.shape, codes.device, codes.get_device(), _code_ld(codes)
         self._transposed: tuple | None = None   # (codes [K, N], version of self.codes, stream, event until it has passed)
 
     def __getstate__(self):
@@ -275,6 +276,10 @@ def _check_out(t: torch.Tensor, shape: tuple[int, int], dtypes: tuple, label: st
 
 def _bias_args(n: int, *biases: torch.Tensor | None) -> tuple[list[torch.Tensor | None], int]:
     """Biases as contiguous vectors of one floating type, and that type's code."""
+    if len(biases) == 1 and biases[0] is not None:   # the usual case, as it is
+        b = biases[0]
+        if b.ndim == 1 and b.dtype in _DTYPE_CODES and b.shape[0] == n and b.is_contiguous():
+            return list(biases), _DTYPE_CODES[b.dtype]
     dtype = None
     for b in biases:
         if b is not None:
@@ -355,15 +360,14 @@ def int8_gemm(
     return c, y
 
 
-def _code_buffers(rows: torch.Tensor, n: int, gated: bool, keep: bool):
+def _code_buffers(rows: torch.Tensor, m: int, k: int, n: int, gated: bool, x_type: int, keep: bool):
     """Room for the codes and scales of x rows: (codes, scale, their addresses); the tensors are kept by the
     caller if it wants them, and all is None when the product quantises the rows itself."""
-    m, k = rows.shape
-    ld = _round_up(max(k, 1), 16)
+    ld = (k + 15) // 16 * 16 or 16
     if keep:
         q, scale = rows.new_empty((m, ld), dtype=torch.int8), rows.new_empty((m,), dtype=torch.float32)
         return q, scale, q.data_ptr(), ld, scale.data_ptr()
-    if nat.lib().ima_int8_fused(m, n, k, gated, _DTYPE_CODES[rows.dtype]):
+    if nat.lib().ima_int8_fused(m, n, k, gated, x_type):
         return None, None, None, ld, None
     ws = rows.new_empty((m * (ld + 4),), dtype=torch.uint8)
     at = ws.data_ptr()
@@ -391,13 +395,13 @@ def _linear_forward(rows: torch.Tensor, weight: Int8Weight, src: torch.Tensor | 
     """(y [M, N], codes, scale) of x rows; codes and scale only with keep.  src: weight rows to be quantised."""
     m, k = rows.shape
     n = weight.shape[0]
-    y = rows.new_empty((m, n))
-    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, n, False, keep)
+    y, x_type = rows.new_empty((m, n)), _DTYPE_CODES[rows.dtype]
+    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, m, k, n, False, x_type, keep)
     bias_dtype = 0
     if bias is not None:
         (bias,), bias_dtype = _bias_args(n, bias)
-    _call(rows.device, "ima_int8_linear", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q_ptr, ld, scale_ptr,
-          keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(), _ptr(src), _code(src),
+    _call(rows.device, "ima_int8_linear", rows.data_ptr(), x_type, m, k, rows.stride(0) if m > 1 else k or 1, q_ptr, ld,
+          scale_ptr, keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(), _ptr(src), _code(src),
           0 if src is None else _ld(src), _ptr(bias), bias_dtype, y.data_ptr(), n or 1)
     return y, q[:, :k] if keep and ld != k else q, scale
 
@@ -409,13 +413,13 @@ def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_sr
     if gate_src is not None and up_src is not None and gate_src.dtype != up_src.dtype:
         _quantise_into(up, up_src)   # weights of two types: the second on its own
         up_src = None
-    h = rows.new_empty((m, n))
-    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, n, True, keep)
+    h, x_type = rows.new_empty((m, n)), _DTYPE_CODES[rows.dtype]
+    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, m, k, n, True, x_type, keep)
     bias_dtype = 0
     if gate_bias is not None or up_bias is not None:
         (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(rows.device, "ima_int8_gated", rows.data_ptr(), _DTYPE_CODES[rows.dtype], m, k, _ld(rows), q_ptr, ld, scale_ptr,
-          keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n, gate.scale.data_ptr(),
+    _call(rows.device, "ima_int8_gated", rows.data_ptr(), x_type, m, k, rows.stride(0) if m > 1 else k or 1, q_ptr, ld,
+          scale_ptr, keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n, gate.scale.data_ptr(),
           up.scale.data_ptr(), _ptr(gate_src), 0 if gate_src is None else _ld(gate_src), _ptr(up_src),
           0 if up_src is None else _ld(up_src), _code(gate_src if gate_src is not None else up_src), _ptr(gate_bias),
           _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], h.data_ptr(), n or 1)
@@ -580,7 +584,7 @@ def _gated_backward(grad, codes, scale, gate, up, gate_bias, up_bias, activation
 def _check_gated(k: int, gate, up, activation: str) -> None:
     if activation not in ACTIVATIONS:
         raise RuntimeError(f"unknown activation {activation!r}; choose one of: {', '.join(sorted(ACTIVATIONS))}")
-    if tuple(gate.shape) != tuple(up.shape):
+    if gate.shape != up.shape:
         raise RuntimeError(f"gate and up weights differ in shape: {tuple(gate.shape)} vs {tuple(up.shape)}")
     if gate.shape[1] != k:
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={gate.shape[1]}")
@@ -619,12 +623,12 @@ def _record(function, leaves, *args):
 
 
 def _versions(*weights: Int8Weight) -> tuple:
-    return tuple(nat.tensor_version(w.codes) for w in weights)
+    return tuple(nat.tensor_version(t) for w in weights for t in (w.codes, w.scale))
 
 
 def _check_versions(before: tuple, *weights: Int8Weight) -> None:
     if before != _versions(*weights):
-        raise RuntimeError("int8 weight codes were modified in place between the forward and the backward pass")
+        raise RuntimeError("int8 weight codes or scales were modified in place between the forward and the backward pass")
 
 
 def _wanted_types(ctx, inputs) -> tuple:
@@ -677,6 +681,18 @@ class _GatedFunction(torch.autograd.Function):
         return (*(None if g is None else g.reshape(shape) for g, shape in zip(grads, ctx.shapes)), None, None, None)
 
 
+def _beside(x: torch.Tensor, weights: tuple, biases: tuple) -> bool:
+    """Whether Int8Weights and floating biases (or None) lie on x's device: what _check_inputs finds, sooner."""
+    index = x.get_device()
+    for w in weights:
+        if w.index != index:
+            return False
+    for b in biases:
+        if b is not None and (type(b) is not torch.Tensor or b.get_device() != index or b.dtype not in _DTYPE_CODES):
+            return False
+    return True
+
+
 def _check_inputs(x: torch.Tensor, *named) -> None:
     if not x.is_cuda:
         _require_cuda(x, "int8 input")
@@ -706,7 +722,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
     weight: an Int8Weight (frozen) or a floating tensor, quantised in the call and differentiable.
     """
     frozen = type(weight) is Int8Weight
-    if not (frozen and x.is_cuda and bias is None and x.dtype in _DTYPE_CODES and x.device == weight.device):
+    if not (frozen and x.is_cuda and x.ndim and x.dtype in _DTYPE_CODES and _beside(x, (weight,), (bias,))):
         _check_inputs(x, ("weight", weight), ("bias", bias))
     k = x.shape[-1]
     if weight.shape[-1] != k:
@@ -736,7 +752,9 @@ def int8_gated(
 
     Both projections, the activation ("silu", "gelu" with the error function, or "gelu_tanh") and the
     product run in one kernel; g and u never reach memory.  Weights as in int8_linear."""
-    _check_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
+    if not (type(gate) is Int8Weight is type(up) and x.is_cuda and x.ndim and x.dtype in _DTYPE_CODES
+            and _beside(x, (gate, up), (gate_bias, up_bias))):
+        _check_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
     k = x.shape[-1]
     _check_gated(k, gate, up, activation)
     if k > MAX_K:

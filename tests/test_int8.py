@@ -1063,3 +1063,15 @@ def test_codes_without_columns_as_they_come(cuda_device):
                                             db_dtype=torch.float32)
     assert dx.shape == (4, 0) and torch.equal(db, torch.full((3,), 4.0, device=cuda_device))
     status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_scales_edited_between_forward_and_backward_are_refused(cuda_device, gated):
+    x, w, _ = make(8, 16, 32, torch.float32, 33, cuda_device)
+    x.requires_grad_()
+    wt, up = int8.Int8Weight.from_float(w), int8.Int8Weight.from_float(w)
+    y = int8.int8_gated(x, wt, up) if gated else int8.int8_linear(x, wt)
+    (up if gated else wt).scale.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified in place"):
+        y.sum().backward()
