@@ -224,10 +224,19 @@ IMA_DEVINL uint64_t sum2(uint32_t a, uint32_t b) {
     return sums_to_float2<1>(x, y);
 }
 
-// (sum * x scale) * column scale + bias of two neighbouring columns; the biases lie `half` floats behind the scales
-IMA_DEVINL uint64_t projection(uint32_t a, uint32_t b, bool zero, uint64_t x2, const float* col, int half) {
-    const float2 w = *reinterpret_cast<const float2*>(col), t = *reinterpret_cast<const float2*>(col + half);
-    return add2(mul2(mul2(zero ? 0ull : sum2(a, b), x2), pair2(w.x, w.y)), pair2(t.x, t.y));
+// (sum * x scale) * column scale + bias of four neighbouring columns
+template <bool BIASED>
+IMA_DEVINL void rescaled4(const uint32_t* sums, bool zero, uint64_t x2, const float* scale, const float* bias, float (&o)[4]) {
+    const float4 w = *reinterpret_cast<const float4*>(scale);
+    uint64_t a = mul2(mul2(zero ? 0ull : sum2(sums[0], sums[1]), x2), pair2(w.x, w.y));
+    uint64_t b = mul2(mul2(zero ? 0ull : sum2(sums[2], sums[3]), x2), pair2(w.z, w.w));
+    if (BIASED) {
+        const float4 t = *reinterpret_cast<const float4*>(bias);
+        a = add2(a, pair2(t.x, t.y));
+        b = add2(b, pair2(t.z, t.w));
+    }
+    const float2 lo = halves(a), hi = halves(b);
+    o[0] = lo.x; o[1] = lo.y; o[2] = hi.x; o[3] = hi.y;
 }
 
 IMA_DEVINL uint32_t pack_bf16(float lo, float hi) {
@@ -536,21 +545,24 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                     }
                     if (p.y) {
                         float v[32];
+                        auto scaled = [&](auto with_bias) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 w = *reinterpret_cast<const float4*>(cols + c0 + j);
-                            const uint64_t a = mul2(mul2(sum2(r[j], r[j + 1]), x2), pair2(w.x, w.y));
-                            const uint64_t b = mul2(mul2(sum2(r[j + 2], r[j + 3]), x2), pair2(w.z, w.w));
-                            const float4 t = *reinterpret_cast<const float4*>(cols + HALF + c0 + j);
-                            const float2 va = halves(add2(a, pair2(t.x, t.y))), vb = halves(add2(b, pair2(t.z, t.w)));
-                            v[j] = va.x; v[j + 1] = va.y; v[j + 2] = vb.x; v[j + 3] = vb.y;
-                        }
+                            for (int j = 0; j < 32; j += 4) {
+                                float f[4];
+                                rescaled4<decltype(with_bias)::value>(r + j, false, x2, cols + c0 + j, cols + HALF + c0 + j, f);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) v[j + e] = f[e];
+                            }
+                        };
+                        if (p.bias[0]) scaled(std::true_type{});
+                        else scaled(std::false_type{});
                         store_y32(p, st, lane, v, row0, rows, n0 + c0, p.y);
                     }
                 }
             } else if constexpr (EPI == I8_GATED) {
-                auto chunks = [&](auto tag) {
+                auto chunks = [&](auto tag, auto with_bias) {
                     constexpr int ACT = decltype(tag)::value;
+                    constexpr bool BIASED = decltype(with_bias)::value;
 #pragma unroll 1
                     for (int c0 = 0; c0 < HALF; c0 += 32) {
                         uint32_t rg[32], ru[32];
@@ -560,18 +572,23 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                         if (n0 + c0 >= p.N || rows == 0) continue;
                         float v[32];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float2 g = halves(projection(rg[j], rg[j + 1], zero, x2, cols + c0 + j, HALF));
-                            const float2 u = halves(projection(ru[j], ru[j + 1], zero, x2, cols + 2 * HALF + c0 + j, HALF));
-                            v[j] = act_value<ACT>(g.x) * u.x;
-                            v[j + 1] = act_value<ACT>(g.y) * u.y;
+                        for (int j = 0; j < 32; j += 4) {
+                            float g[4], u[4];
+                            rescaled4<BIASED>(rg + j, zero, x2, cols + c0 + j, cols + HALF + c0 + j, g);
+                            rescaled4<BIASED>(ru + j, zero, x2, cols + 2 * HALF + c0 + j, cols + 3 * HALF + c0 + j, u);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[j + e] = act_value<ACT>(g[e]) * u[e];
                         }
                         store_y32(p, st, lane, v, row0, rows, n0 + c0, p.y);
                     }
                 };
-                if (p.act == IMA_ACT_SILU) chunks(std::integral_constant<int, IMA_ACT_SILU>{});
-                else if (p.act == IMA_ACT_GELU) chunks(std::integral_constant<int, IMA_ACT_GELU>{});
-                else chunks(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
+                auto both = [&](auto tag) {
+                    if (p.bias[0] || p.bias[1]) chunks(tag, std::true_type{});
+                    else chunks(tag, std::false_type{});
+                };
+                if (p.act == IMA_ACT_SILU) both(std::integral_constant<int, IMA_ACT_SILU>{});
+                else if (p.act == IMA_ACT_GELU) both(std::integral_constant<int, IMA_ACT_GELU>{});
+                else both(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
             } else if constexpr (EPI == I8_GATED_BWD) {
                 uint32_t rm = 0;
                 auto chunks = [&](auto tag) {

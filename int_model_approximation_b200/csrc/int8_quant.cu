@@ -91,6 +91,18 @@ IMA_DEVINL float i8_row_scale(float amax, bool nan) {
     return s < 1e-12f ? 1e-12f : s;
 }
 
+// N words that start d bytes (0..15) into the N + 4 aligned ones of w.
+template <int N>
+IMA_DEVINL void shift_words(const uint32_t (&w)[N + 4], uint32_t d, uint32_t (&o)[N]) {
+    uint32_t x[N + 2], y[N + 1];
+#pragma unroll
+    for (int j = 0; j < N + 2; ++j) x[j] = d & 8 ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < N + 1; ++j) y[j] = d & 4 ? x[j + 1] : x[j];
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = __funnelshift_r(y[j], y[j + 1], (d & 3) * 8);
+}
+
 // Eight consecutive elements as loaded (16 bytes of a 16-bit type, 32 of fp32).  max_bits() is the fp32
 // bit pattern of the largest magnitude: magnitudes order like their bit patterns, NaN above all.
 template <int DT>
@@ -106,6 +118,17 @@ struct Raw8<IMA_DTYPE_F32> {
         const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + k0);
         const float4 a = __ldg(p), b = __ldg(p + 1);
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+    // the same from a row that lies d bytes behind a 16-byte boundary, by aligned loads (all of which
+    // touch bytes of the eight elements)
+    IMA_DEVINL void load_shifted(const void* row, int64_t k0, uint32_t d) {
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(row) + k0 * 4 - d);
+        const uint4 a = __ldg(p), b = __ldg(p + 1), c = __ldg(p + 2);
+        const uint32_t w[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+        uint32_t o[8];
+        shift_words<8>(w, d, o);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(o[j]);
     }
     IMA_DEVINL void load(const void* row, int64_t k0, int64_t K, bool vec) { load8(row, IMA_DTYPE_F32, k0, K, vec, v); }
     IMA_DEVINL void unpack(float (&o)[8]) const {
@@ -125,6 +148,14 @@ struct RawHalf8 {
     IMA_DEVINL void clear() { u = make_uint4(0, 0, 0, 0); }
     IMA_DEVINL void load_whole(const void* row, int64_t k0) {
         u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + k0));
+    }
+    IMA_DEVINL void load_shifted(const void* row, int64_t k0, uint32_t d) {
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(row) + k0 * 2 - d);
+        const uint4 a = __ldg(p), b = __ldg(p + 1);
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        uint32_t o[4];
+        shift_words<4>(w, d, o);
+        u = make_uint4(o[0], o[1], o[2], o[3]);
     }
     IMA_DEVINL void load(const void* row, int64_t k0, int64_t K, bool vec) {
         u = qz_load_half8(reinterpret_cast<const uint16_t*>(row), k0, K, vec);
@@ -186,22 +217,38 @@ __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const __grid
         const int which = (row_at >= a.end[0]) + (row_at >= a.end[1]);
         const int64_t m = row_at - (which ? a.end[which - 1] : 0);
         const unsigned char* row = reinterpret_cast<const unsigned char*>(a.x[which]) + m * a.ldx[which] * dtype_bytes(DT);
-        const bool vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-        // whole aligned groups of eight that this thread keeps; the rest is loaded twice
-        const int64_t whole = vec ? min(K / 8 * 8, (int64_t)V * TPR * 8) : 0;
-        Raw8<DT> keep[V];
+        const uint32_t d = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15;   // the same for a warp
+        const bool vec = d == 0;
+        // whole groups of eight that this thread keeps; the rest is loaded twice
+        const int64_t whole = min(K / 8 * 8, (int64_t)V * TPR * 8);
+        // the last K % 8 elements, where all groups before them are kept
+        const bool ends = whole == K / 8 * 8;
+        const int64_t rest = ends ? K : whole;
+        Raw8<DT> keep[V], last;
+        last.clear();
+        if (ends && whole < K && tid == 0) last.load(row, whole, K, vec);
         uint32_t mx = 0;
+        if (vec) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            keep[i].clear();
-            if ((i * TPR + tid) * 8 < whole) keep[i].load_whole(row, (int64_t)(i * TPR + tid) * 8);
+            for (int i = 0; i < V; ++i) {
+                keep[i].clear();
+                if ((i * TPR + tid) * 8 < whole) keep[i].load_whole(row, (int64_t)(i * TPR + tid) * 8);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                keep[i].clear();
+                if ((i * TPR + tid) * 8 < whole) keep[i].load_shifted(row, (int64_t)(i * TPR + tid) * 8, d);
+            }
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) mx = max(mx, keep[i].max_bits());
+        mx = max(mx, last.max_bits());
 #pragma unroll 1
-        for (int64_t k0 = whole + tid * 8; k0 < K; k0 += TPR * 8) {
+        for (int64_t k0 = rest + tid * 8; k0 < K; k0 += TPR * 8) {
             Raw8<DT> r;
-            r.load(row, k0, K, vec);
+            if (vec || k0 + 8 > K) r.load(row, k0, K, vec);
+            else r.load_shifted(row, k0, d);
             mx = max(mx, r.max_bits());
         }
         const float amax = __uint_as_float(row_max<TPR>(mx, s_max));
@@ -217,10 +264,12 @@ __global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if ((i * TPR + tid) * 8 < whole) emit(keep[i], (int64_t)(i * TPR + tid) * 8);
+        if (ends && whole < K && tid == 0) emit(last, whole);
 #pragma unroll 1
-        for (int64_t k0 = whole + tid * 8; k0 < K; k0 += TPR * 8) {
+        for (int64_t k0 = rest + tid * 8; k0 < K; k0 += TPR * 8) {
             Raw8<DT> r;
-            r.load(row, k0, K, vec);
+            if (vec || k0 + 8 > K) r.load(row, k0, K, vec);
+            else r.load_shifted(row, k0, d);
             emit(r, k0);
         }
     }
