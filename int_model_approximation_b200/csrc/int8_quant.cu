@@ -193,8 +193,9 @@ IMA_DEVINL uint32_t row_max(uint32_t m, uint32_t* s_max) {
 // ---------------------------------------------------------------------------
 // Row quantiser.  TPR threads take one row; a row of up to TPR * 8 * V elements is read once
 // and kept in registers between the maximum and the codes, a longer one is read again (from
-// L2).  Bound by memory: 2 or 4 bytes in and 1 out per element.  16384 x 3584 from bf16 takes 37 us (27 at the
-// measured copy rate), 16384 x 18944 177 (142); fp32 rows are at the copy rate.
+// L2).  Bound by memory: 2 or 4 bytes in and 1 out per element.  16384 x 3584 from bf16 takes 35 us (27 at the
+// measured copy rate), 16384 x 18944 156 (142; 177 with two blocks per SM instead of three); fp32 rows are at the
+// copy rate.
 // ---------------------------------------------------------------------------
 struct QuantRows {           // up to three matrices of K columns, one after the other (activations, weights)
     const void* x[3];
@@ -205,7 +206,7 @@ struct QuantRows {           // up to three matrices of K columns, one after the
 };
 
 template <int DT, int TPR, int V>
-__global__ void __launch_bounds__(256, 2) int8_quantize_rows_kernel(const __grid_constant__ QuantRows a) {
+__global__ void __launch_bounds__(256, DT != IMA_DTYPE_F32 && V <= 10 ? 3 : 2) int8_quantize_rows_kernel(const __grid_constant__ QuantRows a) {
     // a product launched to follow this kernel may start now; it waits for this kernel's end before it reads
     allow_next_kernel();
     __shared__ uint32_t s_max[8];
@@ -641,15 +642,22 @@ int launch_quantize(const QuantRows& a, cudaStream_t st) {
     if (M == 0) return IMA_OK;
     // As few threads per row as hold it in registers, when the rows fill the machine: 8 KB of a row in flight
     // per warp and no barrier, or a barrier of two to eight warps.  Few rows: a block each, for latency.
+    // Rows off 16 bytes take two loads per group, so half as many groups per thread (12638 x 2269 from bf16: 44 us,
+    // 54 with 16; aligned rows 35 us either way at 16384 x 3584).
     constexpr bool F = DT == IMA_DTYPE_F32;
     const bool many = M >= 148 * 8;
+    bool shifted = false;
+    for (int i = 0; i < 3; ++i)
+        shifted |= a.end[i] > (i ? a.end[i - 1] : 0) &&
+                   ((reinterpret_cast<uintptr_t>(a.x[i]) | (uintptr_t)(a.ldx[i] * dtype_bytes(DT))) & 15) != 0;
     auto run = [&](auto tpr, auto v) {
         constexpr int TPR = decltype(tpr)::value, V = decltype(v)::value;
         const unsigned grid = (unsigned)std::min<int64_t>((M * TPR + 255) / 256, 148 * 32);
         int8_quantize_rows_kernel<DT, TPR, V><<<grid, 256, 0, st>>>(a);
     };
     if (K <= 1024) run(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{});
-    else if (many && K <= (F ? 2048 : 4096)) run(std::integral_constant<int, 32>{}, std::integral_constant<int, F ? 8 : 16>{});
+    else if (many && K <= (F ? 2048 : 4096) && (F || !shifted)) run(std::integral_constant<int, 32>{}, std::integral_constant<int, F ? 8 : 16>{});
+    else if (many && !F && K <= 4096) run(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
     else if (many && K <= 5120) run(std::integral_constant<int, 64>{}, std::integral_constant<int, 10>{});
     else if (many && K <= 10240) run(std::integral_constant<int, 128>{}, std::integral_constant<int, 10>{});
     else if (K <= 4096) run(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});

@@ -1075,3 +1075,18 @@ def test_scales_edited_between_forward_and_backward_are_refused(cuda_device, gat
     (up if gated else wt).scale.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified in place"):
         y.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(1, 8), (3, 9), (5, 1), (4, 1025), (2, 4100), (2, 21003), (1300, 1100), (1300, 4093),
+                                 (1300, 5001), (1300, 10001)])
+def test_quantiser_rows_at_every_alignment(cuda_device, dtype, m, k):
+    g = torch.Generator(device=cuda_device).manual_seed(k)
+    for at in range(1, 16 // dtype.itemsize + 1):
+        flat = torch.randn((m * (k + at % 3) + at,), generator=g, device=cuda_device).to(dtype)
+        x = flat[at:].view(m, k + at % 3)[:, :k]
+        q, s = int8.per_token_int8(x)
+        want_q, want_s = plain_codes(x)
+        assert torch.equal(s.flatten().double(), want_s) and torch.equal(q.double(), want_q)
+    status_clean(cuda_device)
