@@ -178,12 +178,6 @@ def _quantise(rows: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
-def _quantise_into(weight: "Int8Weight", src: torch.Tensor) -> None:
-    n, k = src.shape
-    _call(src.device, "ima_int8_quantize_rows", src.data_ptr(), _DTYPE_CODES[src.dtype], n, k, _ld(src),
-          weight.codes.data_ptr(), weight.ld, weight.scale.data_ptr())
-
-
 def _transpose(t: torch.Tensor) -> torch.Tensor:
     """int8 [rows, cols] (aligned) -> [cols, rows]."""
     rows, cols = t.shape
@@ -360,18 +354,25 @@ def int8_gemm(
     return c, y
 
 
-def _code_buffers(rows: torch.Tensor, m: int, k: int, n: int, gated: bool, x_type: int, keep: bool):
-    """Room for the codes and scales of x rows: (codes, scale, their addresses); the tensors are kept by the
-    caller if it wants them, and all is None when the product quantises the rows itself."""
+def _code_buffers(rows: torch.Tensor, m: int, k: int, n: int, gated: bool, x_type: int):
+    """Room for the codes and scales of x rows: (workspace, codes, row stride, scales), addresses but for the
+    first; None when the product quantises the rows itself."""
     ld = (k + 15) // 16 * 16 or 16
-    if keep:
-        q, scale = rows.new_empty((m, ld), dtype=torch.int8), rows.new_empty((m,), dtype=torch.float32)
-        return q, scale, q.data_ptr(), ld, scale.data_ptr()
     if nat.lib().ima_int8_fused(m, n, k, gated, x_type):
-        return None, None, None, ld, None
+        return None, None, ld, None
     ws = rows.new_empty((m * (ld + 4),), dtype=torch.uint8)
     at = ws.data_ptr()
-    return ws, None, at, ld, at + m * ld
+    return ws, at, ld, at + m * ld
+
+
+def _kept_block(m: int, ld: int, *weights: int) -> tuple[list[int], int]:
+    """Layout of what a forward pass keeps: codes [m, ld] and scales of its rows, then of each weight with that many
+    rows, in one allocation: (offsets of scales, codes, scales, ..., bytes)."""
+    at, end = [m * ld], _round_up(m * (ld + 4), 256)
+    for n in weights:
+        at += (end, end + n * ld)
+        end = _round_up(end + n * (ld + 4), 256)
+    return at, end
 
 
 def _weight_args(weight) -> tuple[Int8Weight, torch.Tensor | None]:
@@ -383,47 +384,62 @@ def _weight_args(weight) -> tuple[Int8Weight, torch.Tensor | None]:
     src = _rows(weight.detach())
     n, k = src.shape
     made = Int8Weight.__new__(Int8Weight)
-    if k == 0:   # nothing to quantise: the scales of rows of zeros
-        made._set(_empty_codes(n, k, src), src.new_full((n,), 1e-12, dtype=torch.float32))
-        return made, None
     made._set(_empty_codes(n, k, src), src.new_empty((n,), dtype=torch.float32))
     return made, src
 
 
-def _linear_forward(rows: torch.Tensor, weight: Int8Weight, src: torch.Tensor | None, bias: torch.Tensor | None,
-                    keep: bool = False):
-    """(y [M, N], codes, scale) of x rows; codes and scale only with keep.  src: weight rows to be quantised."""
-    m, k = rows.shape
-    n = weight.shape[0]
-    y, x_type = rows.new_empty((m, n)), _DTYPE_CODES[rows.dtype]
-    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, m, k, n, False, x_type, keep)
+def _at(weight: Int8Weight) -> tuple[int, int, int]:
+    return weight.codes.data_ptr(), weight.ld, weight.scale.data_ptr()
+
+
+def _linear_call(rows, m, k, n, x_type, q, keep, w, src, bias, y) -> None:
+    """q, w: (codes, row stride, scales), as addresses; src: weight rows to be quantised into w, or None."""
     bias_dtype = 0
     if bias is not None:
         (bias,), bias_dtype = _bias_args(n, bias)
-    _call(rows.device, "ima_int8_linear", rows.data_ptr(), x_type, m, k, rows.stride(0) if m > 1 else k or 1, q_ptr, ld,
-          scale_ptr, keep, weight.codes.data_ptr(), weight.ld, n, weight.scale.data_ptr(), _ptr(src), _code(src),
-          0 if src is None else _ld(src), _ptr(bias), bias_dtype, y.data_ptr(), n or 1)
-    return y, q[:, :k] if keep and ld != k else q, scale
+    if src is None:
+        src_at, src_type, src_ld = None, 0, 0
+    else:   # without columns there is no address: any but NULL, and zeros are quantised
+        src_at, src_type, src_ld = src.data_ptr() or w[2], _DTYPE_CODES[src.dtype], _ld(src)
+    _call(rows.device, "ima_int8_linear", rows.data_ptr(), x_type, m, k, rows.stride(0) if m > 1 else k or 1, *q, keep,
+          w[0], w[1], n, w[2], src_at, src_type, src_ld, _ptr(bias), bias_dtype, y.data_ptr(), n or 1)
 
 
-def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, gate_src, up_src, gate_bias, up_bias,
-                   activation: str, keep: bool = False):
+def _linear_forward(rows: torch.Tensor, weight: Int8Weight, src: torch.Tensor | None, bias: torch.Tensor | None):
+    """y [M, N] of x rows.  src: weight rows to be quantised."""
     m, k = rows.shape
-    n = gate.shape[0]
-    if gate_src is not None and up_src is not None and gate_src.dtype != up_src.dtype:
-        _quantise_into(up, up_src)   # weights of two types: the second on its own
-        up_src = None
-    h, x_type = rows.new_empty((m, n)), _DTYPE_CODES[rows.dtype]
-    q, scale, q_ptr, ld, scale_ptr = _code_buffers(rows, m, k, n, True, x_type, keep)
+    n = weight.shape[0]
+    y, x_type = rows.new_empty((m, n)), _DTYPE_CODES[rows.dtype]
+    ws, *q = _code_buffers(rows, m, k, n, False, x_type)
+    _linear_call(rows, m, k, n, x_type, q, False, _at(weight), src, bias, y)
+    return y
+
+
+def _gated_call(rows, m, k, n, x_type, q, keep, g, u, g_src, u_src, gate_bias, up_bias, activation, h) -> None:
+    """As _linear_call."""
+    if g_src is not None and u_src is not None and g_src.dtype != u_src.dtype:
+        # weights of two types: the second on its own
+        _call(rows.device, "ima_int8_quantize_rows", u_src.data_ptr(), _DTYPE_CODES[u_src.dtype], n, k, _ld(u_src), *u)
+        u_src = None
     bias_dtype = 0
     if gate_bias is not None or up_bias is not None:
         (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(rows.device, "ima_int8_gated", rows.data_ptr(), x_type, m, k, rows.stride(0) if m > 1 else k or 1, q_ptr, ld,
-          scale_ptr, keep, gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(), up.ld, n, gate.scale.data_ptr(),
-          up.scale.data_ptr(), _ptr(gate_src), 0 if gate_src is None else _ld(gate_src), _ptr(up_src),
-          0 if up_src is None else _ld(up_src), _code(gate_src if gate_src is not None else up_src), _ptr(gate_bias),
-          _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], h.data_ptr(), n or 1)
-    return h, q[:, :k] if keep and ld != k else q, scale
+    src_type = _code(g_src if g_src is not None else u_src)
+    _call(rows.device, "ima_int8_gated", rows.data_ptr(), x_type, m, k, rows.stride(0) if m > 1 else k or 1, *q, keep,
+          g[0], g[1], u[0], u[1], n, g[2], u[2], None if g_src is None else g_src.data_ptr() or g[2],
+          0 if g_src is None else _ld(g_src), None if u_src is None else u_src.data_ptr() or u[2],
+          0 if u_src is None else _ld(u_src), src_type, _ptr(gate_bias), _ptr(up_bias), bias_dtype,
+          ACTIVATIONS[activation], h.data_ptr(), n or 1)
+
+
+def _gated_forward(rows: torch.Tensor, gate: Int8Weight, up: Int8Weight, g_src, u_src, gate_bias, up_bias,
+                   activation: str):
+    m, k = rows.shape
+    n = gate.shape[0]
+    h, x_type = rows.new_empty((m, n)), _DTYPE_CODES[rows.dtype]
+    ws, *q = _code_buffers(rows, m, k, n, True, x_type)
+    _gated_call(rows, m, k, n, x_type, q, False, _at(gate), _at(up), g_src, u_src, gate_bias, up_bias, activation, h)
+    return h
 
 
 def _code(t: torch.Tensor | None) -> int:
@@ -496,22 +512,25 @@ def int8_linear_backward(
     nat.require_device(codes.device, ("weight", weight.codes), ("scale", scale))
     _check_types(dx_dtype, dw_dtype, db_dtype)
     _check_backward(m, n if dx_dtype is not None else 0, dw_dtype is not None)
-    return _linear_backward(grad, codes, _scales(scale, m, "scale"), weight, dx_dtype, dw_dtype, db_dtype, keep_transposed)
+    scale = _scales(scale, m, "scale")
+    return _linear_backward(grad, codes, (m, n, k), (codes.data_ptr(), _code_ld(codes), scale.data_ptr()), _at(weight),
+                            weight if keep_transposed else None, (dx_dtype, dw_dtype, db_dtype))
 
 
-def _linear_backward(grad, codes, scale, weight, dx_dtype, dw_dtype, db_dtype, keep_transposed):
-    (m, k), n = codes.shape, weight.shape[0]
-    d = _grad_rows(grad, m, n, codes.device)
+def _linear_backward(grad, like, sizes, q, w, weight, types):
+    """q, w: (codes, row stride, scales), as addresses; weight: the Int8Weight that keeps transposed codes, or None."""
+    m, n, k = sizes
+    dx_dtype, dw_dtype, db_dtype = types
+    d = _grad_rows(grad, m, n, like.device)
     planes = _digit_count(d.dtype, dx_dtype, dw_dtype)
-    dx, dw, db = _out(scale, (m, k), dx_dtype), _out(scale, (n, k), dw_dtype), _out(scale, (n,), db_dtype)
-    wt = weight.transposed() if dx is not None and keep_transposed else None
+    dx, dw, db = _out(like, (m, k), dx_dtype), _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
+    wt = weight.transposed() if dx is not None and weight is not None else None
     nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 0, planes, dx is not None, dw is not None,
                                                          db is not None, wt is None)
-    ws = scale.new_empty((nbytes,), dtype=torch.uint8)
-    _call(codes.device, "ima_int8_linear_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k,
-          codes.data_ptr(), _code_ld(codes), scale.data_ptr(), weight.codes.data_ptr(), weight.ld, _ptr(wt),
-          _code_ld(wt) if wt is not None else 0, weight.scale.data_ptr(), planes, _ptr(dx), _code(dx), _ptr(dw),
-          _code(dw), _ptr(db), _code(db), ws.data_ptr())
+    ws = like.new_empty((nbytes,), dtype=torch.uint8)
+    _call(like.device, "ima_int8_linear_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, *q, w[0], w[1],
+          _ptr(wt), _code_ld(wt) if wt is not None else 0, w[2], planes, _ptr(dx), _code(dx), _ptr(dw), _code(dw),
+          _ptr(db), _code(db), ws.data_ptr())
     return dx, dw, db
 
 
@@ -546,31 +565,32 @@ def int8_gated_backward(
     _check_types(*types)
     _check_backward(m, _round_up(n, 128) + n if dx_dtype is not None else 0,
                     dgate_dtype is not None or dup_dtype is not None)
-    return _gated_backward(grad, codes, _scales(scale, m, "scale"), gate, up, gate_bias, up_bias, activation, types,
-                           keep_transposed)
+    scale = _scales(scale, m, "scale")
+    return _gated_backward(grad, codes, (m, n, k), (codes.data_ptr(), _code_ld(codes), scale.data_ptr()), _at(gate),
+                           _at(up), (gate, up) if keep_transposed else None, gate_bias, up_bias, activation, types)
 
 
-def _gated_backward(grad, codes, scale, gate, up, gate_bias, up_bias, activation, types, keep_transposed):
+def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, activation, types):
+    """As _linear_backward; weights: both Int8Weights if they keep transposed codes, else None."""
+    m, n, k = sizes
     dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype = types
-    (m, k), n = codes.shape, gate.shape[0]
-    d = _grad_rows(grad, m, n, codes.device)
+    d = _grad_rows(grad, m, n, like.device)
     want_dw = dgate_dtype is not None or dup_dtype is not None
     planes = _digit_count(d.dtype, dx_dtype, dgate_dtype, dup_dtype)
     w_type, b_type = _one_type(dgate_dtype, dup_dtype), _one_type(gate_db_dtype, up_db_dtype)
-    dx = _out(scale, (m, k), dx_dtype)
-    dgate, dup = _out(scale, (n, k), w_type, dgate_dtype is not None), _out(scale, (n, k), w_type, dup_dtype is not None)
-    dgb, dub = _out(scale, (n,), b_type, gate_db_dtype is not None), _out(scale, (n,), b_type, up_db_dtype is not None)
+    dx = _out(like, (m, k), dx_dtype)
+    dgate, dup = _out(like, (n, k), w_type, dgate_dtype is not None), _out(like, (n, k), w_type, dup_dtype is not None)
+    dgb, dub = _out(like, (n,), b_type, gate_db_dtype is not None), _out(like, (n,), b_type, up_db_dtype is not None)
     gt = ut = None
-    if dx is not None and keep_transposed:
-        gt, ut = gate.transposed(), up.transposed()
+    if dx is not None and weights is not None:
+        gt, ut = weights[0].transposed(), weights[1].transposed()
     nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 1, planes, dx is not None, want_dw, b_type is not None,
                                                          gt is None or ut is None)
-    ws = scale.new_empty((nbytes,), dtype=torch.uint8)
+    ws = like.new_empty((nbytes,), dtype=torch.uint8)
     (gate_bias, up_bias), bias_dtype = _bias_args(n, gate_bias, up_bias)
-    _call(codes.device, "ima_int8_gated_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, codes.data_ptr(),
-          _code_ld(codes), scale.data_ptr(), gate.codes.data_ptr(), gate.ld, up.codes.data_ptr(),
-          up.ld, _ptr(gt), _code_ld(gt) if gt is not None else 0, _ptr(ut),
-          _code_ld(ut) if ut is not None else 0, gate.scale.data_ptr(), up.scale.data_ptr(), _ptr(gate_bias),
+    _call(like.device, "ima_int8_gated_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, *q, g[0], g[1],
+          u[0], u[1], _ptr(gt), _code_ld(gt) if gt is not None else 0, _ptr(ut),
+          _code_ld(ut) if ut is not None else 0, g[2], u[2], _ptr(gate_bias),
           _ptr(up_bias), bias_dtype, ACTIVATIONS[activation], planes, _ptr(dx), _code(dx), _ptr(dgate), _ptr(dup),
           _code(dgate if dgate is not None else dup), _ptr(dgb), _ptr(dub), _code(dgb if dgb is not None else dub),
           ws.data_ptr())
@@ -635,23 +655,48 @@ def _wanted_types(ctx, inputs) -> tuple:
     return tuple(t.dtype if need else None for t, need in zip(inputs, ctx.needs_input_grad))
 
 
+def _source(weight) -> torch.Tensor:
+    if weight.ndim != 2:
+        raise RuntimeError(f"int8 weight source must be 2-D, got {tuple(weight.shape)}")
+    return _rows(weight)
+
+
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, handle):
-        w, src = _weight_args(handle if handle is not None else weight)
-        y, q, scale = _linear_forward(_rows(x.detach()), w, src, bias, keep=True)
-        ctx.save_for_backward(q, scale)
-        ctx.weight, ctx.frozen, ctx.version = w, handle is not None, _versions(w)
+        rows = _rows(x)
+        m, k = rows.shape
+        src = None if handle is not None else _source(weight)
+        n = (src if handle is None else handle).shape[0]
+        ld = (k + 15) // 16 * 16 or 16
+        at, nbytes = _kept_block(m, ld) if handle is not None else _kept_block(m, ld, n)
+        y, block = rows.new_empty((m, n)), rows.new_empty((nbytes,), dtype=torch.uint8)
+        base = block.data_ptr()
+        q = base, ld, base + at[0]
+        w = (base + at[1], ld, base + at[2]) if handle is None else _at(handle)
+        _linear_call(rows, m, k, n, _DTYPE_CODES[rows.dtype], q, True, w, src, bias, y)
+        ctx.save_for_backward(block)
+        ctx.sizes, ctx.handle, ctx.version = (m, n, k), handle, None if handle is None else _versions(handle)
         ctx.types = _wanted_types(ctx, (x, weight, bias))
         ctx.shapes = (x.shape, None if bias is None else bias.shape)
-        return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
+        return y if x.ndim == 2 else y.reshape(*x.shape[:-1], n)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, scale = ctx.saved_tensors
-        _check_versions(ctx.version, ctx.weight)
-        dx, dw, db = _linear_backward(grad, q, scale, ctx.weight, *ctx.types, ctx.frozen)
+        block, = ctx.saved_tensors
+        handle, sizes = ctx.handle, ctx.sizes
+        m, n, k = sizes
+        ld = (k + 15) // 16 * 16 or 16
+        base = block.data_ptr()
+        if handle is None:
+            at, _ = _kept_block(m, ld, n)
+            w = base + at[1], ld, base + at[2]
+        else:
+            _check_versions(ctx.version, handle)
+            at, _ = _kept_block(m, ld)
+            w = _at(handle)
+        dx, dw, db = _linear_backward(grad, block, sizes, (base, ld, base + at[0]), w, handle, ctx.types)
         if dx is not None and len(ctx.shapes[0]) != 2:
             dx = dx.reshape(ctx.shapes[0])
         return dx, dw, None if db is None else db.reshape(ctx.shapes[1]), None
@@ -660,25 +705,49 @@ class _LinearFunction(torch.autograd.Function):
 class _GatedFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, gate, up, activation):
-        g, g_src = _weight_args(gate if gate is not None else gate_weight)
-        u, u_src = _weight_args(up if up is not None else up_weight)
-        h, q, scale = _gated_forward(_rows(x.detach()), g, u, g_src, u_src, gate_bias, up_bias, activation, keep=True)
-        ctx.save_for_backward(q, scale, gate_bias, up_bias)
-        ctx.gate, ctx.up, ctx.activation, ctx.version = g, u, activation, _versions(g, u)
-        ctx.frozen = gate is not None and up is not None
+        rows = _rows(x)
+        m, k = rows.shape
+        g_src = None if gate is not None else _source(gate_weight)
+        u_src = None if up is not None else _source(up_weight)
+        n = (g_src if gate is None else gate).shape[0]
+        ld = (k + 15) // 16 * 16 or 16
+        h = rows.new_empty((m, n))
+        block = rows.new_empty((_kept_block(m, ld, *_GatedFunction.made(n, gate, up))[1],), dtype=torch.uint8)
+        q, g, u = _GatedFunction.parts(block, m, ld, n, gate, up)
+        _gated_call(rows, m, k, n, _DTYPE_CODES[rows.dtype], q, True, g, u, g_src, u_src, gate_bias, up_bias, activation, h)
+        ctx.save_for_backward(block, gate_bias, up_bias)
+        ctx.sizes, ctx.gate, ctx.up, ctx.activation = (m, n, k), gate, up, activation
+        ctx.version = _versions(*(w for w in (gate, up) if w is not None))
         inputs = (x, gate_weight, up_weight, gate_bias, up_bias)
         ctx.types = _wanted_types(ctx, inputs)
         ctx.shapes = tuple(None if t is None else t.shape for t in inputs)
-        return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])
+        return h if x.ndim == 2 else h.reshape(*x.shape[:-1], n)
+
+    @staticmethod
+    def made(n, gate, up) -> tuple:
+        """Rows of the weights that are quantised in the call."""
+        return (n,) * ((gate is None) + (up is None))
+
+    @staticmethod
+    def parts(block, m, ld, n, gate, up):
+        """(codes, row stride, scales) of x, gate and up, as addresses."""
+        at, _ = _kept_block(m, ld, *_GatedFunction.made(n, gate, up))
+        base = block.data_ptr()
+        g = (base + at[1], ld, base + at[2]) if gate is None else _at(gate)
+        u = (base + at[-2], ld, base + at[-1]) if up is None else _at(up)
+        return (base, ld, base + at[0]), g, u
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, scale, gate_bias, up_bias = ctx.saved_tensors
-        _check_versions(ctx.version, ctx.gate, ctx.up)
-        grads = _gated_backward(grad, q, scale, ctx.gate, ctx.up, gate_bias, up_bias, ctx.activation, ctx.types,
-                                ctx.frozen)
-        return (*(None if g is None else g.reshape(shape) for g, shape in zip(grads, ctx.shapes)), None, None, None)
+        block, gate_bias, up_bias = ctx.saved_tensors
+        gate, up = ctx.gate, ctx.up
+        _check_versions(ctx.version, *(w for w in (gate, up) if w is not None))
+        m, n, k = ctx.sizes
+        q, g, u = _GatedFunction.parts(block, m, (k + 15) // 16 * 16 or 16, n, gate, up)
+        frozen = (gate, up) if gate is not None and up is not None else None
+        grads = _gated_backward(grad, block, ctx.sizes, q, g, u, frozen, gate_bias, up_bias, ctx.activation, ctx.types)
+        return (*(None if t is None else t.reshape(shape) for t, shape in zip(grads, ctx.shapes)), None, None, None)
 
 
 def _beside(x: torch.Tensor, weights: tuple, biases: tuple) -> bool:
@@ -735,7 +804,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
         w = None if frozen else weight
         return _record(_LinearFunction, (x, w, bias), x, w, bias, weight if frozen else None)
     w, src = (weight, None) if frozen else _weight_args(weight)
-    y = _linear_forward(_rows(x), w, src, bias)[0]
+    y = _linear_forward(_rows(x), w, src, bias)
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
 
 
@@ -768,5 +837,5 @@ def int8_gated(
         return _record(_GatedFunction, inputs, *inputs, gate if frozen[0] else None, up if frozen[1] else None,
                        activation)
     (g, g_src), (u, u_src) = _weight_args(gate), _weight_args(up)
-    h = _gated_forward(_rows(x), g, u, g_src, u_src, gate_bias, up_bias, activation)[0]
+    h = _gated_forward(_rows(x), g, u, g_src, u_src, gate_bias, up_bias, activation)
     return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])
