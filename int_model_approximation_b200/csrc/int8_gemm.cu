@@ -23,7 +23,7 @@
 // Measured.  Long contractions are bound by power: 16384 x 18944 x 3584 in 0.75 ms with its quantiser (2.95e15
 // operations/s, 0.92 of twice the measured bf16 rate), the gated form in 1.49 (2.99e15); with zeros for operands
 // the same kernel reaches 3.75e15.  Below 14 k-tiles or so the epilogue bounds: 4096 x 4864 x 896 to
-// bf16 takes 26 us, its products alone 12; per 128 x 256 outputs it takes 5700 clocks, most of them in
+// bf16 takes 25 us, its products alone 12; per 128 x 256 outputs it takes 5700 clocks, most of them in
 // the shared-memory pipe (tensor memory out, staging in and out).  Small products are bound by the
 // latency of launch, first loads and last epilogue, 8 us.
 //
@@ -255,7 +255,8 @@ IMA_DEVINL uint32_t pack_half2(float lo, float hi, int dtype) {
 template <int W>
 IMA_DEVINL void stage_out(const unsigned char* st, int lane, unsigned char* base, int64_t pitch, int rows, int bytes,
                           int esize) {
-    using T = std::conditional_t<W == 16, uint4, std::conditional_t<W == 8, uint2, std::conditional_t<W == 4, uint32_t, uint16_t>>>;
+    using Small = std::conditional_t<W == 4, uint32_t, uint16_t>;
+    using T = std::conditional_t<W == 16, uint4, std::conditional_t<W == 8, uint2, Small>>;
     constexpr int ACROSS = 64 / W;
     const int o = lane % ACROSS * W, left = bytes - o;
 #pragma unroll 4
@@ -492,7 +493,9 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
 #pragma unroll
                 for (int o = 0; o < OPS; ++o) {
                     ahead[(2 * o) * EACH + i] = n < p.N && p.ws[o] ? p.ws[o][n] : 0.0f;
-                    ahead[(2 * o + 1) * EACH + i] = n < p.N && p.bias[o] ? load_as_f32(p.bias[o], p.bias_dtype, n) : -0.0f;   // x + -0 is x
+                    // no bias is -0, which changes no sum
+                    ahead[(2 * o + 1) * EACH + i] =
+                        n < p.N && p.bias[o] ? load_as_f32(p.bias[o], p.bias_dtype, n) : -0.0f;
                 }
             }
         };

@@ -45,7 +45,7 @@ struct __align__(64) SkParams {
     const void* bias[2];
     void* y2;                      // I8_DIGIT: rows from split_row on, seg_rows of each part (NULL: all to y)
     int64_t ldx, ldc, ldy, K, split_row, seg_rows;
-    int32_t M, N, tm, k_steps, seg_steps, splits, stages, codes_bytes, partial_bytes, tmem_cols;
+    int32_t M, N, tm, k_steps, seg_steps, splits, stages, codes_bytes, tmem_cols;
     int32_t y_dtype, bias_dtype, act, vec_c, vec_y;
     int32_t dependent;             // launched while the kernel before it still runs: 1: it writes the tokens, 2: weights too
     uint64_t stall_ns;             // test knob (ima_set_gemm_wait_test); 0 in normal use
@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
             named_barrier_sync(1, SK_WORKERS * 32);
         }
         // scales and biases while the products run: of the lane's weight row (one CTA), or of the four
-        // columns that the thread will own (a cluster)
+        // columns that the thread will own (a cluster).  Plain loads: the kernel before this one may have written the
+        // scales since this one started.  No bias is -0, which changes no sum.
         const int q = warp & 3, hw = (warp - 2) >> 2, wt = threadIdx.x - 64;
         const int own = SK_ROWS / S, per = own / 4, j4 = (wt % per) * 4;
         const int32_t nq = S > 1 ? n0 + (int32_t)rank * own + j4 : n0 + q * 32 + lane;
@@ -295,8 +296,8 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
         for (int o = 0; o < OPS; ++o)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? p.ws[o][nq + e] : 0.0f;   // a kernel that still ran at this one's start may have written it: not __ldg
-                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, nq + e) : -0.0f;   // x + -0 is x
+                ws[o][e] = EPI != I8_DIGIT && p.y && e < valid ? p.ws[o][nq + e] : 0.0f;
+                bias[o][e] = EPI != I8_DIGIT && p.bias[o] && e < valid ? load_as_f32(p.bias[o], p.bias_dtype, nq + e) : -0.0f;
             }
         // the value of one output from its exact sums: a[plane], or a[0] of the operand(s)
         auto value = [&](const int32_t (&a)[P], int32_t b, float xs, int e) {
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(SK_THREADS, 2) int8_skinny_kernel(const __grid
 // host side
 // ---------------------------------------------------------------------------
 struct SkPlan {
-    int tm, m_tiles, n_tiles, k_steps, splits, stages, codes_bytes, partial_bytes, smem;
+    int tm, m_tiles, n_tiles, k_steps, splits, stages, codes_bytes, smem;
     bool ok;
     double ns;   // estimate
 };
@@ -471,15 +472,18 @@ SkPlan sk_plan(int64_t M, int64_t N, int64_t k_steps, int planes, int ops, int x
         if (stages < least) continue;
         stages = std::min<int64_t>(stages, std::max<int64_t>(steps, 1));
         q.tm = (int)tm; q.m_tiles = (int)m_tiles; q.n_tiles = (int)n_tiles; q.k_steps = (int)k_steps;
-        q.splits = s; q.stages = (int)stages; q.codes_bytes = (int)codes; q.partial_bytes = (int)partial;
+        q.splits = s; q.stages = (int)stages; q.codes_bytes = (int)codes;
         q.smem = (int)(fixed + stages * stage);
         const int64_t ctas = m_tiles * n_tiles * s;
         // clusters of 8 leave some SMs out, and so do those of 4
         const int64_t room = std::max<int64_t>(1, gemm_grid_limit() * per_sm * (s == 8 ? 14 : s == 4 ? 15 : 16) / 16);
         const double rounds = (double)((ctas + room - 1) / room);
-        const double stream = std::max(rounds * (double)steps * ((double)(ops * SK_ROWS * I8_KT) / 45.0 + (double)(stage - ops * SK_ROWS * I8_KT) / 100.0),
+        const int64_t w_bytes = ops * SK_ROWS * I8_KT;
+        const double stream = std::max(rounds * (double)steps * ((double)w_bytes / 45.0 + (double)(stage - w_bytes) / 100.0),
                                        (double)(N * k_steps * I8_KT * ops * m_tiles) / 5500.0);
-        q.ns = rounds * ((fused ? 6000.0 + 100.0 * (double)M : 5000.0) + (4.0 + 16.0 * (double)per_sm / (double)s) * (double)(ops * planes * tm)) + stream + (s > 1 ? 1000.0 : 0.0);
+        const double column = 4.0 + 16.0 * (double)per_sm / (double)s;
+        q.ns = rounds * ((fused ? 6000.0 + 100.0 * (double)M : 5000.0) + column * (double)(ops * planes * tm)) + stream +
+               (s > 1 ? 1000.0 : 0.0);
         q.ok = true;
         if (!best.ok || q.ns < best.ns) best = q;
     }
@@ -497,7 +501,6 @@ int launch_skinny(SkParams& p, const SkPlan& q, cudaStream_t stream) {
     p.splits = q.splits;
     p.stages = q.stages;
     p.codes_bytes = q.codes_bytes;
-    p.partial_bytes = q.partial_bytes;
     p.stall_ns = g_gemm_stall_ns;
     p.tmem_cols = 32;
     while (p.tmem_cols < (EPI == I8_GATED ? 2 : 1) * P * q.tm) p.tmem_cols *= 2;

@@ -604,6 +604,8 @@ def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, act
 def _check_gated(k: int, gate, up, activation: str) -> None:
     if activation not in ACTIVATIONS:
         raise RuntimeError(f"unknown activation {activation!r}; choose one of: {', '.join(sorted(ACTIVATIONS))}")
+    if len(gate.shape) != 2:
+        raise RuntimeError(f"int8 weight source must be 2-D, got {tuple(gate.shape)}")
     if gate.shape != up.shape:
         raise RuntimeError(f"gate and up weights differ in shape: {tuple(gate.shape)} vs {tuple(up.shape)}")
     if gate.shape[1] != k:

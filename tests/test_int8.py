@@ -1090,3 +1090,16 @@ def test_quantiser_rows_at_every_alignment(cuda_device, dtype, m, k):
         want_q, want_s = plain_codes(x)
         assert torch.equal(s.flatten().double(), want_s) and torch.equal(q.double(), want_q)
     status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+def test_weights_of_other_ranks_are_refused(cuda_device):
+    x = torch.randn((4, 32), device=cuda_device)
+    for w in (torch.randn(32, device=cuda_device), torch.randn((2, 3, 32), device=cuda_device)):
+        for grad in (False, True):
+            w.requires_grad_(grad)
+            with pytest.raises(RuntimeError, match="2-D"):
+                int8.int8_linear(x, w)
+            with pytest.raises(RuntimeError, match="2-D"):
+                int8.int8_gated(x, w, w)
+    status_clean(cuda_device)
