@@ -235,6 +235,8 @@ class Int8Weight:
         kept = self._transposed
         if version is None:
             return None
+        if kept is not None and kept[1] == version and kept[2].cuda_stream == _raw_stream(self.index):
+            return kept[0]   # made on this stream, which keeps it in order
         stream = torch.cuda.current_stream(self.device)
         if kept is None or kept[1] != version:
             if _capturing():    # what a capture writes is not there before its replay
@@ -270,10 +272,13 @@ def _check_out(t: torch.Tensor, shape: tuple[int, int], dtypes: tuple, label: st
 
 def _bias_args(n: int, *biases: torch.Tensor | None) -> tuple[list[torch.Tensor | None], int]:
     """Biases as contiguous vectors of one floating type, and that type's code."""
-    if len(biases) == 1 and biases[0] is not None:   # the usual case, as it is
-        b = biases[0]
-        if b.ndim == 1 and b.dtype in _DTYPE_CODES and b.shape[0] == n and b.is_contiguous():
-            return list(biases), _DTYPE_CODES[b.dtype]
+    dtype = None if biases[0] is None else biases[0].dtype
+    for b in biases:   # the usual case, as it is
+        if b is None or b.dtype is not dtype or b.ndim != 1 or b.shape[0] != n or not b.is_contiguous():
+            break
+    else:
+        if dtype in _DTYPE_CODES:
+            return biases, _DTYPE_CODES[dtype]
     dtype = None
     for b in biases:
         if b is not None:
@@ -701,7 +706,9 @@ class _LinearFunction(torch.autograd.Function):
         dx, dw, db = _linear_backward(grad, block, sizes, (base, ld, base + at[0]), w, handle, ctx.types)
         if dx is not None and len(ctx.shapes[0]) != 2:
             dx = dx.reshape(ctx.shapes[0])
-        return dx, dw, None if db is None else db.reshape(ctx.shapes[1]), None
+        if db is not None and len(ctx.shapes[1]) != 1:
+            db = db.reshape(ctx.shapes[1])
+        return dx, dw, db, None
 
 
 class _GatedFunction(torch.autograd.Function):
@@ -749,7 +756,8 @@ class _GatedFunction(torch.autograd.Function):
         q, g, u = _GatedFunction.parts(block, m, (k + 15) // 16 * 16 or 16, n, gate, up)
         frozen = (gate, up) if gate is not None and up is not None else None
         grads = _gated_backward(grad, block, ctx.sizes, q, g, u, frozen, gate_bias, up_bias, ctx.activation, ctx.types)
-        return (*(None if t is None else t.reshape(shape) for t, shape in zip(grads, ctx.shapes)), None, None, None)
+        return (*(t if t is None or t.shape == shape else t.reshape(shape) for t, shape in zip(grads, ctx.shapes)),
+                None, None, None)
 
 
 def _beside(x: torch.Tensor, weights: tuple, biases: tuple) -> bool:
