@@ -186,8 +186,12 @@ def _transpose(t: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _capturing() -> bool:
-    return torch.cuda.is_current_stream_capturing()
+def _capturing(index: int) -> bool:
+    """Whether the current stream of device `index` records a CUDA graph."""
+    if _current_device() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
 
 
 class Int8Weight:
@@ -195,7 +199,8 @@ class Int8Weight:
 
     `codes` and `scale` stay the caller's tensors where their layout allows it (rows on 16-byte
     boundaries); the transposed codes that a backward pass contracts over are made at the first
-    one and kept until the codes change."""
+    one and kept until the codes change.  A captured backward pass makes its own at every replay,
+    so that replays follow edits of the codes."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
         codes = _aligned_codes(codes.detach(), "int8 weight")
@@ -229,18 +234,18 @@ class Int8Weight:
         return made
 
     def transposed(self) -> torch.Tensor | None:
-        """The transposed codes [K, N], made once.  None where the kept copy cannot be used (codes without
-        a version counter; a capture before it exists or is complete): the caller makes its own."""
+        """The transposed codes [K, N], made once.  None for codes without a version counter and during a
+        capture; the caller then makes its own.  A graph would hold the address of the kept copy, which
+        an edit of the codes outdates and the next call afterwards frees, and a copy made in a
+        capture is not there before its replay."""
         version = nat.tensor_version(self.codes)
-        kept = self._transposed
-        if version is None:
+        if version is None or _capturing(self.index):
             return None
+        kept = self._transposed
         if kept is not None and kept[1] == version and kept[2].cuda_stream == _raw_stream(self.index):
             return kept[0]   # made on this stream, which keeps it in order
         stream = torch.cuda.current_stream(self.device)
         if kept is None or kept[1] != version:
-            if _capturing():    # what a capture writes is not there before its replay
-                return None
             with torch.inference_mode(False):
                 t = _transpose(self.codes)
             event = torch.cuda.Event()
@@ -249,13 +254,11 @@ class Int8Weight:
             return t
         t, _version, maker, event = kept
         if event is not None and stream != maker:
-            if _capturing():
-                return None
             if event.query():
                 self._transposed = (t, version, maker, None)
             else:
                 stream.wait_event(event)
-        if stream != maker and not _capturing():
+        if stream != maker:
             t.record_stream(stream)
         return t
 
@@ -509,7 +512,7 @@ def int8_linear_backward(
 
     grad: output gradient [..., N]; codes, scale: per_token_int8 of the activations.  keep_transposed:
     the transposed weight that dx needs stays with `weight` for the next call (one more byte per
-    weight), else it is temporary.  Launches only, on the current stream."""
+    weight), else, and in a capture, it is temporary.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
     (m, k), n = codes.shape, weight.shape[0]
     if weight.shape[1] != k:
@@ -632,8 +635,9 @@ def _record(function, leaves, *args):
     the stream it was made on, and lives as long as any graph with the leaf.  A capture that records a
     backward pass through a node of another stream ends the process when it runs that pass: eager
     recordings leave a mark on the nodes, and a capture that finds one is refused before it records."""
-    stream = _raw_stream(args[0].device.index)
-    if not _capturing():
+    index = args[0].device.index
+    stream = _raw_stream(index)
+    if not _capturing(index):
         out = function.apply(*args)
         for node, _ in out.grad_fn.next_functions:
             if type(node).__name__ == "AccumulateGrad":

@@ -1,0 +1,90 @@
+"""Int8Weight handles over their lifetime: captures, edits, replaced tensors.  The CPU tests replace the
+transposing launch and the stream queries by host ones; what the handle decides is the same."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from int_model_approximation_b200 import int8
+from test_int8 import make, status_clean
+
+
+class FakeStream:
+    cuda_stream = 7
+
+
+class FakeEvent:
+    def record(self, stream):
+        pass
+
+    def query(self):
+        return True
+
+
+@pytest.fixture
+def host_handle(monkeypatch):
+    """An Int8Weight of host tensors, and a switch that says whether a capture runs."""
+    stream, capturing = FakeStream(), [False]
+    monkeypatch.setattr(int8, "_transpose", lambda t: t.t().contiguous())
+    monkeypatch.setattr(int8, "_raw_stream", lambda index: stream.cuda_stream)
+    monkeypatch.setattr(int8, "_capturing", lambda *index: capturing[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *device: stream)
+    monkeypatch.setattr(torch.cuda, "Event", FakeEvent)
+    wt = int8.Int8Weight.__new__(int8.Int8Weight)
+    wt._set(torch.randint(-127, 128, (5, 16), dtype=torch.int8), torch.ones(5))
+    return wt, capturing
+
+
+def test_a_capture_takes_no_kept_transposed_codes(host_handle):
+    wt, capturing = host_handle
+    kept = wt.transposed()
+    assert torch.equal(kept, wt.codes.t()) and wt.transposed() is kept
+    capturing[0] = True
+    assert wt.transposed() is None
+    capturing[0] = False
+    assert wt.transposed() is kept
+    wt.codes[2].zero_()
+    assert torch.equal(wt.transposed(), wt.codes.t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("own_stream", [False, True])
+@pytest.mark.parametrize("gated", [False, True])
+def test_replays_follow_edited_codes(cuda_device, own_stream, gated):
+    """A backward pass captured while transposed copies are kept (made on the capturing stream, or on another one
+    and complete), then the codes edited, an eager pass that renews the copies, and memory reused."""
+    m, n, k = 40, 70, 200
+    x, w, _ = make(m, n, k, torch.float32, 51, cuda_device)
+    _x, w2, _ = make(m, n, k, torch.float32, 52, cuda_device)
+    dy = torch.randn((m, n), device=cuda_device)
+    q, s = int8.per_token_int8(x)
+    g, u = int8.Int8Weight.from_float(w), int8.Int8Weight.from_float(w2)
+
+    def step(g, u):
+        if gated:
+            return int8.int8_gated_backward(dy, q, s, g, u, dx_dtype=torch.float32)[0]
+        return int8.int8_linear_backward(dy, q, s, g, dx_dtype=torch.float32)[0]
+
+    capturing = torch.cuda.Stream()
+    with torch.cuda.stream(capturing if own_stream else torch.cuda.current_stream()):
+        step(g, u)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(capturing):
+        for _ in range(2):      # the copies are known to be complete here
+            step(g, u)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=capturing):
+        got = step(g, u)
+    for wt in (g, u):
+        wt.codes[3].zero_()
+        wt.codes[:, 5].fill_(100)
+    want = step(*(int8.Int8Weight(wt.codes.clone(), wt.scale) for wt in (g, u)))
+    step(g, u)
+    scribble = [torch.full((k, 80), 77, dtype=torch.int8, device=cuda_device) for _ in range(64)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(step(g, u), want)
+    del scribble
+    status_clean(cuda_device)
