@@ -210,12 +210,50 @@ class Int8Weight:
         self._set(codes, _scales(scale, codes.shape[0], "weight scale"))
 
     def _set(self, codes: torch.Tensor, scale: torch.Tensor) -> None:
-        self.codes, self.scale = codes, scale
+        self._codes, self._scale, self._looks = codes, scale, 0
+        self._look()
+        self._transposed: tuple | None = None   # (codes [K, N], state() of then, stream, event until it has passed)
+
+    def _look(self) -> None:
+        codes = self._codes
+        # aliases of what was looked at: they tell a replaced tensor, and keep its memory from being used again
+        self._seen = codes.detach(), self._scale.detach()
+        self._looks += 1
         self.shape, self.device, self.index, self.ld = codes.shape, codes.device, codes.get_device(), _code_ld(codes)
-        self._transposed: tuple | None = None   # (codes [K, N], version of self.codes, stream, event until it has passed)
+        self.codes_at, self.scale_at = codes.data_ptr(), self._scale.data_ptr()
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self._scale
+
+    def moved(self) -> bool:
+        """Whether codes or scales are other memory than when they were looked at last (tensor.data = other)."""
+        return not (self._codes.is_set_to(self._seen[0]) and self._scale.is_set_to(self._seen[1]))
+
+    def follow(self) -> None:
+        """Look at codes and scales again if they have moved."""
+        if not self.moved():
+            return
+        codes, scale = self._codes, self._scale
+        _check_codes(codes, "int8 weight")
+        if _layout(codes, *codes.shape) is None:
+            raise RuntimeError("int8 weight codes were replaced by rows that do not start on 16 bytes; make a new Int8Weight")
+        nat.require_device(codes.device, ("weight scale", scale))
+        if _scales(scale, codes.shape[0], "weight scale") is not scale:
+            raise RuntimeError("int8 weight scales were replaced by ones that are not contiguous fp32; make a new Int8Weight")
+        self._look()
+
+    def state(self) -> tuple:
+        """What an edit changes: the times that codes or scales were replaced, and their counts of in-place edits."""
+        self.follow()
+        return self._looks, nat.tensor_version(self._codes), nat.tensor_version(self._scale)
 
     def __getstate__(self):
-        return self.codes, self.scale   # copies make their own transposed codes
+        return self._codes, self._scale   # copies make their own transposed codes
 
     def __setstate__(self, state) -> None:
         self._set(*state)
@@ -238,24 +276,24 @@ class Int8Weight:
         capture; the caller then makes its own.  A graph would hold the address of the kept copy, which
         an edit of the codes outdates and the next call afterwards frees, and a copy made in a
         capture is not there before its replay."""
-        version = nat.tensor_version(self.codes)
-        if version is None or _capturing(self.index):
+        state = self.state()[:2]
+        if state[1] is None or _capturing(self.index):
             return None
         kept = self._transposed
-        if kept is not None and kept[1] == version and kept[2].cuda_stream == _raw_stream(self.index):
+        if kept is not None and kept[1] == state and kept[2].cuda_stream == _raw_stream(self.index):
             return kept[0]   # made on this stream, which keeps it in order
         stream = torch.cuda.current_stream(self.device)
-        if kept is None or kept[1] != version:
+        if kept is None or kept[1] != state:
             with torch.inference_mode(False):
-                t = _transpose(self.codes)
+                t = _transpose(self._codes)
             event = torch.cuda.Event()
             event.record(stream)
-            self._transposed = (t, version, stream, event)
+            self._transposed = (t, state, stream, event)
             return t
-        t, _version, maker, event = kept
+        t, _, maker, event = kept
         if event is not None and stream != maker:
             if event.query():
-                self._transposed = (t, version, maker, None)
+                self._transposed = (t, state, maker, None)
             else:
                 stream.wait_event(event)
         if stream != maker:
@@ -397,7 +435,7 @@ def _weight_args(weight) -> tuple[Int8Weight, torch.Tensor | None]:
 
 
 def _at(weight: Int8Weight) -> tuple[int, int, int]:
-    return weight.codes.data_ptr(), weight.ld, weight.scale.data_ptr()
+    return weight.codes_at, weight.ld, weight.scale_at
 
 
 def _linear_call(rows, m, k, n, x_type, q, keep, w, src, bias, y) -> None:
@@ -514,6 +552,7 @@ def int8_linear_backward(
     the transposed weight that dx needs stays with `weight` for the next call (one more byte per
     weight), else, and in a capture, it is temporary.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
+    weight.follow()
     (m, k), n = codes.shape, weight.shape[0]
     if weight.shape[1] != k:
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={weight.shape[1]}")
@@ -565,6 +604,8 @@ def int8_gated_backward(
     int8_linear_backward.  Both projections are formed again from the codes, so a forward pass keeps
     one byte per activation and nothing of width N.  Launches only, on the current stream."""
     codes = _aligned_codes(codes, "int8 activation matrix")
+    gate.follow()
+    up.follow()
     (m, k), n = codes.shape, gate.shape[0]
     _check_gated(k, gate, up, activation)
     nat.require_device(codes.device, ("gate weight", gate.codes), ("up weight", up.codes), ("scale", scale),
@@ -654,7 +695,7 @@ def _record(function, leaves, *args):
 
 
 def _versions(*weights: Int8Weight) -> tuple:
-    return tuple(nat.tensor_version(t) for w in weights for t in (w.codes, w.scale))
+    return tuple(w.state() for w in weights)
 
 
 def _check_versions(before: tuple, *weights: Int8Weight) -> None:
@@ -768,7 +809,7 @@ def _beside(x: torch.Tensor, weights: tuple, biases: tuple) -> bool:
     """Whether Int8Weights and floating biases (or None) lie on x's device: what _check_inputs finds, sooner."""
     index = x.get_device()
     for w in weights:
-        if w.index != index:
+        if w.index != index or w.moved():
             return False
     for b in biases:
         if b is not None and (type(b) is not torch.Tensor or b.get_device() != index or b.dtype not in _DTYPE_CODES):
@@ -788,6 +829,7 @@ def _check_inputs(x: torch.Tensor, *named) -> None:
         if t is None:
             continue
         if type(t) is Int8Weight:
+            t.follow()
             if t.device != dev:
                 nat.require_device(dev, (label, t.codes))
         elif isinstance(t, torch.Tensor):

@@ -26,6 +26,8 @@ class FakeEvent:
 def host_handle(monkeypatch):
     """An Int8Weight of host tensors, and a switch that says whether a capture runs."""
     stream, capturing = FakeStream(), [False]
+    monkeypatch.setattr(int8, "_require_cuda", lambda *named: None)
+    monkeypatch.setattr(int8.nat, "require_device", lambda *named: None)
     monkeypatch.setattr(int8, "_transpose", lambda t: t.t().contiguous())
     monkeypatch.setattr(int8, "_raw_stream", lambda index: stream.cuda_stream)
     monkeypatch.setattr(int8, "_capturing", lambda *index: capturing[0])
@@ -88,3 +90,75 @@ def test_replays_follow_edited_codes(cuda_device, own_stream, gated):
     assert torch.equal(got, want) and torch.equal(step(g, u), want)
     del scribble
     status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# codes and scales that lie elsewhere than before
+# ---------------------------------------------------------------------------
+def test_repointed_codes_are_transposed_anew(host_handle):
+    wt, _capturing = host_handle
+    wt.transposed()
+    version = wt.codes._version
+    wt.codes.data = torch.randint(-127, 128, (5, 16), dtype=torch.int8)
+    assert wt.codes._version == version       # the version alone does not tell
+    assert torch.equal(wt.transposed(), wt.codes.t())
+
+
+def test_codes_and_scales_are_not_assigned(host_handle):
+    wt, _capturing = host_handle
+    for name in ("codes", "scale"):
+        with pytest.raises(AttributeError):
+            setattr(wt, name, getattr(wt, name).clone())
+
+
+@pytest.mark.gpu
+def test_repointed_codes_and_scales(cuda_device):
+    """tensor.data = other, of another shape too: forward and backward follow; between the two it is refused."""
+    dev = cuda_device
+    x, w, _ = make(9, 40, 64, torch.float32, 53, dev)
+    _x, w2, _ = make(9, 130, 64, torch.float32, 54, dev)
+    x.requires_grad_()
+    dy, dy2 = torch.randn((9, 40), device=dev), torch.randn((9, 130), device=dev)
+    wt = int8.Int8Weight.from_float(w)
+    torch.autograd.grad(int8.int8_linear(x, wt), x, dy)
+    other = int8.Int8Weight.from_float(w2)
+    y = int8.int8_linear(x, wt)
+    wt.codes.data, wt.scale.data = other.codes.clone(), other.scale.clone()
+    with pytest.raises(RuntimeError, match="modified in place"):
+        torch.autograd.grad(y, x, dy, retain_graph=True)
+    y, want = int8.int8_linear(x, wt), int8.int8_linear(x, other)
+    assert torch.equal(y, want)
+    want, = torch.autograd.grad(want, x, dy2)
+    assert torch.equal(torch.autograd.grad(y, x, dy2)[0], want)
+    q, s = int8.per_token_int8(x)
+    assert torch.equal(int8.int8_linear_backward(dy2, q, s, wt, dx_dtype=torch.float32)[0], want)
+    h = int8.int8_gated(x.detach(), wt, other)
+    assert torch.equal(h, int8.int8_gated(x.detach(), other, other))
+    # back and forth: memory of the same address, other values
+    wt = int8.Int8Weight.from_float(w)
+    y = int8.int8_linear(x, wt)
+    torch.autograd.grad(y, x, dy, retain_graph=True)
+    for fill in (3, 5, 7):
+        wt.codes.data = torch.full((40, 64), fill, dtype=torch.int8, device=dev)
+        fresh = int8.Int8Weight(wt.codes.clone(), wt.scale.clone())
+        z, want = int8.int8_linear(x, wt), int8.int8_linear(x, fresh)
+        assert torch.equal(z, want)
+        assert torch.equal(torch.autograd.grad(z, x, dy)[0], torch.autograd.grad(want, x, dy)[0])
+        with pytest.raises(RuntimeError, match="modified in place"):
+            torch.autograd.grad(y, x, dy, retain_graph=True)
+    # the same memory, fewer rows
+    wt.codes.data, wt.scale.data = wt.codes[:17], wt.scale[:17]
+    assert int8.int8_linear(x, wt).shape == (9, 17)
+    wt = int8.Int8Weight(other.codes.clone(), other.scale.clone())
+    # layouts that the kernels cannot read
+    wt.scale.data = torch.ones(7, device=dev)
+    with pytest.raises(RuntimeError, match="entries, expected"):
+        int8.int8_linear(x, wt)
+    wt.scale.data = torch.ones(260, device=dev)[::2]
+    with pytest.raises(RuntimeError, match="contiguous fp32"):
+        int8.int8_linear(x, wt)
+    wt.scale.data = other.scale.clone()
+    wt.codes.data = torch.zeros((130, 65), dtype=torch.int8, device=dev)[:, 1:]
+    with pytest.raises(RuntimeError, match="do not start on 16 bytes"):
+        int8.int8_gated(x, wt, other)
+    status_clean(dev)
