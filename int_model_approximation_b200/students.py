@@ -434,11 +434,20 @@ def _expanded_block_scale(weight: torch.Tensor, scale: torch.Tensor) -> torch.Te
     ]
 
 
+def _channel_scale(weight: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """weight_scale of an FP8 linear as a factor of weight [N, K]: one scale, or one per output channel in any
+    shape of N entries, as CodebookLinear reads it."""
+    if scale.numel() not in (1, weight.shape[0]):
+        raise RuntimeError(f"FP8 weight_scale has shape {tuple(scale.shape)}, expected one entry or one per output channel "
+                           f"({weight.shape[0]})")
+    return scale.to(torch.float32).reshape(-1, 1)
+
+
 def _dequantized_weight(module: nn.Linear) -> torch.Tensor:
     weight = module.weight.detach()
     if weight.dtype == torch.float8_e4m3fn:
         if hasattr(module, "weight_scale"):
-            return weight.to(torch.float32) * module.weight_scale.detach().to(torch.float32)
+            return weight.to(torch.float32) * _channel_scale(weight, module.weight_scale.detach())
         if hasattr(module, "weight_scale_inv"):
             scale = module.weight_scale_inv.detach().to(torch.float32)
             return weight.to(torch.float32) * _expanded_block_scale(weight, scale)
