@@ -13,12 +13,15 @@ runs on the sm_100a kernels of libima_b200.so; there is no CPU execution path.
 
 from __future__ import annotations
 
+import functools
+import inspect
 import math
 import os
 from typing import Any
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from . import _native as nat
 from .codebook import DigitPlanes, codebook_planes_from_fp8, int_gemm, per_token_fp8, planes_from_int32
@@ -393,24 +396,75 @@ def _bump_probe(products: int) -> None:
 
 
 def _gated_activation(module: nn.Module) -> str | None:
-    """The activation of a module whose children are exactly gate_proj, up_proj, down_proj and act_fn,
-    down(act(gate(x)) * up(x)) in the layout of every gated block this package's shapes come from; None
-    for anything else."""
+    """The activation of a module that computes down(act(gate(x)) * up(x)) on children gate_proj, up_proj, down_proj
+    and act_fn, in the layout of every gated block this package's shapes come from; None for anything else.
+    The names only propose: a fused block replaces the module's own forward and no longer calls gate_proj, up_proj
+    and act_fn, so own parameters or buffers, hooks on any of them and a forward that computes something else decline."""
     children = dict(module.named_children())
     if set(children) != {"gate_proj", "up_proj", "down_proj", "act_fn"}:
         return None
-    if next(module.parameters(recurse=False), None) is not None:
+    own = (*module.parameters(recurse=False), *module.buffers(recurse=False))
+    if own or any(map(_hooked, (module, children["gate_proj"], children["up_proj"], children["act_fn"]))):
         return None
     act = children["act_fn"]
     if isinstance(act, nn.SiLU):
-        return "silu"
-    if isinstance(act, nn.GELU):
-        return "gelu_tanh" if act.approximate == "tanh" else "gelu"
-    return None
+        activation = "silu"
+    elif isinstance(act, nn.GELU):
+        activation = "gelu_tanh" if act.approximate == "tanh" else "gelu"
+    else:
+        return None
+    return activation if _computes_gated(module, activation) else None
+
+
+_ACTIVATION_FUNCTIONS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": functools.partial(F.gelu, approximate="tanh")}
+
+
+def _hooked(module: nn.Module) -> bool:
+    return any(getattr(module, hooks, None) for hooks in (
+        "_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks"))
+
+
+class _Picked(nn.Module):
+    """Stand-in for a projection: every output is one of the inputs times a factor."""
+
+    def __init__(self, linear: nn.Module, step: int):
+        super().__init__()
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        i = torch.arange(self.out_features, device="cpu", dtype=torch.float64)
+        self.index, self.factor = (step * (i + 1)).long() % self.in_features, 0.5 + (0.618 * step * (i + 1)) % 1.0
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return x[..., self.index] * self.factor
+
+
+def _computes_gated(module: nn.Module, activation: str) -> bool:
+    """Whether module.forward(x) is down(act(gate(x)) * up(x)): run on the host in 64 bits with stand-ins for the
+    three projections, on values of both signs from 1e-3 to 1e4, in training and in evaluation mode."""
+    try:
+        if "forward" in vars(module) or len(inspect.signature(module.forward).parameters) != 1:
+            return False
+        gate, up, down = (_Picked(getattr(module, name), step)
+                          for name, step in (("gate_proj", 7), ("up_proj", 11), ("down_proj", 13)))
+        i = torch.arange(6 * gate.in_features, device="cpu", dtype=torch.float64).reshape(2, 3, -1)
+        x = torch.where(i * 0.7548 % 1.0 < 0.5, -1.0, 1.0) * 10.0 ** (7.0 * (i * 0.5698 % 1.0) - 3.0)
+        want = down(_ACTIVATION_FUNCTIONS[activation](gate(x)) * up(x))
+        bound = 1e-5 * want.abs() + down(1e-6 * up(x).abs())   # covers an activation taken in fp32
+        for training in (False, True):
+            twin = object.__new__(type(module))   # the module's own forward and attributes, other projections
+            vars(twin).update(vars(module), training=training, _modules={
+                **module._modules, "gate_proj": gate, "up_proj": up, "down_proj": down})
+            with torch.no_grad(), torch.random.fork_rng(devices=[]):
+                got = twin.forward(x.clone())
+            if not (isinstance(got, torch.Tensor) and got.shape == want.shape and
+                    bool(((got.double() - want).abs() <= bound).all())):
+                return False
+    except Exception:   # a forward that needs more than its projections' outputs is not this formula
+        return False
+    return True
 
 
 def _fuse_gated_blocks(model: nn.Module) -> None:
-    """Replace every gated block whose three projections are Int8Linear by an Int8GatedMLP."""
+    """Replace every gated block (_gated_activation) whose three projections are Int8Linear by an Int8GatedMLP."""
     blocks = [(name, module) for name, module in model.named_modules() if name]
     for name, module in blocks:
         activation = _gated_activation(module)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from int_model_approximation_b200 import int8, students, synthetic
-from test_int8 import status_clean
+from test_int8 import GatedBlock, status_clean
 
 
 def fp8_linear(n, k, scale, seed=0, device="cpu"):
@@ -56,4 +56,127 @@ def test_square_fp8_linear_beside_the_codebook_student(cuda_device, monkeypatch,
         assert torch.equal(model(x), int8.int8_linear(x, lin.weight.float() * scale.to(cuda_device).reshape(-1, 1)))
     # e4m3 carries 2^-4 of each activation, int8 half a step of 1/127 of the row's maximum
     assert float((got - want).norm() / want.norm()) < 0.1
+    status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# which modules are gated blocks
+# ---------------------------------------------------------------------------
+class Fp32Activation(GatedBlock):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x).float()).to(x.dtype) * self.up_proj(x))
+
+
+class OtherOrder(GatedBlock):
+    def forward(self, hidden_states):
+        return self.down_proj(self.up_proj(hidden_states) * self.act_fn(self.gate_proj(hidden_states)))
+
+
+class Clamped(GatedBlock):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x).clamp(max=7.0)) * self.up_proj(x))
+
+
+class Shifted(GatedBlock):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x)) * (self.up_proj(x) + 1))
+
+
+class Scaled(GatedBlock):
+    multiplier = 0.5
+
+    def forward(self, x):
+        return self.down_proj(self.act_fn(self.gate_proj(x) * self.multiplier) * self.up_proj(x))
+
+
+class Residual(GatedBlock):
+    def forward(self, x):
+        return x + self.down_proj(self.act_fn(self.gate_proj(x)) * self.up_proj(x))
+
+
+class Swapped(GatedBlock):
+    def forward(self, x):
+        return self.down_proj(self.gate_proj(x) * self.act_fn(self.up_proj(x)))
+
+
+class Dropping(GatedBlock):
+    def forward(self, x):
+        h = self.act_fn(self.gate_proj(x)) * self.up_proj(x)
+        return self.down_proj(torch.nn.functional.dropout(h, 0.5, self.training))
+
+
+class WithMask(GatedBlock):
+    def forward(self, x, mask=None):
+        h = self.act_fn(self.gate_proj(x)) * self.up_proj(x)
+        return self.down_proj(h if mask is None else h * mask)
+
+
+class Raising(GatedBlock):
+    def forward(self, x):
+        return self.down_proj(self.act_fn(x @ self.gate_proj.weight.t()) * self.up_proj(x))
+
+
+ACT_MODULES = {"silu": torch.nn.SiLU(), "gelu": torch.nn.GELU(), "gelu_tanh": torch.nn.GELU(approximate="tanh")}
+
+
+@pytest.mark.parametrize("act", sorted(ACT_MODULES))
+@pytest.mark.parametrize("sizes", [(4, 8), (1, 3), (7, 5), (64, 200)])
+def test_blocks_of_the_formula_are_recognised(act, sizes):
+    for cls in (GatedBlock, Fp32Activation, OtherOrder):
+        block = cls(*sizes, ACT_MODULES[act])
+        before = torch.random.get_rng_state()
+        assert students._gated_activation(block) == act
+        assert students._gated_activation(block.double().eval()) == act
+        assert torch.equal(before, torch.random.get_rng_state()) and isinstance(block.gate_proj, torch.nn.Linear)
+
+
+@pytest.mark.parametrize("act", sorted(ACT_MODULES))
+@pytest.mark.parametrize("cls", [Clamped, Shifted, Scaled, Residual, Swapped, Dropping, WithMask, Raising])
+def test_blocks_of_another_formula_are_left_alone(cls, act):
+    for block in (cls(16, 24, ACT_MODULES[act]), cls(16, 24, ACT_MODULES[act]).eval()):
+        assert students._gated_activation(block) is None
+
+
+def test_blocks_with_something_of_their_own_are_left_alone():
+    block = GatedBlock(4, 8, torch.nn.SiLU())
+    block.register_buffer("scale", torch.ones(1))
+    assert students._gated_activation(block) is None
+    block = GatedBlock(4, 8, torch.nn.SiLU())
+    block.gain = torch.nn.Parameter(torch.ones(1))
+    assert students._gated_activation(block) is None
+    block = GatedBlock(4, 8, torch.nn.SiLU())
+    block.forward = lambda x: GatedBlock.forward(block, x)
+    assert students._gated_activation(block) is None
+
+    class Leaky(torch.nn.SiLU):     # an activation of that class that computes another
+        def forward(self, x):
+            return torch.nn.functional.leaky_relu(x)
+
+    assert students._gated_activation(GatedBlock(4, 8, Leaky())) is None
+    for part in (None, "gate_proj", "up_proj", "act_fn"):
+        for register in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook",
+                         "register_full_backward_pre_hook"):
+            block = GatedBlock(4, 8, torch.nn.SiLU())
+            handle = getattr(block if part is None else getattr(block, part), register)(lambda *args: None)
+            assert students._gated_activation(block) is None
+            handle.remove()
+            assert students._gated_activation(block) == "silu"
+
+
+@pytest.mark.gpu
+def test_students_of_other_blocks_compute_what_the_blocks_do(cuda_device, monkeypatch):
+    """Through the replacement pass: fused or not, a block's student stays near the block."""
+    monkeypatch.setattr(students, "STUDENT_KERNEL", "int8")
+    torch.manual_seed(1)
+    x = torch.randn((30, 64), device=cuda_device) * 4
+    for cls in (GatedBlock, Fp32Activation, Clamped, Shifted, Scaled, Residual, Swapped, WithMask):
+        model = torch.nn.Sequential(cls(64, 96, torch.nn.SiLU(), bias=True)).to(cuda_device).eval()
+        with torch.no_grad():
+            model[0].gate_proj.weight.mul_(4)   # gates beyond the clamp
+            want = model(x)
+            students._replace_int32_linears(model)
+            got = model(x)
+        assert isinstance(model[0], students.Int8GatedMLP) == (cls in (GatedBlock, Fp32Activation))
+        # a percent or two from three linears of half a step of 1/127; every other formula is tens of percent off
+        assert float((got - want).norm() / want.norm()) < 0.05, cls
     status_clean(cuda_device)
