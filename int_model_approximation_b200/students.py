@@ -373,7 +373,8 @@ class Int8Linear(nn.Module):
 
 class Int8GatedMLP(nn.Module):
     """Gated feed-forward block down(act(gate(x)) * up(x)) on three Int8Linear: gate, up, activation and
-    product in one kernel, then the down projection."""
+    product in one kernel, then the down projection.  While gate_proj or up_proj has a hook, both are
+    called as modules and their outputs rounded to x's type."""
 
     def __init__(self, gate_proj: Int8Linear, up_proj: Int8Linear, down_proj: Int8Linear, activation: str):
         super().__init__()
@@ -383,6 +384,8 @@ class Int8GatedMLP(nn.Module):
         self.activation = activation
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if _hooked(self.gate_proj) or _hooked(self.up_proj):
+            return self.down_proj(_ACTIVATION_FUNCTIONS[self.activation](self.gate_proj(x)) * self.up_proj(x))
         _require_cuda_tensor(x, "int8 input")
         _bump_probe(2)
         h = int8_gated(x, self.gate_proj.int8_weight(), self.up_proj.int8_weight(), self.gate_proj.bias,

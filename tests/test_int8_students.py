@@ -180,3 +180,34 @@ def test_students_of_other_blocks_compute_what_the_blocks_do(cuda_device, monkey
         # a percent or two from three linears of half a step of 1/127; every other formula is tens of percent off
         assert float((got - want).norm() / want.norm()) < 0.05, cls
     status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", sorted(ACT_MODULES))
+def test_hooks_on_the_projections_of_a_fused_block(cuda_device, monkeypatch, act):
+    monkeypatch.setattr(students, "STUDENT_KERNEL", "int8")
+    torch.manual_seed(2)
+    model = torch.nn.Sequential(GatedBlock(64, 96, ACT_MODULES[act], bias=True)).to(cuda_device)
+    students._replace_int32_linears(model)
+    block = model[0]
+    assert isinstance(block, students.Int8GatedMLP)
+    x = torch.randn((5, 64), device=cuda_device, requires_grad=True)
+    plain = model(x)
+    seen = []
+    handles = [block.gate_proj.register_forward_hook(lambda m, args, out: seen.append(out.detach())),
+               block.up_proj.register_forward_pre_hook(lambda m, args: (args[0] * 2,)),
+               block.down_proj.register_forward_hook(lambda m, args, out: seen.append(args[0].detach()))]
+    with students._Int32KernelProbe() as probe:
+        y = model(x)
+    assert probe.count == 3 and len(seen) == 2
+    g = int8.int8_linear(x, block.gate_proj.int8_weight(), block.gate_proj.bias).detach()
+    u = int8.int8_linear(x * 2, block.up_proj.int8_weight(), block.up_proj.bias).detach()
+    assert torch.equal(seen[0], g) and torch.equal(seen[1], ACT_MODULES[act](g) * u)
+    grads = []
+    handles.append(block.gate_proj.register_full_backward_hook(lambda m, gi, go: grads.append(go[0])))
+    model(x).sum().backward()
+    assert len(grads) == 1 and grads[0].shape == (5, 96)
+    for handle in handles:
+        handle.remove()
+    assert torch.equal(model(x), plain) and not torch.equal(y, plain)
+    status_clean(cuda_device)
