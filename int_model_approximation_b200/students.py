@@ -357,6 +357,15 @@ class Int8Linear(nn.Module):
         self.in_features = weight.shape[1]
         self.out_features = weight.shape[0]
 
+    def _apply(self, fn, recurse=True):
+        """The module moved (model.to and the like).  The scales belong to the codes: a cast of the model's floating
+        tensors leaves them in fp32."""
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
     def int8_weight(self) -> Int8Weight:
         """The codes and scales as int8_linear takes them (laid out anew if a buffer was replaced,
         e.g. by moving the module)."""

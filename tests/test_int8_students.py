@@ -211,3 +211,41 @@ def test_hooks_on_the_projections_of_a_fused_block(cuda_device, monkeypatch, act
         handle.remove()
     assert torch.equal(model(x), plain) and not torch.equal(y, plain)
     status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# modules that are moved or cast
+# ---------------------------------------------------------------------------
+def host_linear(n=6, k=16, bias=True):
+    """An Int8Linear of host tensors, without the launch that quantises."""
+    made = students.Int8Linear.__new__(students.Int8Linear)
+    torch.nn.Module.__init__(made)
+    made.register_buffer("weight", torch.randint(-127, 128, (n, k), dtype=torch.int8), persistent=False)
+    made.register_buffer("weight_scale", torch.logspace(-9, 2, n), persistent=False)
+    made.register_buffer("bias", torch.randn(n), persistent=False)
+    made.in_features, made.out_features = k, n
+    return made
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_a_cast_leaves_the_scales_of_the_codes(dtype):
+    lin = host_linear()
+    codes, scale = lin.weight.clone(), lin.weight_scale.clone()
+    model = torch.nn.Sequential(lin).to(dtype)
+    assert model[0] is lin and lin.bias.dtype == dtype
+    assert torch.equal(lin.weight, codes) and lin.weight_scale.dtype == torch.float32
+    assert torch.equal(lin.weight_scale, scale)
+    meta = model.to(device="meta", dtype=dtype)[0]
+    assert meta.weight_scale.dtype == torch.float32 and meta.weight_scale.device.type == "meta"
+
+
+@pytest.mark.gpu
+def test_a_cast_model_computes_with_its_own_scales(cuda_device):
+    w = torch.randn((40, 64), device=cuda_device) * torch.logspace(-9, 0, 40, device=cuda_device)[:, None]
+    lin = students.Int8Linear(w, None)
+    x = torch.randn((3, 64), device=cuda_device).to(torch.float16)
+    want = int8.int8_linear(x, int8.Int8Weight.from_float(w))
+    for cast in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.float(), lambda m: m.cpu().to(cuda_device)):
+        lin = cast(lin)
+        assert torch.equal(lin(x), want)
+    status_clean(cuda_device)
