@@ -14,8 +14,9 @@ There is no counterpart in the reference.
                     in one kernel
   int8_linear_backward, int8_gated_backward   their gradients as plain calls
 
-int8_linear and int8_gated take part in autograd (a whole training step can be captured into a CUDA
-graph if no eager autograd graph of the same leaves is alive; the *_backward calls can always).
+int8_linear and int8_gated take part in reverse-mode autograd; forward-mode tangents are refused.  A
+whole training step can be captured into a CUDA graph if no eager autograd graph of the same leaves
+is alive; the *_backward calls, which record nothing, can always.
 Gradients pass straight through the rounding: they are the derivatives at the dequantised
 activations and weights, with the scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
 gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
@@ -33,6 +34,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -668,6 +670,15 @@ def _wants_grad(*tensors) -> bool:
     return False
 
 
+def _refuse_tangents(*tensors) -> None:
+    """The operators have gradients but no forward-mode derivative: a tangent is refused, not dropped."""
+    if getattr(forward_ad, "_current_level", 0) < 0:   # no dual level is open
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the int8 operators have no forward-mode derivative; an input carries a tangent")
+
+
 _STREAM_MARK = "int8_recorded_on"
 
 
@@ -854,6 +865,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={weight.shape[-1]}")
     if k > MAX_K:
         raise RuntimeError(f"int8 linear: contraction of {k} exceeds {MAX_K} (exact int32 sums)")
+    _refuse_tangents(x, weight, bias)
     if torch.is_grad_enabled() and _wants_grad(x, weight, bias):
         _check_backward(x.numel() // max(k, 1), weight.shape[0] if x.requires_grad else 0,
                         not frozen and weight.requires_grad)
@@ -884,6 +896,7 @@ def int8_gated(
     _check_gated(k, gate, up, activation)
     if k > MAX_K:
         raise RuntimeError(f"int8 gated block: contraction of {k} exceeds {MAX_K} (exact int32 sums)")
+    _refuse_tangents(x, gate, up, gate_bias, up_bias)
     if torch.is_grad_enabled() and _wants_grad(x, gate, up, gate_bias, up_bias):
         frozen = [isinstance(w, Int8Weight) for w in (gate, up)]
         _check_backward(x.numel() // max(k, 1),
