@@ -24,9 +24,10 @@ products of a backward pass run on the int8 tensor cores too: the gradient is wr
 base-256 digits of its row maximum (two digits for bf16 tensors, three for fp16 and fp32; see
 csrc/int8_quant.cu).
 
-Shapes: every contraction (K; in the backward pass also N, the padded pair of N for the gated
-block, and the number of tokens for a weight gradient) is at most 131071, so that int32 sums are
-exact.  Rows whose activations hold a NaN or an infinity come out as NaN.
+Shapes: every contraction (K; in the backward pass also the padded pair of N for the gated block, and
+the number of tokens for a weight gradient) is at most 131071, so that int32 sums are exact.  N of a
+linear is not limited: the activations' gradient of a wider one (a vocabulary head) is summed from
+parts.  Rows whose activations hold a NaN or an infinity come out as NaN.
 """
 
 from __future__ import annotations
@@ -560,10 +561,21 @@ def int8_linear_backward(
         raise RuntimeError(f"int8 matmul shape mismatch: K={k} vs K={weight.shape[1]}")
     nat.require_device(codes.device, ("weight", weight.codes), ("scale", scale))
     _check_types(dx_dtype, dw_dtype, db_dtype)
-    _check_backward(m, n if dx_dtype is not None else 0, dw_dtype is not None)
+    _check_backward(m, 0, dw_dtype is not None)
     scale = _scales(scale, m, "scale")
     return _linear_backward(grad, codes, (m, n, k), (codes.data_ptr(), _code_ld(codes), scale.data_ptr()), _at(weight),
                             weight if keep_transposed else None, (dx_dtype, dw_dtype, db_dtype))
+
+
+def _parts(n: int) -> list[tuple[int, int]]:
+    """(first, count) of the parts of an N-long contraction whose int32 sums are exact: as few as do, of much the
+    same length, starting on multiples of 16."""
+    if n <= MAX_K:
+        return [(0, n)]
+    longest = MAX_K // 16 * 16
+    count = (n + longest - 1) // longest
+    step = _round_up((n + count - 1) // count, 16)
+    return [(first, min(step, n - first)) for first in range(0, n, step)]
 
 
 def _linear_backward(grad, like, sizes, q, w, weight, types):
@@ -572,15 +584,25 @@ def _linear_backward(grad, like, sizes, q, w, weight, types):
     dx_dtype, dw_dtype, db_dtype = types
     d = _grad_rows(grad, m, n, like.device)
     planes = _digit_count(d.dtype, dx_dtype, dw_dtype)
-    dx, dw, db = _out(like, (m, k), dx_dtype), _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
+    parts = _parts(n) if dx_dtype is not None else [(0, n)]
+    dx = _out(like, (m, k), dx_dtype if len(parts) == 1 else torch.float32, dx_dtype is not None)
+    dw, db = _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
     wt = weight.transposed() if dx is not None and weight is not None else None
-    nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 0, planes, dx is not None, dw is not None,
-                                                         db is not None, wt is None)
-    ws = like.new_empty((nbytes,), dtype=torch.uint8)
-    _call(like.device, "ima_int8_linear_backward", d.data_ptr(), _DTYPE_CODES[d.dtype], _ld(d), m, n, k, *q, w[0], w[1],
-          _ptr(wt), _code_ld(wt) if wt is not None else 0, w[2], planes, _ptr(dx), _code(dx), _ptr(dw), _code(dw),
-          _ptr(db), _code(db), ws.data_ptr())
-    return dx, dw, db
+    ws = None
+    for first, count in parts:
+        if ws is None:   # the first part is the longest
+            nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, count, k, 0, planes, dx is not None, dw is not None,
+                                                                 db is not None, wt is None)
+            ws = like.new_empty((nbytes,), dtype=torch.uint8)
+        part = dx if first == 0 else torch.empty_like(dx)
+        _call(like.device, "ima_int8_linear_backward", d.data_ptr() + first * d.element_size(), _DTYPE_CODES[d.dtype],
+              _ld(d), m, count, k, *q, w[0] + first * w[1], w[1], None if wt is None else wt.data_ptr() + first,
+              _code_ld(wt) if wt is not None else 0, w[2] + 4 * first, planes, _ptr(part), _code(part),
+              None if dw is None else dw.data_ptr() + first * k * dw.element_size(), _code(dw),
+              None if db is None else db.data_ptr() + first * db.element_size(), _code(db), ws.data_ptr())
+        if first:
+            dx.add_(part)
+    return dx if dx is None or dx.dtype == dx_dtype else dx.to(dx_dtype), dw, db
 
 
 def int8_gated_backward(
@@ -867,8 +889,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
         raise RuntimeError(f"int8 linear: contraction of {k} exceeds {MAX_K} (exact int32 sums)")
     _refuse_tangents(x, weight, bias)
     if torch.is_grad_enabled() and _wants_grad(x, weight, bias):
-        _check_backward(x.numel() // max(k, 1), weight.shape[0] if x.requires_grad else 0,
-                        not frozen and weight.requires_grad)
+        _check_backward(x.numel() // max(k, 1), 0, not frozen and weight.requires_grad)
         w = None if frozen else weight
         return _record(_LinearFunction, (x, w, bias), x, w, bias, weight if frozen else None)
     w, src = (weight, None) if frozen else _weight_args(weight)

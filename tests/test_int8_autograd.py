@@ -6,8 +6,9 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from int_model_approximation_b200 import int8
-from test_int8 import make, status_clean
+from int_model_approximation_b200 import int8, students
+from test_int8 import (U32, assert_within, digit_limit, grad_bound, half_step, make, plain_codes, smallest,
+                       status_clean)
 
 
 # ---------------------------------------------------------------------------
@@ -42,4 +43,72 @@ def test_tangents_are_refused(cuda_device, requires_grad):
     assert torch.equal(y, int8.int8_linear(x, wt))
     with pytest.raises(RuntimeError, match="forward-mode"):
         torch.func.jvp(lambda t: int8.int8_linear(t, wt), (x.detach(),), (torch.ones_like(x),))
+    status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# linears wider than one exact contraction
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [0, 1, 17, int8.MAX_K - 1, int8.MAX_K, int8.MAX_K + 1, 152064, 262111, 262112, 262113, 393217,
+                               1_000_003])
+def test_parts_cover_the_contraction(n):
+    parts = int8._parts(n)
+    assert sum(count for _, count in parts) == n and all(0 <= count <= int8.MAX_K for _, count in parts)
+    ends = [0]
+    for first, count in parts:
+        assert first == ends[-1] and first % 16 == 0 and (count > 0 or n == 0)
+        ends.append(first + count)
+    assert parts[0][1] == max(count for _, count in parts)
+    assert (len(parts) == 1) == (n <= int8.MAX_K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(1, 131072, 64), (3, 131075, 33), (40, 152064, 96), (130, 262150, 48), (2, 131071, 32)])
+@pytest.mark.parametrize("frozen", [False, True])
+def test_gradients_of_a_vocabulary_head(cuda_device, dtype, m, n, k, frozen):
+    x, w, b = make(m, n, k, dtype, 62, cuda_device, bias=True)
+    g = torch.Generator(device=cuda_device).manual_seed(63)
+    dy = torch.randn((m, n), generator=g, device=cuda_device)
+    dy[:, n // 2:] *= 2.0**-6         # parts of different sizes
+    dy = dy.to(dtype)
+    (q, s), (wq, t) = plain_codes(x), plain_codes(w)
+    for leaf in (x, b) if frozen else (x, w, b):
+        leaf.requires_grad_()
+    if frozen:
+        y = int8.int8_linear(x, int8.Int8Weight.from_float(w), b)
+        (dx, db), dw = torch.autograd.grad(y, (x, b), dy), None
+    else:
+        y = int8.int8_linear(x, w, b)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    want = (dy.double() * t) @ wq
+    none = torch.zeros((m, n), dtype=torch.float64, device=cuda_device)
+    # the parts' sums, each rounded to fp32, and their addition: within the six roundings of the bound
+    assert_within(dx, want, grad_bound(dy.double(), none, t, wq, digit_limit(dtype), dtype, want))
+    assert dx.dtype == dtype and db.dtype == dtype
+    want = dy.double().sum(dim=0)
+    assert_within(db, want, half_step(dtype) * want.abs() + (m + 2) * U32 * dy.double().abs().sum(dim=0) + smallest(dtype))
+    if dw is not None:
+        want = (dy.double() * s[:, None]).T @ q
+        none = torch.zeros((n, m), dtype=torch.float64, device=cuda_device)
+        assert_within(dw, want, grad_bound(dy.double().T, none, s, q, digit_limit(dtype), dtype, want))
+    # the plain call, without and with kept transposed codes, gives the same
+    wt = int8.Int8Weight.from_float(w)
+    codes, scale = int8.per_token_int8(x)
+    for keep in (False, True, True):
+        got = int8.int8_linear_backward(dy, codes, scale, wt, dx_dtype=dtype, keep_transposed=keep)[0]
+        assert torch.equal(got, dx) or not frozen
+    status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+def test_gradients_reach_the_input_of_a_model_with_a_wide_head(cuda_device, monkeypatch):
+    monkeypatch.setattr(students, "STUDENT_KERNEL", "int8")
+    torch.manual_seed(3)
+    model = torch.nn.Sequential(torch.nn.Linear(64, 48), torch.nn.Linear(48, 131200, bias=False)).to(cuda_device)
+    students._replace_int32_linears(model)
+    x = torch.randn((7, 64), device=cuda_device, requires_grad=True)
+    loss = torch.nn.functional.cross_entropy(model(x), torch.arange(7, device=cuda_device) * 18000)
+    loss.backward()
+    assert torch.isfinite(x.grad).all() and float(x.grad.abs().max()) > 0
     status_clean(cuda_device)
