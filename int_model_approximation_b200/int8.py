@@ -21,8 +21,8 @@ Gradients pass straight through the rounding: they are the derivatives at the de
 activations and weights, with the scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
 gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
 products of a backward pass run on the int8 tensor cores too: the gradient is written in
-base-256 digits of its row maximum (two digits for bf16 tensors, three for fp16 and fp32; see
-csrc/int8_quant.cu).
+base-256 digits of its row maximum (two digits for bf16 tensors and sums of up to 49,152, else three;
+see csrc/int8_quant.cu).
 
 Shapes: every contraction (K; in the backward pass also the padded pair of N for the gated block, and
 the number of tokens for a weight gradient) is at most 131071, so that int32 sums are exact.  N of a
@@ -498,11 +498,12 @@ def _code(t: torch.Tensor | None) -> int:
 # ---------------------------------------------------------------------------
 # gradients
 # ---------------------------------------------------------------------------
-def _digit_count(*dtypes: torch.dtype | None) -> int:
-    """Digits of a gradient: two reach 2^-16 of its row maximum, three 2^-24.  Over rows whose elements
-    differ a lot (a column of token gradients) two are off by up to 6e-4 of the result's norm: below
-    bf16's own rounding (2e-3), above fp16's (2e-4)."""
-    return 2 if all(t in (None, torch.bfloat16) for t in dtypes) else 3
+def _digit_count(contraction: int, *dtypes: torch.dtype | None) -> int:
+    """Digits of a gradient: two are off by at most 2^-16 of its row maximum, three by 2^-24.  Over L summands that is
+    at most sqrt(L / 3) 2^-16 of the norm of a result that its largest summand carries (less where others do; 6e-4
+    measured over 4096 tokens of very different sizes).  Two where that is at most 2^-9, half of bf16's own half step:
+    bf16 tensors and L <= 3 * 2^14."""
+    return 2 if contraction <= 3 << 14 and all(t in (None, torch.bfloat16) for t in dtypes) else 3
 
 
 def _check_backward(m: int, contraction: int, want_dw: bool) -> None:
@@ -583,8 +584,9 @@ def _linear_backward(grad, like, sizes, q, w, weight, types):
     m, n, k = sizes
     dx_dtype, dw_dtype, db_dtype = types
     d = _grad_rows(grad, m, n, like.device)
-    planes = _digit_count(d.dtype, dx_dtype, dw_dtype)
     parts = _parts(n) if dx_dtype is not None else [(0, n)]
+    planes = _digit_count(max(parts[0][1] if dx_dtype is not None else 0, m if dw_dtype is not None else 0), d.dtype,
+                          dx_dtype, dw_dtype)
     dx = _out(like, (m, k), dx_dtype if len(parts) == 1 else torch.float32, dx_dtype is not None)
     dw, db = _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
     wt = weight.transposed() if dx is not None and weight is not None else None
@@ -649,7 +651,8 @@ def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, act
     dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype = types
     d = _grad_rows(grad, m, n, like.device)
     want_dw = dgate_dtype is not None or dup_dtype is not None
-    planes = _digit_count(d.dtype, dx_dtype, dgate_dtype, dup_dtype)
+    planes = _digit_count(max(2 * n if dx_dtype is not None else 0, m if want_dw else 0), d.dtype, dx_dtype, dgate_dtype,
+                          dup_dtype)
     w_type, b_type = _one_type(dgate_dtype, dup_dtype), _one_type(gate_db_dtype, up_db_dtype)
     dx = _out(like, (m, k), dx_dtype)
     dgate, dup = _out(like, (n, k), w_type, dgate_dtype is not None), _out(like, (n, k), w_type, dup_dtype is not None)

@@ -7,7 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 from int_model_approximation_b200 import int8, students
-from test_int8 import (U32, assert_within, digit_limit, grad_bound, half_step, make, plain_codes, smallest,
+from test_int8 import (U32, assert_within, digit_limit, grad_bound, half_step, make, plain_act, plain_codes, smallest,
                        status_clean)
 
 
@@ -111,4 +111,44 @@ def test_gradients_reach_the_input_of_a_model_with_a_wide_head(cuda_device, monk
     loss = torch.nn.functional.cross_entropy(model(x), torch.arange(7, device=cuda_device) * 18000)
     loss.backward()
     assert torch.isfinite(x.grad).all() and float(x.grad.abs().max()) > 0
+    status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# digits of gradients over long sums
+# ---------------------------------------------------------------------------
+def test_digits_follow_types_and_lengths():
+    b, h, f = torch.bfloat16, torch.float16, torch.float32
+    assert int8._digit_count(1, b) == int8._digit_count(49152, b, None, b) == 2
+    assert int8._digit_count(49153, b, b, None) == int8._digit_count(1, b, f) == int8._digit_count(1, h) == 3
+    # the worst case of two digits over the longest sum that gets them is half of bf16's half step
+    assert (49152 / 3) ** 0.5 * 2.0**-16 <= torch.finfo(b).eps / 4 < (49153 / 3) ** 0.5 * 2.0**-16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [70000, 131071])
+@pytest.mark.parametrize("gated", [False, True])
+def test_weight_gradient_that_one_token_carries(cuda_device, tokens, gated):
+    """One token 2^14 times the others: the digits' error e is spread over all tokens, the result's norm is
+    the one's.  A value that is off by e rounds to another bf16 number with probability e / step, and is then a step
+    (2^-7 of it at most) off: sqrt(e 2^-7) of the norm.  Three digits: e <= sqrt(131071 / 3) 2^-24 < 2^-16, below
+    2^-11 of the norm; with two it would be 5e-3."""
+    n, k = 64, 96
+    g = torch.Generator(device=cuda_device).manual_seed(64)
+    x = torch.randn((tokens, k), generator=g, device=cuda_device).to(torch.bfloat16)
+    w = (torch.randn((n, k), generator=g, device=cuda_device) * 0.05).to(torch.bfloat16).requires_grad_()
+    dy = torch.randn((tokens, n), generator=g, device=cuda_device) * 2.0**-14
+    dy[0] = torch.where(dy[0] < 0, -1.0, 1.0)
+    dy = dy.to(torch.bfloat16)
+    q, s = plain_codes(x)
+    if gated:       # up at the constant bias 1, so that the gate's gradient is dy act'(g)
+        up, one = torch.zeros((n, k), device=cuda_device), torch.ones(n, device=cuda_device)
+        got, = torch.autograd.grad(int8.int8_gated(x, w, up, None, one), w, dy)
+        wq, t = plain_codes(w)
+        d = dy.double() * plain_act((q @ wq.T) * s[:, None] * t, "silu")[1]
+    else:
+        got, = torch.autograd.grad(int8.int8_linear(x, w), w, dy)
+        d = dy.double()
+    want = (d * s[:, None]).T @ q
+    assert float((got.double() - want.to(torch.bfloat16).double()).norm()) <= 2.0**-10 * float(want.norm())
     status_clean(cuda_device)
