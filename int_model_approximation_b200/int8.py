@@ -498,11 +498,14 @@ def _code(t: torch.Tensor | None) -> int:
 # ---------------------------------------------------------------------------
 # gradients
 # ---------------------------------------------------------------------------
-def _digit_count(contraction: int, *dtypes: torch.dtype | None) -> int:
-    """Digits of a gradient: two are off by at most 2^-16 of its row maximum, three by 2^-24.  Over L summands that is
+def _digit_count(contraction: int, *dtypes: torch.dtype | None, wanted: int | None = None) -> int:
+    """The wanted digits of a gradient, or by default those that its result's type needs.  Digits of a gradient: two are off by at most 2^-16 of its row maximum, three by 2^-24.  Over L summands that is
     at most sqrt(L / 3) 2^-16 of the norm of a result that its largest summand carries (less where others do; 6e-4
     measured over 4096 tokens of very different sizes).  Two where that is at most 2^-9, half of bf16's own half step:
-    bf16 tensors and L <= 3 * 2^14."""
+    bf16 tensors and L <= 3 * 2^14.  That is by norms: a summand below 2^-16 of its row's largest vanishes, which a
+    caller may want kept."""
+    if wanted is not None:
+        return wanted
     return 2 if contraction <= 3 << 14 and all(t in (None, torch.bfloat16) for t in dtypes) else 3
 
 
@@ -511,6 +514,11 @@ def _check_backward(m: int, contraction: int, want_dw: bool) -> None:
         raise RuntimeError(f"int8 backward: contraction of {contraction} exceeds {MAX_K} (exact int32 sums)")
     if want_dw and m > MAX_K:
         raise RuntimeError(f"int8 weight gradient over {m} tokens exceeds {MAX_K} (exact int32 sums); split the batch")
+
+
+def _check_digits(digits: int | None) -> None:
+    if digits not in (None, 2, 3):
+        raise RuntimeError(f"gradients are written in 2 or 3 digits, not {digits!r}")
 
 
 def _check_types(*dtypes: torch.dtype | None) -> None:
@@ -549,12 +557,15 @@ def int8_linear_backward(
     dw_dtype: torch.dtype | None = None,
     db_dtype: torch.dtype | None = None,
     keep_transposed: bool = True,
+    digits: int | None = None,
 ):
     """Gradients of int8_linear as (dx [M, K], dw [N, K], db [N]); None where no type is given.
 
     grad: output gradient [..., N]; codes, scale: per_token_int8 of the activations.  keep_transposed:
     the transposed weight that dx needs stays with `weight` for the next call (one more byte per
-    weight), else, and in a capture, it is temporary.  Launches only, on the current stream."""
+    weight), else, and in a capture, it is temporary.  digits:
+    as in int8_linear.  Launches only, on the current stream."""
+    _check_digits(digits)
     codes = _aligned_codes(codes, "int8 activation matrix")
     weight.follow()
     (m, k), n = codes.shape, weight.shape[0]
@@ -565,7 +576,7 @@ def int8_linear_backward(
     _check_backward(m, 0, dw_dtype is not None)
     scale = _scales(scale, m, "scale")
     return _linear_backward(grad, codes, (m, n, k), (codes.data_ptr(), _code_ld(codes), scale.data_ptr()), _at(weight),
-                            weight if keep_transposed else None, (dx_dtype, dw_dtype, db_dtype))
+                            weight if keep_transposed else None, (dx_dtype, dw_dtype, db_dtype), digits)
 
 
 def _parts(n: int) -> list[tuple[int, int]]:
@@ -579,14 +590,14 @@ def _parts(n: int) -> list[tuple[int, int]]:
     return [(first, min(step, n - first)) for first in range(0, n, step)]
 
 
-def _linear_backward(grad, like, sizes, q, w, weight, types):
+def _linear_backward(grad, like, sizes, q, w, weight, types, digits):
     """q, w: (codes, row stride, scales), as addresses; weight: the Int8Weight that keeps transposed codes, or None."""
     m, n, k = sizes
     dx_dtype, dw_dtype, db_dtype = types
     d = _grad_rows(grad, m, n, like.device)
     parts = _parts(n) if dx_dtype is not None else [(0, n)]
-    planes = _digit_count(max(parts[0][1] if dx_dtype is not None else 0, m if dw_dtype is not None else 0), d.dtype,
-                          dx_dtype, dw_dtype)
+    planes = _digit_count(max(parts[0][1] if dx_dtype is not None else 0, m if dw_dtype is not None else 0),
+                          d.dtype, dx_dtype, dw_dtype, wanted=digits)
     dx = _out(like, (m, k), dx_dtype if len(parts) == 1 else torch.float32, dx_dtype is not None)
     dw, db = _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
     wt = weight.transposed() if dx is not None and weight is not None else None
@@ -623,12 +634,14 @@ def int8_gated_backward(
     gate_db_dtype: torch.dtype | None = None,
     up_db_dtype: torch.dtype | None = None,
     keep_transposed: bool = True,
+    digits: int | None = None,
 ):
     """Gradients of int8_gated as (dx, dgate, dup, dgate_bias, dup_bias); None where no type is given.
 
-    grad: gradient of h [..., N]; codes, scale: per_token_int8 of the activations; keep_transposed as in
-    int8_linear_backward.  Both projections are formed again from the codes, so a forward pass keeps
+    grad: gradient of h [..., N]; codes, scale: per_token_int8 of the activations; keep_transposed and digits
+    as in int8_linear_backward.  Both projections are formed again from the codes, so a forward pass keeps
     one byte per activation and nothing of width N.  Launches only, on the current stream."""
+    _check_digits(digits)
     codes = _aligned_codes(codes, "int8 activation matrix")
     gate.follow()
     up.follow()
@@ -642,17 +655,17 @@ def int8_gated_backward(
                     dgate_dtype is not None or dup_dtype is not None)
     scale = _scales(scale, m, "scale")
     return _gated_backward(grad, codes, (m, n, k), (codes.data_ptr(), _code_ld(codes), scale.data_ptr()), _at(gate),
-                           _at(up), (gate, up) if keep_transposed else None, gate_bias, up_bias, activation, types)
+                           _at(up), (gate, up) if keep_transposed else None, gate_bias, up_bias, activation, types, digits)
 
 
-def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, activation, types):
+def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, activation, types, digits):
     """As _linear_backward; weights: both Int8Weights if they keep transposed codes, else None."""
     m, n, k = sizes
     dx_dtype, dgate_dtype, dup_dtype, gate_db_dtype, up_db_dtype = types
     d = _grad_rows(grad, m, n, like.device)
     want_dw = dgate_dtype is not None or dup_dtype is not None
     planes = _digit_count(max(2 * n if dx_dtype is not None else 0, m if want_dw else 0), d.dtype, dx_dtype, dgate_dtype,
-                          dup_dtype)
+                          dup_dtype, wanted=digits)
     w_type, b_type = _one_type(dgate_dtype, dup_dtype), _one_type(gate_db_dtype, up_db_dtype)
     dx = _out(like, (m, k), dx_dtype)
     dgate, dup = _out(like, (n, k), w_type, dgate_dtype is not None), _out(like, (n, k), w_type, dup_dtype is not None)
@@ -751,7 +764,7 @@ def _source(weight) -> torch.Tensor:
 
 class _LinearFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, handle):
+    def forward(ctx, x, weight, bias, handle, digits):
         rows = _rows(x)
         m, k = rows.shape
         src = None if handle is not None else _source(weight)
@@ -765,6 +778,7 @@ class _LinearFunction(torch.autograd.Function):
         _linear_call(rows, m, k, n, _DTYPE_CODES[rows.dtype], q, True, w, src, bias, y)
         ctx.save_for_backward(block)
         ctx.sizes, ctx.handle, ctx.version = (m, n, k), handle, None if handle is None else _versions(handle)
+        ctx.digits = digits
         ctx.types = _wanted_types(ctx, (x, weight, bias))
         ctx.shapes = (x.shape, None if bias is None else bias.shape)
         return y if x.ndim == 2 else y.reshape(*x.shape[:-1], n)
@@ -784,17 +798,17 @@ class _LinearFunction(torch.autograd.Function):
             _check_versions(ctx.version, handle)
             at, _ = _kept_block(m, ld)
             w = _at(handle)
-        dx, dw, db = _linear_backward(grad, block, sizes, (base, ld, base + at[0]), w, handle, ctx.types)
+        dx, dw, db = _linear_backward(grad, block, sizes, (base, ld, base + at[0]), w, handle, ctx.types, ctx.digits)
         if dx is not None and len(ctx.shapes[0]) != 2:
             dx = dx.reshape(ctx.shapes[0])
         if db is not None and len(ctx.shapes[1]) != 1:
             db = db.reshape(ctx.shapes[1])
-        return dx, dw, db, None
+        return dx, dw, db, None, None
 
 
 class _GatedFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, gate, up, activation):
+    def forward(ctx, x, gate_weight, up_weight, gate_bias, up_bias, gate, up, activation, digits):
         rows = _rows(x)
         m, k = rows.shape
         g_src = None if gate is not None else _source(gate_weight)
@@ -806,7 +820,7 @@ class _GatedFunction(torch.autograd.Function):
         q, g, u = _GatedFunction.parts(block, m, ld, n, gate, up)
         _gated_call(rows, m, k, n, _DTYPE_CODES[rows.dtype], q, True, g, u, g_src, u_src, gate_bias, up_bias, activation, h)
         ctx.save_for_backward(block, gate_bias, up_bias)
-        ctx.sizes, ctx.gate, ctx.up, ctx.activation = (m, n, k), gate, up, activation
+        ctx.sizes, ctx.gate, ctx.up, ctx.activation, ctx.digits = (m, n, k), gate, up, activation, digits
         ctx.version = _versions(*(w for w in (gate, up) if w is not None))
         inputs = (x, gate_weight, up_weight, gate_bias, up_bias)
         ctx.types = _wanted_types(ctx, inputs)
@@ -836,9 +850,10 @@ class _GatedFunction(torch.autograd.Function):
         m, n, k = ctx.sizes
         q, g, u = _GatedFunction.parts(block, m, (k + 15) // 16 * 16 or 16, n, gate, up)
         frozen = (gate, up) if gate is not None and up is not None else None
-        grads = _gated_backward(grad, block, ctx.sizes, q, g, u, frozen, gate_bias, up_bias, ctx.activation, ctx.types)
+        grads = _gated_backward(grad, block, ctx.sizes, q, g, u, frozen, gate_bias, up_bias, ctx.activation, ctx.types,
+                                ctx.digits)
         return (*(t if t is None or t.shape == shape else t.reshape(shape) for t, shape in zip(grads, ctx.shapes)),
-                None, None, None)
+                None, None, None, None)
 
 
 def _beside(x: torch.Tensor, weights: tuple, biases: tuple) -> bool:
@@ -877,11 +892,16 @@ def _check_inputs(x: torch.Tensor, *named) -> None:
             raise RuntimeError(f"{label} must be a tensor or an Int8Weight, got {type(t).__name__}")
 
 
-def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.Tensor | None = None, *,
+                digits: int | None = None) -> torch.Tensor:
     """y = x W^T + b with int8 codes on both sides, in x's type: x [..., K], weight [N, K].
 
     weight: an Int8Weight (frozen) or a floating tensor, quantised in the call and differentiable.
+    digits: of the output's gradient in the backward pass.  2 keep it to 2^-16 of the largest in its row (for dx) or
+    column (for dW), 3 to 2^-24 for about half as much time again in the products; by default 2 for bf16 and sums of
+    up to 49,152, else 3.
     """
+    _check_digits(digits)
     frozen = type(weight) is Int8Weight
     if not (frozen and x.is_cuda and x.ndim and x.dtype in _DTYPE_CODES and _beside(x, (weight,), (bias,))):
         _check_inputs(x, ("weight", weight), ("bias", bias))
@@ -894,7 +914,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
     if torch.is_grad_enabled() and _wants_grad(x, weight, bias):
         _check_backward(x.numel() // max(k, 1), 0, not frozen and weight.requires_grad)
         w = None if frozen else weight
-        return _record(_LinearFunction, (x, w, bias), x, w, bias, weight if frozen else None)
+        return _record(_LinearFunction, (x, w, bias), x, w, bias, weight if frozen else None, digits)
     w, src = (weight, None) if frozen else _weight_args(weight)
     y = _linear_forward(_rows(x), w, src, bias)
     return y if x.ndim == 2 else y.reshape(*x.shape[:-1], w.shape[0])
@@ -908,11 +928,13 @@ def int8_gated(
     up_bias: torch.Tensor | None = None,
     *,
     activation: str = "silu",
+    digits: int | None = None,
 ) -> torch.Tensor:
     """h = act(x Wg^T + bg) * (x Wu^T + bu) in x's type: x [..., K], gate and up [N, K].
 
     Both projections, the activation ("silu", "gelu" with the error function, or "gelu_tanh") and the
-    product run in one kernel; g and u never reach memory.  Weights as in int8_linear."""
+    product run in one kernel; g and u never reach memory.  Weights and digits as in int8_linear."""
+    _check_digits(digits)
     if not (type(gate) is Int8Weight is type(up) and x.is_cuda and x.ndim and x.dtype in _DTYPE_CODES
             and _beside(x, (gate, up), (gate_bias, up_bias))):
         _check_inputs(x, ("gate weight", gate), ("up weight", up), ("gate bias", gate_bias), ("up bias", up_bias))
@@ -928,7 +950,7 @@ def int8_gated(
                         any(not f and w.requires_grad for f, w in zip(frozen, (gate, up))))
         inputs = (x, None if frozen[0] else gate, None if frozen[1] else up, gate_bias, up_bias)
         return _record(_GatedFunction, inputs, *inputs, gate if frozen[0] else None, up if frozen[1] else None,
-                       activation)
+                       activation, digits)
     (g, g_src), (u, u_src) = _weight_args(gate), _weight_args(up)
     h = _gated_forward(_rows(x), g, u, g_src, u_src, gate_bias, up_bias, activation)
     return h if x.ndim == 2 else h.reshape(*x.shape[:-1], g.shape[0])

@@ -152,3 +152,56 @@ def test_weight_gradient_that_one_token_carries(cuda_device, tokens, gated):
     want = (d * s[:, None]).T @ q
     assert float((got.double() - want.to(torch.bfloat16).double()).norm()) <= 2.0**-10 * float(want.norm())
     status_clean(cuda_device)
+
+
+def test_other_numbers_of_digits_are_refused():
+    x, w = torch.zeros(2, 16), torch.zeros(4, 16)
+    for digits in (0, 1, 4, 2.5, "2"):
+        with pytest.raises(RuntimeError, match="2 or 3 digits"):
+            int8.int8_linear(x, w, digits=digits)
+        with pytest.raises(RuntimeError, match="2 or 3 digits"):
+            int8.int8_gated(x, w, w, digits=digits)
+        with pytest.raises(RuntimeError, match="2 or 3 digits"):
+            int8.int8_linear_backward(x, x, x, w, digits=digits)
+        with pytest.raises(RuntimeError, match="2 or 3 digits"):
+            int8.int8_gated_backward(x, x, x, w, w, digits=digits)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,digits", [(torch.bfloat16, 2), (torch.bfloat16, 3), (torch.float32, 2), (torch.float32, 3)])
+@pytest.mark.parametrize("m,n,k", [(3, 70, 33), (300, 130, 250)])
+def test_wanted_digits(cuda_device, dtype, digits, m, n, k):
+    """Every gradient within the digits that were asked for; a small token beside one of 2^18 times its size is kept
+    by three digits and lost by two."""
+    limit = {2: 32639.0, 3: 8355000.0}[digits]
+    x, w, b = make(m, n, k, dtype, 65, cuda_device, bias=True)
+    g = torch.Generator(device=cuda_device).manual_seed(66)
+    dy = torch.randn((m, n), generator=g, device=cuda_device)
+    dy[0] = torch.where(dy[0] < 0, -1.0, 1.0)
+    dy[1:] = dy[1:].clamp(-1, 1) * 2.0**-18
+    dy = dy.to(dtype)
+    x.detach()[0, 1:] = 0     # the large token reaches one column of dW only; the scales stay alike
+    x.detach()[0, 0] = 4.0
+    for t in (x, w, b):
+        t.requires_grad_()
+    (q, s), (wq, t) = plain_codes(x), plain_codes(w)
+    dx, dw, _ = torch.autograd.grad(int8.int8_linear(x, w, b, digits=digits), (x, w, b), dy)
+    want = (dy.double() * t) @ wq
+    none = torch.zeros((m, n), dtype=torch.float64, device=cuda_device)
+    assert_within(dx, want, grad_bound(dy.double(), none, t, wq, limit, dtype, want))
+    want = (dy.double() * s[:, None]).T @ q
+    assert_within(dw, want, grad_bound(dy.double().T, none.T, s, q, limit, dtype, want))
+    small = (dw.double()[:, 1:] - want[:, 1:]).norm() / want[:, 1:].norm()
+    assert (float(small) < 0.2) == (digits == 3)
+    codes, scale = int8.per_token_int8(x)
+    got = int8.int8_linear_backward(dy, codes, scale, int8.Int8Weight.from_float(w), dx_dtype=dtype, dw_dtype=dtype,
+                                    digits=digits)
+    assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+    # the gated block: the same digits through autograd and the plain call, and three closer than two
+    h = int8.int8_gated(x, w, w, b, None, digits=digits)
+    dx, dw = torch.autograd.grad(h, (x, w), dy)
+    wt = int8.Int8Weight.from_float(w)
+    got = int8.int8_gated_backward(dy, codes, scale, wt, wt, b, None, dx_dtype=dtype, dgate_dtype=dtype, dup_dtype=dtype,
+                                   digits=digits)
+    assert torch.equal(got[0], dx)
+    status_clean(cuda_device)
