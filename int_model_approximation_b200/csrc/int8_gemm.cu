@@ -743,17 +743,10 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
 // box_rows(, 1)} box, 128-byte swizzle.
 int make_i8_map(CUtensorMap* map, const int8_t* base, int64_t K, int64_t ld, int64_t rows, int planes,
                 int64_t plane_stride, int box_rows) {
-    const bool three_d = plane_stride != 0;
-    auto enc = get_encode_fn();
-    if (!enc) return IMA_ERR_CUDA;
-    cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)planes};
-    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)plane_stride};
-    cuuint32_t box[3] = {(cuuint32_t)I8_KT, (cuuint32_t)box_rows, 1};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, three_d ? 3 : 2, const_cast<int8_t*>(base), dims, strides, box,
-                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? IMA_OK : IMA_ERR_INVALID_ARGUMENT;
+    const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)plane_stride};
+    const cuuint32_t box[3] = {(cuuint32_t)I8_KT, (cuuint32_t)box_rows, 1};
+    return encode_bytes(map, plane_stride ? 3 : 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Allow `kern` its dynamic shared memory, once per device (a bit each for the first 64).

@@ -515,18 +515,32 @@ PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
     return fn;
 }
 
-// 3-D map over planes [P][rows][ld] int8 with a {64 B, box_rows, 1} box, 64-byte swizzle.
-int make_plane_map(CUtensorMap* map, const int8_t* base, int64_t ld, int64_t rows, int planes, int box_rows) {
+// A tiled map of bytes.  Encoding needs a current context and makes none, unlike the runtime's calls: where it is a
+// thread's first call (a worker's product, autograd's thread), the device's is made current and it is tried again.
+int encode_bytes(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                 const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
     auto enc = get_encode_fn();
     if (!enc) return IMA_ERR_CUDA;
-    cuuint64_t dims[3] = {(cuuint64_t)ld, (cuuint64_t)rows, (cuuint64_t)planes};
-    cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(ld * rows)};
-    cuuint32_t box[3] = {(cuuint32_t)GM_KT, (cuuint32_t)box_rows, 1};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t*>(base), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? IMA_OK : IMA_ERR_INVALID_ARGUMENT;
+    const cuuint32_t estr[3] = {1, 1, 1};
+    auto encode = [&] {
+        return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    if (encode() == CUDA_SUCCESS) return IMA_OK;
+    int dev = 0;
+    int rc = ima_note_cuda(cudaGetDevice(&dev));
+    if (rc == IMA_OK) rc = ima_note_cuda(cudaSetDevice(dev));
+    if (rc != IMA_OK) return rc;
+    return encode() == CUDA_SUCCESS ? IMA_OK : IMA_ERR_INVALID_ARGUMENT;
+}
+
+// 3-D map over planes [P][rows][ld] int8 with a {64 B, box_rows, 1} box, 64-byte swizzle.
+int make_plane_map(CUtensorMap* map, const int8_t* base, int64_t ld, int64_t rows, int planes, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)ld, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld, (cuuint64_t)(ld * rows)};
+    const cuuint32_t box[3] = {(cuuint32_t)GM_KT, (cuuint32_t)box_rows, 1};
+    return encode_bytes(map, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int num_sms() {
