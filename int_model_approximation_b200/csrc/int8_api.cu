@@ -117,7 +117,7 @@ int int8_gated_entry(const int8_t* a, int64_t lda, const int8_t* gate, int64_t l
     I8Params p;
     memset(&p, 0, sizeof(p));
     p.y = y; p.xs = x_scale; p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias;
-    p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = activation;
+    p.bias_dtype = bias_dtype; p.ldy = ldy; p.y_dtype = y_dtype; p.act = act_form(activation, y_dtype == IMA_DTYPE_F32);
     p.M = (int32_t)M; p.N = (int32_t)N; p.dependent = dependent;
     p.y_width = store_width(y, ldy, dtype_bytes(y_dtype));
     return run_codes<1, I8_GATED>(p, {a, gate, up, lda, ldg, ldu, K, K, M * lda}, 2, (cudaStream_t)stream);
@@ -193,7 +193,7 @@ int ima_int8_gated(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx
         SkParams p;
         memset(&p, 0, sizeof(p));
         p.x = x; p.ldx = ldx; p.K = K; p.M = (int32_t)M; p.N = (int32_t)N;
-        p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.act = activation;
+        p.y = y; p.ldy = ldy; p.y_dtype = x_dtype; p.act = act_form(activation, x_dtype == IMA_DTYPE_F32);
         p.ws[0] = gate_scale; p.ws[1] = up_scale; p.bias[0] = gate_bias; p.bias[1] = up_bias; p.bias_dtype = bias_dtype;
         p.vec_y = store_width(y, ldy, dtype_bytes(x_dtype)) >= 4 * dtype_bytes(x_dtype);
         rc = sk_weight_maps(p, {nullptr, gate, up, 0, ldg, ldu, K, K, 0});

@@ -85,7 +85,7 @@ struct __align__(64) I8Params {
     int32_t full_tiles;             // tiles taken whole; each of the rest is split over tail_splits workers
     int32_t tail_splits;
     int32_t M, N, m_tiles, n_tiles, k_tiles, group_m;
-    int32_t y_dtype, bias_dtype, dh_dtype, act, c_width, y_width;   // width: see stage_store
+    int32_t y_dtype, bias_dtype, dh_dtype, act, c_width, y_width;   // act: act_form() (I8_GATED_BWD: the activation); width: see stage_store
     int32_t dependent;              // launched while the kernel before it (a quantiser) still runs
     int32_t seg_tiles;              // I8_DIGIT: k-tiles of the first B; later ones read the second (mb2)
     uint64_t stall_ns;              // test knob (ima_set_gemm_wait_test); 0 in normal use
@@ -126,30 +126,70 @@ struct I8Work {
 // ---------------------------------------------------------------------------
 // activations and their derivatives, fp32
 // ---------------------------------------------------------------------------
-template <int ACT>
-IMA_DEVINL float act_value(float g) {
-    if (ACT == IMA_ACT_SILU) return __fdividef(g, 1.0f + __expf(-g));
-    if (ACT == IMA_ACT_GELU) return 0.5f * g * erfcf(-0.70710678f * g);
-    const float z = 0.79788456f * (g + 0.044715f * g * g * g);
-    return 0.5f * g * (1.0f + tanhf(z));
+// An activation as the forward epilogues take it: IMA_ACT_..., with ACT_FINE for fp32 results.  Results of 16 bits take the
+// hardware's 2^x for e^-|z|: off by 2^-22 + |z| 2^-24 of it, and 0 from |z| = 87 on, where the activation is below 2^-119.
+// 4096 x 4864 x 896 takes 52.7 us to bf16 so, 57.6 with expf.
+constexpr int ACT_FINE = 4;
+inline int act_form(int activation, bool fine) { return activation + (fine ? ACT_FINE : 0); }
+
+template <bool FINE>
+IMA_DEVINL float exp_minus(float x) {   // e^-x, x >= 0
+    if (FINE) return expf(-x);
+    float t;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(x * -1.44269504f));
+    return t;
 }
-// value a = act(g) and slope act'(g)
+// r = 1 / (1 + e^-z) and c = 1 - r, both from e^-|z|, so that neither cancels, overflows or divides by more than 2 (where
+// the estimate of the reciprocal is off by a unit in the last place).
+template <bool FINE>
+IMA_DEVINL void sigmoid_both(float z, float& r, float& c) {
+    const float t = exp_minus<FINE>(fabsf(z));
+    float hi;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(1.0f + t));
+    const float lo = t * hi;
+    r = z < 0.0f ? lo : hi;
+    c = z < 0.0f ? hi : lo;
+}
+// gelu_tanh(g) = g / (1 + e^-z) with z = 2 sqrt(2 / pi) (g + 0.044715 g^3); slope: z'.  Both quotients are 0
+// or 1 from |g| = 13 on, where g may stop: its cube does not overflow.
+IMA_DEVINL float gelu_tanh_z(float g, float& slope) {
+    const float x = fminf(fmaxf(g, -32.0f), 32.0f), x2 = x * x;
+    slope = 1.5957691f + 0.21406444f * x2;
+    return x * (1.5957691f + 0.071354814f * x2);
+}
+template <int FORM>
+IMA_DEVINL float act_value(float g) {
+    constexpr int ACT = FORM % ACT_FINE;
+    if (ACT == IMA_ACT_GELU) return 0.5f * g * erfcf(-0.70710678f * g);
+    float r, c, slope, z = g;
+    if (ACT == IMA_ACT_GELU_TANH) z = gelu_tanh_z(g, slope);
+    sigmoid_both<(FORM >= ACT_FINE)>(z, r, c);
+    return g * r;
+}
+// value a = act(g) and slope act'(g), as exact as fp32 results need for all types: the gradients are formed in fp32,
+// and the estimate would save 0.5 % of a backward pass
 template <int ACT>
 IMA_DEVINL void act_both(float g, float& a, float& da) {
-    if (ACT == IMA_ACT_SILU) {
-        const float s = __fdividef(1.0f, 1.0f + __expf(-g));
-        a = g * s;
-        da = s * (1.0f + g * (1.0f - s));
-    } else if (ACT == IMA_ACT_GELU) {
+    if (ACT == IMA_ACT_GELU) {
         const float cdf = 0.5f * erfcf(-0.70710678f * g);
         a = g * cdf;
-        da = cdf + g * 0.39894228f * __expf(-0.5f * g * g);
+        da = cdf + g * 0.39894228f * expf(-0.5f * g * g);
     } else {
-        const float z = 0.79788456f * (g + 0.044715f * g * g * g);
-        const float t = tanhf(z);
-        a = 0.5f * g * (1.0f + t);
-        da = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g * g);
+        float r, c, slope = 1.0f, z = g;
+        if (ACT == IMA_ACT_GELU_TANH) z = gelu_tanh_z(g, slope);
+        sigmoid_both<true>(z, r, c);
+        a = g * r;
+        da = r + a * c * slope;
     }
+}
+// f(integral_constant of the form); gelu has one, with erfc
+template <typename F>
+IMA_DEVINL void with_form(int form, F&& f) {
+    if (form == IMA_ACT_SILU) f(std::integral_constant<int, IMA_ACT_SILU>{});
+    else if (form == IMA_ACT_GELU_TANH) f(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
+    else if (form == IMA_ACT_SILU + ACT_FINE) f(std::integral_constant<int, IMA_ACT_SILU + ACT_FINE>{});
+    else if (form == IMA_ACT_GELU_TANH + ACT_FINE) f(std::integral_constant<int, IMA_ACT_GELU_TANH + ACT_FINE>{});
+    else f(std::integral_constant<int, IMA_ACT_GELU>{});
 }
 
 // Two fp32 values in one register pair, and arithmetic on both in one instruction; each rounds as the plain form does.
@@ -589,9 +629,7 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
                     if (p.bias[0] || p.bias[1]) chunks(tag, std::true_type{});
                     else chunks(tag, std::false_type{});
                 };
-                if (p.act == IMA_ACT_SILU) both(std::integral_constant<int, IMA_ACT_SILU>{});
-                else if (p.act == IMA_ACT_GELU) both(std::integral_constant<int, IMA_ACT_GELU>{});
-                else both(std::integral_constant<int, IMA_ACT_GELU_TANH>{});
+                with_form(p.act, both);
             } else if constexpr (EPI == I8_GATED_BWD) {
                 uint32_t rm = 0;
                 auto chunks = [&](auto tag) {

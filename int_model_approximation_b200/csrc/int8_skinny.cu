@@ -78,10 +78,10 @@ IMA_DEVINL void store_quad(void* y, int dtype, int64_t off, const float (&v)[4],
     }
 }
 
-IMA_DEVINL float gated_value(int act, float g, float u) {
-    if (act == IMA_ACT_SILU) return act_value<IMA_ACT_SILU>(g) * u;
-    if (act == IMA_ACT_GELU) return act_value<IMA_ACT_GELU>(g) * u;
-    return act_value<IMA_ACT_GELU_TANH>(g) * u;
+IMA_DEVINL float gated_value(int form, float g, float u) {
+    float h;
+    with_form(form, [&](auto tag) { h = act_value<decltype(tag)::value>(g) * u; });
+    return h;
 }
 
 // EPI: I8_LINEAR, I8_GATED or I8_DIGIT; P digit planes (1 otherwise); DT: type of the activations when
