@@ -251,8 +251,8 @@ class Int8Weight:
         self._look()
 
     def state(self) -> tuple:
-        """What an edit changes: the times that codes or scales were replaced, and their counts of in-place edits."""
-        self.follow()
+        """What an edit changes, after follow(): the times that codes or scales were replaced, and their counts of
+        in-place edits."""
         return self._looks, nat.tensor_version(self._codes), nat.tensor_version(self._scale)
 
     def __getstate__(self):
@@ -279,6 +279,11 @@ class Int8Weight:
         capture; the caller then makes its own.  A graph would hold the address of the kept copy, which
         an edit of the codes outdates and the next call afterwards frees, and a copy made in a
         capture is not there before its replay."""
+        self.follow()
+        return self._kept_transposed()
+
+    def _kept_transposed(self) -> torch.Tensor | None:
+        """transposed(), after follow()."""
         state = self.state()[:2]
         if state[1] is None or _capturing(self.index):
             return None
@@ -600,7 +605,7 @@ def _linear_backward(grad, like, sizes, q, w, weight, types, digits):
                           d.dtype, dx_dtype, dw_dtype, wanted=digits)
     dx = _out(like, (m, k), dx_dtype if len(parts) == 1 else torch.float32, dx_dtype is not None)
     dw, db = _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
-    wt = weight.transposed() if dx is not None and weight is not None else None
+    wt = weight._kept_transposed() if dx is not None and weight is not None else None
     ws = None
     for first, count in parts:
         if ws is None:   # the first part is the longest
@@ -672,7 +677,7 @@ def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, act
     dgb, dub = _out(like, (n,), b_type, gate_db_dtype is not None), _out(like, (n,), b_type, up_db_dtype is not None)
     gt = ut = None
     if dx is not None and weights is not None:
-        gt, ut = weights[0].transposed(), weights[1].transposed()
+        gt, ut = weights[0]._kept_transposed(), weights[1]._kept_transposed()
     nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 1, planes, dx is not None, want_dw, b_type is not None,
                                                          gt is None or ut is None)
     ws = like.new_empty((nbytes,), dtype=torch.uint8)
@@ -743,11 +748,13 @@ def _record(function, leaves, *args):
     return function.apply(*args)
 
 
-def _versions(*weights: Int8Weight) -> tuple:
-    return tuple(w.state() for w in weights)
+def _versions(*weights: Int8Weight) -> list:
+    return [w.state() for w in weights]
 
 
-def _check_versions(before: tuple, *weights: Int8Weight) -> None:
+def _check_versions(before: list, *weights: Int8Weight) -> None:
+    for w in weights:
+        w.follow()
     if before != _versions(*weights):
         raise RuntimeError("int8 weight codes or scales were modified in place between the forward and the backward pass")
 
