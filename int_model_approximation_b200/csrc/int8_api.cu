@@ -248,7 +248,7 @@ BwdPlan bwd_plan(int64_t M, int64_t N, int64_t K, int segs, int planes, int want
         b.q_t = take(K * b.ldm);
     }
     if (want & BWD_OWN_WT) b.w_t = take(segs * K * b.ldwt);
-    if (want & BWD_DB) b.partial = take((M + 127) / 128 * b.W * 4);
+    if (want & BWD_DB) b.partial = take((M + 127) / 128 * b.W * 8);
     // more 128 x 128 blocks than workers: the tiled form may have a tail to split
     const int64_t kb = (K + 127) / 128;
     b.has_tail = (dx && (M + 127) / 128 * kb > 74) || (dw && (b.W + 127) / 128 * kb > 74);
@@ -411,7 +411,7 @@ int run_backward(const BwdArgs& a, cudaStream_t st) {
         d.cols = reinterpret_cast<int8_t*>(ws + b.cols);
         d.col_scale = reinterpret_cast<float*>(ws + b.col_scale);
     }
-    if (want_db) d.partial = reinterpret_cast<float*>(ws + b.partial);
+    if (want_db) d.partial = reinterpret_cast<double*>(ws + b.partial);
     d.ldm = b.ldm;
     rc = run_grad_digits(d, src_dtype, a.planes, st);
     if (rc != IMA_OK) return rc;

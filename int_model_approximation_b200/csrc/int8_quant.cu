@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(256) int8_grad_max_kernel(const GradSrc a) {
     if (col < a.n) atomicMax(a.col_max + col, m);
 }
 
-// Digit planes of both forms, and partial column sums of D, in one pass over D.  A block takes 128 rows
+// Digit planes of both forms, and partial column sums of D (in 64 bits), in one pass over D.  A block takes 128 rows
 // by 64 columns; the transposed form goes through shared memory.  There a row is 16 quads of columns, the
 // two of its thread t at t ^ (row / 16) and (t + 8) ^ (row / 16): eight threads that write a row, and eight
 // 16-row groups that read a quad, meet no bank conflicts.  Every plane row is written
@@ -384,7 +384,7 @@ struct GradDigits {
     float* row_scale;         // [M]
     int8_t* cols;             // [P][W][ldm]
     float* col_scale;         // [W]
-    float* partial;           // [ceil(M / 128)][W]
+    double* partial;          // [ceil(M / 128)][W]
     int64_t ldm;
 };
 
@@ -497,9 +497,9 @@ __global__ void __launch_bounds__(256) int8_grad_digits_kernel(const GradDigits 
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = from[i * 64];
         if (a.partial) {
-            float sum = 0.0f;
+            double sum = 0.0;   // 64 bits throughout: one rounding, to the bias' type, at the end
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += v[i];
+            for (int i = 0; i < 16; ++i) sum += (double)v[i];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
             if (lane < 4 && c < valid) a.partial[(int64_t)blockIdx.y * g.W + c0 + c] = sum;
@@ -526,17 +526,16 @@ __global__ void __launch_bounds__(256) int8_grad_digits_kernel(const GradDigits 
 
 // out[j] = sum over chunks of partial[chunk][j], in the type of the bias; blockIdx.y: which of two
 // segments, `pitch` columns apart (out NULL: not wanted).
-__global__ void __launch_bounds__(256) int8_col_sum_kernel(const float* partial, int64_t chunks, int64_t W, int64_t n,
+__global__ void __launch_bounds__(256) int8_col_sum_kernel(const double* partial, int64_t chunks, int64_t W, int64_t n,
                                                            int64_t pitch, void* out0, void* out1, int dtype) {
     const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
     void* out = blockIdx.y ? out1 : out0;
     if (j >= n || !out) return;
     double t = 0.0;
-    for (int64_t c = 0; c < chunks; ++c) t += (double)partial[c * W + blockIdx.y * pitch + j];
-    const float f = (float)t;
-    if (dtype == IMA_DTYPE_F32) reinterpret_cast<float*>(out)[j] = f;
-    else if (dtype == IMA_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(out)[j] = __float2bfloat16_rn(f);
-    else reinterpret_cast<__half*>(out)[j] = __float2half_rn(f);
+    for (int64_t c = 0; c < chunks; ++c) t += partial[c * W + blockIdx.y * pitch + j];
+    if (dtype == IMA_DTYPE_F32) reinterpret_cast<float*>(out)[j] = (float)t;
+    else if (dtype == IMA_DTYPE_BF16) reinterpret_cast<__nv_bfloat16*>(out)[j] = __double2bfloat16(t);
+    else reinterpret_cast<__half*>(out)[j] = __double2half(t);
 }
 
 // dst[c][r] = src[r][c], int8; columns rows..round16(rows) of dst are zero.  A block turns 128 x 128

@@ -205,3 +205,26 @@ def test_wanted_digits(cuda_device, dtype, digits, m, n, k):
                                    digits=digits)
     assert torch.equal(got[0], dx)
     status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# bias gradients
+# ---------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n", [(2, 33), (129, 64), (1000, 70), (4096, 130)])
+def test_bias_gradient_of_sums_that_cancel(cuda_device, dtype, m, n):
+    """Pairs of rows of 2^10 and their negatives around rows of size 1: the 64-bit sums are off by m 2^-53 of the
+    magnitudes, then rounded once."""
+    g = torch.Generator(device=cuda_device).manual_seed(67)
+    dy = torch.randn((m, n), generator=g, device=cuda_device)
+    big = torch.randn((m // 2, n), generator=g, device=cuda_device) * 2.0**10
+    dy[: m // 2] += big
+    dy = dy.to(dtype)
+    dy[m // 2 : m // 2 * 2] -= dy[: m // 2].flip(0)
+    x, w, b = make(m, n, 32, dtype, 68, cuda_device, bias=True)
+    b.requires_grad_()
+    got, = torch.autograd.grad(int8.int8_linear(x, int8.Int8Weight.from_float(w), b), b, dy)
+    want = dy.double().sum(dim=0)
+    assert_within(got, want, half_step(dtype) * want.abs() + m * 2.0**-52 * dy.double().abs().sum(dim=0) + smallest(dtype))
+    status_clean(cuda_device)
