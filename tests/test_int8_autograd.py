@@ -228,3 +228,30 @@ def test_bias_gradient_of_sums_that_cancel(cuda_device, dtype, m, n):
     want = dy.double().sum(dim=0)
     assert_within(got, want, half_step(dtype) * want.abs() + m * 2.0**-52 * dy.double().abs().sum(dim=0) + smallest(dtype))
     status_clean(cuda_device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [49152, 49153, 60000, 140000])
+@pytest.mark.parametrize("digits", [None, 2, 3])
+def test_long_sums_of_two_digits_come_in_parts(cuda_device, n, digits):
+    """One channel that carries dx.  See test_weight_gradient_that_one_token_carries: three digits are off by less
+    than 2^-10 of the norm behind bf16's own rounding, two by sqrt(2^-9 2^-7) at most where a part is no longer than
+    49,152 and by sqrt(sqrt(131071 / 3) 2^-16 2^-7), 2^-7.6, where it is."""
+    m, k = 5, 64
+    x, w, _ = make(m, n, k, torch.bfloat16, 69, cuda_device)
+    w[0] = torch.randn((k,), device=cuda_device).to(torch.bfloat16)
+    g = torch.Generator(device=cuda_device).manual_seed(70)
+    dy = torch.randn((m, n), generator=g, device=cuda_device) * 2.0**-12
+    dy[:, 0] = 1.0
+    dy = dy.to(torch.bfloat16)
+    x.requires_grad_()
+    wt = int8.Int8Weight.from_float(w)
+    got, = torch.autograd.grad(int8.int8_linear(x, wt, digits=digits), x, dy)
+    wq, t = plain_codes(w)
+    want = (dy.double() * t) @ wq
+    none = torch.zeros((m, n), dtype=torch.float64, device=cuda_device)
+    limit = 8355000.0 if digits == 3 else 32639.0
+    assert_within(got, want, grad_bound(dy.double(), none, t, wq, limit, torch.bfloat16, want))
+    off = float((got.double() - want.to(torch.bfloat16).double()).norm() / want.norm())
+    assert off <= (2.0**-10 if digits == 3 else 2.0**-8 if digits is None else 2.0**-7.6)
+    status_clean(cuda_device)
