@@ -281,12 +281,12 @@ class Int8Weight:
         an edit of the codes outdates and the next call afterwards frees, and a copy made in a
         capture is not there before its replay."""
         self.follow()
-        return self._kept_transposed()
+        return None if _capturing(self.index) else self._kept_transposed()
 
     def _kept_transposed(self) -> torch.Tensor | None:
-        """transposed(), after follow()."""
-        state = self.state()[:2]
-        if state[1] is None or _capturing(self.index):
+        """transposed(), after follow() and outside a capture."""
+        state = self._looks, nat.tensor_version(self._codes)
+        if state[1] is None:
             return None
         kept = self._transposed
         if kept is not None and kept[1] == state and kept[2].cuda_stream == _raw_stream(self.index):
@@ -611,7 +611,9 @@ def _linear_backward(grad, like, sizes, q, w, weight, types, digits):
                           d.dtype, dx_dtype, dw_dtype, wanted=digits)
     dx = _out(like, (m, k), dx_dtype if len(parts) == 1 else torch.float32, dx_dtype is not None)
     dw, db = _out(like, (n, k), dw_dtype), _out(like, (n,), db_dtype)
-    wt = weight._kept_transposed() if dx is not None and weight is not None else None
+    wt = None
+    if dx is not None and weight is not None and not _capturing(like.device.index):
+        wt = weight._kept_transposed()
     ws = None
     for first, count in parts:
         if ws is None:   # the first part is the longest
@@ -682,7 +684,7 @@ def _gated_backward(grad, like, sizes, q, g, u, weights, gate_bias, up_bias, act
     dgate, dup = _out(like, (n, k), w_type, dgate_dtype is not None), _out(like, (n, k), w_type, dup_dtype is not None)
     dgb, dub = _out(like, (n,), b_type, gate_db_dtype is not None), _out(like, (n,), b_type, up_db_dtype is not None)
     gt = ut = None
-    if dx is not None and weights is not None:
+    if dx is not None and weights is not None and not _capturing(like.device.index):
         gt, ut = weights[0]._kept_transposed(), weights[1]._kept_transposed()
     nbytes = nat.lib().ima_int8_backward_workspace_bytes(m, n, k, 1, planes, dx is not None, want_dw, b_type is not None,
                                                          gt is None or ut is None)
