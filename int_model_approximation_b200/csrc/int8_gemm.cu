@@ -20,9 +20,10 @@
 // gated forms put 128 rows of G and 128 rows of U into one B tile: a single MMA of N = 256 forms g and u of
 // the same 128 output columns, and A is read once for both.
 //
-// Measured.  Long contractions are bound by power: 16384 x 18944 x 3584 in 0.75 ms with its quantiser (2.95e15
-// operations/s, 0.92 of twice the measured bf16 rate), the gated form in 1.49 (2.99e15); with zeros for operands
-// the same kernel reaches 3.75e15.  Below 14 k-tiles or so the epilogue bounds: 4096 x 4864 x 896 to
+// Measured.  Long contractions are bound by power: 16384 x 18944 x 3584 with its quantiser takes 0.74 to 0.79 ms (cards
+// differ) in the first 20 ms after a pause, 0.92 after seconds of it, when the card draws 1 kW and clocks 1.24 GHz:
+// 2.85e15 and 2.42e15 operations/s, 0.89 and 0.88 of twice the bf16 rates measured the same two ways.  The gated form
+// takes 1.53 and 1.78 (2.91e15 and 2.50e15); with zeros for operands the kernel reaches 3.75e15.  Below 14 k-tiles or so the epilogue bounds: 4096 x 4864 x 896 to
 // bf16 takes 25 us, its products alone 12; per 128 x 256 outputs it takes 5700 clocks, most of them in
 // the shared-memory pipe (tensor memory out, staging in and out).  Small products are bound by the
 // latency of launch, first loads and last epilogue, 8 us.
@@ -376,6 +377,8 @@ __global__ void __launch_bounds__(64 + 32 * i8_epi_warps(EPI), 1) int8_gemm_kern
     constexpr int HALF = TN / (L::EW / 4);                          // output columns of an epilogue warp
     constexpr int COLS = L::EW == 16 ? 128 : 256;                   // its scales and biases
     static_assert((PAIR ? 4 : 2) * HALF <= COLS, "scales and biases of an epilogue warp");
+    // The gated forward forms spill a few registers: 5 loads and 4 stores per warp and tile whatever the activation, 0.1 to
+    // 0.4 % of the instructions (counted for 256 and 4096 x 4864 x 896).
     extern __shared__ unsigned char i8_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(i8_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::BAR_OFFSET);

@@ -2,8 +2,9 @@
 
 The codebook student reproduces an FP8 linear bit for bit and pays nine int8 products per
 multiplication for it.  The operators here pay one: activations are quantised per token and
-weights per output channel to int8, the product is exact in int32 (and Freivalds-checkable
-like every integer product of this package), and the scales are applied in the epilogue.
+weights per output channel to int8, the product is exact in int32, and the scales are applied in
+the epilogue.  int8_gemm returns the int32 product, which Freivalds checks like every integer
+product of this package; int8_linear and int8_gated keep theirs on the chip.
 There is no counterpart in the reference.
 
   per_token_int8    the quantiser of both sides
@@ -16,7 +17,8 @@ There is no counterpart in the reference.
 
 int8_linear and int8_gated take part in reverse-mode autograd; forward-mode tangents are refused.  A
 whole training step can be captured into a CUDA graph if no eager autograd graph of the same leaves
-is alive; the *_backward calls, which record nothing, can always.
+is alive (refused where these operators recorded it; nothing tells of one that others recorded); the
+*_backward calls, which record nothing, can always.
 Gradients pass straight through the rounding: they are the derivatives at the dequantised
 activations and weights, with the scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
 gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
@@ -358,7 +360,7 @@ def int8_gemm(
     c_out: torch.Tensor | None = None,
     y_out: torch.Tensor | None = None,
 ):
-    """C = A B^T exactly (int32) and/or y = (fp32(C) * x_scale[m]) * w_scale[n] (+ bias).
+    """C = A B^T exactly (int32) and/or y = (fp32(C) * x_scale[m]) * w_scale[n] (+ bias).  Records nothing for autograd.
 
     a: int8 [M, K]; b: int8 [N, K], any strides (rows that do not start on 16 bytes are copied).
     Returns (c int32 [M, N] or None, y [M, N] or None)."""

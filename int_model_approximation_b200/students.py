@@ -339,8 +339,8 @@ class HawkeyeClassCountsLinear(nn.Module):
 
 class Int8Linear(nn.Module):
     """Linear with int8 activations (one scale per token) and int8 weights (one per output channel):
-    one exact int32 product per forward.  No counterpart in the reference; weight is the
-    dequantised one, like Int32Linear's."""
+    one exact int32 product per forward, counted by the probe.  No counterpart in the reference.  Made from
+    the dequantised weight, like Int32Linear; the buffers weight and weight_scale hold its codes and scales."""
 
     def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None):
         super().__init__()
