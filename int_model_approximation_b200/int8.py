@@ -206,7 +206,8 @@ class Int8Weight:
     `codes` and `scale` stay the caller's tensors where their layout allows it (rows on 16-byte
     boundaries); the transposed codes that a backward pass contracts over are made at the first
     one and kept until the codes change.  A captured backward pass makes its own at every replay,
-    so that replays follow edits of the codes."""
+    so that replays follow edits of the codes.  A replayed graph that itself writes codes leaves no trace on
+    the tensor: after one, make a new Int8Weight."""
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
         codes = _aligned_codes(codes.detach(), "int8 weight")

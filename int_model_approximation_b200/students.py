@@ -13,6 +13,7 @@ runs on the sm_100a kernels of libima_b200.so; there is no CPU execution path.
 
 from __future__ import annotations
 
+import copy
 import functools
 import inspect
 import math
@@ -411,21 +412,16 @@ def _gated_activation(module: nn.Module) -> str | None:
     """The activation of a module that computes down(act(gate(x)) * up(x)) on children gate_proj, up_proj, down_proj
     and act_fn, in the layout of every gated block this package's shapes come from; None for anything else.
     The names only propose: a fused block replaces the module's own forward and no longer calls gate_proj, up_proj
-    and act_fn, so own parameters or buffers, hooks on any of them and a forward that computes something else decline."""
+    and act_fn, so own parameters or buffers (the activation's too), hooks on any of them and a forward that computes
+    something else decline.  The activation may be of any class."""
     children = dict(module.named_children())
     if set(children) != {"gate_proj", "up_proj", "down_proj", "act_fn"}:
         return None
-    own = (*module.parameters(recurse=False), *module.buffers(recurse=False))
-    if own or any(map(_hooked, (module, children["gate_proj"], children["up_proj"], children["act_fn"]))):
-        return None
     act = children["act_fn"]
-    if isinstance(act, nn.SiLU):
-        activation = "silu"
-    elif isinstance(act, nn.GELU):
-        activation = "gelu_tanh" if act.approximate == "tanh" else "gelu"
-    else:
+    own = (*module.parameters(recurse=False), *module.buffers(recurse=False), *act.parameters(), *act.buffers())
+    if own or any(map(_hooked, (module, children["gate_proj"], children["up_proj"], *act.modules()))):
         return None
-    return activation if _computes_gated(module, activation) else None
+    return next((name for name in _ACTIVATION_FUNCTIONS if _computes_gated(module, name)), None)
 
 
 _ACTIVATION_FUNCTIONS = {"silu": F.silu, "gelu": F.gelu, "gelu_tanh": functools.partial(F.gelu, approximate="tanh")}
@@ -457,14 +453,15 @@ def _computes_gated(module: nn.Module, activation: str) -> bool:
             return False
         gate, up, down = (_Picked(getattr(module, name), step)
                           for name, step in (("gate_proj", 7), ("up_proj", 11), ("down_proj", 13)))
-        i = torch.arange(6 * gate.in_features, device="cpu", dtype=torch.float64).reshape(2, 3, -1)
+        tokens = max(3, -(-4096 // gate.in_features))   # narrow blocks too see every magnitude
+        i = torch.arange(2 * tokens * gate.in_features, device="cpu", dtype=torch.float64).reshape(2, tokens, -1)
         x = torch.where(i * 0.7548 % 1.0 < 0.5, -1.0, 1.0) * 10.0 ** (7.0 * (i * 0.5698 % 1.0) - 3.0)
         want = down(_ACTIVATION_FUNCTIONS[activation](gate(x)) * up(x))
         bound = 1e-5 * want.abs() + down(1e-6 * up(x).abs())   # covers an activation taken in fp32
         for training in (False, True):
             twin = object.__new__(type(module))   # the module's own forward and attributes, other projections
             vars(twin).update(vars(module), training=training, _modules={
-                **module._modules, "gate_proj": gate, "up_proj": up, "down_proj": down})
+                "gate_proj": gate, "up_proj": up, "down_proj": down, "act_fn": copy.deepcopy(module.act_fn).train(training)})
             with torch.no_grad(), torch.random.fork_rng(devices=[]):
                 got = twin.forward(x.clone())
             if not (isinstance(got, torch.Tensor) and got.shape == want.shape and

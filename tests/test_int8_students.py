@@ -249,3 +249,39 @@ def test_a_cast_model_computes_with_its_own_scales(cuda_device):
         lin = cast(lin)
         assert torch.equal(lin(x), want)
     status_clean(cuda_device)
+
+
+# ---------------------------------------------------------------------------
+# activations of other classes
+# ---------------------------------------------------------------------------
+class OwnGelu(torch.nn.Module):
+    def forward(self, x):
+        return 0.5 * x * (1.0 + torch.tanh(0.7978845608028654 * (x + 0.044715 * x**3)))
+
+
+class OwnSilu(torch.nn.Module):
+    def forward(self, x):
+        return x * torch.sigmoid(x)
+
+
+class ScaledSilu(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.beta = torch.nn.Parameter(torch.ones(1))
+
+    def forward(self, x):
+        return x * torch.sigmoid(self.beta * x)
+
+
+def test_activations_of_other_classes():
+    assert students._gated_activation(GatedBlock(4, 8, OwnGelu())) == "gelu_tanh"
+    assert students._gated_activation(GatedBlock(4, 8, OwnSilu())) == "silu"
+    assert students._gated_activation(GatedBlock(4, 8, torch.nn.Sequential(torch.nn.SiLU()))) == "silu"
+    quick = torch.nn.Module()
+    quick.forward = lambda x: x * torch.sigmoid(1.702 * x)
+    dropping = torch.nn.Sequential(torch.nn.SiLU(), torch.nn.Dropout(0.5))
+    for act in (ScaledSilu(), quick, dropping, dropping.eval(), torch.nn.Mish(), torch.nn.Tanh(), torch.nn.Identity()):
+        assert students._gated_activation(GatedBlock(4, 8, act)) is None
+    hooked = torch.nn.Sequential(torch.nn.SiLU())
+    hooked[0].register_forward_hook(lambda *args: None)
+    assert students._gated_activation(GatedBlock(4, 8, hooked)) is None
