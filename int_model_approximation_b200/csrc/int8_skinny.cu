@@ -17,9 +17,9 @@
 // saves a launch and a round trip of the codes.  Otherwise the row quantiser runs before, and this
 // kernel is launched so that it starts, and loads its first weight tiles, while that one finishes.
 //
-// Measured: 16 tokens by 3584 x 18944 (68 MB of weights) 19.1 us, where a kernel that only loads them takes
-// 15.0 and the measured copy rate would allow 10.4; the gated form of one token by 18944 x 3584 (136 MB) 28.2 us,
-// 4.8 TB/s; one token by 4864 x 896 8.8 us, all of it latency.
+// Measured: 16 tokens by 3584 x 18944 (68 MB of weights) 18.3 to 18.9 us, where a kernel that only loads them takes
+// 15.0 and the measured copy rate would allow 10.4; the gated form of one token by 18944 x 3584 (136 MB) 27.8 us,
+// 4.9 TB/s; one token by 4864 x 896 8.5 us, all of it latency.
 #include "sm100_pair.cuh"
 
 namespace {
