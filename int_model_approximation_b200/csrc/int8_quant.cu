@@ -16,7 +16,7 @@
 // element carries the whole row: 1.7e-3 over the 37888 columns of a pair, 3.2e-3 over the longest sum.
 // Measured: 4e-5 for Gaussian rows, 6e-4 for columns of 4096 token gradients of very different sizes.  bf16 rounds
 // by up to 2^-8 of a value, 1.6e-3 of a norm, fp16 by an eighth of that: the callers take P = 2 for bf16 and L <=
-// 49152, where the worst case is at most 2^-9, else P = 3.
+// 65536, where the worst case is 2.3e-3, else P = 3.
 #include <algorithm>
 #include <type_traits>
 #include "sm100_pair.cuh"

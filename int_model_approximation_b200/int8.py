@@ -23,13 +23,14 @@ Gradients pass straight through the rounding: they are the derivatives at the de
 activations and weights, with the scales held fixed.  A weight given as a floating tensor is quantised in the call and gets a
 gradient (training with a master weight); an Int8Weight is frozen and gets none.  The two
 products of a backward pass run on the int8 tensor cores too: the gradient is written in
-base-256 digits of its row maximum (two digits for bf16 tensors and sums of up to 49,152, else three;
+base-256 digits of its row maximum (two digits for bf16 tensors and sums of up to 65,536, else three;
 see csrc/int8_quant.cu).
 
 Shapes: every contraction (K; in the backward pass also the padded pair of N for the gated block, and
 the number of tokens for a weight gradient) is at most 131071, so that int32 sums are exact.  N of a
 linear is not limited: the activations' gradient of a wider one (a vocabulary head) is summed in fp32
-from parts, of at most 49,152 outputs where two digits are taken.  Rows whose activations hold a NaN or an infinity come out as NaN.
+from parts, of at most 65,536 outputs where two digits are taken.  Rows whose activations hold a NaN
+or an infinity come out as NaN, as do rows of a product with a gradient that does.
 """
 
 from __future__ import annotations
@@ -43,7 +44,7 @@ from torch.autograd.function import once_differentiable
 from . import _native as nat
 
 MAX_K = 131071
-TWO_DIGITS = 3 << 14   # longest sum that two digits of a bf16 gradient do for (_digit_count)
+TWO_DIGITS = 1 << 16   # longest sum that two digits of a bf16 gradient do for (_digit_count)
 ACTIVATIONS = {"silu": nat.IMA_ACT_SILU, "gelu": nat.IMA_ACT_GELU, "gelu_tanh": nat.IMA_ACT_GELU_TANH}
 
 
@@ -508,11 +509,11 @@ def _code(t: torch.Tensor | None) -> int:
 # gradients
 # ---------------------------------------------------------------------------
 def _digit_count(contraction: int, *dtypes: torch.dtype | None, wanted: int | None = None) -> int:
-    """The wanted digits of a gradient, or by default those that its result's type needs.  Digits of a gradient: two are off by at most 2^-16 of its row maximum, three by 2^-24.  Over L summands that is
-    at most sqrt(L / 3) 2^-16 of the norm of a result that its largest summand carries (less where others do; 6e-4
-    measured over 4096 tokens of very different sizes).  Two where that is at most 2^-9, half of bf16's own half step:
-    bf16 tensors and L <= TWO_DIGITS.  That is by norms: a summand below 2^-16 of its row's largest vanishes, which a
-    caller may want kept."""
+    """The wanted digits of a gradient, or by default those that its result's type needs.  Two are off by at most
+    2^-16 of its row maximum, three by 2^-24.  Over L summands that is at most sqrt(L / 3) 2^-16 of the norm of a
+    result that its largest summand carries (less where others do; 6e-4 measured over 4096 tokens of very different
+    sizes).  Two where that is below 0.6 of bf16's own half step of 2^-8: bf16 tensors and L <= TWO_DIGITS.  That is
+    by norms: a summand below 2^-16 of its row's largest vanishes, which a caller may want kept."""
     if wanted is not None:
         return wanted
     return 2 if contraction <= TWO_DIGITS and all(t in (None, torch.bfloat16) for t in dtypes) else 3
@@ -606,8 +607,8 @@ def _linear_backward(grad, like, sizes, q, w, weight, types, digits):
     d = _grad_rows(grad, m, n, like.device)
     parts = [(0, n)]
     if dx_dtype is not None and n > TWO_DIGITS:
-        # sums that two digits do for: 4096 tokens through 152064 outputs of 896 columns take 1.9 ms in four such
-        # parts and 2.8 in two of three digits
+        # sums that two digits do for: 4096 tokens through 152064 outputs of 896 columns take 1.9 ms in three or four
+        # such parts and 2.8 in two of three digits
         short = digits is None and _digit_count(m if dw_dtype is not None else 0, d.dtype, dx_dtype, dw_dtype) == 2
         parts = _parts(n, TWO_DIGITS if short else MAX_K)
     planes = _digit_count(max(parts[0][1] if dx_dtype is not None else 0, m if dw_dtype is not None else 0),
@@ -917,7 +918,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight | torch.Tensor, bias: torch.
     weight: an Int8Weight (frozen) or a floating tensor, quantised in the call and differentiable.
     digits: of the output's gradient in the backward pass.  2 keep it to 2^-16 of the largest in its row (for dx) or
     column (for dW), 3 to 2^-24 for about half as much time again in the products; by default 2 for bf16 and sums of
-    up to 49,152, else 3.
+    up to 65,536, else 3.
     """
     _check_digits(digits)
     frozen = type(weight) is Int8Weight

@@ -119,10 +119,10 @@ def test_gradients_reach_the_input_of_a_model_with_a_wide_head(cuda_device, monk
 # ---------------------------------------------------------------------------
 def test_digits_follow_types_and_lengths():
     b, h, f = torch.bfloat16, torch.float16, torch.float32
-    assert int8._digit_count(1, b) == int8._digit_count(49152, b, None, b) == 2
-    assert int8._digit_count(49153, b, b, None) == int8._digit_count(1, b, f) == int8._digit_count(1, h) == 3
-    # the worst case of two digits over the longest sum that gets them is half of bf16's half step
-    assert (49152 / 3) ** 0.5 * 2.0**-16 <= torch.finfo(b).eps / 4 < (49153 / 3) ** 0.5 * 2.0**-16
+    assert int8._digit_count(1, b) == int8._digit_count(65536, b, None, b) == 2
+    assert int8._digit_count(65537, b, b, None) == int8._digit_count(1, b, f) == int8._digit_count(1, h) == 3
+    # the worst case of two digits over the longest sum that gets them is 0.6 of bf16's half step
+    assert (65536 / 3) ** 0.5 * 2.0**-16 <= 0.6 * torch.finfo(b).eps / 2
 
 
 @pytest.mark.gpu
@@ -231,12 +231,12 @@ def test_bias_gradient_of_sums_that_cancel(cuda_device, dtype, m, n):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("n", [49152, 49153, 60000, 140000])
+@pytest.mark.parametrize("n", [65536, 65537, 70000, 140000])
 @pytest.mark.parametrize("digits", [None, 2, 3])
 def test_long_sums_of_two_digits_come_in_parts(cuda_device, n, digits):
     """One channel that carries dx.  See test_weight_gradient_that_one_token_carries: three digits are off by less
-    than 2^-10 of the norm behind bf16's own rounding, two by sqrt(2^-9 2^-7) at most where a part is no longer than
-    49,152 and by sqrt(sqrt(131071 / 3) 2^-16 2^-7), 2^-7.6, where it is."""
+    than 2^-10 of the norm behind bf16's own rounding, two by sqrt(sqrt(65536 / 3) 2^-16 2^-7), 2^-7.8, where a part is
+    no longer than 65,536 and by sqrt(sqrt(131071 / 3) 2^-16 2^-7), 2^-7.6, where it is."""
     m, k = 5, 64
     x, w, _ = make(m, n, k, torch.bfloat16, 69, cuda_device)
     w[0] = torch.randn((k,), device=cuda_device).to(torch.bfloat16)
@@ -253,5 +253,5 @@ def test_long_sums_of_two_digits_come_in_parts(cuda_device, n, digits):
     limit = 8355000.0 if digits == 3 else 32639.0
     assert_within(got, want, grad_bound(dy.double(), none, t, wq, limit, torch.bfloat16, want))
     off = float((got.double() - want.to(torch.bfloat16).double()).norm() / want.norm())
-    assert off <= (2.0**-10 if digits == 3 else 2.0**-8 if digits is None else 2.0**-7.6)
+    assert off <= (2.0**-10 if digits == 3 else 2.0**-7.8 if digits is None else 2.0**-7.6)
     status_clean(cuda_device)

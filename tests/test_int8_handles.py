@@ -162,3 +162,36 @@ def test_repointed_codes_and_scales(cuda_device):
     with pytest.raises(RuntimeError, match="do not start on 16 bytes"):
         int8.int8_gated(x, wt, other)
     status_clean(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated,n", [(False, 70), (False, 131080), (True, 70)])
+def test_replayed_training_steps_follow_edited_codes(cuda_device, gated, n):
+    """Forward and backward through autograd, captured while transposed copies are kept; then codes and scales edited."""
+    m, k = 20, 48
+    x, w, _ = make(m, n, k, torch.float32, 55, cuda_device)
+    x.requires_grad_()
+    dy = torch.randn((m, n), device=cuda_device)
+    wt = int8.Int8Weight.from_float(w)
+
+    def step(wt):
+        y = int8.int8_gated(x, wt, wt) if gated else int8.int8_linear(x, wt)
+        return y.detach(), *torch.autograd.grad(y, x, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(wt)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(wt)
+    for edit in (lambda: wt.codes[3].fill_(100), lambda: wt.scale.mul_(1.5), lambda: wt.codes[:, 1].zero_()):
+        edit()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(int8.Int8Weight(wt.codes.clone(), wt.scale.clone()))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del want
+    status_clean(cuda_device)
